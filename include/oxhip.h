@@ -549,6 +549,137 @@ int oxh_moe_route(const float *d_logits, size_t n_tok, size_t n_expert, size_t t
                   int32_t *d_ids, float *d_weights, uint32_t *d_counts, uint32_t *d_offsets,
                   uint32_t *d_perm, uint32_t *d_slot_pos, void *stream);
 
+/* Routers of models with many experts, beside oxh_moe_route (which keeps the
+ * reference's softmax and its order among equal probabilities).  Per token:
+ *   score   softmax over the experts, or a sigmoid of each logit, in 64 bits
+ *   key     score + d_bias[e] (d_bias NULL: the score).  The bias keeps the
+ *           experts' loads even: it takes part in the choice, not in the weight
+ *   groups  n_group > 1: the experts are n_group runs of n_expert / n_group;
+ *           a group ranks by its best key, or by the sum of its best two
+ *           (group_best 1 or 2), and only the experts of the top_group best
+ *           groups can be chosen.  n_group <= 1: all experts
+ *   choice  the top_k largest keys, largest first; equal keys, and equal
+ *           groups, go to the lower index
+ *   weight  score, divided by the sum of the chosen scores when `renorm`,
+ *           times `scale`; rounded once, to f32
+ * An expert whose logit is -inf or NaN, or whose key is NaN or -inf, is
+ * masked: its weight is 0, it is chosen only where the kept groups hold fewer
+ * than top_k others (lowest index first), and it does not count in its group's
+ * rank; a group with no other expert ranks last.  A token whose experts are
+ * all masked gets weights of 0.  A logit of +inf counts as the largest f32.
+ * Weights are 0 where the sum to divide by is 0.
+ * Then the pairs are sorted by expert, token order kept, as oxh_moe_route
+ * leaves them: what oxh_moe_ffn_i8 takes. */
+#define OXH_SCORE_SOFTMAX 0u
+#define OXH_SCORE_SIGMOID 1u
+#define OXH_SELECT_MAX_EXPERTS 512u
+#define OXH_SELECT_MAX_TOPK     16u
+#define OXH_SELECT_MAX_GROUPS   64u
+#define OXH_SELECT_MAX_TOKENS 65535u
+typedef struct OxhMoeRouter {
+    uint32_t     score;               /* OXH_SCORE_*                                     */
+    uint32_t     group_best;          /* 1 or 2; read when n_group > 1                   */
+    size_t       n_expert, top_k;
+    size_t       n_group, top_group;  /* top_group is read when n_group > 1              */
+    const float *d_bias;              /* NULL or n_expert values                         */
+    int          renorm;
+    float        scale;
+} OxhMoeRouter;
+/* Where a routing lies on the device.  ids, weights, perm, slot_pos:
+ * n_tok * top_k entries, pair (t, j) of ids, weights and slot_pos at
+ * t * top_k + j; counts: n_expert; offsets: n_expert + 1 (see oxh_moe_route). */
+typedef struct OxhRouting {
+    int32_t  *d_ids;
+    float    *d_weights;
+    uint32_t *d_counts, *d_offsets, *d_perm, *d_slot_pos;
+} OxhRouting;
+/* Bytes of workspace a call takes (0 up to 64 tokens). */
+int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes);
+/* d_logits: n_tok rows of n_expert values of `logits_type` (OXH_F32, OXH_F16,
+ * OXH_BF16), logits_stride elements apart.  d_workspace: 16-byte aligned,
+ * overwritten; NULL where none is needed. */
+int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const void *d_logits, size_t logits_stride,
+                   size_t n_tok, const OxhRouting *out, void *d_workspace, size_t workspace_bytes, void *stream);
+
+/* int8 rows with ONE scale per row: weights with a scale per output channel
+ * against tokens with a scale each.  The integer sum runs over the whole row, so
+ * a prompt's product has no float step per block (oxh_mmq's 32- and 256-value
+ * formats have, and are paced by it).  Any packed matrix gets there in two
+ * calls: oxh_get_rows expands rows to f32, oxh_i8_quantize writes codes and
+ * scales.  No counterpart in the reference.
+ * Row r of such a matrix: `cols` codes at d + r * stride; d 16-byte aligned,
+ * stride a multiple of 16 and at least cols (64 or 128 read fastest).  The
+ * bytes between cols and the next multiple of 16 are read and not used.  Any
+ * cols from 1 to OXH_I8_MAX_COLS (the int32 sums of codes -128..127 cannot
+ * overflow); more is OXH_ERR_TOO_WIDE. */
+#define OXH_I8_MAX_COLS 131071u
+/* element types of the float side (not GGUF type ids) */
+#define OXH_F32  0u
+#define OXH_F16  1u
+#define OXH_BF16 2u
+typedef struct OxhI8Matrix {
+    const int8_t *d_w;
+    size_t        stride;             /* bytes from row to row                           */
+    const float  *d_scale;            /* rows values                                     */
+    size_t        rows, cols;
+} OxhI8Matrix;
+/* Rows of floats to codes and scales:  v = x, or silu(x) * up with d_up (laid
+ * out like d_x; f32 arithmetic),
+ *   scale = max|v| / 127 rounded to f32,  code = the integer nearest to
+ *   v / scale (of the exact quotient; ties to even), within -127..127.
+ * A row of zeros, or one whose scale would lie below 2^-126, gets scale 0 and
+ * codes 0; a row that holds an infinity or a NaN gets scale NaN and codes 0,
+ * so that what is computed from it, and nothing else, is NaN.
+ * x_stride in elements, at least cols, also for one row; d_x and d_up aligned
+ * to their elements; d_q 16-byte aligned, q_stride a multiple of 16.  The bytes
+ * between cols and the next multiple of 16 are written as 0, those behind are
+ * left alone.  d_q may not overlap the inputs. */
+int oxh_i8_quantize(uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, size_t cols,
+                    const void *d_up, int8_t *d_q, size_t q_stride, float *d_scale, void *stream);
+/* out[t * out_stride + r] = (sum_k q[t][k] * w[r][k]) * q_scale[t] * w_scale[r]
+ * + bias[r], for t < n_vec (any count) in out_type; the sum is an exact
+ * integer, the rest f32, rounded once.  d_bias NULL or `rows` floats.  d_out
+ * aligned to its elements.  Few results over long rows are shared out over
+ * the columns when there is a workspace (oxh_i8_matmul_workspace bytes,
+ * 16-byte aligned, overwritten; with less, or NULL, the call does without,
+ * and with the same results). */
+size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec);
+int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
+                  const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,
+                  void *d_workspace, size_t workspace_bytes, void *stream);
+/* oxh_i8_matmul over float tokens, quantised on the way (oxh_i8_quantize's
+ * codes and scales; the results are those of the two calls): one launch for a
+ * few tokens, so that a decode step needs no quantiser of its own.  The
+ * workspace is not optional here: oxh_i8_linear_workspace bytes, 16-byte
+ * aligned, overwritten (0 where the call needs none). */
+size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec);
+int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
+                  const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,
+                  void *d_workspace, size_t workspace_bytes, void *stream);
+/* A mixture-of-experts feed-forward over int8 stacks under a given routing
+ * (oxh_moe_select's, or oxh_moe_route's):
+ *   x of every token to codes; per expert and only for its own pairs gate and
+ *   up, h = silu(gate) * up in f32, h to codes, down in f32;
+ *   out[t] = sum over t's pairs j, in their order, of weight[t][j] * down.
+ * Matrices are stacked expert-major as in OxhMoe (expert e of gate / up at rows
+ * [e*ffn, (e+1)*ffn), of down at rows [e*hidden, (e+1)*hidden)), a scale per
+ * row.  n_expert <= 512, top_k <= 16, n_tok <= 65535.  The routing must be one
+ * of n_tok tokens over n_expert experts with top_k choices; entries out of
+ * range are clamped, never followed.  A fixed sequence of launches, capturable.
+ * No output may overlap an input. */
+typedef struct OxhMoeI8 {
+    const int8_t *d_w_gate, *d_w_up, *d_w_down;
+    const float  *d_s_gate, *d_s_up, *d_s_down;
+    size_t        gate_up_stride, down_stride;   /* bytes from row to row                */
+    size_t        n_expert, top_k, hidden, ffn;
+} OxhMoeI8;
+int oxh_moe_i8_workspace_bytes(const OxhMoeI8 *m, size_t n_tok, size_t *bytes);
+/* d_workspace: oxh_moe_i8_workspace_bytes() of device memory, 256-byte aligned,
+ * overwritten by every call: calls that overlap in time need one each. */
+int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint32_t x_type, const void *d_x, size_t x_stride,
+                   size_t n_tok, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
+                   size_t workspace_bytes, void *stream);
+
 /* Device memory / stream / event plumbing so that C callers never include
  * HIP headers (as cuda_mmq.h does with its void* stream). */
 int  oxh_malloc(void **d_ptr, size_t bytes);

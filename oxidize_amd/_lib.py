@@ -38,6 +38,24 @@ class OxhMoe(ctypes.Structure):
                 ("n_expert", Z), ("top_k", Z), ("hidden", Z), ("ffn", Z), ("renorm", I)]
 
 
+class OxhMoeRouter(ctypes.Structure):
+    _fields_ = [("score", U32), ("group_best", U32), ("n_expert", Z), ("top_k", Z), ("n_group", Z), ("top_group", Z),
+                ("d_bias", V), ("renorm", I), ("scale", ctypes.c_float)]
+
+
+class OxhRouting(ctypes.Structure):
+    _fields_ = [("d_ids", V), ("d_weights", V), ("d_counts", V), ("d_offsets", V), ("d_perm", V), ("d_slot_pos", V)]
+
+
+class OxhI8Matrix(ctypes.Structure):
+    _fields_ = [("d_w", V), ("stride", Z), ("d_scale", V), ("rows", Z), ("cols", Z)]
+
+
+class OxhMoeI8(ctypes.Structure):
+    _fields_ = [("d_w_gate", V), ("d_w_up", V), ("d_w_down", V), ("d_s_gate", V), ("d_s_up", V), ("d_s_down", V),
+                ("gate_up_stride", Z), ("down_stride", Z), ("n_expert", Z), ("top_k", Z), ("hidden", Z), ("ffn", Z)]
+
+
 class OxhTensor(ctypes.Structure):
     _fields_ = [("name", ctypes.c_char_p), ("qtype", U32), ("ggml_type", U32), ("n_dims", U32),
                 ("dims", ctypes.c_uint64 * 8), ("offset", ctypes.c_uint64), ("data", V), ("nbytes", Z),
@@ -106,6 +124,15 @@ SIGNATURES = {
     "oxh_moe_ffn": (I, [ctypes.POINTER(OxhMoe), V, V, Z, Z, V, Z, V, Z, V]),
     "oxh_moe_ffn_static": (I, [ctypes.POINTER(OxhMoe), V, V, Z, Z, V, Z, V]),
     "oxh_moe_route": (I, [V, Z, Z, Z, I, V, V, V, V, V, V, V]),
+    "oxh_moe_select_workspace": (I, [ctypes.POINTER(OxhMoeRouter), Z, ctypes.POINTER(Z)]),
+    "oxh_moe_select": (I, [ctypes.POINTER(OxhMoeRouter), U32, V, Z, Z, ctypes.POINTER(OxhRouting), V, Z, V]),
+    "oxh_i8_quantize": (I, [U32, V, Z, Z, Z, V, V, Z, V, V]),
+    "oxh_i8_matmul_workspace": (Z, [ctypes.POINTER(OxhI8Matrix), Z]),
+    "oxh_i8_matmul": (I, [ctypes.POINTER(OxhI8Matrix), V, Z, V, Z, V, U32, V, Z, V, Z, V]),
+    "oxh_i8_linear_workspace": (Z, [ctypes.POINTER(OxhI8Matrix), Z]),
+    "oxh_i8_linear": (I, [ctypes.POINTER(OxhI8Matrix), U32, V, Z, Z, V, U32, V, Z, V, Z, V]),
+    "oxh_moe_i8_workspace_bytes": (I, [ctypes.POINTER(OxhMoeI8), Z, ctypes.POINTER(Z)]),
+    "oxh_moe_ffn_i8": (I, [ctypes.POINTER(OxhMoeI8), ctypes.POINTER(OxhRouting), U32, V, Z, Z, U32, V, Z, V, Z, V]),
     "oxh_malloc": (I, [ctypes.POINTER(V), Z]),
     "oxh_host_alloc": (I, [ctypes.POINTER(V), Z]),
     "oxh_host_free": (I, [V]),

@@ -1,0 +1,414 @@
+/* oxh_select.hip — routing for models with many experts: softmax or sigmoid scores, a bias on the choice, expert groups,
+ * up to 512 experts and 16 choices, and the pairs sorted by expert (oxh_moe_select).
+ *
+ * A wave per token, lane l the experts l, l + 64, ...  Scores are 64-bit: two keys next to each other at the border
+ * of the choice are told apart as the definition tells them, which 32 bits do not always do (among 256 sigmoids the
+ * eighth and ninth lie within 1e-7 of each other in about one token of 40 000).
+ *
+ * Sorting needs no sort: a workgroup takes at most 64 tokens, and a token chooses an expert at most once, so the
+ * tokens of an expert are a 64-bit mask in LDS; its count is the mask's population and a pair's rank the population
+ * below its token.  Up to 64 tokens one workgroup does all of it in one launch.  Above, every workgroup leaves its
+ * counts (a byte each) and a second launch adds up those of the workgroups before it. */
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "oxhip.h"
+#include "oxh_internal.h"
+#include "oxh_device.inc"
+
+#pragma clang fp contract(off)
+
+#define SEL_TOKENS 64u              /* a workgroup's tokens, at most: bits of a mask */
+#define SEL_WAVES 16u
+
+struct SelectArgs {
+    const void *logits;
+    size_t stride;
+    const float *bias;
+    int32_t *ids;
+    float *weights;
+    uint32_t *counts, *offsets, *perm, *slot_pos;
+    uint8_t *hist;                  /* [workgroup][hist_stride] counts; NULL for a launch of one workgroup */
+    uint32_t n_tok, tok_per_wg, n_expert, k, n_group, top_group, group_best, score, renorm, hist_stride;
+    float scale;
+};
+
+/* The order of 64-bit keys as the order of integers; 0 is left for experts that cannot be chosen, 1 for masked ones
+ * (the least key there is, -inf, maps to more). */
+__device__ __forceinline__ uint64_t sortable(double key)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(key);
+    return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d)
+{
+    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, d), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d);
+    return ((uint64_t)hi << 32) | lo;
+}
+
+__device__ __forceinline__ double wave_sum64(double v)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v += __longlong_as_double((long long)shfl_xor64((uint64_t)__double_as_longlong(v), d));
+    return v;
+}
+
+/* what a wave's lanes wrote to LDS before, its other lanes read after */
+__device__ __forceinline__ void sel_wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+template <typename T> __device__ __forceinline__ float sel_load(const void *p, size_t i);
+template <> __device__ __forceinline__ float sel_load<float>(const void *p, size_t i) { return ((const float *)p)[i]; }
+template <> __device__ __forceinline__ float sel_load<_Float16>(const void *p, size_t i) { return (float)((const _Float16 *)p)[i]; }
+template <> __device__ __forceinline__ float sel_load<__bf16>(const void *p, size_t i)
+{
+    return __uint_as_float((uint32_t)((const uint16_t *)p)[i] << 16);
+}
+
+/* exclusive prefix of the experts' totals (in s_total) into s_base; one wave */
+__device__ __forceinline__ void sel_scan(const uint32_t *s_total, uint32_t *s_base, uint32_t n_expert, uint32_t lane)
+{
+    uint32_t own[8], sum = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        own[i] = 8u * lane + i < n_expert ? s_total[8u * lane + i] : 0u;
+        sum += own[i];
+    }
+    uint32_t upto = sum;
+#pragma unroll
+    for (uint32_t d = 1; d < 64u; d <<= 1) {
+        const uint32_t v = __shfl_up(upto, d);
+        if (lane >= d) upto += v;
+    }
+    uint32_t at = upto - sum;
+#pragma unroll
+    for (uint32_t i = 0; i < 8u; i++) {
+        s_base[8u * lane + i] = at;
+        at += own[i];
+    }
+}
+
+template <typename T, int NPL>
+__global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
+{
+    __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
+    __shared__ double s_key[SEL_WAVES][NPL * 64];
+    __shared__ uint16_t s_id[SEL_TOKENS * OXH_SELECT_MAX_TOPK];
+    __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
+    const uint32_t t0 = blockIdx.x * a.tok_per_wg, here = min(a.tok_per_wg, a.n_tok - t0), E = a.n_expert;
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += blockDim.x) s_mask[e] = 0ull;
+    __syncthreads();
+    for (uint32_t tt = wave; tt < here; tt += SEL_WAVES) {
+        const size_t row = (size_t)(t0 + tt) * a.stride;
+        double p[NPL];
+        uint64_t key[NPL];
+        float x[NPL], top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < NPL; i++) {
+            const uint32_t e = lane + 64u * i;
+            float v = e < E ? sel_load<T>(a.logits, row + e) : -__builtin_inff();
+            v = v != v ? -__builtin_inff() : fminf(v, 3.402823466e38f);
+            x[i] = v;
+            top = fmaxf(top, v);
+        }
+        top = wave_max(top);
+        if (a.score == OXH_SCORE_SOFTMAX) {
+            double z = 0.0;
+#pragma unroll
+            for (int i = 0; i < NPL; i++) {
+                p[i] = x[i] > -__builtin_inff() ? exp((double)x[i] - (double)top) : 0.0;
+                z += p[i];
+            }
+            z = wave_sum64(z);
+#pragma unroll
+            for (int i = 0; i < NPL; i++) p[i] = z > 0.0 ? p[i] / z : 0.0;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NPL; i++) p[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+        }
+#pragma unroll
+        for (int i = 0; i < NPL; i++) {
+            const uint32_t e = lane + 64u * i;
+            double kv = p[i];
+            if (a.bias && e < E) kv += (double)a.bias[e];
+            const bool live = x[i] > -__builtin_inff() && kv > -__builtin_inf();      /* a NaN is not */
+            key[i] = e >= E ? 0ull : live ? sortable(kv) : 1ull;
+            if (!live) p[i] = 0.0;
+            if (a.n_group > 1u) s_key[wave][e] = live ? kv : -__builtin_inf();
+        }
+        if (a.n_group > 1u) {
+            sel_wave_sync();
+            const uint32_t size = E / a.n_group;
+            double b1 = -__builtin_inf(), b2 = -__builtin_inf();
+            if (lane < a.n_group)
+                for (uint32_t j = 0; j < size; j++) {
+                    const double v = s_key[wave][lane * size + j];
+                    b2 = v > b1 ? b1 : v > b2 ? v : b2;
+                    b1 = v > b1 ? v : b1;
+                }
+            const uint64_t rank = sortable(a.group_best == 2u && b2 > -__builtin_inf() ? b1 + b2 : b1);
+            uint32_t before = 0;
+            for (uint32_t g = 0; g < a.n_group; g++) {
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, (int)g);
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(rank >> 32), (int)g);
+                const uint64_t other = ((uint64_t)hi << 32) | lo;
+                before += other > rank || (other == rank && g < lane) ? 1u : 0u;
+            }
+            const unsigned long long kept = __ballot(lane < a.n_group && before < a.top_group);
+#pragma unroll
+            for (int i = 0; i < NPL; i++) {
+                const uint32_t e = lane + 64u * i;
+                if (e < E && !((kept >> (e / size)) & 1ull)) key[i] = 0ull;
+            }
+            sel_wave_sync();
+        }
+        double my_p = 0.0;
+        uint32_t my_id = 0;
+        for (uint32_t j = 0; j < a.k; j++) {
+            uint64_t best = key[0];
+            uint32_t at = lane;
+            double bp = p[0];
+#pragma unroll
+            for (int i = 1; i < NPL; i++)
+                if (key[i] > best) {
+                    best = key[i];
+                    at = lane + 64u * i;
+                    bp = p[i];
+                }
+            uint64_t m = best;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint64_t o = shfl_xor64(m, d);
+                m = o > m ? o : m;
+            }
+            unsigned long long who = __ballot(best == m);
+            uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)at, __builtin_ctzll(who));
+            if (who & (who - 1ull)) {               /* equal keys: the lowest expert */
+                uint32_t low = best == m ? at : 0xFFFFFFFFu;
+#pragma unroll
+                for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d));
+                id = low;
+            }
+            const int owner = (int)(id & 63u);
+            const uint64_t bits = (uint64_t)__double_as_longlong(bp);
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, owner);
+            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), owner);
+            if (lane == j) {
+                my_id = id;
+                my_p = __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+            }
+#pragma unroll
+            for (int i = 0; i < NPL; i++)
+                if (id == lane + 64u * i) key[i] = 0ull;
+        }
+        const double sum = wave_sum64(my_p);                    /* lanes from k on hold 0 */
+        double w = my_p;
+        if (a.renorm) w = sum > 0.0 ? my_p / sum : 0.0;
+        if (lane < a.k) {
+            const size_t pair = (size_t)(t0 + tt) * a.k + lane;
+            a.ids[pair] = (int32_t)my_id;
+            a.weights[pair] = (float)(w * (double)a.scale);
+            s_id[tt * a.k + lane] = (uint16_t)my_id;
+            atomicOr(&s_mask[my_id], 1ull << tt);
+        }
+    }
+    __syncthreads();
+    if (a.hist) {
+        for (uint32_t e = tid; e < a.hist_stride; e += blockDim.x)
+            a.hist[(size_t)blockIdx.x * a.hist_stride + e] = e < E ? (uint8_t)__popcll(s_mask[e]) : (uint8_t)0;
+        return;
+    }
+    for (uint32_t e = tid; e < E; e += blockDim.x) s_total[e] = (uint32_t)__popcll(s_mask[e]);
+    __syncthreads();
+    if (wave == 0u) sel_scan(s_total, s_base, E, lane);
+    __syncthreads();
+    for (uint32_t e = tid; e < E; e += blockDim.x) {
+        a.counts[e] = s_total[e];
+        a.offsets[e] = s_base[e];
+    }
+    if (tid == 0u) a.offsets[E] = a.n_tok * a.k;
+    for (uint32_t i = tid; i < here * a.k; i += blockDim.x) {
+        const uint32_t tt = i / a.k, e = s_id[i];
+        const uint32_t pos = s_base[e] + (uint32_t)__popcll(s_mask[e] & ((1ull << tt) - 1ull));
+        a.perm[pos] = t0 + tt;
+        a.slot_pos[i] = pos;
+    }
+}
+
+/* The positions of the pairs of many workgroups' tokens: the counts of all workgroups give the experts' runs, those of
+ * the workgroups before this one where its own pairs start in them.  Four counts to a dword, rows dealt to the threads. */
+__global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
+{
+    __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
+    __shared__ uint16_t s_id[SEL_TOKENS * OXH_SELECT_MAX_TOPK];
+    __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_before[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_expert;
+    const uint32_t t0 = blockIdx.x * a.tok_per_wg, here = min(a.tok_per_wg, a.n_tok - t0);
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += blockDim.x) {
+        s_mask[e] = 0ull;
+        s_total[e] = s_before[e] = 0u;
+    }
+    __syncthreads();
+    for (uint32_t i = tid; i < here * a.k; i += blockDim.x) {
+        const uint32_t e = (uint32_t)a.ids[(size_t)t0 * a.k + i];
+        s_id[i] = (uint16_t)e;
+        atomicOr(&s_mask[e], 1ull << (i / a.k));
+    }
+    const uint32_t quads = a.hist_stride / 4u, slices = blockDim.x / quads;
+    if (tid < slices * quads) {
+        const uint32_t q = tid % quads;
+        uint32_t all[4] = { 0u, 0u, 0u, 0u }, bef[4] = { 0u, 0u, 0u, 0u };
+        for (uint32_t b = tid / quads; b < gridDim.x; b += slices) {
+            const uint32_t c = *reinterpret_cast<const uint32_t *>(a.hist + (size_t)b * a.hist_stride + 4u * q);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const uint32_t v = (c >> (8 * i)) & 0xFFu;
+                all[i] += v;
+                bef[i] += b < blockIdx.x ? v : 0u;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (all[i]) {
+                atomicAdd(&s_total[4u * q + i], all[i]);
+                atomicAdd(&s_before[4u * q + i], bef[i]);
+            }
+    }
+    __syncthreads();
+    if (wave == 0u) sel_scan(s_total, s_base, E, lane);
+    __syncthreads();
+    if (blockIdx.x == 0u) {
+        for (uint32_t e = tid; e < E; e += blockDim.x) {
+            a.counts[e] = s_total[e];
+            a.offsets[e] = s_base[e];
+        }
+        if (tid == 0u) a.offsets[E] = a.n_tok * a.k;
+    }
+    for (uint32_t i = tid; i < here * a.k; i += blockDim.x) {
+        const uint32_t tt = i / a.k, e = s_id[i];
+        const uint32_t pos = s_base[e] + s_before[e] + (uint32_t)__popcll(s_mask[e] & ((1ull << tt) - 1ull));
+        a.perm[pos] = t0 + tt;
+        a.slot_pos[(size_t)t0 * a.k + i] = pos;
+    }
+}
+
+/* ─── host side ───────────────────────────────────────────────────────── */
+
+static uint32_t sel_tok_per_wg(size_t n_tok)
+{
+    if (n_tok <= SEL_TOKENS) return SEL_TOKENS;
+    return n_tok <= 16u * 256u ? 16u : n_tok <= 32u * 256u ? 32u : SEL_TOKENS;
+}
+
+static uint32_t sel_hist_stride(size_t n_expert) { return ((uint32_t)n_expert + 3u) & ~3u; }
+
+static int sel_check(const OxhMoeRouter *r, size_t n_tok, const char *who)
+{
+    if (!r) return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: NULL router", who);
+    if (r->score != OXH_SCORE_SOFTMAX && r->score != OXH_SCORE_SIGMOID)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: score %u is not one of OXH_SCORE_*", who, r->score);
+    if (r->n_expert == 0 || r->n_expert > OXH_SELECT_MAX_EXPERTS)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: n_expert must be 1..%u", who, OXH_SELECT_MAX_EXPERTS);
+    size_t open = r->n_expert;
+    if (r->n_group > 1) {
+        if (r->n_group > OXH_SELECT_MAX_GROUPS || r->n_expert % r->n_group)
+            return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: n_group must be at most %u and divide n_expert", who,
+                                       OXH_SELECT_MAX_GROUPS);
+        if (r->top_group == 0 || r->top_group > r->n_group)
+            return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: top_group must be 1..n_group", who);
+        if (r->group_best != 1 && r->group_best != 2)
+            return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: group_best must be 1 or 2", who);
+        open = r->n_expert / r->n_group * r->top_group;
+    }
+    if (r->top_k == 0 || r->top_k > OXH_SELECT_MAX_TOPK || r->top_k > open)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: top_k must be 1..%u and at most the experts of the kept groups (%zu)",
+                                   who, OXH_SELECT_MAX_TOPK, open);
+    if (n_tok > OXH_SELECT_MAX_TOKENS)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: at most %u tokens per call", who, OXH_SELECT_MAX_TOKENS);
+    return OXH_OK;
+}
+
+static size_t sel_workspace(const OxhMoeRouter *r, size_t n_tok)
+{
+    const uint32_t per = sel_tok_per_wg(n_tok);
+    return n_tok <= SEL_TOKENS ? 0 : (n_tok + per - 1u) / per * sel_hist_stride(r->n_expert);
+}
+
+extern "C" int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes)
+{
+    const int rc = sel_check(r, n_tok, "oxh_moe_select_workspace");
+    if (rc) return rc;
+    if (bytes) *bytes = sel_workspace(r, n_tok);
+    return OXH_OK;
+}
+
+template <typename T> static void sel_launch(const SelectArgs &a, uint32_t wgs, hipStream_t st)
+{
+    const dim3 grid(wgs), block(64u * SEL_WAVES);
+    if (a.n_expert <= 64u) hipLaunchKernelGGL((k_moe_select<T, 1>), grid, block, 0, st, a);
+    else if (a.n_expert <= 128u) hipLaunchKernelGGL((k_moe_select<T, 2>), grid, block, 0, st, a);
+    else if (a.n_expert <= 256u) hipLaunchKernelGGL((k_moe_select<T, 4>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((k_moe_select<T, 8>), grid, block, 0, st, a);
+}
+
+extern "C" int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const void *d_logits, size_t logits_stride,
+                              size_t n_tok, const OxhRouting *out, void *d_workspace, size_t workspace_bytes, void *stream)
+{
+    static const char who[] = "oxh_moe_select";
+    int rc = sel_check(r, n_tok, who);
+    if (rc) return rc;
+    if (logits_type != OXH_F32 && logits_type != OXH_F16 && logits_type != OXH_BF16)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: logits_type %u is not OXH_F32, OXH_F16 or OXH_BF16", who, logits_type);
+    if (n_tok == 0) return OXH_OK;
+    if (!d_logits || !out || !out->d_ids || !out->d_weights || !out->d_counts || !out->d_offsets || !out->d_perm || !out->d_slot_pos)
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: NULL pointer", who);
+    if ((uintptr_t)d_logits % (logits_type == OXH_F32 ? 4u : 2u))
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: d_logits is not aligned to its elements", who);
+    if (logits_stride < r->n_expert) return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: logits_stride < n_expert", who);
+    const size_t need = sel_workspace(r, n_tok);
+    if (need && (!d_workspace || workspace_bytes < need))
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: workspace too small (see oxh_moe_select_workspace)", who);
+    if (need && ((uintptr_t)d_workspace & 15u))
+        return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: workspace must be 16-byte aligned", who);
+    if (oxh_internal_device() < 0 && (rc = oxh_init(0))) return rc;
+    SelectArgs a = {};
+    a.logits = d_logits;
+    a.stride = logits_stride;
+    a.bias = r->d_bias;
+    a.ids = out->d_ids;
+    a.weights = out->d_weights;
+    a.counts = out->d_counts;
+    a.offsets = out->d_offsets;
+    a.perm = out->d_perm;
+    a.slot_pos = out->d_slot_pos;
+    a.hist = need ? (uint8_t *)d_workspace : nullptr;
+    a.n_tok = (uint32_t)n_tok;
+    a.tok_per_wg = sel_tok_per_wg(n_tok);
+    a.n_expert = (uint32_t)r->n_expert;
+    a.k = (uint32_t)r->top_k;
+    a.n_group = r->n_group > 1 ? (uint32_t)r->n_group : 1u;
+    a.top_group = (uint32_t)r->top_group;
+    a.group_best = r->group_best;
+    a.score = r->score;
+    a.renorm = r->renorm ? 1u : 0u;
+    a.hist_stride = sel_hist_stride(r->n_expert);
+    a.scale = r->scale;
+    const uint32_t wgs = (a.n_tok + a.tok_per_wg - 1u) / a.tok_per_wg;
+    hipStream_t st = (hipStream_t)(stream ? stream : oxh_internal_stream());
+    if (logits_type == OXH_F32) sel_launch<float>(a, wgs, st);
+    else if (logits_type == OXH_F16) sel_launch<_Float16>(a, wgs, st);
+    else sel_launch<__bf16>(a, wgs, st);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && need) {
+        hipLaunchKernelGGL(k_moe_place, dim3(wgs), dim3(1024), 0, st, a);
+        e = hipGetLastError();
+    }
+    if (e != hipSuccess) return oxh_internal_errorf(OXH_ERR_HIP, "HIP error in %s: %s", who, hipGetErrorString(e));
+    return OXH_OK;
+}

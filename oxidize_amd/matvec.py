@@ -238,6 +238,33 @@ def moe_route(d_logits, n_tok, n_expert, top_k, renorm, d_ids, d_wts, d_counts, 
                               vp(d_counts), vp(d_offsets), vp(d_perm), vp(d_slot_pos), stream))
 
 
+SCORE = {"softmax": 0, "sigmoid": 1}
+
+
+def make_routing(d_ids, d_weights, d_counts, d_offsets, d_perm, d_slot_pos):
+    """Device addresses of a routing (oxh_moe_select writes it, the expert layers read it)."""
+    return _lib.OxhRouting(d_ids, d_weights, d_counts, d_offsets, d_perm, d_slot_pos)
+
+
+class MoeRouter:
+    """How tokens choose their experts: softmax or sigmoid scores, a bias on the choice, groups, top-k
+    (oxh_moe_select; up to 512 experts and 16 choices).  The workspace is the caller's."""
+
+    def __init__(self, n_expert, top_k, score="softmax", n_group=1, top_group=1, group_best=1, d_bias=None, renorm=True,
+                 scale=1.0):
+        self.desc = _lib.OxhMoeRouter(SCORE[score], group_best, n_expert, top_k, n_group, top_group, d_bias, int(renorm), scale)
+
+    def workspace_bytes(self, n_tok):
+        need = ctypes.c_size_t()
+        check(lib().oxh_moe_select_workspace(ctypes.byref(self.desc), n_tok, ctypes.byref(need)))
+        return need.value
+
+    def select(self, logits_type, d_logits, logits_stride, n_tok, routing, d_ws=None, ws_bytes=0, stream=None):
+        """`routing` from make_routing(); logits_type one of int8.F32, F16, BF16."""
+        check(lib().oxh_moe_select(ctypes.byref(self.desc), logits_type, d_logits, logits_stride, n_tok, ctypes.byref(routing),
+                                   d_ws, ws_bytes, stream))
+
+
 class MoeLayer:
     """One mixture-of-experts feed-forward layer resident on the device
     (routing, grouping, expert matrices and combination as
