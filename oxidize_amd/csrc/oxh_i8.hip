@@ -2,14 +2,14 @@
  * products of a mixture-of-experts layer (oxh_i8_*, oxh_moe_ffn_i8). */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
+#include <stdlib.h>
 
 #include "oxhip.h"
 #include "oxh_internal.h"
 #include "oxh_device.inc"
+#include "i8_tiles.inc"
 
 #pragma clang fp contract(off)
-
-typedef int v4i __attribute__((ext_vector_type(4)));
 
 /* ─── floats ──────────────────────────────────────────────────────────── */
 
@@ -107,26 +107,115 @@ __device__ __forceinline__ v4i i8_wave_sums(const int8_t *w_row, const int8_t *q
     return acc;
 }
 
-template <typename T>
-__global__ __launch_bounds__(256) void
-k_i8_matmul(const OxhI8Matrix w, const int8_t *__restrict__ q, size_t q_stride, const float *__restrict__ q_scale, uint32_t n_vec,
-            const float *__restrict__ bias, T *__restrict__ out, size_t out_stride)
+/* Four neighbouring results of a token, aligned to their elements only; the last rows of a matrix one by one. */
+template <typename T> __device__ __forceinline__ void i8_store4(T *out, const float (&v)[4], uint32_t rows_left)
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, rows = (uint32_t)w.rows;
-    const uint32_t r0 = blockIdx.x * 64u + 16u * wave, t = blockIdx.y * 16u + (lane & 15u);
-    if (r0 >= rows) return;
-    const v4i acc = i8_wave_sums(w.d_w + (size_t)min(r0 + (lane & 15u), rows - 1u) * w.stride,
-                                 q + (size_t)min(t, n_vec - 1u) * q_stride, (uint32_t)w.cols, lane);
-    if (t >= n_vec) return;
-    const float st = q_scale[t];
+    if (rows_left >= 4u) {
+        Run<T, 4> r;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const uint32_t r = r0 + 4u * (lane >> 4) + i;
-        if (r >= rows) break;
-        float v = (float)acc[i] * st * w.d_scale[r];
-        if (bias) v += bias[r];
-        out[(size_t)t * out_stride + r] = from_f32<T>(v);
+        for (int i = 0; i < 4; i++) r.v[i] = from_f32<T>(v[i]);
+        *reinterpret_cast<Run<T, 4> *>(out) = r;
+    } else
+#pragma unroll
+        for (uint32_t i = 0; i < 3u; i++)
+            if (i < rows_left) out[i] = from_f32<T>(v[i]);
+}
+
+/* The tile of workgroup b of row_tiles * tok_tiles.  The workgroups of an XCD (every eighth one) take neighbouring tiles of an
+ * order that goes through the token tiles with up to eight row tiles at each: what an XCD's 32 CUs read at a time is
+ * then 8 + 4 operand tiles through its L2, where one row tile under 32 token tiles is 33. */
+__device__ __forceinline__ void i8_tile_of(uint32_t b, uint32_t row_tiles, uint32_t tok_tiles, uint32_t &row, uint32_t &tok)
+{
+    const uint32_t n = row_tiles * tok_tiles, per = n / 8u, more = n % 8u, x = b % 8u;
+    const uint32_t i = x * per + min(x, more) + b / 8u;
+    const uint32_t group = i / (8u * tok_tiles), in = i - group * 8u * tok_tiles, high = min(8u, row_tiles - 8u * group);
+    row = 8u * group + in % high;
+    tok = in / high;
+}
+
+/* What the product's kernels take: the matrix, quantised tokens, and where the results go. */
+struct I8Product {
+    OxhI8Matrix w;
+    const int8_t *q;
+    size_t q_stride;
+    const float *q_scale, *bias;
+    void *out;
+    size_t out_stride;
+    int *parts;                     /* partial sums [split][token][rows_pad] of a product whose columns are shared out */
+    uint32_t n_vec, splits, row_tiles, tok_tiles, rows_pad, out_type;
+};
+
+/* four rows' results of a token from their sums, in out_type */
+__device__ __forceinline__ void i8_results(const I8Product &p, uint32_t r, uint32_t t, const v4i &sums, const float (&sw)[4],
+                                           const float (&b)[4], float st)
+{
+    const uint32_t rows = (uint32_t)p.w.rows;
+    float v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        v[k] = (float)sums[k] * st * sw[k];
+        if (p.bias) v[k] += b[k];
     }
+    const size_t at = (size_t)t * p.out_stride + r;
+    if (p.out_type == OXH_F32) i8_store4((float *)p.out + at, v, rows - r);
+    else if (p.out_type == OXH_F16) i8_store4((_Float16 *)p.out + at, v, rows - r);
+    else i8_store4((__bf16 *)p.out + at, v, rows - r);
+}
+
+__device__ __forceinline__ void i8_row_factors(const I8Product &p, uint32_t r, float (&sw)[4], float (&b)[4])
+{
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        const uint32_t rk = min(r + k, (uint32_t)p.w.rows - 1u);
+        sw[k] = p.w.d_scale[rk];
+        b[k] = p.bias ? p.bias[rk] : 0.0f;
+    }
+}
+
+template <typename G>
+__global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles(const I8Product p)
+{
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, tiles = p.row_tiles * p.tok_tiles;
+    const uint32_t split = blockIdx.x / tiles;
+    uint32_t r0, t0;
+    i8_tile_of(blockIdx.x - split * tiles, p.row_tiles, p.tok_tiles, r0, t0);
+    r0 *= G::ROWS;
+    t0 *= G::TOK;
+    const uint32_t ws = (uint32_t)p.w.stride, qs = (uint32_t)p.q_stride;
+    /* this workgroup's stages of 128 columns */
+    const uint32_t stages = (cols + 127u) / 128u, first = split * stages / p.splits, end = (split + 1u) * stages / p.splits;
+    const uint32_t k0 = 128u * first, kn = min(cols, 128u * end) - k0;
+    v4i acc[G::RF][G::TF];
+    i8_tile<G>(p.w.d_w + (size_t)r0 * p.w.stride + k0, p.q + (size_t)t0 * p.q_stride + k0, kn,
+               [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; }, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, acc);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+#pragma unroll
+    for (uint32_t i = 0; i < G::RF; i++) {
+        const uint32_t r = r0 + (wr * G::RF + i) * 16u + 4u * (lane >> 4);
+        if (r >= rows) break;
+        float sw[4], b[4];
+        if (!p.parts) i8_row_factors(p, r, sw, b);
+#pragma unroll
+        for (uint32_t j = 0; j < G::TF; j++) {
+            const uint32_t t = t0 + (wt * G::TF + j) * 16u + (lane & 15u);
+            if (t >= p.n_vec) break;
+            if (p.parts) *reinterpret_cast<v4i *>(p.parts + ((size_t)split * p.n_vec + t) * p.rows_pad + r) = acc[i][j];
+            else i8_results(p, r, t, acc[i][j], sw, b, p.q_scale[t]);
+        }
+    }
+}
+
+/* The sums of a product whose columns were shared out: integers, the same in any order.  Four rows to a thread. */
+__global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
+{
+    const uint32_t r = (blockIdx.x * 256u + threadIdx.x) * 4u, t = blockIdx.y;
+    if (r >= (uint32_t)p.w.rows) return;
+    v4i sums = { 0, 0, 0, 0 };
+    for (uint32_t s = 0; s < p.splits; s++)
+        sums += *reinterpret_cast<const v4i *>(p.parts + ((size_t)s * p.n_vec + t) * p.rows_pad + r);
+    float sw[4], b[4];
+    i8_row_factors(p, r, sw, b);
+    i8_results(p, r, t, sums, sw, b, p.q_scale[t]);
 }
 
 /* An expert's run of the sorted pairs, as far as it lies among them. */
@@ -224,12 +313,16 @@ static int launched(const char *who)
 /* rows or tokens: the launches count them in 32 bits, in grids of up to 2^31 threads a dimension */
 #define I8_MAX_ROWS ((size_t)1 << 23)
 
+/* a tile's rows lie within 32 bits of its first one */
+#define I8_MAX_STRIDE ((size_t)1 << 23)
+
 static int check_rows(const char *who, const char *name, const void *d, size_t stride, size_t cols)
 {
     if (!d) return I8_ARG("%s: NULL pointer (%s)", who, name);
     if ((uintptr_t)d & 15u) return I8_ARG("%s: %s must be 16-byte aligned", who, name);
     if (stride % 16u) return I8_ARG("%s: the stride of %s must be a multiple of 16", who, name);
     if (stride < cols) return I8_ARG("%s: the stride of %s is less than cols", who, name);
+    if (stride > I8_MAX_STRIDE) return I8_ARG("%s: the stride of %s is more than %zu bytes", who, name, I8_MAX_STRIDE);
     return OXH_OK;
 }
 
@@ -294,28 +387,66 @@ static int check_matrix(const char *who, const OxhI8Matrix *w)
     return OXH_OK;
 }
 
-static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, const float *bias,
-                         uint32_t out_type, void *out, size_t out_stride, hipStream_t st, const char *who)
+typedef I8Geom<8, 4, 2, 4> I8Large;        /* 256 x 256, a workgroup per CU */
+typedef I8Geom<4, 4, 2, 2> I8Mid;          /* 128 x 128, two */
+typedef I8Geom<2, 2, 2, 2> I8Small;        /* 64 x 64, four */
+
+/* How a product runs: on which tile, its columns in how many parts. */
+struct I8Way {
+    int tile;                       /* 0 large, 1 mid, 2 small */
+    uint32_t splits;
+};
+
+static int forced_tile(void) { const char *v = getenv("OXH_I8_TILE"); return v ? atoi(v) : -1; }
+static int forced_split(void) { const char *v = getenv("OXH_I8_SPLIT"); return v ? atoi(v) : 0; }
+static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes)
 {
-    for (size_t t0 = 0; t0 < n; t0 += 65535u * 16u) {
-        const size_t here = n - t0 < 65535u * 16u ? n - t0 : 65535u * 16u;
-        const dim3 grid((uint32_t)((w->rows + 63u) / 64u), (uint32_t)((here + 15u) / 16u)), block(256);
-#define OXH_MM(T)                                                                                                                \
-    hipLaunchKernelGGL(k_i8_matmul<T>, grid, block, 0, st, *w, q + t0 * q_stride, q_stride, q_scale + t0, (uint32_t)here, bias,  \
-                       (T *)out + t0 * out_stride, out_stride)
-        if (out_type == OXH_F32) OXH_MM(float);
-        else if (out_type == OXH_F16) OXH_MM(_Float16);
-        else OXH_MM(__bf16);
-#undef OXH_MM
-    }
+    I8Way w = { 0, 1 };
+    if (forced_tile() >= 0) w.tile = forced_tile();
+    if (forced_split() > 0) w.splits = (uint32_t)forced_split();
+    return w;
+}
+
+static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return splits > 1 ? (size_t)splits * n * ((rows + 3u) & ~(size_t)3u) * 4u : 0; }
+
+template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
+{
+    p.row_tiles = (uint32_t)((p.w.rows + G::ROWS - 1u) / G::ROWS);
+    p.tok_tiles = (p.n_vec + G::TOK - 1u) / G::TOK;
+    hipLaunchKernelGGL(k_i8_tiles<G>, dim3(p.row_tiles * p.tok_tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
+}
+
+static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, const float *bias,
+                         uint32_t out_type, void *out, size_t out_stride, void *ws, size_t ws_bytes, hipStream_t st, const char *who)
+{
+    const I8Way way = i8_way(w->rows, w->cols, n, ws_bytes);
+    I8Product p = { *w, q, q_stride, q_scale, bias, out, out_stride, way.splits > 1 ? (int *)ws : nullptr, (uint32_t)n, way.splits, 0, 0,
+                    (uint32_t)((w->rows + 3u) & ~(size_t)3u), out_type };
+    if (way.tile == 0) tiles_launch<I8Large>(p, st);
+    else if (way.tile == 1) tiles_launch<I8Mid>(p, st);
+    else tiles_launch<I8Small>(p, st);
+    if (way.splits > 1) hipLaunchKernelGGL(k_i8_join, dim3((p.rows_pad / 4u + 255u) / 256u, p.n_vec), dim3(256), 0, st, p);
     return launched(who);
+}
+
+template <typename K> static hipError_t whole_lds(K kernel)
+{
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, 160 * 1024);
+}
+
+extern "C" int oxh_internal_i8_init(void)
+{
+    hipError_t e;
+    if ((e = whole_lds(k_i8_tiles<I8Large>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
+    return (int)hipSuccess;
 }
 
 extern "C" size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    (void)w;
-    (void)n_vec;
-    return 0;
+    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > I8_MAX_ROWS || n_vec > I8_MAX_ROWS)
+        return 0;
+    return parts_bytes(w->rows, n_vec, i8_way(w->rows, w->cols, n_vec, SIZE_MAX).splits);
 }
 
 extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
@@ -332,7 +463,8 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
     if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
     if (d_workspace && workspace_bytes && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
     if ((rc = ready())) return rc;
-    return matmul_launch(w, d_q, q_stride, d_q_scale, n_vec, d_bias, out_type, d_out, out_stride, stream_of(stream), who);
+    return matmul_launch(w, d_q, q_stride, d_q_scale, n_vec, d_bias, out_type, d_out, out_stride, d_workspace,
+                         d_workspace ? workspace_bytes : 0, stream_of(stream), who);
 }
 
 /* the codes and scales of the tokens */
@@ -373,7 +505,7 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
     int8_t *q = (int8_t *)d_workspace;
     float *scale = (float *)((uint8_t *)d_workspace + p.scale);
     if ((rc = quantize_launch(x_type, d_x, x_stride, n_vec, w->cols, nullptr, q, p.q_stride, scale, stream_of(stream), who))) return rc;
-    return matmul_launch(w, q, p.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, stream_of(stream), who);
+    return matmul_launch(w, q, p.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, nullptr, 0, stream_of(stream), who);
 }
 
 /* ─── experts ─────────────────────────────────────────────────────────── */

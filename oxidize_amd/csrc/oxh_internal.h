@@ -79,6 +79,8 @@ int oxh_internal_experts_batch_takes(int fmt, size_t n_mat, size_t n_expert, siz
 int oxh_internal_experts_batch(int fmt, int tile_major, const void *const *d_w, float *const *d_out, size_t n_mat,
                                size_t n_expert, size_t rows, size_t blocks, const void *d_acts, size_t out_stride,
                                const uint32_t *d_counts, const uint32_t *d_offsets, size_t pairs, size_t max_tokens, void *stream);
+/* Products over int8 rows (oxh_i8.hip); a hipError_t. */
+int oxh_internal_i8_init(void);
 /* Whether the runtime knows all of this memory (page-locked, managed or on the device) and so copies it without a
  * detour through staging of its own. */
 int oxh_internal_runtime_memory(const void *p, size_t bytes);

@@ -948,6 +948,7 @@ static hipError_t raise_all_lds_ceilings(void)
     if ((e = (hipError_t)oxh_internal_mmq6_init()) != hipSuccess) return e;
     if ((e = (hipError_t)oxh_internal_mmq32_init()) != hipSuccess) return e;
     if ((e = (hipError_t)oxh_internal_batch_init()) != hipSuccess) return e;
+    if ((e = (hipError_t)oxh_internal_i8_init()) != hipSuccess) return e;
     return hipSuccess;
 }
 
