@@ -2,7 +2,6 @@
  * products of a mixture-of-experts layer (oxh_i8_*, oxh_moe_ffn_i8). */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
-#include <stdlib.h>
 
 #include "oxhip.h"
 #include "oxh_internal.h"
@@ -19,20 +18,82 @@ template <typename T> __device__ __forceinline__ T from_f32(float v) { return (T
 /* N neighbouring values that are aligned to their elements only */
 template <typename T, int N> struct __attribute__((packed, aligned(sizeof(T)))) Run { T v[N]; };
 
+__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
+
 /* ─── rows of floats to codes ─────────────────────────────────────────── */
 
 /* The integer nearest to v / s, ties to even.  v * inv is within 2^-15 of the quotient, so its rounding is off by one at
  * most, next to a half; the remainder v - t * s has no more bits than an f32 holds (it is a multiple of half a unit of
  * s's last place and no larger than half of s and a bit), the fused operation gives it exactly, and which side of the half it lies
  * on says whether the rounding was right. */
-__device__ __forceinline__ int i8_code(float v, float s, float inv)
+__device__ __forceinline__ float i8_settle(float v, float t, float s)
 {
-    float t = rintf(v * inv);
     const float r = __builtin_fmaf(-t, s, v), twice = r + r;
     const bool odd = ((int)t & 1) != 0;
-    if (twice > s || (twice == s && odd)) t += 1.0f;
-    else if (twice < -s || (twice == -s && odd)) t -= 1.0f;
-    return (int)t;
+    if (twice > s || (twice == s && odd)) return t + 1.0f;
+    if (twice < -s || (twice == -s && odd)) return t - 1.0f;
+    return t;
+}
+
+/* The codes of eight values as bytes.  Only where a product lies within 2^-14 of a half (eight values in a thousand) is the
+ * remainder looked at: five instructions a value instead of a dozen. */
+__device__ __forceinline__ uint2 i8_codes8(const float (&v)[8], float s, float inv)
+{
+    float t[8], far = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const float x = v[i] * inv;
+        t[i] = rintf(x);
+        far = fmaxf(far, fabsf(x - t[i]));
+    }
+    if (far > 0.5f - 0x1p-14f) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) t[i] = i8_settle(v[i], t[i], s);
+    }
+    uint32_t b[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) b[i] = (uint32_t)(int)t[i];
+    auto four = [](uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+        return __builtin_amdgcn_perm(__builtin_amdgcn_perm(d, c, 0x0C0C0400u), __builtin_amdgcn_perm(b, a, 0x0C0C0400u), 0x05040100u);
+    };
+    return make_uint2(four(b[0], b[1], b[2], b[3]), four(b[4], b[5], b[6], b[7]));
+}
+
+/* Values c .. c + 7 of a row of cols, those behind the last one 0; up: NULL, or the row of SwiGLU's other factor. */
+template <typename T, bool GLU>
+__device__ __forceinline__ void i8_values8(const T *__restrict__ x, const T *__restrict__ up, uint32_t c, uint32_t cols, float (&v)[8])
+{
+    if (c + 8u <= cols) {
+        const Run<T, 8> r = *reinterpret_cast<const Run<T, 8> *>(x + c);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(r.v[i]);
+        if (GLU) {
+            const Run<T, 8> u = *reinterpret_cast<const Run<T, 8> *>(up + c);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = silu(v[i]) * to_f32(u.v[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            v[i] = c + i < cols ? to_f32(x[c + i]) : 0.0f;
+            if (GLU) v[i] = c + i < cols ? silu(v[i]) * to_f32(up[c + i]) : 0.0f;
+        }
+    }
+}
+
+__device__ __forceinline__ uint32_t i8_top8(const float (&v)[8])
+{
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; i++) top = max(top, __float_as_uint(v[i]) & 0x7FFFFFFFu);
+    return top;
+}
+
+__device__ __forceinline__ uint32_t wave_top(uint32_t top)
+{
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
+    return top;
 }
 
 /* scale and 1 / scale of a row whose largest magnitude has the bits `top` (those of an infinity or a NaN are the
@@ -47,33 +108,51 @@ __device__ __forceinline__ float i8_scale(uint32_t top, float &inv)
     return s;
 }
 
-__device__ __forceinline__ float silu(float g) { return g / (1.0f + expf(-g)); }
-
-/* A workgroup per row, eight values to a thread and step: once for the largest magnitude, once for the codes. */
-template <typename T, bool GLU>
-__global__ __launch_bounds__(256) void
+/* A workgroup per row, eight values to a thread and step: once for the largest magnitude, once for the codes.  The first
+ * HELD steps' values stay in registers; what is longer is read (and, GLU, computed) a second time. */
+template <typename T, bool GLU, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void
 k_i8_quantize(const T *__restrict__ x, size_t x_stride, uint32_t cols, const T *__restrict__ up, int8_t *__restrict__ q,
               size_t q_stride, float *__restrict__ scale)
 {
-    __shared__ uint32_t s_top[4];
+    constexpr uint32_t STEP = 8u * THREADS;
+    __shared__ uint32_t s_top[THREADS / 64];
     const size_t row = blockIdx.x;
     const T *xr = x + row * x_stride, *ur = GLU ? up + row * x_stride : nullptr;
-    auto value = [&](uint32_t c) {
-        const float v = to_f32(xr[c]);
-        return GLU ? silu(v) * to_f32(ur[c]) : v;
-    };
+    const uint32_t c0 = 8u * threadIdx.x;
+    float v[HELD][8];
     uint32_t top = 0;
-    for (uint32_t c = threadIdx.x; c < cols; c += 256u) top = max(top, __float_as_uint(value(c)) & 0x7FFFFFFFu);
 #pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    if ((threadIdx.x & 63u) == 0u) s_top[threadIdx.x >> 6] = top;
-    __syncthreads();
-    top = max(max(s_top[0], s_top[1]), max(s_top[2], s_top[3]));
+    for (int i = 0; i < HELD; i++) i8_values8<T, GLU>(xr, ur, c0 + STEP * i, cols, v[i]);
+#pragma unroll
+    for (int i = 0; i < HELD; i++) top = max(top, i8_top8(v[i]));
+    for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
+        float t[8];
+        i8_values8<T, GLU>(xr, ur, c, cols, t);
+        top = max(top, i8_top8(t));
+    }
+    top = wave_top(top);
+    if (THREADS > 64) {
+        if ((threadIdx.x & 63u) == 0u) s_top[threadIdx.x >> 6] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) top = max(top, s_top[i]);
+    }
     float inv;
     const float s = i8_scale(top, inv);
     if (threadIdx.x == 0u) scale[row] = s;
-    for (uint32_t c = threadIdx.x; c < ((cols + 15u) & ~15u); c += 256u)
-        q[row * q_stride + c] = (int8_t)(inv != 0.0f && c < cols ? i8_code(value(c), s, inv) : 0);
+    const uint32_t end = (cols + 15u) & ~15u;
+    int8_t *qr = q + row * q_stride;
+    auto store = [&](uint32_t c, const float (&t)[8]) {
+        if (c < end) *reinterpret_cast<uint2 *>(qr + c) = inv != 0.0f ? i8_codes8(t, s, inv) : make_uint2(0u, 0u);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) store(c0 + STEP * i, v[i]);
+    for (uint32_t c = c0 + STEP * HELD; c < end; c += STEP) {
+        float t[8];
+        i8_values8<T, GLU>(xr, ur, c, cols, t);
+        store(c, t);
+    }
 }
 
 /* ─── products ────────────────────────────────────────────────────────── */
@@ -121,13 +200,18 @@ template <typename T> __device__ __forceinline__ void i8_store4(T *out, const fl
             if (i < rows_left) out[i] = from_f32<T>(v[i]);
 }
 
-/* The tile of workgroup b of row_tiles * tok_tiles.  The workgroups of an XCD (every eighth one) take neighbouring tiles of an
- * order that goes through the token tiles with up to eight row tiles at each: what an XCD's 32 CUs read at a time is
- * then 8 + 4 operand tiles through its L2, where one row tile under 32 token tiles is 33. */
-__device__ __forceinline__ void i8_tile_of(uint32_t b, uint32_t row_tiles, uint32_t tok_tiles, uint32_t &row, uint32_t &tok)
+/* Workgroup b of n takes place i8_place() of the tiles' order: the workgroups of an XCD (every eighth one) take a run of it. */
+__device__ __forceinline__ uint32_t i8_place(uint32_t b, uint32_t n)
 {
-    const uint32_t n = row_tiles * tok_tiles, per = n / 8u, more = n % 8u, x = b % 8u;
-    const uint32_t i = x * per + min(x, more) + b / 8u;
+    const uint32_t per = n / 8u, more = n % 8u, x = b % 8u;
+    return x * per + min(x, more) + b / 8u;
+}
+
+/* The tile at place i: an order that goes through the token tiles with up to eight row tiles at each, so that what an XCD's
+ * 32 CUs read at a time is 8 + 4 operand tiles through its L2, where one row tile under 32 token tiles is 33 (8192 x
+ * 8192 x 8192: 473 us, 435 in this order). */
+__device__ __forceinline__ void i8_tile_at(uint32_t i, uint32_t row_tiles, uint32_t tok_tiles, uint32_t &row, uint32_t &tok)
+{
     const uint32_t group = i / (8u * tok_tiles), in = i - group * 8u * tok_tiles, high = min(8u, row_tiles - 8u * group);
     row = 8u * group + in % high;
     tok = in / high;
@@ -142,7 +226,7 @@ struct I8Product {
     void *out;
     size_t out_stride;
     int *parts;                     /* partial sums [split][token][rows_pad] of a product whose columns are shared out */
-    uint32_t n_vec, splits, row_tiles, tok_tiles, rows_pad, out_type;
+    uint32_t n_vec, splits, row_tiles, tok_tiles, whole, rows_pad, out_type;
 };
 
 /* four rows' results of a token from their sums, in out_type */
@@ -172,17 +256,11 @@ __device__ __forceinline__ void i8_row_factors(const I8Product &p, uint32_t r, f
     }
 }
 
-template <typename G>
-__global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles(const I8Product p)
+/* The tile at rows r0.., tokens t0.., over part `split` of the columns: results, or partial sums. */
+template <typename G> __device__ __forceinline__ void i8_product_tile(const I8Product &p, uint32_t r0, uint32_t t0, uint32_t split)
 {
-    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, tiles = p.row_tiles * p.tok_tiles;
-    const uint32_t split = blockIdx.x / tiles;
-    uint32_t r0, t0;
-    i8_tile_of(blockIdx.x - split * tiles, p.row_tiles, p.tok_tiles, r0, t0);
-    r0 *= G::ROWS;
-    t0 *= G::TOK;
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols;
     const uint32_t ws = (uint32_t)p.w.stride, qs = (uint32_t)p.q_stride;
-    /* this workgroup's stages of 128 columns */
     const uint32_t stages = (cols + 127u) / 128u, first = split * stages / p.splits, end = (split + 1u) * stages / p.splits;
     const uint32_t k0 = 128u * first, kn = min(cols, 128u * end) - k0;
     v4i acc[G::RF][G::TF];
@@ -205,6 +283,33 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles(const I8Product p
     }
 }
 
+template <typename G>
+__global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles(const I8Product p)
+{
+    const uint32_t tiles = p.row_tiles * p.tok_tiles, split = blockIdx.x / tiles;
+    uint32_t row, tok;
+    i8_tile_at(i8_place(blockIdx.x - split * tiles, tiles), p.row_tiles, p.tok_tiles, row, tok);
+    i8_product_tile<G>(p, row * G::ROWS, tok * G::TOK, split);
+}
+
+/* A last round that would leave half of the CUs idle and more is done in tiles of half the rows: places from p.whole on, two
+ * workgroups to each. */
+template <typename G, typename H>
+__global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles_tail(const I8Product p)
+{
+    static_assert(G::TOK == H::TOK && G::ROWS == 2u * H::ROWS && G::WAVES == H::WAVES && G::LDS_BYTES == H::LDS_BYTES, "the same launch");
+    uint32_t row, tok;
+    if (blockIdx.x < p.whole) {
+        i8_tile_at(i8_place(blockIdx.x, p.whole), p.row_tiles, p.tok_tiles, row, tok);
+        i8_product_tile<G>(p, row * G::ROWS, tok * G::TOK, 0u);
+    } else {
+        const uint32_t h = i8_place(blockIdx.x - p.whole, gridDim.x - p.whole);
+        i8_tile_at(p.whole + h / 2u, p.row_tiles, p.tok_tiles, row, tok);
+        const uint32_t r0 = row * G::ROWS + (h & 1u) * H::ROWS;
+        if (r0 < (uint32_t)p.w.rows) i8_product_tile<H>(p, r0, tok * H::TOK, 0u);
+    }
+}
+
 /* The sums of a product whose columns were shared out: integers, the same in any order.  Four rows to a thread. */
 __global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
 {
@@ -216,6 +321,134 @@ __global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
     float sw[4], b[4];
     i8_row_factors(p, r, sw, b);
     i8_results(p, r, t, sums, sw, b, p.q_scale[t]);
+}
+
+/* ─── few tokens ──────────────────────────────────────────────────────── */
+
+/* Up to sixteen tokens: the matrix is streamed once and everything else has to stay out of its way.  A workgroup of
+ * sixteen waves per CU keeps the tokens' codes in LDS, in the order the MFMA takes them ([16-column piece][token], what
+ * lies behind the last column 0), and goes through groups of 16 rows: `team` waves share a group's columns, each
+ * straight from memory to operand registers, eight steps of 64 columns in flight beside the eight being multiplied, the next
+ * group's first ones requested before this one's sums are joined in LDS.  The first weights are requested before
+ * the tokens are even looked at.
+ *
+ * XT: the type of float tokens, which every workgroup quantises for itself (k_i8_quantize's codes); int8_t: codes and scales
+ * are there.  Bound by HBM; few rows by the latency of one trip to it. */
+#define FEW_TOKENS 16u
+#define FEW_WAVES 16u
+#define FEW_STEPS 8u
+#define FEW_RED_BYTES (2u * FEW_WAVES * 1024u)
+#define FEW_HEAD_BYTES (FEW_RED_BYTES + 256u)          /* and the scales, a maximum per wave */
+
+template <typename XT>
+__global__ __launch_bounds__(1024) void
+k_i8_few(const I8Product p, const XT *__restrict__ x, size_t x_stride, uint32_t team, uint32_t groups)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t few_shared[];
+    v4i *const red = reinterpret_cast<v4i *>(few_shared);
+    float *const s_scale = reinterpret_cast<float *>(few_shared + FEW_RED_BYTES);
+    uint32_t *const s_top = reinterpret_cast<uint32_t *>(few_shared + FEW_RED_BYTES + 64u);
+    uint8_t *const codes = few_shared + FEW_HEAD_BYTES;
+    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
+    const uint32_t r16 = lane & 15u, kq = lane >> 4;
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, n = p.n_vec;
+    const uint32_t teams = FEW_WAVES / team, mine = wave / team, part = wave % team;
+    const uint32_t steps = (cols + 63u) / 64u, first = part * steps / team, end = (part + 1u) * steps / team;
+    const uint32_t chunks = max(1u, ((steps + team - 1u) / team + FEW_STEPS - 1u) / FEW_STEPS);
+    const uint32_t rounds = (groups + gridDim.x * teams - 1u) / (gridDim.x * teams);
+    const uint32_t last_piece = (cols - 1u) / 16u;
+    v4i w[2][FEW_STEPS];
+    auto group_of = [&](uint32_t round) { return (round * gridDim.x + blockIdx.x) * teams + mine; };
+    /* columns behind the wave's part are requested as its last ones and not used */
+    auto fetch = [&](v4i (&to)[FEW_STEPS], uint32_t round, uint32_t chunk) {
+        const uint32_t row = min(min(group_of(round), groups - 1u) * 16u + r16, rows - 1u);
+        const int8_t *base = p.w.d_w + (size_t)row * p.w.stride;
+#pragma unroll
+        for (uint32_t i = 0; i < FEW_STEPS; i++) {
+            const uint32_t step = min(first + chunk * FEW_STEPS + i, steps - 1u);
+            to[i] = *reinterpret_cast<const v4i *>(base + 16u * min(4u * step + kq, last_piece));
+        }
+    };
+    fetch(w[0], 0u, 0u);
+
+    /* tokens to LDS: waves n_waves * t .. of token t */
+    const uint32_t pieces = 4u * steps;
+    if constexpr (sizeof(XT) == 1) {
+        for (uint32_t i = tid; i < pieces * n; i += 1024u) {
+            const uint32_t t = i / pieces, c = i - t * pieces;
+            *reinterpret_cast<v4i *>(codes + 16u * (c * n + t)) = i8_piece(reinterpret_cast<const int8_t *>(x) + (size_t)t * x_stride, 16u * c, cols);
+        }
+        if (tid < n) s_scale[tid] = p.q_scale[tid];
+    } else {
+        const uint32_t per = n == 1u ? 16u : n == 2u ? 8u : n <= 4u ? 4u : n <= 8u ? 2u : 1u;
+        const uint32_t t = wave / per, w0 = wave % per;
+        const XT *xr = x + (size_t)min(t, n - 1u) * x_stride;
+        const uint32_t c0 = 8u * (64u * w0 + lane), step = 8u * 64u * per;
+        uint32_t top = 0;
+        if (t < n)
+            for (uint32_t c = c0; c < cols; c += step) {
+                float v[8];
+                i8_values8<XT, false>(xr, nullptr, c, cols, v);
+                top = max(top, i8_top8(v));
+            }
+        top = wave_top(top);
+        if (lane == 0u) s_top[wave] = top;
+        __syncthreads();
+        for (uint32_t k = 0; k < per; k++) top = max(top, s_top[wave - w0 + k]);
+        float inv;
+        const float s = i8_scale(top, inv);
+        if (t < n) {
+            if (w0 == 0u && lane == 0u) s_scale[t] = s;
+            for (uint32_t c = c0; c < 16u * pieces; c += step) {
+                float v[8];
+                i8_values8<XT, false>(xr, nullptr, c, cols, v);
+                *reinterpret_cast<uint2 *>(codes + 16u * ((c / 16u) * n + t) + (c & 8u)) = inv != 0.0f ? i8_codes8(v, s, inv) : make_uint2(0u, 0u);
+            }
+        }
+    }
+    __syncthreads();
+
+    const uint8_t *mine_codes = codes + 16u * (kq * n + min(r16, n - 1u));
+    uint32_t buf = 0;
+    v4i acc = { 0, 0, 0, 0 };
+    uint32_t round = 0, chunk = 0;
+    /* one chunk from `now` while the one behind it comes to `then` */
+    auto work = [&](v4i (&now)[FEW_STEPS], v4i (&then)[FEW_STEPS]) {
+        const bool last = chunk + 1u == chunks;
+        fetch(then, last ? round + 1u : round, last ? 0u : chunk + 1u);
+#pragma unroll
+        for (uint32_t i = 0; i < FEW_STEPS; i++) {
+            const uint32_t step = first + chunk * FEW_STEPS + i;
+            if (step < end) {
+                const v4i b = *reinterpret_cast<const v4i *>(mine_codes + 64u * step * n);
+                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[i], b, acc, 0, 0, 0);
+            }
+        }
+        if (last) {
+            red[(buf * FEW_WAVES + wave) * 64u + lane] = acc;
+            acc = v4i{ 0, 0, 0, 0 };
+            __syncthreads();
+            if (wave < teams) {
+                const uint32_t g = (round * gridDim.x + blockIdx.x) * teams + wave, r = 16u * g + 4u * kq;
+                if (g < groups && r < rows && r16 < n) {
+                    v4i sums = { 0, 0, 0, 0 };
+                    for (uint32_t k = 0; k < team; k++) sums += red[(buf * FEW_WAVES + wave * team + k) * 64u + lane];
+                    float sw[4], b[4];
+                    i8_row_factors(p, r, sw, b);
+                    i8_results(p, r, r16, sums, sw, b, s_scale[r16]);
+                }
+            }
+            buf ^= 1u;
+            chunk = 0;
+            round++;
+        } else chunk++;
+    };
+    while (true) {
+        work(w[0], w[1]);
+        if (round == rounds) break;
+        work(w[1], w[0]);
+        if (round == rounds) break;
+    }
 }
 
 /* An expert's run of the sorted pairs, as far as it lies among them. */
@@ -310,8 +543,8 @@ static int launched(const char *who)
     return e == hipSuccess ? OXH_OK : oxh_internal_errorf(OXH_ERR_HIP, "HIP error in %s: %s", who, hipGetErrorString(e));
 }
 
-/* rows or tokens: the launches count them in 32 bits, in grids of up to 2^31 threads a dimension */
-#define I8_MAX_ROWS ((size_t)1 << 23)
+/* rows or tokens: a workgroup of 1024 threads each is a grid of 2^31 threads */
+#define I8_MAX_ROWS ((size_t)1 << 21)
 
 /* a tile's rows lie within 32 bits of its first one */
 #define I8_MAX_STRIDE ((size_t)1 << 23)
@@ -346,18 +579,28 @@ static int check_floats(const char *who, const char *name, uint32_t type, const 
 static int quantize_launch(uint32_t type, const void *x, size_t x_stride, size_t n, size_t cols, const void *up, int8_t *q,
                            size_t q_stride, float *scale, hipStream_t st, const char *who)
 {
-    const dim3 grid((uint32_t)n), block(256);
+    const dim3 grid((uint32_t)n);
+#define OXH_QUANT_K(T, GLU, THREADS, HELD)                                                                                       \
+    hipLaunchKernelGGL((k_i8_quantize<T, GLU, THREADS, HELD>), grid, dim3(THREADS), 0, st, (const T *)x, x_stride, (uint32_t)cols, \
+                       (const T *)up, q, q_stride, scale)
+#define OXH_QUANT_S(T, GLU)                                                                                                      \
+    do {                                                                                                                         \
+        if (cols <= 512u) OXH_QUANT_K(T, GLU, 64, 1);                                                                            \
+        else if (cols <= 2048u) OXH_QUANT_K(T, GLU, 256, 1);                                                                     \
+        else if (cols <= 8192u && n >= 512u) OXH_QUANT_K(T, GLU, 256, 4);                                                        \
+        else OXH_QUANT_K(T, GLU, 1024, 2);                                                                                       \
+    } while (0)
 #define OXH_QUANT(T)                                                                                                             \
     do {                                                                                                                         \
-        if (up) hipLaunchKernelGGL((k_i8_quantize<T, true>), grid, block, 0, st, (const T *)x, x_stride, (uint32_t)cols,         \
-                                   (const T *)up, q, q_stride, scale);                                                           \
-        else hipLaunchKernelGGL((k_i8_quantize<T, false>), grid, block, 0, st, (const T *)x, x_stride, (uint32_t)cols,           \
-                                (const T *)nullptr, q, q_stride, scale);                                                         \
+        if (up) OXH_QUANT_S(T, true);                                                                                            \
+        else OXH_QUANT_S(T, false);                                                                                              \
     } while (0)
     if (type == OXH_F32) OXH_QUANT(float);
     else if (type == OXH_F16) OXH_QUANT(_Float16);
     else OXH_QUANT(__bf16);
 #undef OXH_QUANT
+#undef OXH_QUANT_S
+#undef OXH_QUANT_K
     return launched(who);
 }
 
@@ -387,43 +630,134 @@ static int check_matrix(const char *who, const OxhI8Matrix *w)
     return OXH_OK;
 }
 
-typedef I8Geom<8, 4, 2, 4> I8Large;        /* 256 x 256, a workgroup per CU */
-typedef I8Geom<4, 4, 2, 2> I8Mid;          /* 128 x 128, two */
-typedef I8Geom<2, 2, 2, 2> I8Small;        /* 64 x 64, four */
+typedef I8Geom<8, 4, 2, 4, 5> I8Large;        /* 256 x 256, a workgroup per CU */
+typedef I8Geom<4, 4, 2, 4, 5> I8Half;         /* 128 x 256, one */
+typedef I8Geom<2, 4, 4, 2, 5> I8Mid;          /* 128 x 128, two */
+typedef I8Geom<2, 2, 2, 2, 5> I8Small;        /* 64 x 64, four */
 
 /* How a product runs: on which tile, its columns in how many parts. */
+enum { I8_LARGE = 0, I8_HALF, I8_MID, I8_SMALL, I8_TILES };
 struct I8Way {
-    int tile;                       /* 0 large, 1 mid, 2 small */
+    int tile;
     uint32_t splits;
 };
 
-static int forced_tile(void) { const char *v = getenv("OXH_I8_TILE"); return v ? atoi(v) : -1; }
-static int forced_split(void) { const char *v = getenv("OXH_I8_SPLIT"); return v ? atoi(v) : 0; }
-static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes)
+static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return splits > 1 ? (size_t)splits * n * ((rows + 3u) & ~(size_t)3u) * 4u : 0; }
+#define I8_MAX_PARTS_BYTES ((size_t)64 << 20)
+
+/* Microseconds that a stage of 128 columns takes a CU that works on `c` tiles at a time: 1.3 (large; 1.5 round after round), 0.88 (0.95), 0.48 / 0.8
+ * and 0.36 / 0.4 / 0.55 / 0.75, from launches that give every CU exactly that many (for instance 512 x 4096 x 4096 in small
+ * tiles, two to a CU, 32 stages: 18.5 us, of which 3 are launch and first loads and 1.7 the results). */
+static double stage_us(int tile, size_t c, bool full)
 {
-    I8Way w = { 0, 1 };
-    if (forced_tile() >= 0) w.tile = forced_tile();
-    if (forced_split() > 0) w.splits = (uint32_t)forced_split();
-    return w;
+    static const double mid[3] = { 0, 0.48, 0.8 }, small[5] = { 0, 0.36, 0.40, 0.55, 0.75 };
+    switch (tile) {
+    case I8_LARGE: return full ? 1.5 : 1.3;
+    case I8_HALF:  return full ? 0.95 : 0.88;
+    case I8_MID:   return mid[c];
+    default:       return small[c];
+    }
 }
 
-static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return splits > 1 ? (size_t)splits * n * ((rows + 3u) & ~(size_t)3u) * 4u : 0; }
+/* What a product takes: rounds of what the CUs hold at a time, the last one with as many tiles to a CU as are left; results
+ * at 5 TB/s; partial sums written and read at 4 TB/s and a second launch. */
+static double product_us(int tile, uint32_t splits, size_t rows, size_t stages, size_t n, size_t cus)
+{
+    static const size_t tile_rows[I8_TILES] = { 256, 128, 128, 64 }, tile_tok[I8_TILES] = { 256, 256, 128, 64 }, held[I8_TILES] = { 1, 1, 2, 4 };
+    const size_t tiles = ((rows + tile_rows[tile] - 1) / tile_rows[tile]) * ((n + tile_tok[tile] - 1) / tile_tok[tile]) * splits;
+    const size_t k = (stages + splits - 1) / splits, rounds = tiles / (cus * held[tile]), rest = tiles - rounds * cus * held[tile];
+    double us = 3.0 + (double)rounds * ((double)k * stage_us(tile, held[tile], true) + 1.5);
+    if (rest) {
+        const bool halves = tile == I8_LARGE && splits == 1 && rest <= cus / 2;
+        us += (double)k * stage_us(halves ? I8_HALF : tile, (rest + cus - 1) / cus, rounds != 0) + 1.5;
+    }
+    us += (double)n * (double)rows * 4.0 / 5e6;
+    if (splits > 1) us += 2.5 + (double)splits * (double)n * (double)rows * 8.0 / 4e6;
+    return us;
+}
+
+static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes, size_t cus)
+{
+    const size_t stages = (cols + 127u) / 128u;
+    I8Way best = { I8_SMALL, 1 };
+    double least = 1e30;
+    for (uint32_t splits = 1; splits <= 12 && splits <= stages; splits++) {
+        const size_t need = parts_bytes(rows, n, splits);
+        if (splits > 1 && (need > ws_bytes || need > I8_MAX_PARTS_BYTES || n > 65535u)) break;
+        for (int tile = 0; tile < I8_TILES; tile++) {
+            const double us = product_us(tile, splits, rows, stages, n, cus);
+            if (us < least) {
+                least = us;
+                best = { tile, splits };
+            }
+        }
+    }
+    return best;
+}
+
+/* compute units; a count to plan a workspace with when there is no device yet */
+static size_t i8_cus(void) { return oxh_internal_n_cu() > 0 ? (size_t)oxh_internal_n_cu() : 256u; }
 
 template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
 {
     p.row_tiles = (uint32_t)((p.w.rows + G::ROWS - 1u) / G::ROWS);
     p.tok_tiles = (p.n_vec + G::TOK - 1u) / G::TOK;
-    hipLaunchKernelGGL(k_i8_tiles<G>, dim3(p.row_tiles * p.tok_tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
+    const uint32_t tiles = p.row_tiles * p.tok_tiles;
+    if constexpr (G::ROWS == I8Large::ROWS) {
+        const uint32_t cus = (uint32_t)i8_cus(), rest = tiles % cus;
+        if (p.splits == 1u && rest && rest <= cus / 2u) {
+            p.whole = tiles - rest;
+            hipLaunchKernelGGL((k_i8_tiles_tail<I8Large, I8Half>), dim3(p.whole + 2u * rest), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
+            return;
+        }
+    }
+    hipLaunchKernelGGL(k_i8_tiles<G>, dim3(tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
+}
+
+/* The kernel for few tokens: how many waves share a group of 16 rows (0: it does not take the product).  All 4096 waves should
+ * have something to read, in as few rounds as may be; a round costs a join of its own, about six steps. */
+static size_t few_lds(size_t cols, size_t n) { return FEW_HEAD_BYTES + n * up64(cols); }
+static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
+{
+    if (n > FEW_TOKENS || few_lds(cols, n) > 160u * 1024u) return 0;
+    const size_t groups = (rows + 15u) / 16u, steps = (cols + 63u) / 64u;
+    uint32_t best = FEW_WAVES;
+    double least = 1e30;
+    for (uint32_t team = FEW_WAVES; team; team /= 2u) {
+        const double rounds = (double)((groups * team + cus * FEW_WAVES - 1u) / (cus * FEW_WAVES));
+        const double t = rounds * ((double)((steps + team - 1u) / team) + 6.0);
+        if (t < least) {
+            least = t;
+            best = team;
+        }
+    }
+    return best;
+}
+
+template <typename XT> static void few_launch(I8Product &p, const XT *x, size_t x_stride, uint32_t team, hipStream_t st)
+{
+    const uint32_t groups = (uint32_t)((p.w.rows + 15u) / 16u), teams = FEW_WAVES / team, need = (groups + teams - 1u) / teams;
+    const uint32_t cus = (uint32_t)i8_cus();
+    hipLaunchKernelGGL(k_i8_few<XT>, dim3(need < cus ? need : cus), dim3(64u * FEW_WAVES), few_lds(p.w.cols, p.n_vec), st, p, x, x_stride, team,
+                       groups);
 }
 
 static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, const float *bias,
                          uint32_t out_type, void *out, size_t out_stride, void *ws, size_t ws_bytes, hipStream_t st, const char *who)
 {
-    const I8Way way = i8_way(w->rows, w->cols, n, ws_bytes);
-    I8Product p = { *w, q, q_stride, q_scale, bias, out, out_stride, way.splits > 1 ? (int *)ws : nullptr, (uint32_t)n, way.splits, 0, 0,
+    I8Product p = { *w, q, q_stride, q_scale, bias, out, out_stride, nullptr, (uint32_t)n, 1u, 0u, 0u, 0u,
                     (uint32_t)((w->rows + 3u) & ~(size_t)3u), out_type };
-    if (way.tile == 0) tiles_launch<I8Large>(p, st);
-    else if (way.tile == 1) tiles_launch<I8Mid>(p, st);
+    const uint32_t team = few_team(w->rows, w->cols, n, i8_cus());
+    if (team) {
+        few_launch<int8_t>(p, q, q_stride, team, st);
+        return launched(who);
+    }
+    const I8Way way = i8_way(w->rows, w->cols, n, ws_bytes, i8_cus());
+    p.splits = way.splits;
+    if (way.splits > 1) p.parts = (int *)ws;
+    if (way.tile == I8_LARGE) tiles_launch<I8Large>(p, st);
+    else if (way.tile == I8_HALF) tiles_launch<I8Half>(p, st);
+    else if (way.tile == I8_MID) tiles_launch<I8Mid>(p, st);
     else tiles_launch<I8Small>(p, st);
     if (way.splits > 1) hipLaunchKernelGGL(k_i8_join, dim3((p.rows_pad / 4u + 255u) / 256u, p.n_vec), dim3(256), 0, st, p);
     return launched(who);
@@ -438,7 +772,13 @@ extern "C" int oxh_internal_i8_init(void)
 {
     hipError_t e;
     if ((e = whole_lds(k_i8_tiles<I8Large>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_tiles_tail<I8Large, I8Half>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_few<int8_t>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_few<float>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_few<_Float16>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_few<__bf16>)) != hipSuccess) return (int)e;
     return (int)hipSuccess;
 }
 
@@ -446,7 +786,8 @@ extern "C" size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
     if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > I8_MAX_ROWS || n_vec > I8_MAX_ROWS)
         return 0;
-    return parts_bytes(w->rows, n_vec, i8_way(w->rows, w->cols, n_vec, SIZE_MAX).splits);
+    if (few_team(w->rows, w->cols, n_vec, i8_cus())) return 0;
+    return parts_bytes(w->rows, n_vec, i8_way(w->rows, w->cols, n_vec, SIZE_MAX, i8_cus()).splits);
 }
 
 extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
@@ -467,23 +808,31 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
                          d_workspace ? workspace_bytes : 0, stream_of(stream), who);
 }
 
-/* the codes and scales of the tokens */
+/* Whether a product quantises its tokens in the launch itself: every workgroup does it again, so for few values only
+ * (the second launch costs about 3 us, the values of one token of 4096 about 1). */
+static bool linear_fused(size_t rows, size_t cols, size_t n) { return n * cols <= 16384u && few_team(rows, cols, n, i8_cus()) != 0; }
+
+/* the workspace otherwise: codes and scales of the tokens, the partial sums of the product */
 struct LinearParts {
-    size_t q_stride, q, scale, total;
+    size_t q_stride, q, scale, parts, parts_bytes, total;
 };
-static LinearParts linear_parts(size_t cols, size_t n)
+static LinearParts linear_parts(size_t rows, size_t cols, size_t n)
 {
     LinearParts p;
     p.q_stride = up64(cols);
     p.q = 0;
     p.scale = p.q_stride * n;
-    p.total = p.scale + up16(4u * n);
+    p.parts = p.scale + up16(4u * n);
+    p.parts_bytes = few_team(rows, cols, n, i8_cus()) ? 0 : parts_bytes(rows, n, i8_way(rows, cols, n, SIZE_MAX, i8_cus()).splits);
+    p.total = linear_fused(rows, cols, n) ? 0 : p.parts + p.parts_bytes;
     return p;
 }
 
 extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    return w && w->cols && w->cols <= OXH_I8_MAX_COLS && n_vec <= I8_MAX_ROWS ? linear_parts(w->cols, n_vec).total : 0;
+    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > I8_MAX_ROWS || n_vec > I8_MAX_ROWS)
+        return 0;
+    return linear_parts(w->rows, w->cols, n_vec).total;
 }
 
 extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
@@ -498,14 +847,24 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
         (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)))
         return rc;
     if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
-    const LinearParts p = linear_parts(w->cols, n_vec);
-    if (!d_workspace || workspace_bytes < p.total) return I8_ARG("%s: workspace too small (see oxh_i8_linear_workspace)", who);
-    if ((uintptr_t)d_workspace & 15u) return I8_ARG("%s: workspace must be 16-byte aligned", who);
+    const LinearParts l = linear_parts(w->rows, w->cols, n_vec);
+    if (l.total && (!d_workspace || workspace_bytes < l.total)) return I8_ARG("%s: workspace too small (see oxh_i8_linear_workspace)", who);
+    if (l.total && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
     if ((rc = ready())) return rc;
+    hipStream_t st = stream_of(stream);
+    if (l.total == 0) {
+        I8Product p = { *w, nullptr, 0, nullptr, d_bias, d_out, out_stride, nullptr, (uint32_t)n_vec, 1u, 0u, 0u, 0u, 0u, out_type };
+        const uint32_t team = few_team(w->rows, w->cols, n_vec, i8_cus());
+        if (x_type == OXH_F32) few_launch(p, (const float *)d_x, x_stride, team, st);
+        else if (x_type == OXH_F16) few_launch(p, (const _Float16 *)d_x, x_stride, team, st);
+        else few_launch(p, (const __bf16 *)d_x, x_stride, team, st);
+        return launched(who);
+    }
     int8_t *q = (int8_t *)d_workspace;
-    float *scale = (float *)((uint8_t *)d_workspace + p.scale);
-    if ((rc = quantize_launch(x_type, d_x, x_stride, n_vec, w->cols, nullptr, q, p.q_stride, scale, stream_of(stream), who))) return rc;
-    return matmul_launch(w, q, p.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, nullptr, 0, stream_of(stream), who);
+    float *scale = (float *)((uint8_t *)d_workspace + l.scale);
+    if ((rc = quantize_launch(x_type, d_x, x_stride, n_vec, w->cols, nullptr, q, l.q_stride, scale, st, who))) return rc;
+    return matmul_launch(w, q, l.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, (uint8_t *)d_workspace + l.parts, l.parts_bytes,
+                         st, who);
 }
 
 /* ─── experts ─────────────────────────────────────────────────────────── */
