@@ -186,6 +186,14 @@ __device__ __forceinline__ v4i i8_wave_sums(const int8_t *w_row, const int8_t *q
     return acc;
 }
 
+/* what a wave's lanes wrote to LDS before, its other lanes read after (LDS serves a wave in order) */
+__device__ __forceinline__ void i8_wave_sync()
+{
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
 /* Four neighbouring results of a token, aligned to their elements only; the last rows of a matrix one by one. */
 template <typename T> __device__ __forceinline__ void i8_store4(T *out, const float (&v)[4], uint32_t rows_left)
 {
@@ -264,8 +272,9 @@ template <typename G> __device__ __forceinline__ void i8_product_tile(const I8Pr
     const uint32_t stages = (cols + 127u) / 128u, first = split * stages / p.splits, end = (split + 1u) * stages / p.splits;
     const uint32_t k0 = 128u * first, kn = min(cols, 128u * end) - k0;
     v4i acc[G::RF][G::TF];
-    i8_tile<G>(p.w.d_w + (size_t)r0 * p.w.stride + k0, p.q + (size_t)t0 * p.q_stride + k0, kn,
-               [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; }, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, acc);
+    const int8_t *w = p.w.d_w + (size_t)r0 * p.w.stride + k0;
+    i8_tile<G>([&](uint32_t) { return w; }, [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; },
+               p.q + (size_t)t0 * p.q_stride + k0, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, kn, acc);
     const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
 #pragma unroll
     for (uint32_t i = 0; i < G::RF; i++) {
@@ -325,129 +334,186 @@ __global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
 
 /* ─── few tokens ──────────────────────────────────────────────────────── */
 
-/* Up to sixteen tokens: the matrix is streamed once and everything else has to stay out of its way.  A workgroup of
- * sixteen waves per CU keeps the tokens' codes in LDS, in the order the MFMA takes them ([16-column piece][token], what
- * lies behind the last column 0), and goes through groups of 16 rows: `team` waves share a group's columns, each
- * straight from memory to operand registers, eight steps of 64 columns in flight beside the eight being multiplied, the next
- * group's first ones requested before this one's sums are joined in LDS.  The first weights are requested before
- * the tokens are even looked at.
- *
- * XT: the type of float tokens, which every workgroup quantises for itself (k_i8_quantize's codes); int8_t: codes and scales
- * are there.  Bound by HBM; few rows by the latency of one trip to it. */
+/* Up to sixteen tokens: the matrix is streamed once and everything else has to stay out of its way.  `team` waves of a
+ * workgroup of sixteen share the columns of a group of 16 rows, at most ST stages of 128 columns a wave.  A wave requests all
+ * that it multiplies at once: weights eight rows of 128 bytes an instruction, turned into operands through 2 KiB of LDS of its own
+ * (loaded in the operand's order, sixteen rows of 64 bytes an instruction, one wave per CU takes 9.0 us for 16.8 MB where it
+ * takes 5.5 this way); tokens straight from L2, which all workgroups read.  The waves' sums are joined in LDS, where
+ * each leaves its own at the start of its 2 KiB.  Bound by HBM; few rows by the latency of one trip to it. */
 #define FEW_TOKENS 16u
 #define FEW_WAVES 16u
-#define FEW_STEPS 8u
-#define FEW_RED_BYTES (2u * FEW_WAVES * 1024u)
-#define FEW_HEAD_BYTES (FEW_RED_BYTES + 256u)          /* and the scales, a maximum per wave */
+#define FEW_TURN_BYTES (FEW_WAVES * 2048u)
 
-template <typename XT>
+/* This wave's weights: stages first .. of the group's rows at `rows` (this lane's, lane / 8 and lane / 8 + 8); stages that are not
+ * there are the last one again. */
+template <int ST>
+__device__ __forceinline__ void few_weights(v4i (&w)[ST][2], const int8_t *const (&rows)[2], uint32_t first, uint32_t stages, uint32_t last_piece)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+#pragma unroll
+    for (uint32_t i = 0; i < ST; i++)
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++)
+            w[i][h] = *reinterpret_cast<const v4i *>(rows[h] + 16u * min(8u * min(first + i, stages - 1u) + (lane & 7u), last_piece));
+}
+
+/* acc += a stage's weights, through `turn`, times tokens b(0), b(1).  Piece c of row r lies at slot c ^ ((r >> 1) & 7) of its
+ * 128 bytes, as in i8_tiles.inc. */
+template <typename B> __device__ __forceinline__ void few_stage(v4i &acc, const v4i (&w)[2], uint8_t *turn, B b)
+{
+    const uint32_t lane = threadIdx.x & 63u, r16 = lane & 15u, kq = lane >> 4, swz = (r16 >> 1) & 7u;
+    const uint32_t wr = 128u * (lane >> 3) + 16u * ((lane & 7u) ^ ((lane >> 4) & 7u));
+    *reinterpret_cast<v4i *>(turn + wr) = w[0];
+    *reinterpret_cast<v4i *>(turn + 1024u + (wr ^ 64u)) = w[1];
+    i8_wave_sync();
+    const v4i a0 = *reinterpret_cast<const v4i *>(turn + 128u * r16 + 16u * (kq ^ swz));
+    const v4i a1 = *reinterpret_cast<const v4i *>(turn + 128u * r16 + 16u * ((4u + kq) ^ swz));
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a0, b(0u), acc, 0, 0, 0);
+    acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a1, b(1u), acc, 0, 0, 0);
+    i8_wave_sync();
+}
+
+/* The sums of a group of rows and up to sixteen tokens over `mine` stages from `first` on, left in this wave's `turn`.
+ * q_row: this lane's token, lane % 16. */
+template <int ST>
+__device__ __forceinline__ void few_sums(const int8_t *const (&rows)[2], const int8_t *q_row, uint32_t cols, uint32_t first, uint32_t mine,
+                                         uint8_t *turn)
+{
+    const uint32_t lane = threadIdx.x & 63u, kq = lane >> 4, stages = (cols + 127u) / 128u, last_piece = (cols - 1u) / 16u;
+    v4i w[ST][2], q[2][2];
+    auto tokens = [&](uint32_t i) {
+#pragma unroll
+        for (uint32_t h = 0; h < 2u; h++)
+            q[i & 1u][h] = *reinterpret_cast<const v4i *>(q_row + 16u * min(8u * min(first + i, stages - 1u) + 4u * h + kq, last_piece));
+    };
+    tokens(0u);
+    few_weights<ST>(w, rows, first, stages, last_piece);
+    v4i acc = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t i = 0; i < ST; i++) {
+        if (i + 1u < ST) tokens(i + 1u);
+        if (i < mine) {
+            if (128u * (first + i + 1u) > cols) {           /* the tokens' columns behind the last one count as 0 */
+#pragma unroll
+                for (uint32_t h = 0; h < 2u; h++)
+#pragma unroll
+                    for (uint32_t d = 0; d < 4u; d++) {
+                        const uint32_t at = 128u * (first + i) + 64u * h + 16u * kq + 4u * d, left = cols > at ? cols - at : 0u;
+                        if (left < 4u) q[i & 1u][h][d] &= (int)((1u << (8u * left)) - 1u);
+                    }
+            }
+            few_stage(acc, w[i], turn, [&](uint32_t h) { return q[i & 1u][h]; });
+        }
+    }
+    *reinterpret_cast<v4i *>(turn + 16u * lane) = acc;
+}
+
+/* Part `part` of `parts` of a row's stages. */
+__device__ __forceinline__ void few_part(uint32_t stages, uint32_t part, uint32_t parts, uint32_t &first, uint32_t &mine)
+{
+    first = part * stages / parts;
+    mine = (part + 1u) * stages / parts - first;
+}
+
+/* The joined sums of the `count` waves from `wave` on. */
+__device__ __forceinline__ v4i few_join(const uint8_t *turns, uint32_t wave, uint32_t count)
+{
+    v4i sums = { 0, 0, 0, 0 };
+    for (uint32_t k = 0; k < count; k++) sums += *reinterpret_cast<const v4i *>(turns + 2048u * (wave + k) + 16u * (threadIdx.x & 63u));
+    return sums;
+}
+
+/* quantised tokens */
+template <int ST>
+__global__ __launch_bounds__(1024) void k_i8_few(const I8Product p, uint32_t team, uint32_t groups)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_TURN_BYTES];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, teams = FEW_WAVES / team, r16 = lane & 15u;
+    const uint32_t r0 = 16u * min(blockIdx.x * teams + wave / team, groups - 1u);
+    uint32_t first, mine;
+    few_part((cols + 127u) / 128u, wave % team, team, first, mine);
+    const int8_t *w[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; h++) w[h] = p.w.d_w + (size_t)min(r0 + 8u * h + (lane >> 3), rows - 1u) * p.w.stride;
+    few_sums<ST>(w, p.q + (size_t)min(r16, p.n_vec - 1u) * p.q_stride, cols, first, mine, turns + 2048u * wave);
+    __syncthreads();
+    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * (lane >> 4);
+    if (wave < teams && g < groups && r < rows && r16 < p.n_vec) {
+        float sw[4], b[4];
+        i8_row_factors(p, r, sw, b);
+        i8_results(p, r, r16, few_join(turns, wave * team, team), sw, b, p.q_scale[r16]);
+    }
+}
+
+/* Float tokens, which every workgroup quantises for itself (k_i8_quantize's codes): their values are requested before the weights
+ * and wait in registers; the codes lie in LDS in the order the MFMA takes them, [16-column piece][token]. */
+#define FEW_HELD 4u                                    /* times eight values of a token that a lane holds */
+#define FEW_HEAD_BYTES (FEW_TURN_BYTES + 128u)         /* and the scales, a maximum per wave */
+
+template <typename XT, int ST>
 __global__ __launch_bounds__(1024) void
-k_i8_few(const I8Product p, const XT *__restrict__ x, size_t x_stride, uint32_t team, uint32_t groups)
+k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uint32_t team, uint32_t groups)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_shared[];
-    v4i *const red = reinterpret_cast<v4i *>(few_shared);
-    float *const s_scale = reinterpret_cast<float *>(few_shared + FEW_RED_BYTES);
-    uint32_t *const s_top = reinterpret_cast<uint32_t *>(few_shared + FEW_RED_BYTES + 64u);
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    float *const s_scale = reinterpret_cast<float *>(few_shared + FEW_TURN_BYTES);
+    uint32_t *const s_top = reinterpret_cast<uint32_t *>(few_shared + FEW_TURN_BYTES + 64u);
     uint8_t *const codes = few_shared + FEW_HEAD_BYTES;
-    const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(tid >> 6));
     const uint32_t r16 = lane & 15u, kq = lane >> 4;
-    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, n = p.n_vec;
-    const uint32_t teams = FEW_WAVES / team, mine = wave / team, part = wave % team;
-    const uint32_t steps = (cols + 63u) / 64u, first = part * steps / team, end = (part + 1u) * steps / team;
-    const uint32_t chunks = max(1u, ((steps + team - 1u) / team + FEW_STEPS - 1u) / FEW_STEPS);
-    const uint32_t rounds = (groups + gridDim.x * teams - 1u) / (gridDim.x * teams);
-    const uint32_t last_piece = (cols - 1u) / 16u;
-    v4i w[2][FEW_STEPS];
-    auto group_of = [&](uint32_t round) { return (round * gridDim.x + blockIdx.x) * teams + mine; };
-    /* columns behind the wave's part are requested as its last ones and not used */
-    auto fetch = [&](v4i (&to)[FEW_STEPS], uint32_t round, uint32_t chunk) {
-        const uint32_t row = min(min(group_of(round), groups - 1u) * 16u + r16, rows - 1u);
-        const int8_t *base = p.w.d_w + (size_t)row * p.w.stride;
-#pragma unroll
-        for (uint32_t i = 0; i < FEW_STEPS; i++) {
-            const uint32_t step = min(first + chunk * FEW_STEPS + i, steps - 1u);
-            to[i] = *reinterpret_cast<const v4i *>(base + 16u * min(4u * step + kq, last_piece));
-        }
-    };
-    fetch(w[0], 0u, 0u);
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, n = p.n_vec, teams = FEW_WAVES / team;
+    const uint32_t stages = (cols + 127u) / 128u, pieces = 8u * stages;
+    uint32_t first, mine;
+    few_part(stages, wave % team, team, first, mine);
 
-    /* tokens to LDS: waves n_waves * t .. of token t */
-    const uint32_t pieces = 4u * steps;
-    if constexpr (sizeof(XT) == 1) {
-        for (uint32_t i = tid; i < pieces * n; i += 1024u) {
-            const uint32_t t = i / pieces, c = i - t * pieces;
-            *reinterpret_cast<v4i *>(codes + 16u * (c * n + t)) = i8_piece(reinterpret_cast<const int8_t *>(x) + (size_t)t * x_stride, 16u * c, cols);
-        }
-        if (tid < n) s_scale[tid] = p.q_scale[tid];
-    } else {
-        const uint32_t per = n == 1u ? 16u : n == 2u ? 8u : n <= 4u ? 4u : n <= 8u ? 2u : 1u;
-        const uint32_t t = wave / per, w0 = wave % per;
-        const XT *xr = x + (size_t)min(t, n - 1u) * x_stride;
-        const uint32_t c0 = 8u * (64u * w0 + lane), step = 8u * 64u * per;
-        uint32_t top = 0;
-        if (t < n)
-            for (uint32_t c = c0; c < cols; c += step) {
-                float v[8];
-                i8_values8<XT, false>(xr, nullptr, c, cols, v);
-                top = max(top, i8_top8(v));
-            }
-        top = wave_top(top);
-        if (lane == 0u) s_top[wave] = top;
-        __syncthreads();
-        for (uint32_t k = 0; k < per; k++) top = max(top, s_top[wave - w0 + k]);
-        float inv;
-        const float s = i8_scale(top, inv);
-        if (t < n) {
-            if (w0 == 0u && lane == 0u) s_scale[t] = s;
-            for (uint32_t c = c0; c < 16u * pieces; c += step) {
-                float v[8];
-                i8_values8<XT, false>(xr, nullptr, c, cols, v);
-                *reinterpret_cast<uint2 *>(codes + 16u * ((c / 16u) * n + t) + (c & 8u)) = inv != 0.0f ? i8_codes8(v, s, inv) : make_uint2(0u, 0u);
-            }
+    /* tokens: waves per * t .. of token t */
+    const uint32_t per = n == 1u ? 16u : n == 2u ? 8u : n <= 4u ? 4u : n <= 8u ? 2u : 1u;
+    const uint32_t t = wave / per, w0 = wave % per, c0 = 8u * (64u * w0 + lane), step = 512u * per;
+    float v[FEW_HELD][8];
+    const XT *xr = x + (size_t)min(t, n - 1u) * x_stride;
+#pragma unroll
+    for (uint32_t i = 0; i < FEW_HELD; i++) i8_values8<XT, false>(xr, nullptr, c0 + step * i, t < n ? cols : 0u, v[i]);
+    const uint32_t r0 = 16u * min(blockIdx.x * teams + wave / team, groups - 1u);
+    const int8_t *wrow[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; h++) wrow[h] = p.w.d_w + (size_t)min(r0 + 8u * h + (lane >> 3), rows - 1u) * p.w.stride;
+    v4i w[ST][2];
+    few_weights<ST>(w, wrow, first, stages, (cols - 1u) / 16u);
+
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < FEW_HELD; i++) top = max(top, i8_top8(v[i]));
+    top = wave_top(top);
+    if (lane == 0u) s_top[wave] = top;
+    __syncthreads();
+    for (uint32_t k = 0; k < per; k++) top = max(top, s_top[wave - w0 + k]);
+    float inv;
+    const float s = i8_scale(top, inv);
+    if (t < n) {
+        if (w0 == 0u && lane == 0u) s_scale[t] = s;
+#pragma unroll
+        for (uint32_t i = 0; i < FEW_HELD; i++) {
+            const uint32_t c = c0 + step * i;
+            if (c < 16u * pieces)
+                *reinterpret_cast<uint2 *>(codes + 16u * ((c / 16u) * n + t) + (c & 8u)) = inv != 0.0f ? i8_codes8(v[i], s, inv) : make_uint2(0u, 0u);
         }
     }
     __syncthreads();
 
     const uint8_t *mine_codes = codes + 16u * (kq * n + min(r16, n - 1u));
-    uint32_t buf = 0;
     v4i acc = { 0, 0, 0, 0 };
-    uint32_t round = 0, chunk = 0;
-    /* one chunk from `now` while the one behind it comes to `then` */
-    auto work = [&](v4i (&now)[FEW_STEPS], v4i (&then)[FEW_STEPS]) {
-        const bool last = chunk + 1u == chunks;
-        fetch(then, last ? round + 1u : round, last ? 0u : chunk + 1u);
 #pragma unroll
-        for (uint32_t i = 0; i < FEW_STEPS; i++) {
-            const uint32_t step = first + chunk * FEW_STEPS + i;
-            if (step < end) {
-                const v4i b = *reinterpret_cast<const v4i *>(mine_codes + 64u * step * n);
-                acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(now[i], b, acc, 0, 0, 0);
-            }
-        }
-        if (last) {
-            red[(buf * FEW_WAVES + wave) * 64u + lane] = acc;
-            acc = v4i{ 0, 0, 0, 0 };
-            __syncthreads();
-            if (wave < teams) {
-                const uint32_t g = (round * gridDim.x + blockIdx.x) * teams + wave, r = 16u * g + 4u * kq;
-                if (g < groups && r < rows && r16 < n) {
-                    v4i sums = { 0, 0, 0, 0 };
-                    for (uint32_t k = 0; k < team; k++) sums += red[(buf * FEW_WAVES + wave * team + k) * 64u + lane];
-                    float sw[4], b[4];
-                    i8_row_factors(p, r, sw, b);
-                    i8_results(p, r, r16, sums, sw, b, s_scale[r16]);
-                }
-            }
-            buf ^= 1u;
-            chunk = 0;
-            round++;
-        } else chunk++;
-    };
-    while (true) {
-        work(w[0], w[1]);
-        if (round == rounds) break;
-        work(w[1], w[0]);
-        if (round == rounds) break;
+    for (uint32_t i = 0; i < ST; i++)
+        if (i < mine)
+            few_stage(acc, w[i], few_shared + 2048u * wave,
+                      [&](uint32_t h) { return *reinterpret_cast<const v4i *>(mine_codes + 16u * n * (8u * (first + i) + 4u * h)); });
+    *reinterpret_cast<v4i *>(few_shared + 2048u * wave + 16u * lane) = acc;
+    __syncthreads();
+    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * kq;
+    if (wave < teams && g < groups && r < rows && r16 < n) {
+        float sw[4], b[4];
+        i8_row_factors(p, r, sw, b);
+        i8_results(p, r, r16, few_join(few_shared, wave * team, team), sw, b, s_scale[r16]);
     }
 }
 
@@ -714,32 +780,49 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
     hipLaunchKernelGGL(k_i8_tiles<G>, dim3(tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
 }
 
-/* The kernel for few tokens: how many waves share a group of 16 rows (0: it does not take the product).  All 4096 waves should
- * have something to read, in as few rounds as may be; a round costs a join of its own, about six steps. */
-static size_t few_lds(size_t cols, size_t n) { return FEW_HEAD_BYTES + n * up64(cols); }
+/* The kernels for few tokens: how many waves share a group of 16 rows (0: they do not take the product).  Four stages a wave
+ * leave room for two workgroups on a CU (151936 x 896 under one token: 27 us, 33 with eight); where the groups are few, all
+ * of a CU's sixteen waves are wanted. */
+#define FEW_MAX_STAGES 8u
 static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
 {
-    if (n > FEW_TOKENS || few_lds(cols, n) > 160u * 1024u) return 0;
-    const size_t groups = (rows + 15u) / 16u, steps = (cols + 63u) / 64u;
-    uint32_t best = FEW_WAVES;
-    double least = 1e30;
-    for (uint32_t team = FEW_WAVES; team; team /= 2u) {
-        const double rounds = (double)((groups * team + cus * FEW_WAVES - 1u) / (cus * FEW_WAVES));
-        const double t = rounds * ((double)((steps + team - 1u) / team) + 6.0);
-        if (t < least) {
-            least = t;
-            best = team;
-        }
-    }
-    return best;
+    const size_t groups = (rows + 15u) / 16u, stages = (cols + 127u) / 128u;
+    if (n > FEW_TOKENS || stages > FEW_MAX_STAGES * FEW_WAVES) return 0;
+    uint32_t team = 1;
+    while (team < FEW_WAVES && (stages > 4u * team || groups * team < cus * FEW_WAVES)) team *= 2u;
+    return team;
 }
 
-template <typename XT> static void few_launch(I8Product &p, const XT *x, size_t x_stride, uint32_t team, hipStream_t st)
+struct FewGrid {
+    uint32_t groups, wgs, stages;   /* stages of a wave, at most */
+};
+static FewGrid few_grid(size_t rows, size_t cols, uint32_t team)
 {
-    const uint32_t groups = (uint32_t)((p.w.rows + 15u) / 16u), teams = FEW_WAVES / team, need = (groups + teams - 1u) / teams;
-    const uint32_t cus = (uint32_t)i8_cus();
-    hipLaunchKernelGGL(k_i8_few<XT>, dim3(need < cus ? need : cus), dim3(64u * FEW_WAVES), few_lds(p.w.cols, p.n_vec), st, p, x, x_stride, team,
-                       groups);
+    FewGrid g;
+    g.groups = (uint32_t)((rows + 15u) / 16u);
+    g.wgs = (g.groups + FEW_WAVES / team - 1u) / (FEW_WAVES / team);
+    g.stages = ((uint32_t)((cols + 127u) / 128u) + team - 1u) / team;
+    return g;
+}
+
+static void few_launch(const I8Product &p, uint32_t team, hipStream_t st)
+{
+    const FewGrid g = few_grid(p.w.rows, p.w.cols, team);
+    const dim3 grid(g.wgs), block(64u * FEW_WAVES);
+    if (g.stages <= 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
+    else if (g.stages <= 4u) hipLaunchKernelGGL(k_i8_few<4>, grid, block, 0, st, p, team, g.groups);
+    else hipLaunchKernelGGL(k_i8_few<8>, grid, block, 0, st, p, team, g.groups);
+}
+
+static size_t few_float_lds(size_t cols, size_t n) { return FEW_HEAD_BYTES + n * ((cols + 127u) & ~(size_t)127u); }
+template <typename XT> static void few_float_launch(const I8Product &p, const XT *x, size_t x_stride, uint32_t team, hipStream_t st)
+{
+    const FewGrid g = few_grid(p.w.rows, p.w.cols, team);
+    const dim3 grid(g.wgs), block(64u * FEW_WAVES);
+    const size_t lds = few_float_lds(p.w.cols, p.n_vec);
+    if (g.stages <= 2u) hipLaunchKernelGGL((k_i8_few_float<XT, 2>), grid, block, lds, st, p, x, x_stride, team, g.groups);
+    else if (g.stages <= 4u) hipLaunchKernelGGL((k_i8_few_float<XT, 4>), grid, block, lds, st, p, x, x_stride, team, g.groups);
+    else hipLaunchKernelGGL((k_i8_few_float<XT, 8>), grid, block, lds, st, p, x, x_stride, team, g.groups);
 }
 
 static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, const float *bias,
@@ -749,7 +832,7 @@ static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride,
                     (uint32_t)((w->rows + 3u) & ~(size_t)3u), out_type };
     const uint32_t team = few_team(w->rows, w->cols, n, i8_cus());
     if (team) {
-        few_launch<int8_t>(p, q, q_stride, team, st);
+        few_launch(p, team, st);
         return launched(who);
     }
     const I8Way way = i8_way(w->rows, w->cols, n, ws_bytes, i8_cus());
@@ -775,10 +858,6 @@ extern "C" int oxh_internal_i8_init(void)
     if ((e = whole_lds(k_i8_tiles_tail<I8Large, I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_few<int8_t>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_few<float>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_few<_Float16>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_few<__bf16>)) != hipSuccess) return (int)e;
     return (int)hipSuccess;
 }
 
@@ -808,9 +887,15 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
                          d_workspace ? workspace_bytes : 0, stream_of(stream), who);
 }
 
-/* Whether a product quantises its tokens in the launch itself: every workgroup does it again, so for few values only
- * (the second launch costs about 3 us, the values of one token of 4096 about 1). */
-static bool linear_fused(size_t rows, size_t cols, size_t n) { return n * cols <= 16384u && few_team(rows, cols, n, i8_cus()) != 0; }
+/* Whether a product quantises its tokens in the launch itself: every workgroup does it again, so for few values (a second
+ * launch costs about 3 us, the values of one token of 4096 about 1) and while there is no more than a workgroup per CU
+ * (14336 x 4096 under one token, 448 workgroups: 16.5 us fused, 15.2 in two). */
+static bool linear_fused(size_t rows, size_t cols, size_t n)
+{
+    const size_t per = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;      /* waves a token, as in the kernel */
+    const uint32_t team = few_team(rows, cols, n, i8_cus());
+    return team && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= i8_cus();
+}
 
 /* the workspace otherwise: codes and scales of the tokens, the partial sums of the product */
 struct LinearParts {
@@ -855,9 +940,9 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
     if (l.total == 0) {
         I8Product p = { *w, nullptr, 0, nullptr, d_bias, d_out, out_stride, nullptr, (uint32_t)n_vec, 1u, 0u, 0u, 0u, 0u, out_type };
         const uint32_t team = few_team(w->rows, w->cols, n_vec, i8_cus());
-        if (x_type == OXH_F32) few_launch(p, (const float *)d_x, x_stride, team, st);
-        else if (x_type == OXH_F16) few_launch(p, (const _Float16 *)d_x, x_stride, team, st);
-        else few_launch(p, (const __bf16 *)d_x, x_stride, team, st);
+        if (x_type == OXH_F32) few_float_launch(p, (const float *)d_x, x_stride, team, st);
+        else if (x_type == OXH_F16) few_float_launch(p, (const _Float16 *)d_x, x_stride, team, st);
+        else few_float_launch(p, (const __bf16 *)d_x, x_stride, team, st);
         return launched(who);
     }
     int8_t *q = (int8_t *)d_workspace;
