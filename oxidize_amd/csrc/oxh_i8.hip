@@ -108,17 +108,14 @@ __device__ __forceinline__ float i8_scale(uint32_t top, float &inv)
     return s;
 }
 
-/* A workgroup per row, eight values to a thread and step: once for the largest magnitude, once for the codes.  The first
+/* A row by a workgroup, eight values to a thread and step: once for the largest magnitude, once for the codes.  The first
  * HELD steps' values stay in registers; what is longer is read (and, GLU, computed) a second time. */
 template <typename T, bool GLU, int THREADS, int HELD>
-__global__ __launch_bounds__(THREADS) void
-k_i8_quantize(const T *__restrict__ x, size_t x_stride, uint32_t cols, const T *__restrict__ up, int8_t *__restrict__ q,
-              size_t q_stride, float *__restrict__ scale)
+__device__ __forceinline__ void i8_quantize_row(const T *__restrict__ xr, const T *__restrict__ ur, uint32_t cols, int8_t *__restrict__ qr,
+                                                float *__restrict__ scale)
 {
     constexpr uint32_t STEP = 8u * THREADS;
     __shared__ uint32_t s_top[THREADS / 64];
-    const size_t row = blockIdx.x;
-    const T *xr = x + row * x_stride, *ur = GLU ? up + row * x_stride : nullptr;
     const uint32_t c0 = 8u * threadIdx.x;
     float v[HELD][8];
     uint32_t top = 0;
@@ -140,9 +137,8 @@ k_i8_quantize(const T *__restrict__ x, size_t x_stride, uint32_t cols, const T *
     }
     float inv;
     const float s = i8_scale(top, inv);
-    if (threadIdx.x == 0u) scale[row] = s;
+    if (threadIdx.x == 0u) *scale = s;
     const uint32_t end = (cols + 15u) & ~15u;
-    int8_t *qr = q + row * q_stride;
     auto store = [&](uint32_t c, const float (&t)[8]) {
         if (c < end) *reinterpret_cast<uint2 *>(qr + c) = inv != 0.0f ? i8_codes8(t, s, inv) : make_uint2(0u, 0u);
     };
@@ -153,6 +149,15 @@ k_i8_quantize(const T *__restrict__ x, size_t x_stride, uint32_t cols, const T *
         i8_values8<T, GLU>(xr, ur, c, cols, t);
         store(c, t);
     }
+}
+
+template <typename T, bool GLU, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void
+k_i8_quantize(const T *__restrict__ x, size_t x_stride, uint32_t cols, const T *__restrict__ up, int8_t *__restrict__ q,
+              size_t q_stride, float *__restrict__ scale)
+{
+    const size_t row = blockIdx.x;
+    i8_quantize_row<T, GLU, THREADS, HELD>(x + row * x_stride, GLU ? up + row * x_stride : nullptr, cols, q + row * q_stride, scale + row);
 }
 
 /* ─── products ────────────────────────────────────────────────────────── */
@@ -171,19 +176,6 @@ __device__ __forceinline__ v4i i8_piece(const int8_t *row, uint32_t k, uint32_t 
             }
     }
     return v;
-}
-
-/* 16 rows x 16 tokens of a wave: lane l supplies sixteen columns of row l % 16 and of token l % 16, and receives the sums
- * of token l % 16 and rows 4 * (l / 16) .. +3.  Zeroing one operand behind the last column is enough. */
-__device__ __forceinline__ v4i i8_wave_sums(const int8_t *w_row, const int8_t *q_row, uint32_t cols, uint32_t lane)
-{
-    v4i acc = { 0, 0, 0, 0 };
-    for (uint32_t k0 = 0; k0 < cols; k0 += 64u) {
-        const uint32_t k = k0 + 16u * (lane >> 4);
-        const v4i a = i8_piece(w_row, k, cols), b = i8_piece(q_row, k, cols);
-        acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, acc, 0, 0, 0);
-    }
-    return acc;
 }
 
 /* what a wave's lanes wrote to LDS before, its other lanes read after (LDS serves a wave in order) */
@@ -517,63 +509,169 @@ k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uin
     }
 }
 
-/* An expert's run of the sorted pairs, as far as it lies among them. */
-__device__ __forceinline__ uint32_t i8_run(const uint32_t *offsets, uint32_t e, uint32_t pairs, uint32_t &first)
-{
-    first = min(offsets[e], pairs);
-    const uint32_t end = min(offsets[e + 1u], pairs);
-    return end > first ? end - first : 0u;
-}
+/* ─── experts ─────────────────────────────────────────────────────────── */
 
-/* h = silu(gate) * up of an expert's pairs; the pairs' tokens through perm */
-__global__ __launch_bounds__(256) void
-k_i8_experts_up(const OxhMoeI8 m, const OxhRouting rt, const int8_t *__restrict__ q, size_t q_stride,
-                const float *__restrict__ q_scale, uint32_t n_tok, uint32_t pairs, float *__restrict__ h, size_t h_stride)
+/* Up to a number of pairs of an expert: n of them from sorted pair `first` on; n 0: nothing.  all: tiles there are. */
+struct I8ExpertTile {
+    uint32_t expert, first, n, all;
+};
+
+/* The first launch of a layer: a workgroup per token to quantise it, and one that cuts the experts' runs of the sorted pairs into tiles
+ * of `tok`; entries behind the last tile say so. */
+template <typename T, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void
+k_i8_experts_begin(const T *__restrict__ x, size_t x_stride, uint32_t cols, int8_t *__restrict__ q, size_t q_stride,
+                   float *__restrict__ scale, const uint32_t *__restrict__ offsets, uint32_t n_expert, uint32_t pairs, uint32_t tok,
+                   I8ExpertTile *__restrict__ tiles, uint32_t n_tiles)
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, e = blockIdx.y, ffn = (uint32_t)m.ffn;
-    const uint32_t r0 = blockIdx.x * 64u + 16u * wave;
-    if (r0 >= ffn) return;
-    uint32_t first;
-    const uint32_t n = i8_run(rt.d_offsets, e, pairs, first);
-    const size_t row = (size_t)e * ffn + min(r0 + (lane & 15u), ffn - 1u);
-    for (uint32_t j0 = 0; j0 < n; j0 += 16u) {
-        const uint32_t j = first + min(j0 + (lane & 15u), n - 1u), tok = min(rt.d_perm[j], n_tok - 1u);
-        const int8_t *qr = q + (size_t)tok * q_stride;
-        const v4i g = i8_wave_sums(m.d_w_gate + row * m.gate_up_stride, qr, (uint32_t)m.hidden, lane);
-        const v4i u = i8_wave_sums(m.d_w_up + row * m.gate_up_stride, qr, (uint32_t)m.hidden, lane);
-        if (j0 + (lane & 15u) >= n) continue;
-        const float st = q_scale[tok];
+    __shared__ uint32_t s_first[OXH_SELECT_MAX_EXPERTS + 1], s_tile[OXH_SELECT_MAX_EXPERTS + 1];
+    if (blockIdx.x != 0u) {
+        const size_t row = blockIdx.x - 1u;
+        i8_quantize_row<T, false, THREADS, HELD>(x + row * x_stride, nullptr, cols, q + row * q_stride, scale + row);
+        return;
+    }
+    for (uint32_t e = threadIdx.x; e <= n_expert; e += THREADS) s_first[e] = min(offsets[e], pairs);
+    __syncthreads();
+    if (threadIdx.x < 64u) {                        /* eight experts to a lane: where their tiles start */
+        uint32_t own[8], sum = 0;
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t r = r0 + 4u * (lane >> 4) + i;
-            if (r >= ffn) break;
-            const float gv = (float)g[i] * st * m.d_s_gate[(size_t)e * ffn + r], uv = (float)u[i] * st * m.d_s_up[(size_t)e * ffn + r];
-            h[(size_t)j * h_stride + r] = silu(gv) * uv;
+        for (uint32_t i = 0; i < 8u; i++) {
+            const uint32_t e = 8u * threadIdx.x + i;
+            const uint32_t n = e < n_expert && s_first[e + 1u] > s_first[e] ? s_first[e + 1u] - s_first[e] : 0u;
+            own[i] = (n + tok - 1u) / tok;
+            sum += own[i];
         }
+        uint32_t upto = sum;
+#pragma unroll
+        for (uint32_t d = 1; d < 64u; d <<= 1) {
+            const uint32_t v = __shfl_up(upto, d);
+            if (threadIdx.x >= d) upto += v;
+        }
+        uint32_t at = upto - sum;
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) {
+            if (8u * threadIdx.x + i <= n_expert) s_tile[8u * threadIdx.x + i] = at;
+            at += own[i];
+        }
+        if (threadIdx.x == 63u && n_expert == OXH_SELECT_MAX_EXPERTS) s_tile[n_expert] = at;
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n_tiles; i += THREADS) {
+        I8ExpertTile t = { 0u, 0u, 0u, s_tile[n_expert] };
+        if (i < s_tile[n_expert]) {
+            uint32_t lo = 0, hi = n_expert;         /* the last expert whose tiles start at i or before */
+            while (hi - lo > 1u) {
+                const uint32_t mid = (lo + hi) / 2u;
+                if (s_tile[mid] <= i) lo = mid;
+                else hi = mid;
+            }
+            t.expert = lo;
+            t.first = s_first[lo] + tok * (i - s_tile[lo]);
+            t.n = min(tok, s_first[lo + 1u] - t.first);
+        }
+        tiles[i] = t;
     }
 }
 
-__global__ __launch_bounds__(256) void
-k_i8_experts_down(const OxhMoeI8 m, const OxhRouting rt, const int8_t *__restrict__ q, size_t q_stride,
-                  const float *__restrict__ q_scale, uint32_t pairs, float *__restrict__ y, size_t y_stride)
+/* What the experts' products read and write: gate and up (UP) over tokens through perm into h, or down over the pairs' codes
+ * into y. */
+struct I8Experts {
+    const int8_t *w[2];
+    const float *s[2];
+    size_t stride;
+    const int8_t *q;
+    size_t q_stride;
+    const float *q_scale;
+    const uint32_t *perm;
+    const I8ExpertTile *tiles;
+    float *out;
+    size_t out_stride;
+    uint32_t rows, cols, n_tok, n_tiles, row_tiles;
+};
+
+/* the row of codes of a tile's pair j */
+template <bool UP> __device__ __forceinline__ uint32_t i8_pair_row(const I8Experts &p, const I8ExpertTile &t, uint32_t j)
 {
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, e = blockIdx.y, rows = (uint32_t)m.hidden;
-    const uint32_t r0 = blockIdx.x * 64u + 16u * wave;
-    if (r0 >= rows) return;
-    uint32_t first;
-    const uint32_t n = i8_run(rt.d_offsets, e, pairs, first);
-    const size_t row = (size_t)e * rows + min(r0 + (lane & 15u), rows - 1u);
-    for (uint32_t j0 = 0; j0 < n; j0 += 16u) {
-        const uint32_t j = first + min(j0 + (lane & 15u), n - 1u);
-        const v4i s = i8_wave_sums(m.d_w_down + row * m.down_stride, q + (size_t)j * q_stride, (uint32_t)m.ffn, lane);
-        if (j0 + (lane & 15u) >= n) continue;
-        const float st = q_scale[j];
+    const uint32_t pair = t.first + min(j, t.n - 1u);
+    return UP ? min(p.perm[pair], p.n_tok - 1u) : pair;
+}
+
+/* Four rows' results of a pair from its sums. */
+template <bool UP>
+__device__ __forceinline__ void i8_pair_results(const I8Experts &p, const I8ExpertTile &t, uint32_t j, uint32_t r, const v4i &first, const v4i &second)
+{
+    if (r >= p.rows) return;
+    const size_t row0 = (size_t)t.expert * p.rows;
+    const float st = p.q_scale[i8_pair_row<UP>(p, t, j)];
+    float v[4];
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const uint32_t r = r0 + 4u * (lane >> 4) + i;
-            if (r >= rows) break;
-            y[(size_t)j * y_stride + r] = (float)s[i] * st * m.d_s_down[(size_t)e * rows + r];
-        }
+    for (uint32_t k = 0; k < 4u; k++) {
+        const uint32_t rk = min(r + k, p.rows - 1u);
+        v[k] = (float)first[k] * st * p.s[0][row0 + rk];
+        if (UP) v[k] = silu(v[k]) * ((float)second[k] * st * p.s[1][row0 + rk]);
+    }
+    i8_store4(p.out + (size_t)(t.first + j) * p.out_stride + r, v, p.rows - r);
+}
+
+/* A tile of an expert's rows and pairs.  UP: the tile's fragments of 16 rows are gate's and up's by turns, so that a wave holds
+ * both factors of a result. */
+template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(const I8Experts &p, const I8ExpertTile &t, uint32_t row_tile)
+{
+    constexpr uint32_t OUT_ROWS = UP ? G::ROWS / 2u : G::ROWS;
+    const uint32_t r0 = row_tile * OUT_ROWS, stride = (uint32_t)p.stride, qs = (uint32_t)p.q_stride;
+    const size_t at = ((size_t)t.expert * p.rows + r0) * p.stride;
+    const int8_t *w0 = p.w[0] + at, *w1 = p.w[1] + at, *q = UP ? p.q : p.q + (size_t)t.first * p.q_stride;
+    v4i acc[G::RF][G::TF];
+    i8_tile<G>([&](uint32_t o) { return UP && ((o >> 1) & 1u) ? w1 : w0; },
+               [&](uint32_t r) { return min(UP ? 16u * (r >> 5) + (r & 15u) : r, p.rows - 1u - r0) * stride; }, q,
+               [&](uint32_t j) { return (UP ? i8_pair_row<UP>(p, t, j) : min(j, t.n - 1u)) * qs; }, p.cols, acc);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+#pragma unroll
+    for (uint32_t j = 0; j < G::TF; j++) {
+        const uint32_t tok = (wt * G::TF + j) * 16u + (lane & 15u);
+        if (tok >= t.n) break;
+#pragma unroll
+        for (uint32_t i = 0; i < G::RF; i += UP ? 2u : 1u)
+            i8_pair_results<UP>(p, t, tok, r0 + (UP ? (wr * G::RF + i) * 8u : (wr * G::RF + i) * 16u) + 4u * (lane >> 4), acc[i][j],
+                                acc[UP ? i + 1u : i][j]);
+    }
+}
+
+/* G: as many pairs as a table entry can have; H: half of them, for the last ones of an expert's. */
+template <typename G, typename H, bool UP>
+__global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts p)
+{
+    /* those that there are, dealt to the XCDs evenly; which comes first does not matter */
+    const uint32_t all = min(p.tiles[0].all, p.n_tiles) * p.row_tiles;
+    if (blockIdx.x >= all) return;
+    const uint32_t i = i8_place(blockIdx.x, all), row_tile = i % p.row_tiles;
+    const I8ExpertTile t = p.tiles[i / p.row_tiles];
+    if (t.n <= H::TOK) i8_experts_tile<H, UP>(p, t, row_tile);
+    else i8_experts_tile<G, UP>(p, t, row_tile);
+}
+
+/* Up to sixteen pairs of an expert, as k_i8_few: `team` waves share a group of 16 rows; UP: half of them take gate, half up. */
+template <int ST, bool UP>
+__global__ __launch_bounds__(1024) void k_i8_experts_few(const I8Experts p, uint32_t team, uint32_t groups)
+{
+    __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_TURN_BYTES];
+    const I8ExpertTile t = p.tiles[blockIdx.y];
+    if (t.n == 0u) return;
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t teams = FEW_WAVES / team, parts = UP ? team / 2u : team, r16 = lane & 15u;
+    const uint32_t r0 = 16u * min(blockIdx.x * teams + wave / team, groups - 1u), which = wave % team / parts;
+    uint32_t first, mine;
+    few_part((p.cols + 127u) / 128u, wave % parts, parts, first, mine);
+    const int8_t *w[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; h++)
+        w[h] = p.w[which] + ((size_t)t.expert * p.rows + min(r0 + 8u * h + (lane >> 3), p.rows - 1u)) * p.stride;
+    few_sums<ST>(w, p.q + (size_t)i8_pair_row<UP>(p, t, r16) * p.q_stride, p.cols, first, mine, turns + 2048u * wave);
+    __syncthreads();
+    const uint32_t g = blockIdx.x * teams + wave;
+    if (wave < teams && g < groups && r16 < t.n) {
+        const v4i a = few_join(turns, wave * team, parts);
+        i8_pair_results<UP>(p, t, r16, 16u * g + 4u * (lane >> 4), a, UP ? few_join(turns, wave * team + parts, parts) : a);
     }
 }
 
@@ -700,6 +798,11 @@ typedef I8Geom<8, 4, 2, 4, 5> I8Large;        /* 256 x 256, a workgroup per CU *
 typedef I8Geom<4, 4, 2, 4, 5> I8Half;         /* 128 x 256, one */
 typedef I8Geom<2, 4, 4, 2, 5> I8Mid;          /* 128 x 128, two */
 typedef I8Geom<2, 2, 2, 2, 5> I8Small;        /* 64 x 64, four */
+
+typedef I8Geom<2, 4, 4, 2, 5> I8Mid128;     /* 128 rows x 128, 64 pairs */
+typedef I8Geom<2, 2, 4, 2, 5> I8Mid64;
+typedef I8Geom<2, 2, 2, 2, 5> I8Small64;    /* 64 rows x 64, 32 pairs */
+typedef I8Geom<2, 1, 2, 2, 5> I8Small32;
 
 /* How a product runs: on which tile, its columns in how many parts. */
 enum { I8_LARGE = 0, I8_HALF, I8_MID, I8_SMALL, I8_TILES };
@@ -858,6 +961,8 @@ extern "C" int oxh_internal_i8_init(void)
     if ((e = whole_lds(k_i8_tiles_tail<I8Large, I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, true>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, false>)) != hipSuccess) return (int)e;
     return (int)hipSuccess;
 }
 
@@ -954,9 +1059,24 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
 
 /* ─── experts ─────────────────────────────────────────────────────────── */
 
+/* Pairs of a table entry: by how many an expert gets on average. */
+static uint32_t experts_tok(size_t pairs, size_t n_expert)
+{
+    const size_t avg = pairs / n_expert;
+    return avg <= 10 ? FEW_TOKENS : avg <= 44 ? 64u : 128u;
+}
+
+/* The most tiles any routing can need: an expert's runs make at most one tile that is not full. */
+static size_t experts_tiles(size_t pairs, size_t n_expert, uint32_t tok)
+{
+    const size_t most = pairs / tok + n_expert;
+    return most < pairs ? most : pairs;
+}
+
 struct MoeI8Parts {
     size_t q_stride, h_stride, y_stride, qh_stride;    /* bytes, floats, floats, bytes */
-    size_t q, q_scale, h, qh, qh_scale, y, total;
+    size_t tiles, q, q_scale, h, qh, qh_scale, y, total;
+    uint32_t tok, n_tiles;
 };
 
 static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Parts *p)
@@ -973,8 +1093,12 @@ static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Part
     p->qh_stride = up64(m->ffn);
     p->h_stride = up64(m->ffn);
     p->y_stride = up64(m->hidden);
+    if (n_tok * p->q_stride > 0xFFFFFFFFull) return I8_ARG("%s: the tokens' codes exceed 4 GiB", who);
+    p->tok = experts_tok(pairs, m->n_expert);
+    p->n_tiles = (uint32_t)experts_tiles(pairs, m->n_expert, p->tok);
     size_t at = 0;
 #define OXH_PART(FIELD, BYTES) p->FIELD = at; at = up256(at + (BYTES))
+    OXH_PART(tiles, p->n_tiles * sizeof(I8ExpertTile));
     OXH_PART(q, n_tok * p->q_stride);
     OXH_PART(q_scale, n_tok * 4u);
     OXH_PART(h, pairs * p->h_stride * 4u);
@@ -984,6 +1108,48 @@ static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Part
 #undef OXH_PART
     p->total = at;
     return OXH_OK;
+}
+
+template <typename G, typename H, bool UP> static void experts_launch(I8Experts &e, hipStream_t st)
+{
+    const uint32_t out_rows = UP ? G::ROWS / 2u : G::ROWS;
+    e.row_tiles = (e.rows + out_rows - 1u) / out_rows;
+    hipLaunchKernelGGL((k_i8_experts<G, H, UP>), dim3(e.row_tiles * e.n_tiles), dim3(G::WAVES * 64u), G::LDS_BYTES, st, e);
+}
+
+/* the experts' kernel for few pairs: waves to a group of rows, as few_team() */
+template <bool UP> static void experts_few_launch(I8Experts &e, hipStream_t st)
+{
+    const uint32_t groups = (e.rows + 15u) / 16u, stages = (e.cols + 127u) / 128u, cus = (uint32_t)i8_cus();
+    uint32_t team = UP ? 2u : 1u;
+    while (team < FEW_WAVES && (stages * (UP ? 2u : 1u) > 4u * team || (size_t)groups * e.n_tiles * team < cus * FEW_WAVES)) team *= 2u;
+    const uint32_t teams = FEW_WAVES / team, parts = UP ? team / 2u : team, mine = (stages + parts - 1u) / parts;
+    const dim3 grid((groups + teams - 1u) / teams, e.n_tiles), block(64u * FEW_WAVES);
+    if (mine <= 2u) hipLaunchKernelGGL((k_i8_experts_few<2, UP>), grid, block, 0, st, e, team, groups);
+    else if (mine <= 4u) hipLaunchKernelGGL((k_i8_experts_few<4, UP>), grid, block, 0, st, e, team, groups);
+    else hipLaunchKernelGGL((k_i8_experts_few<8, UP>), grid, block, 0, st, e, team, groups);
+}
+
+template <bool UP> static void experts_run(I8Experts &e, uint32_t tok, hipStream_t st)
+{
+    const uint32_t stages = (e.cols + 127u) / 128u;
+    if (tok == FEW_TOKENS && stages <= FEW_MAX_STAGES * FEW_WAVES / (UP ? 2u : 1u)) experts_few_launch<UP>(e, st);
+    else if (tok <= 64u) experts_launch<I8Small64, I8Small32, UP>(e, st);
+    else experts_launch<I8Mid128, I8Mid64, UP>(e, st);
+}
+
+template <typename T>
+static void experts_begin(const void *x, size_t x_stride, size_t n_tok, size_t cols, int8_t *q, size_t q_stride, float *scale,
+                          const uint32_t *offsets, size_t n_expert, size_t pairs, uint32_t tok, I8ExpertTile *tiles, uint32_t n_tiles,
+                          hipStream_t st)
+{
+    const dim3 grid((uint32_t)n_tok + 1u);
+#define OXH_BEGIN(THREADS, HELD)                                                                                                 \
+    hipLaunchKernelGGL((k_i8_experts_begin<T, THREADS, HELD>), grid, dim3(THREADS), 0, st, (const T *)x, x_stride, (uint32_t)cols, q, \
+                       q_stride, scale, offsets, (uint32_t)n_expert, (uint32_t)pairs, tok, tiles, n_tiles)
+    if (cols <= 2048u) OXH_BEGIN(256, 1);
+    else OXH_BEGIN(1024, 2);
+#undef OXH_BEGIN
 }
 
 extern "C" int oxh_moe_i8_workspace_bytes(const OxhMoeI8 *m, size_t n_tok, size_t *bytes)
@@ -1020,13 +1186,19 @@ extern "C" int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint
     int8_t *q = (int8_t *)(ws + p.q), *qh = (int8_t *)(ws + p.qh);
     float *q_scale = (float *)(ws + p.q_scale), *qh_scale = (float *)(ws + p.qh_scale), *h = (float *)(ws + p.h), *y = (float *)(ws + p.y);
     const size_t pairs = n_tok * m->top_k;
-    if ((rc = quantize_launch(x_type, d_x, x_stride, n_tok, m->hidden, nullptr, q, p.q_stride, q_scale, st, who))) return rc;
-    hipLaunchKernelGGL(k_i8_experts_up, dim3((uint32_t)((m->ffn + 63u) / 64u), (uint32_t)m->n_expert), dim3(256), 0, st, *m, *routing,
-                       q, p.q_stride, q_scale, (uint32_t)n_tok, (uint32_t)pairs, h, p.h_stride);
+    I8ExpertTile *tiles = (I8ExpertTile *)(ws + p.tiles);
+    if (x_type == OXH_F32) experts_begin<float>(d_x, x_stride, n_tok, m->hidden, q, p.q_stride, q_scale, routing->d_offsets, m->n_expert, pairs, p.tok, tiles, p.n_tiles, st);
+    else if (x_type == OXH_F16) experts_begin<_Float16>(d_x, x_stride, n_tok, m->hidden, q, p.q_stride, q_scale, routing->d_offsets, m->n_expert, pairs, p.tok, tiles, p.n_tiles, st);
+    else experts_begin<__bf16>(d_x, x_stride, n_tok, m->hidden, q, p.q_stride, q_scale, routing->d_offsets, m->n_expert, pairs, p.tok, tiles, p.n_tiles, st);
+    if ((rc = launched(who))) return rc;
+    I8Experts up = { { m->d_w_gate, m->d_w_up }, { m->d_s_gate, m->d_s_up }, m->gate_up_stride, q, p.q_stride, q_scale, routing->d_perm, tiles,
+                     h, p.h_stride, (uint32_t)m->ffn, (uint32_t)m->hidden, (uint32_t)n_tok, p.n_tiles, 0u };
+    experts_run<true>(up, p.tok, st);
     if ((rc = launched(who))) return rc;
     if ((rc = quantize_launch(OXH_F32, h, p.h_stride, pairs, m->ffn, nullptr, qh, p.qh_stride, qh_scale, st, who))) return rc;
-    hipLaunchKernelGGL(k_i8_experts_down, dim3((uint32_t)((m->hidden + 63u) / 64u), (uint32_t)m->n_expert), dim3(256), 0, st, *m,
-                       *routing, qh, p.qh_stride, qh_scale, (uint32_t)pairs, y, p.y_stride);
+    I8Experts down = { { m->d_w_down, m->d_w_down }, { m->d_s_down, m->d_s_down }, m->down_stride, qh, p.qh_stride, qh_scale, routing->d_perm,
+                       tiles, y, p.y_stride, (uint32_t)m->hidden, (uint32_t)m->ffn, (uint32_t)n_tok, p.n_tiles, 0u };
+    experts_run<false>(down, p.tok, st);
     if ((rc = launched(who))) return rc;
 #define OXH_COMBINE(T)                                                                                                           \
     hipLaunchKernelGGL(k_i8_combine<T>, dim3((uint32_t)((m->hidden + 255u) / 256u), (uint32_t)n_tok), dim3(256), 0, st, y, p.y_stride, \
