@@ -263,23 +263,35 @@ template <typename G> __device__ __forceinline__ void i8_product_tile(const I8Pr
     const uint32_t ws = (uint32_t)p.w.stride, qs = (uint32_t)p.q_stride;
     const uint32_t stages = (cols + 127u) / 128u, first = split * stages / p.splits, end = (split + 1u) * stages / p.splits;
     const uint32_t k0 = 128u * first, kn = min(cols, 128u * end) - k0;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+    const uint32_t row = r0 + wr * G::RF * 16u + 4u * (lane >> 4), tok = t0 + wt * G::TF * 16u + (lane & 15u);
+    /* a wave's factors are asked for before the product, so that no result waits for one; the largest tile has no registers
+     * for that and asks for all of them at its end */
+    constexpr bool EARLY = G::RF * G::TF <= 16u;
+    float sw[G::RF][4], b[G::RF][4], st[G::TF];
+    auto factors = [&]() {
+        if (p.parts) return;
+#pragma unroll
+        for (uint32_t i = 0; i < G::RF; i++) i8_row_factors(p, row + 16u * i, sw[i], b[i]);
+#pragma unroll
+        for (uint32_t j = 0; j < G::TF; j++) st[j] = p.q_scale[min(tok + 16u * j, p.n_vec - 1u)];
+    };
+    if (EARLY) factors();
     v4i acc[G::RF][G::TF];
     const int8_t *w = p.w.d_w + (size_t)r0 * p.w.stride + k0;
     i8_tile<G>([&](uint32_t) { return w; }, [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; },
                p.q + (size_t)t0 * p.q_stride + k0, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, kn, acc);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+    if (!EARLY) factors();
 #pragma unroll
-    for (uint32_t i = 0; i < G::RF; i++) {
-        const uint32_t r = r0 + (wr * G::RF + i) * 16u + 4u * (lane >> 4);
-        if (r >= rows) break;
-        float sw[4], b[4];
-        if (!p.parts) i8_row_factors(p, r, sw, b);
+    for (uint32_t j = 0; j < G::TF; j++) {
+        const uint32_t t = tok + 16u * j;
+        if (t >= p.n_vec) break;
 #pragma unroll
-        for (uint32_t j = 0; j < G::TF; j++) {
-            const uint32_t t = t0 + (wt * G::TF + j) * 16u + (lane & 15u);
-            if (t >= p.n_vec) break;
+        for (uint32_t i = 0; i < G::RF; i++) {
+            const uint32_t r = row + 16u * i;
+            if (r >= rows) break;
             if (p.parts) *reinterpret_cast<v4i *>(p.parts + ((size_t)split * p.n_vec + t) * p.rows_pad + r) = acc[i][j];
-            else i8_results(p, r, t, acc[i][j], sw, b, p.q_scale[t]);
+            else i8_results(p, r, t, acc[i][j], sw[i], b[i], st[j]);
         }
     }
 }
@@ -417,7 +429,7 @@ __device__ __forceinline__ v4i few_join(const uint8_t *turns, uint32_t wave, uin
 
 /* quantised tokens */
 template <int ST>
-__global__ __launch_bounds__(1024) void k_i8_few(const I8Product p, uint32_t team, uint32_t groups)
+__global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_few(const I8Product p, uint32_t team, uint32_t groups)
 {
     __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_TURN_BYTES];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -428,14 +440,20 @@ __global__ __launch_bounds__(1024) void k_i8_few(const I8Product p, uint32_t tea
     const int8_t *w[2];
 #pragma unroll
     for (uint32_t h = 0; h < 2u; h++) w[h] = p.w.d_w + (size_t)min(r0 + 8u * h + (lane >> 3), rows - 1u) * p.w.stride;
-    few_sums<ST>(w, p.q + (size_t)min(r16, p.n_vec - 1u) * p.q_stride, cols, first, mine, turns + 2048u * wave);
-    __syncthreads();
+    /* what the results of this wave's rows need, if it is one that joins */
     const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * (lane >> 4);
-    if (wave < teams && g < groups && r < rows && r16 < p.n_vec) {
-        float sw[4], b[4];
-        i8_row_factors(p, r, sw, b);
-        i8_results(p, r, r16, few_join(turns, wave * team, team), sw, b, p.q_scale[r16]);
-    }
+    float sw[4], b[4];
+    float st;
+    auto factors = [&]() {
+        i8_row_factors(p, min(r, rows - 1u), sw, b);
+        st = p.q_scale[min(r16, p.n_vec - 1u)];
+    };
+    /* asked for early where a trip to memory is what the launch takes; late where the registers are wanted for weights */
+    if (ST <= 2) factors();
+    few_sums<ST>(w, p.q + (size_t)min(r16, p.n_vec - 1u) * p.q_stride, cols, first, mine, turns + 2048u * wave);
+    if (ST > 2) factors();
+    __syncthreads();
+    if (wave < teams && g < groups && r < rows && r16 < p.n_vec) i8_results(p, r, r16, few_join(turns, wave * team, team), sw, b, st);
 }
 
 /* Float tokens, which every workgroup quantises for itself (k_i8_quantize's codes): their values are requested before the weights
@@ -469,6 +487,9 @@ k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uin
     const int8_t *wrow[2];
 #pragma unroll
     for (uint32_t h = 0; h < 2u; h++) wrow[h] = p.w.d_w + (size_t)min(r0 + 8u * h + (lane >> 3), rows - 1u) * p.w.stride;
+    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * kq;
+    float sw[4], b[4];
+    if (ST <= 2) i8_row_factors(p, min(r, rows - 1u), sw, b);
     v4i w[ST][2];
     few_weights<ST>(w, wrow, first, stages, (cols - 1u) / 16u);
 
@@ -500,20 +521,17 @@ k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uin
             few_stage(acc, w[i], few_shared + 2048u * wave,
                       [&](uint32_t h) { return *reinterpret_cast<const v4i *>(mine_codes + 16u * n * (8u * (first + i) + 4u * h)); });
     *reinterpret_cast<v4i *>(few_shared + 2048u * wave + 16u * lane) = acc;
+    if (ST > 2) i8_row_factors(p, min(r, rows - 1u), sw, b);
     __syncthreads();
-    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * kq;
-    if (wave < teams && g < groups && r < rows && r16 < n) {
-        float sw[4], b[4];
-        i8_row_factors(p, r, sw, b);
-        i8_results(p, r, r16, few_join(few_shared, wave * team, team), sw, b, s_scale[r16]);
-    }
+    if (wave < teams && g < groups && r < rows && r16 < n) i8_results(p, r, r16, few_join(few_shared, wave * team, team), sw, b, s_scale[r16]);
 }
 
 /* ─── experts ─────────────────────────────────────────────────────────── */
 
-/* Up to a number of pairs of an expert: n of them from sorted pair `first` on; n 0: nothing.  all: tiles there are. */
+/* Up to a number of pairs of an expert: n of them from sorted pair `first` on; n 0: nothing.  The expert's tiles are `count` from
+ * entry `base` on; all: tiles there are. */
 struct I8ExpertTile {
-    uint32_t expert, first, n, all;
+    uint32_t expert, first, n, all, base, count, unused[2];
 };
 
 /* The first launch of a layer: a workgroup per token to quantise it, and one that cuts the experts' runs of the sorted pairs into tiles
@@ -557,7 +575,7 @@ k_i8_experts_begin(const T *__restrict__ x, size_t x_stride, uint32_t cols, int8
     }
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < n_tiles; i += THREADS) {
-        I8ExpertTile t = { 0u, 0u, 0u, s_tile[n_expert] };
+        I8ExpertTile t = { 0u, 0u, 0u, s_tile[n_expert], 0u, 0u, { 0u, 0u } };
         if (i < s_tile[n_expert]) {
             uint32_t lo = 0, hi = n_expert;         /* the last expert whose tiles start at i or before */
             while (hi - lo > 1u) {
@@ -568,6 +586,8 @@ k_i8_experts_begin(const T *__restrict__ x, size_t x_stride, uint32_t cols, int8
             t.expert = lo;
             t.first = s_first[lo] + tok * (i - s_tile[lo]);
             t.n = min(tok, s_first[lo + 1u] - t.first);
+            t.base = s_tile[lo];
+            t.count = s_tile[lo + 1u] - t.base;
         }
         tiles[i] = t;
     }
@@ -596,19 +616,29 @@ template <bool UP> __device__ __forceinline__ uint32_t i8_pair_row(const I8Exper
     return UP ? min(p.perm[pair], p.n_tok - 1u) : pair;
 }
 
-/* Four rows' results of a pair from its sums. */
-template <bool UP>
-__device__ __forceinline__ void i8_pair_results(const I8Experts &p, const I8ExpertTile &t, uint32_t j, uint32_t r, const v4i &first, const v4i &second)
+/* The scales of four rows of the expert (UP: of gate's and of up's). */
+template <bool UP> __device__ __forceinline__ void i8_pair_scales(const I8Experts &p, const I8ExpertTile &t, uint32_t r, float (&s0)[4], float (&s1)[4])
 {
-    if (r >= p.rows) return;
     const size_t row0 = (size_t)t.expert * p.rows;
-    const float st = p.q_scale[i8_pair_row<UP>(p, t, j)];
-    float v[4];
 #pragma unroll
     for (uint32_t k = 0; k < 4u; k++) {
         const uint32_t rk = min(r + k, p.rows - 1u);
-        v[k] = (float)first[k] * st * p.s[0][row0 + rk];
-        if (UP) v[k] = silu(v[k]) * ((float)second[k] * st * p.s[1][row0 + rk]);
+        s0[k] = p.s[0][row0 + rk];
+        s1[k] = UP ? p.s[1][row0 + rk] : 0.0f;
+    }
+}
+
+/* Four rows' results of a pair from its sums. */
+template <bool UP>
+__device__ __forceinline__ void i8_pair_results(const I8Experts &p, const I8ExpertTile &t, uint32_t j, uint32_t r, const v4i &first, const v4i &second,
+                                                const float (&s0)[4], const float (&s1)[4], float st)
+{
+    if (r >= p.rows) return;
+    float v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        v[k] = (float)first[k] * st * s0[k];
+        if (UP) v[k] = silu(v[k]) * ((float)second[k] * st * s1[k]);
     }
     i8_store4(p.out + (size_t)(t.first + j) * p.out_stride + r, v, p.rows - r);
 }
@@ -621,19 +651,24 @@ template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(c
     const uint32_t r0 = row_tile * OUT_ROWS, stride = (uint32_t)p.stride, qs = (uint32_t)p.q_stride;
     const size_t at = ((size_t)t.expert * p.rows + r0) * p.stride;
     const int8_t *w0 = p.w[0] + at, *w1 = p.w[1] + at, *q = UP ? p.q : p.q + (size_t)t.first * p.q_stride;
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+    constexpr uint32_t PER = UP ? G::RF / 2u : G::RF;               /* results' fragments of a wave */
+    const uint32_t row = r0 + wr * PER * 16u + 4u * (lane >> 4), tok = wt * G::TF * 16u + (lane & 15u);
+    float s0[PER][4], s1[PER][4], st[G::TF];
+#pragma unroll
+    for (uint32_t i = 0; i < PER; i++) i8_pair_scales<UP>(p, t, row + 16u * i, s0[i], s1[i]);
+#pragma unroll
+    for (uint32_t j = 0; j < G::TF; j++) st[j] = p.q_scale[i8_pair_row<UP>(p, t, tok + 16u * j)];
     v4i acc[G::RF][G::TF];
     i8_tile<G>([&](uint32_t o) { return UP && ((o >> 1) & 1u) ? w1 : w0; },
                [&](uint32_t r) { return min(UP ? 16u * (r >> 5) + (r & 15u) : r, p.rows - 1u - r0) * stride; }, q,
                [&](uint32_t j) { return (UP ? i8_pair_row<UP>(p, t, j) : min(j, t.n - 1u)) * qs; }, p.cols, acc);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
 #pragma unroll
     for (uint32_t j = 0; j < G::TF; j++) {
-        const uint32_t tok = (wt * G::TF + j) * 16u + (lane & 15u);
-        if (tok >= t.n) break;
+        if (tok + 16u * j >= t.n) break;
 #pragma unroll
-        for (uint32_t i = 0; i < G::RF; i += UP ? 2u : 1u)
-            i8_pair_results<UP>(p, t, tok, r0 + (UP ? (wr * G::RF + i) * 8u : (wr * G::RF + i) * 16u) + 4u * (lane >> 4), acc[i][j],
-                                acc[UP ? i + 1u : i][j]);
+        for (uint32_t i = 0; i < PER; i++)
+            i8_pair_results<UP>(p, t, tok + 16u * j, row + 16u * i, acc[UP ? 2u * i : i][j], acc[UP ? 2u * i + 1u : i][j], s0[i], s1[i], st[j]);
     }
 }
 
@@ -641,18 +676,20 @@ template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(c
 template <typename G, typename H, bool UP>
 __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts p)
 {
-    /* those that there are, dealt to the XCDs evenly; which comes first does not matter */
+    /* those that there are, dealt to the XCDs evenly; the tiles of an expert that share weights next to each other */
     const uint32_t all = min(p.tiles[0].all, p.n_tiles) * p.row_tiles;
     if (blockIdx.x >= all) return;
-    const uint32_t i = i8_place(blockIdx.x, all), row_tile = i % p.row_tiles;
-    const I8ExpertTile t = p.tiles[i / p.row_tiles];
+    const uint32_t i = i8_place(blockIdx.x, all);
+    const I8ExpertTile any = p.tiles[i / p.row_tiles];
+    const uint32_t in = i - any.base * p.row_tiles, row_tile = in / any.count;
+    const I8ExpertTile t = p.tiles[any.base + in % any.count];
     if (t.n <= H::TOK) i8_experts_tile<H, UP>(p, t, row_tile);
     else i8_experts_tile<G, UP>(p, t, row_tile);
 }
 
 /* Up to sixteen pairs of an expert, as k_i8_few: `team` waves share a group of 16 rows; UP: half of them take gate, half up. */
 template <int ST, bool UP>
-__global__ __launch_bounds__(1024) void k_i8_experts_few(const I8Experts p, uint32_t team, uint32_t groups)
+__global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const I8Experts p, uint32_t team, uint32_t groups)
 {
     __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_TURN_BYTES];
     const I8ExpertTile t = p.tiles[blockIdx.y];
@@ -666,12 +703,19 @@ __global__ __launch_bounds__(1024) void k_i8_experts_few(const I8Experts p, uint
 #pragma unroll
     for (uint32_t h = 0; h < 2u; h++)
         w[h] = p.w[which] + ((size_t)t.expert * p.rows + min(r0 + 8u * h + (lane >> 3), p.rows - 1u)) * p.stride;
-    few_sums<ST>(w, p.q + (size_t)i8_pair_row<UP>(p, t, r16) * p.q_stride, p.cols, first, mine, turns + 2048u * wave);
+    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * (lane >> 4), q_row = i8_pair_row<UP>(p, t, r16);
+    float s0[4], s1[4], st;
+    auto factors = [&]() {
+        i8_pair_scales<UP>(p, t, min(r, p.rows - 1u), s0, s1);
+        st = p.q_scale[q_row];
+    };
+    if (ST <= 2) factors();
+    few_sums<ST>(w, p.q + (size_t)q_row * p.q_stride, p.cols, first, mine, turns + 2048u * wave);
+    if (ST > 2) factors();
     __syncthreads();
-    const uint32_t g = blockIdx.x * teams + wave;
     if (wave < teams && g < groups && r16 < t.n) {
         const v4i a = few_join(turns, wave * team, parts);
-        i8_pair_results<UP>(p, t, r16, 16u * g + 4u * (lane >> 4), a, UP ? few_join(turns, wave * team + parts, parts) : a);
+        i8_pair_results<UP>(p, t, r16, r, a, UP ? few_join(turns, wave * team + parts, parts) : a, s0, s1, st);
     }
 }
 
