@@ -10,6 +10,8 @@
 
 #pragma clang fp contract(off)
 
+typedef float v4f __attribute__((ext_vector_type(4)));
+
 /* ─── floats ──────────────────────────────────────────────────────────── */
 
 template <typename T> __device__ __forceinline__ float to_f32(T v) { return (float)v; }
@@ -217,6 +219,49 @@ __device__ __forceinline__ void i8_tile_at(uint32_t i, uint32_t row_tiles, uint3
     tok = in / high;
 }
 
+/* A tile's results to memory.  A wave holds four rows of each of sixteen tokens, 64 or 32 bytes of an output row at a time;
+ * stored like that a launch writes 2.8 TB/s (131 MB in 47 us; a fill of them takes 22).  So the workgroup's results are gathered in
+ * its LDS, token by token, and written 16 bytes to a lane along the rows.
+ *
+ * PER: a wave's fragments of 16 rows; value(i, j): its four results of fragment i, tokens j, as T.  out: the tile's first
+ * token and row; rows, toks: how many of them there are.  T's of four bytes may be ints as well. */
+template <typename G, typename T, uint32_t PER, typename Value>
+__device__ __forceinline__ void i8_store_tile(Value value, T *out, size_t out_stride, uint32_t rows, uint32_t toks)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
+    constexpr uint32_t ROWS = 16u * PER * G::WR, ROW_BYTES = ROWS * sizeof(T), PITCH = ROW_BYTES + 16u, THREADS = 64u * G::WAVES;
+    constexpr uint32_t JC = G::TF * 16u * G::WT * PITCH <= G::LDS_BYTES ? G::TF : G::TF / 2u;       /* of a wave's tokens at a time */
+    static_assert(JC * 16u * G::WT * PITCH <= G::LDS_BYTES, "half of the tokens fit");
+    constexpr uint32_t CHUNKS = ROW_BYTES / 16u, STEP = 16u / sizeof(T);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+#pragma unroll
+    for (uint32_t j0 = 0; j0 < G::TF; j0 += JC) {
+        __syncthreads();                            /* operands, or the tokens before, are read */
+#pragma unroll
+        for (uint32_t j = j0; j < j0 + JC; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < PER; i++) {
+                const Run<T, 4> r = value(i, j);
+                uint8_t *to = i8_lds + (16u * (wt * JC + j - j0) + (lane & 15u)) * PITCH + (16u * (wr * PER + i) + 4u * (lane >> 4)) * sizeof(T);
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<T4 *>(to) = T4{ r.v[0], r.v[1], r.v[2], r.v[3] };
+            }
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t f = threadIdx.x; f < 16u * G::WT * JC * CHUNKS; f += THREADS) {
+            const uint32_t at = f / CHUNKS, c = f % CHUNKS, tok = 16u * (at / (16u * JC) * G::TF + j0) + at % (16u * JC), r = c * STEP;
+            if (tok >= toks || r >= rows) continue;
+            const Run<T, STEP> v = *reinterpret_cast<const Run<T, STEP> *>(i8_lds + at * PITCH + 16u * c);
+            T *to = out + (size_t)tok * out_stride + r;
+            if (r + STEP <= rows) *reinterpret_cast<Run<T, STEP> *>(to) = v;
+            else
+#pragma unroll
+                for (uint32_t k = 0; k < STEP - 1u; k++)
+                    if (r + k < rows) to[k] = v.v[k];
+        }
+    }
+}
+
 /* What the product's kernels take: the matrix, quantised tokens, and where the results go. */
 struct I8Product {
     OxhI8Matrix w;
@@ -282,18 +327,31 @@ template <typename G> __device__ __forceinline__ void i8_product_tile(const I8Pr
     i8_tile<G>([&](uint32_t) { return w; }, [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; },
                p.q + (size_t)t0 * p.q_stride + k0, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, kn, acc);
     if (!EARLY) factors();
-#pragma unroll
-    for (uint32_t j = 0; j < G::TF; j++) {
-        const uint32_t t = tok + 16u * j;
-        if (t >= p.n_vec) break;
-#pragma unroll
-        for (uint32_t i = 0; i < G::RF; i++) {
-            const uint32_t r = row + 16u * i;
-            if (r >= rows) break;
-            if (p.parts) *reinterpret_cast<v4i *>(p.parts + ((size_t)split * p.n_vec + t) * p.rows_pad + r) = acc[i][j];
-            else i8_results(p, r, t, acc[i][j], sw[i], b[i], st[j]);
-        }
+    const uint32_t rows_here = rows - r0, toks_here = p.n_vec - t0;
+    if (p.parts) {
+        i8_store_tile<G, int, G::RF>([&](uint32_t i, uint32_t j) { return __builtin_bit_cast(Run<int, 4>, acc[i][j]); },
+                                     p.parts + ((size_t)split * p.n_vec + t0) * p.rows_pad + r0, p.rows_pad, rows_here, toks_here);
+        return;
     }
+    auto value = [&](uint32_t i, uint32_t j, auto of) {
+        Run<decltype(of), 4> r;
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) {
+            float v = (float)acc[i][j][k] * st[j] * sw[i][k];
+            if (p.bias) v += b[i][k];
+            r.v[k] = from_f32<decltype(of)>(v);
+        }
+        return r;
+    };
+    const size_t at = (size_t)t0 * p.out_stride + r0;
+    if (p.out_type == OXH_F32)
+        i8_store_tile<G, float, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, 0.0f); }, (float *)p.out + at, p.out_stride, rows_here, toks_here);
+    else if (p.out_type == OXH_F16)
+        i8_store_tile<G, _Float16, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, (_Float16)0.0f); }, (_Float16 *)p.out + at, p.out_stride,
+                                          rows_here, toks_here);
+    else
+        i8_store_tile<G, __bf16, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, (__bf16)0.0f); }, (__bf16 *)p.out + at, p.out_stride,
+                                        rows_here, toks_here);
 }
 
 template <typename G>
@@ -628,19 +686,24 @@ template <bool UP> __device__ __forceinline__ void i8_pair_scales(const I8Expert
     }
 }
 
+/* silu with the hardware's exponential and reciprocal, a unit in the last place each: expf and a division are a third of the vector
+ * instructions of a layer's first product */
+__device__ __forceinline__ float silu_fast(float g)
+{
+    return g * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(g * -1.44269504f));
+}
+
 /* Four rows' results of a pair from its sums. */
 template <bool UP>
-__device__ __forceinline__ void i8_pair_results(const I8Experts &p, const I8ExpertTile &t, uint32_t j, uint32_t r, const v4i &first, const v4i &second,
-                                                const float (&s0)[4], const float (&s1)[4], float st)
+__device__ __forceinline__ Run<float, 4> i8_pair_values(const v4i &first, const v4i &second, const float (&s0)[4], const float (&s1)[4], float st)
 {
-    if (r >= p.rows) return;
-    float v[4];
+    Run<float, 4> r;
 #pragma unroll
     for (uint32_t k = 0; k < 4u; k++) {
-        v[k] = (float)first[k] * st * s0[k];
-        if (UP) v[k] = silu(v[k]) * ((float)second[k] * st * s1[k]);
+        r.v[k] = (float)first[k] * st * s0[k];
+        if (UP) r.v[k] = silu_fast(r.v[k]) * ((float)second[k] * st * s1[k]);
     }
-    i8_store4(p.out + (size_t)(t.first + j) * p.out_stride + r, v, p.rows - r);
+    return r;
 }
 
 /* A tile of an expert's rows and pairs.  UP: the tile's fragments of 16 rows are gate's and up's by turns, so that a wave holds
@@ -663,17 +726,15 @@ template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(c
     i8_tile<G>([&](uint32_t o) { return UP && ((o >> 1) & 1u) ? w1 : w0; },
                [&](uint32_t r) { return min(UP ? 16u * (r >> 5) + (r & 15u) : r, p.rows - 1u - r0) * stride; }, q,
                [&](uint32_t j) { return (UP ? i8_pair_row<UP>(p, t, j) : min(j, t.n - 1u)) * qs; }, p.cols, acc);
-#pragma unroll
-    for (uint32_t j = 0; j < G::TF; j++) {
-        if (tok + 16u * j >= t.n) break;
-#pragma unroll
-        for (uint32_t i = 0; i < PER; i++)
-            i8_pair_results<UP>(p, t, tok + 16u * j, row + 16u * i, acc[UP ? 2u * i : i][j], acc[UP ? 2u * i + 1u : i][j], s0[i], s1[i], st[j]);
-    }
+    i8_store_tile<G, float, PER>(
+        [&](uint32_t i, uint32_t j) {
+            return i8_pair_values<UP>(acc[UP ? 2u * i : i][j], acc[UP ? 2u * i + 1u : i][j], s0[i], s1[i], st[j]);
+        },
+        p.out + (size_t)t.first * p.out_stride + r0, p.out_stride, p.rows - r0, t.n);
 }
 
-/* G: as many pairs as a table entry can have; H: half of them, for the last ones of an expert's. */
-template <typename G, typename H, bool UP>
+/* G: as many pairs as a table entry can have; H, Q: fewer, for the last ones of an expert's. */
+template <typename G, typename H, typename Q, bool UP>
 __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts p)
 {
     /* those that there are, dealt to the XCDs evenly; the tiles of an expert that share weights next to each other */
@@ -683,7 +744,8 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts
     const I8ExpertTile any = p.tiles[i / p.row_tiles];
     const uint32_t in = i - any.base * p.row_tiles, row_tile = in / any.count;
     const I8ExpertTile t = p.tiles[any.base + in % any.count];
-    if (t.n <= H::TOK) i8_experts_tile<H, UP>(p, t, row_tile);
+    if (Q::TOK < H::TOK && t.n <= Q::TOK) i8_experts_tile<Q, UP>(p, t, row_tile);
+    else if (t.n <= H::TOK) i8_experts_tile<H, UP>(p, t, row_tile);
     else i8_experts_tile<G, UP>(p, t, row_tile);
 }
 
@@ -713,24 +775,39 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const 
     few_sums<ST>(w, p.q + (size_t)q_row * p.q_stride, p.cols, first, mine, turns + 2048u * wave);
     if (ST > 2) factors();
     __syncthreads();
-    if (wave < teams && g < groups && r16 < t.n) {
+    if (wave < teams && g < groups && r16 < t.n && r < p.rows) {
         const v4i a = few_join(turns, wave * team, parts);
-        i8_pair_results<UP>(p, t, r16, r, a, UP ? few_join(turns, wave * team + parts, parts) : a, s0, s1, st);
+        const Run<float, 4> v = i8_pair_values<UP>(a, UP ? few_join(turns, wave * team + parts, parts) : a, s0, s1, st);
+        i8_store4(p.out + (size_t)(t.first + r16) * p.out_stride + r, v.v, p.rows - r);
     }
 }
 
-/* out[t] = sum over t's pairs, in their order, of weight * y */
+/* out[t] = sum over t's pairs, in their order, of weight * y.  Four columns to a thread, eight of the token's pairs under way at a time. */
 template <typename T>
 __global__ __launch_bounds__(256) void
 k_i8_combine(const float *__restrict__ y, size_t y_stride, const float *__restrict__ weights, const uint32_t *__restrict__ slot_pos,
              uint32_t k, uint32_t pairs, uint32_t cols, T *__restrict__ out, size_t out_stride)
 {
     const size_t t = blockIdx.y;
-    const uint32_t c = blockIdx.x * 256u + threadIdx.x;
+    const uint32_t c = 4u * (blockIdx.x * 256u + threadIdx.x);
     if (c >= cols) return;
-    float acc = 0.0f;
-    for (uint32_t j = 0; j < k; j++) acc += weights[t * k + j] * y[(size_t)min(slot_pos[t * k + j], pairs - 1u) * y_stride + c];
-    out[t * out_stride + c] = from_f32<T>(acc);
+    float acc[4] = { 0.0f, 0.0f, 0.0f, 0.0f };
+    for (uint32_t j0 = 0; j0 < k; j0 += 8u) {
+        v4f v[8];
+        float w[8];
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j++) {                         /* past the end: the last pair again */
+            const size_t pair = t * k + min(j0 + j, k - 1u);
+            w[j] = weights[pair];
+            v[j] = *reinterpret_cast<const v4f *>(y + (size_t)min(slot_pos[pair], pairs - 1u) * y_stride + c);
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8u; j++)
+            if (j0 + j < k)
+#pragma unroll
+                for (int i = 0; i < 4; i++) acc[i] += w[j] * v[j][i];
+    }
+    i8_store4(out + t * out_stride + c, acc, cols - c);
 }
 
 /* ─── host side ───────────────────────────────────────────────────────── */
@@ -794,6 +871,7 @@ static int quantize_launch(uint32_t type, const void *x, size_t x_stride, size_t
 #define OXH_QUANT_S(T, GLU)                                                                                                      \
     do {                                                                                                                         \
         if (cols <= 512u) OXH_QUANT_K(T, GLU, 64, 1);                                                                            \
+        else if (cols <= 1024u) OXH_QUANT_K(T, GLU, 64, 2);                                                                      \
         else if (cols <= 2048u) OXH_QUANT_K(T, GLU, 256, 1);                                                                     \
         else if (cols <= 8192u && n >= 512u) OXH_QUANT_K(T, GLU, 256, 4);                                                        \
         else OXH_QUANT_K(T, GLU, 1024, 2);                                                                                       \
@@ -843,8 +921,9 @@ typedef I8Geom<4, 4, 2, 4, 5> I8Half;         /* 128 x 256, one */
 typedef I8Geom<2, 4, 4, 2, 5> I8Mid;          /* 128 x 128, two */
 typedef I8Geom<2, 2, 2, 2, 5> I8Small;        /* 64 x 64, four */
 
-typedef I8Geom<2, 4, 4, 2, 5> I8Mid128;     /* 128 rows x 128, 64 pairs */
+typedef I8Geom<2, 4, 4, 2, 5> I8Mid128;     /* 128 rows x 128, 64, 32 pairs */
 typedef I8Geom<2, 2, 4, 2, 5> I8Mid64;
+typedef I8Geom<2, 1, 4, 2, 5> I8Mid32;
 typedef I8Geom<2, 2, 2, 2, 5> I8Small64;    /* 64 rows x 64, 32 pairs */
 typedef I8Geom<2, 1, 2, 2, 5> I8Small32;
 
@@ -1005,8 +1084,8 @@ extern "C" int oxh_internal_i8_init(void)
     if ((e = whole_lds(k_i8_tiles_tail<I8Large, I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, true>)) != hipSuccess) return (int)e;
-    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, false>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, true>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, false>)) != hipSuccess) return (int)e;
     return (int)hipSuccess;
 }
 
@@ -1154,11 +1233,11 @@ static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Part
     return OXH_OK;
 }
 
-template <typename G, typename H, bool UP> static void experts_launch(I8Experts &e, hipStream_t st)
+template <typename G, typename H, typename Q, bool UP> static void experts_launch(I8Experts &e, hipStream_t st)
 {
     const uint32_t out_rows = UP ? G::ROWS / 2u : G::ROWS;
     e.row_tiles = (e.rows + out_rows - 1u) / out_rows;
-    hipLaunchKernelGGL((k_i8_experts<G, H, UP>), dim3(e.row_tiles * e.n_tiles), dim3(G::WAVES * 64u), G::LDS_BYTES, st, e);
+    hipLaunchKernelGGL((k_i8_experts<G, H, Q, UP>), dim3(e.row_tiles * e.n_tiles), dim3(G::WAVES * 64u), G::LDS_BYTES, st, e);
 }
 
 /* the experts' kernel for few pairs: waves to a group of rows, as few_team() */
@@ -1178,8 +1257,8 @@ template <bool UP> static void experts_run(I8Experts &e, uint32_t tok, hipStream
 {
     const uint32_t stages = (e.cols + 127u) / 128u;
     if (tok == FEW_TOKENS && stages <= FEW_MAX_STAGES * FEW_WAVES / (UP ? 2u : 1u)) experts_few_launch<UP>(e, st);
-    else if (tok <= 64u) experts_launch<I8Small64, I8Small32, UP>(e, st);
-    else experts_launch<I8Mid128, I8Mid64, UP>(e, st);
+    else if (tok <= 64u) experts_launch<I8Small64, I8Small32, I8Small32, UP>(e, st);
+    else experts_launch<I8Mid128, I8Mid64, I8Mid32, UP>(e, st);
 }
 
 template <typename T>
@@ -1245,7 +1324,7 @@ extern "C" int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint
     experts_run<false>(down, p.tok, st);
     if ((rc = launched(who))) return rc;
 #define OXH_COMBINE(T)                                                                                                           \
-    hipLaunchKernelGGL(k_i8_combine<T>, dim3((uint32_t)((m->hidden + 255u) / 256u), (uint32_t)n_tok), dim3(256), 0, st, y, p.y_stride, \
+    hipLaunchKernelGGL(k_i8_combine<T>, dim3((uint32_t)((m->hidden + 1023u) / 1024u), (uint32_t)n_tok), dim3(256), 0, st, y, p.y_stride, \
                        routing->d_weights, routing->d_slot_pos, (uint32_t)m->top_k, (uint32_t)pairs, (uint32_t)m->hidden,        \
                        (T *)d_out, out_stride)
     if (out_type == OXH_F32) OXH_COMBINE(float);
