@@ -219,49 +219,6 @@ __device__ __forceinline__ void i8_tile_at(uint32_t i, uint32_t row_tiles, uint3
     tok = in / high;
 }
 
-/* A tile's results to memory.  A wave holds four rows of each of sixteen tokens, 64 or 32 bytes of an output row at a time;
- * stored like that a launch writes 2.8 TB/s (131 MB in 47 us; a fill of them takes 22).  So the workgroup's results are gathered in
- * its LDS, token by token, and written 16 bytes to a lane along the rows.
- *
- * PER: a wave's fragments of 16 rows; value(i, j): its four results of fragment i, tokens j, as T.  out: the tile's first
- * token and row; rows, toks: how many of them there are.  T's of four bytes may be ints as well. */
-template <typename G, typename T, uint32_t PER, typename Value>
-__device__ __forceinline__ void i8_store_tile(Value value, T *out, size_t out_stride, uint32_t rows, uint32_t toks)
-{
-    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
-    constexpr uint32_t ROWS = 16u * PER * G::WR, ROW_BYTES = ROWS * sizeof(T), PITCH = ROW_BYTES + 16u, THREADS = 64u * G::WAVES;
-    constexpr uint32_t JC = G::TF * 16u * G::WT * PITCH <= G::LDS_BYTES ? G::TF : G::TF / 2u;       /* of a wave's tokens at a time */
-    static_assert(JC * 16u * G::WT * PITCH <= G::LDS_BYTES, "half of the tokens fit");
-    constexpr uint32_t CHUNKS = ROW_BYTES / 16u, STEP = 16u / sizeof(T);
-    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
-#pragma unroll
-    for (uint32_t j0 = 0; j0 < G::TF; j0 += JC) {
-        __syncthreads();                            /* operands, or the tokens before, are read */
-#pragma unroll
-        for (uint32_t j = j0; j < j0 + JC; j++)
-#pragma unroll
-            for (uint32_t i = 0; i < PER; i++) {
-                const Run<T, 4> r = value(i, j);
-                uint8_t *to = i8_lds + (16u * (wt * JC + j - j0) + (lane & 15u)) * PITCH + (16u * (wr * PER + i) + 4u * (lane >> 4)) * sizeof(T);
-                typedef T T4 __attribute__((ext_vector_type(4)));
-                *reinterpret_cast<T4 *>(to) = T4{ r.v[0], r.v[1], r.v[2], r.v[3] };
-            }
-        __syncthreads();
-#pragma unroll 4
-        for (uint32_t f = threadIdx.x; f < 16u * G::WT * JC * CHUNKS; f += THREADS) {
-            const uint32_t at = f / CHUNKS, c = f % CHUNKS, tok = 16u * (at / (16u * JC) * G::TF + j0) + at % (16u * JC), r = c * STEP;
-            if (tok >= toks || r >= rows) continue;
-            const Run<T, STEP> v = *reinterpret_cast<const Run<T, STEP> *>(i8_lds + at * PITCH + 16u * c);
-            T *to = out + (size_t)tok * out_stride + r;
-            if (r + STEP <= rows) *reinterpret_cast<Run<T, STEP> *>(to) = v;
-            else
-#pragma unroll
-                for (uint32_t k = 0; k < STEP - 1u; k++)
-                    if (r + k < rows) to[k] = v.v[k];
-        }
-    }
-}
-
 /* What the product's kernels take: the matrix, quantised tokens, and where the results go. */
 struct I8Product {
     OxhI8Matrix w;
@@ -327,31 +284,18 @@ template <typename G> __device__ __forceinline__ void i8_product_tile(const I8Pr
     i8_tile<G>([&](uint32_t) { return w; }, [&](uint32_t r) { return min(r, rows - 1u - r0) * ws; },
                p.q + (size_t)t0 * p.q_stride + k0, [&](uint32_t t) { return min(t, p.n_vec - 1u - t0) * qs; }, kn, acc);
     if (!EARLY) factors();
-    const uint32_t rows_here = rows - r0, toks_here = p.n_vec - t0;
-    if (p.parts) {
-        i8_store_tile<G, int, G::RF>([&](uint32_t i, uint32_t j) { return __builtin_bit_cast(Run<int, 4>, acc[i][j]); },
-                                     p.parts + ((size_t)split * p.n_vec + t0) * p.rows_pad + r0, p.rows_pad, rows_here, toks_here);
-        return;
-    }
-    auto value = [&](uint32_t i, uint32_t j, auto of) {
-        Run<decltype(of), 4> r;
 #pragma unroll
-        for (uint32_t k = 0; k < 4u; k++) {
-            float v = (float)acc[i][j][k] * st[j] * sw[i][k];
-            if (p.bias) v += b[i][k];
-            r.v[k] = from_f32<decltype(of)>(v);
+    for (uint32_t j = 0; j < G::TF; j++) {
+        const uint32_t t = tok + 16u * j;
+        if (t >= p.n_vec) break;
+#pragma unroll
+        for (uint32_t i = 0; i < G::RF; i++) {
+            const uint32_t r = row + 16u * i;
+            if (r >= rows) break;
+            if (p.parts) *reinterpret_cast<v4i *>(p.parts + ((size_t)split * p.n_vec + t) * p.rows_pad + r) = acc[i][j];
+            else i8_results(p, r, t, acc[i][j], sw[i], b[i], st[j]);
         }
-        return r;
-    };
-    const size_t at = (size_t)t0 * p.out_stride + r0;
-    if (p.out_type == OXH_F32)
-        i8_store_tile<G, float, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, 0.0f); }, (float *)p.out + at, p.out_stride, rows_here, toks_here);
-    else if (p.out_type == OXH_F16)
-        i8_store_tile<G, _Float16, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, (_Float16)0.0f); }, (_Float16 *)p.out + at, p.out_stride,
-                                          rows_here, toks_here);
-    else
-        i8_store_tile<G, __bf16, G::RF>([&](uint32_t i, uint32_t j) { return value(i, j, (__bf16)0.0f); }, (__bf16 *)p.out + at, p.out_stride,
-                                        rows_here, toks_here);
+    }
 }
 
 template <typename G>
@@ -704,6 +648,50 @@ __device__ __forceinline__ Run<float, 4> i8_pair_values(const v4i &first, const 
         if (UP) r.v[k] = silu_fast(r.v[k]) * ((float)second[k] * st * s1[k]);
     }
     return r;
+}
+
+/* A tile's results to memory, for products of few columns, which are half stores.  A wave holds four rows of each of sixteen tokens,
+ * 64 bytes of an output row at a time; stored like that a launch writes 2.8 TB/s (131 MB beside the products of 768 columns: 47 us
+ * more; a fill of them takes 22).  So the workgroup's results are gathered in its LDS, token by token, and written 16 bytes
+ * to a lane along the rows (30 us).  Long products (i8_product_tile) are 3 % faster without the two barriers this takes.
+ *
+ * PER: a wave's fragments of 16 rows; value(i, j): its four results of fragment i, tokens j, as T.  out: the tile's first
+ * token and row; rows, toks: how many of them there are.  T's of four bytes may be ints as well. */
+template <typename G, typename T, uint32_t PER, typename Value>
+__device__ __forceinline__ void i8_store_tile(Value value, T *out, size_t out_stride, uint32_t rows, uint32_t toks)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t i8_lds[];
+    constexpr uint32_t ROWS = 16u * PER * G::WR, ROW_BYTES = ROWS * sizeof(T), PITCH = ROW_BYTES + 16u, THREADS = 64u * G::WAVES;
+    constexpr uint32_t JC = G::TF * 16u * G::WT * PITCH <= G::LDS_BYTES ? G::TF : G::TF / 2u;       /* of a wave's tokens at a time */
+    static_assert(JC * 16u * G::WT * PITCH <= G::LDS_BYTES, "half of the tokens fit");
+    constexpr uint32_t CHUNKS = ROW_BYTES / 16u, STEP = 16u / sizeof(T);
+    const uint32_t lane = threadIdx.x & 63u, wave = threadIdx.x >> 6, wr = wave / G::WT, wt = wave % G::WT;
+#pragma unroll
+    for (uint32_t j0 = 0; j0 < G::TF; j0 += JC) {
+        __syncthreads();                            /* operands, or the tokens before, are read */
+#pragma unroll
+        for (uint32_t j = j0; j < j0 + JC; j++)
+#pragma unroll
+            for (uint32_t i = 0; i < PER; i++) {
+                const Run<T, 4> r = value(i, j);
+                uint8_t *to = i8_lds + (16u * (wt * JC + j - j0) + (lane & 15u)) * PITCH + (16u * (wr * PER + i) + 4u * (lane >> 4)) * sizeof(T);
+                typedef T T4 __attribute__((ext_vector_type(4)));
+                *reinterpret_cast<T4 *>(to) = T4{ r.v[0], r.v[1], r.v[2], r.v[3] };
+            }
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t f = threadIdx.x; f < 16u * G::WT * JC * CHUNKS; f += THREADS) {
+            const uint32_t at = f / CHUNKS, c = f % CHUNKS, tok = 16u * (at / (16u * JC) * G::TF + j0) + at % (16u * JC), r = c * STEP;
+            if (tok >= toks || r >= rows) continue;
+            const Run<T, STEP> v = *reinterpret_cast<const Run<T, STEP> *>(i8_lds + at * PITCH + 16u * c);
+            T *to = out + (size_t)tok * out_stride + r;
+            if (r + STEP <= rows) *reinterpret_cast<Run<T, STEP> *>(to) = v;
+            else
+#pragma unroll
+                for (uint32_t k = 0; k < STEP - 1u; k++)
+                    if (r + k < rows) to[k] = v.v[k];
+        }
+    }
 }
 
 /* A tile of an expert's rows and pairs.  UP: the tile's fragments of 16 rows are gate's and up's by turns, so that a wave holds

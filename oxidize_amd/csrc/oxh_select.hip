@@ -41,17 +41,54 @@ __device__ __forceinline__ uint64_t sortable(double key)
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int d)
+/* v's neighbour in a step of a reduction over 16 lanes (lane ^ 1, lane ^ 2, mirrored in 8, mirrored in 16): no trip through LDS */
+template <int STEP> __device__ __forceinline__ uint32_t dpp_step(uint32_t v)
 {
-    const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, d), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), d);
-    return ((uint64_t)hi << 32) | lo;
+    constexpr int ctrl = STEP == 0 ? 0xB1 : STEP == 1 ? 0x4E : STEP == 2 ? 0x141 : 0x140;
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, ctrl, 0xF, 0xF, false);
+}
+template <int STEP> __device__ __forceinline__ double dpp_step(double v)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    return __longlong_as_double((long long)(((uint64_t)dpp_step<STEP>((uint32_t)(b >> 32)) << 32) | dpp_step<STEP>((uint32_t)b)));
+}
+
+__device__ __forceinline__ double lane_double(double v, int lane)
+{
+    const uint64_t b = (uint64_t)__double_as_longlong(v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(b >> 32), lane);
+    return __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
 }
 
 __device__ __forceinline__ double wave_sum64(double v)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v += __longlong_as_double((long long)shfl_xor64((uint64_t)__double_as_longlong(v), d));
-    return v;
+    v += dpp_step<0>(v);
+    v += dpp_step<1>(v);
+    v += dpp_step<2>(v);
+    v += dpp_step<3>(v);
+    return (lane_double(v, 0) + lane_double(v, 16)) + (lane_double(v, 32) + lane_double(v, 48));
+}
+
+__device__ __forceinline__ uint32_t wave_max32(uint32_t v)
+{
+    v = max(v, dpp_step<0>(v));
+    v = max(v, dpp_step<1>(v));
+    v = max(v, dpp_step<2>(v));
+    v = max(v, dpp_step<3>(v));
+    return max(max((uint32_t)__builtin_amdgcn_readlane((int)v, 0), (uint32_t)__builtin_amdgcn_readlane((int)v, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
+}
+
+/* The lanes that hold the largest 64-bit key: by its upper half, and by the lower one only where that does not tell. */
+__device__ __forceinline__ unsigned long long wave_argmax64(uint64_t key)
+{
+    const uint32_t hi = (uint32_t)(key >> 32), top = wave_max32(hi);
+    unsigned long long who = __ballot(hi == top);
+    if (who & (who - 1ull)) {
+        const uint32_t lo = hi == top ? (uint32_t)key : 0u, low = wave_max32(lo);
+        who = __ballot(hi == top && lo == low);
+    }
+    return who;
 }
 
 /* what a wave's lanes wrote to LDS before, its other lanes read after */
@@ -126,8 +163,9 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
                 z += p[i];
             }
             z = wave_sum64(z);
+            const double inv = z > 0.0 ? 1.0 / z : 0.0;
 #pragma unroll
-            for (int i = 0; i < NPL; i++) p[i] = z > 0.0 ? p[i] / z : 0.0;
+            for (int i = 0; i < NPL; i++) p[i] *= inv;
         } else {
 #pragma unroll
             for (int i = 0; i < NPL; i++) p[i] = 1.0 / (1.0 + exp(-(double)x[i]));
@@ -144,14 +182,26 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
         }
         if (a.n_group > 1u) {
             sel_wave_sync();
-            const uint32_t size = E / a.n_group;
+            /* `share` neighbouring lanes look through a group, every one at each share-th of its keys, and put their best two
+             * together */
+            const uint32_t size = E / a.n_group, share = 1u << (31u - (uint32_t)__builtin_clz(64u / a.n_group));
+            const uint32_t mine = lane / share, from = lane % share;
             double b1 = -__builtin_inf(), b2 = -__builtin_inf();
-            if (lane < a.n_group)
-                for (uint32_t j = 0; j < size; j++) {
-                    const double v = s_key[wave][lane * size + j];
-                    b2 = v > b1 ? b1 : v > b2 ? v : b2;
-                    b1 = v > b1 ? v : b1;
+            if (mine < a.n_group)
+#pragma unroll 4
+                for (uint32_t j = from; j < size; j += share) {
+                    const double v = s_key[wave][mine * size + j];
+                    b2 = fmax(b2, fmin(b1, v));
+                    b1 = fmax(b1, v);
                 }
+            for (uint32_t d = 1; d < share; d <<= 1) {
+                const double o1 = __shfl_xor(b1, (int)d), o2 = __shfl_xor(b2, (int)d);
+                b2 = fmax(fmin(b1, o1), fmax(b2, o2));
+                b1 = fmax(b1, o1);
+            }
+            /* group g's at lane g */
+            b1 = __shfl(b1, (int)min(lane * share, 63u));
+            b2 = __shfl(b2, (int)min(lane * share, 63u));
             const uint64_t rank = sortable(a.group_best == 2u && b2 > -__builtin_inf() ? b1 + b2 : b1);
             uint32_t before = 0;
             for (uint32_t g = 0; g < a.n_group; g++) {
@@ -181,27 +231,14 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
                     at = lane + 64u * i;
                     bp = p[i];
                 }
-            uint64_t m = best;
-#pragma unroll
-            for (int d = 1; d < 64; d <<= 1) {
-                const uint64_t o = shfl_xor64(m, d);
-                m = o > m ? o : m;
-            }
-            unsigned long long who = __ballot(best == m);
+            const unsigned long long who = wave_argmax64(best);
             uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)at, __builtin_ctzll(who));
-            if (who & (who - 1ull)) {               /* equal keys: the lowest expert */
-                uint32_t low = best == m ? at : 0xFFFFFFFFu;
-#pragma unroll
-                for (int d = 1; d < 64; d <<= 1) low = min(low, (uint32_t)__shfl_xor((int)low, d));
-                id = low;
-            }
-            const int owner = (int)(id & 63u);
-            const uint64_t bits = (uint64_t)__double_as_longlong(bp);
-            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)bits, owner);
-            const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(bits >> 32), owner);
+            /* equal keys: the lowest expert, which is the first lane's unless a lane holds several */
+            if (NPL > 1 && (who & (who - 1ull))) id = ~wave_max32((who >> lane) & 1ull ? ~at : 0u);
+            const double chosen = lane_double(bp, (int)(id & 63u));
             if (lane == j) {
                 my_id = id;
-                my_p = __longlong_as_double((long long)(((uint64_t)hi << 32) | lo));
+                my_p = chosen;
             }
 #pragma unroll
             for (int i = 0; i < NPL; i++)
@@ -242,44 +279,50 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
 }
 
 /* The positions of the pairs of many workgroups' tokens: the counts of all workgroups give the experts' runs, those of
- * the workgroups before this one where its own pairs start in them.  Four counts to a dword, rows dealt to the threads. */
+ * the workgroups before this one where its own pairs start in them.  Sixteen counts to a load, rows dealt to the threads;
+ * they are added up two to a word (an expert has at most one pair of a token, 65535 in all). */
 __global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
 {
     __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
-    __shared__ uint16_t s_id[SEL_TOKENS * OXH_SELECT_MAX_TOPK];
-    __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_before[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
+    __shared__ uint32_t s_all[OXH_SELECT_MAX_EXPERTS / 2u], s_bef[OXH_SELECT_MAX_EXPERTS / 2u];
+    __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_expert;
     const uint32_t t0 = blockIdx.x * a.tok_per_wg, here = min(a.tok_per_wg, a.n_tok - t0);
-    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += blockDim.x) {
-        s_mask[e] = 0ull;
-        s_total[e] = s_before[e] = 0u;
-    }
-    __syncthreads();
-    for (uint32_t i = tid; i < here * a.k; i += blockDim.x) {
-        const uint32_t e = (uint32_t)a.ids[(size_t)t0 * a.k + i];
-        s_id[i] = (uint16_t)e;
-        atomicOr(&s_mask[e], 1ull << (i / a.k));
-    }
-    const uint32_t quads = a.hist_stride / 4u, slices = blockDim.x / quads;
-    if (tid < slices * quads) {
-        const uint32_t q = tid % quads;
-        uint32_t all[4] = { 0u, 0u, 0u, 0u }, bef[4] = { 0u, 0u, 0u, 0u };
-        for (uint32_t b = tid / quads; b < gridDim.x; b += slices) {
-            const uint32_t c = *reinterpret_cast<const uint32_t *>(a.hist + (size_t)b * a.hist_stride + 4u * q);
+    /* the loads first: this workgroup's choices, the first rows of counts */
+    const uint32_t chunks = a.hist_stride / 16u, slices = blockDim.x / chunks, c = tid % chunks, first = tid / chunks;
+    const uint32_t n_pairs = here * a.k;
+    const uint32_t id = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid, n_pairs - 1u)];
+    uint32_t all[8] = { 0u }, bef[8] = { 0u };         /* experts 4i, 4i + 2 and 4i + 1, 4i + 3 of the chunk */
+    if (tid < slices * chunks)
+#pragma unroll 4
+        for (uint32_t b = first; b < gridDim.x; b += slices) {
+            const u32x4 v = *reinterpret_cast<const u32x4 *>(a.hist + (size_t)b * a.hist_stride + 16u * c);
+            const uint32_t on = b < blockIdx.x ? 0xFFFFFFFFu : 0u;
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const uint32_t v = (c >> (8 * i)) & 0xFFu;
-                all[i] += v;
-                bef[i] += b < blockIdx.x ? v : 0u;
+                const uint32_t even = v[i] & 0x00FF00FFu, odd = (v[i] >> 8) & 0x00FF00FFu;
+                all[2 * i] += even;
+                all[2 * i + 1] += odd;
+                bef[2 * i] += even & on;
+                bef[2 * i + 1] += odd & on;
             }
         }
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (all[i]) {
-                atomicAdd(&s_total[4u * q + i], all[i]);
-                atomicAdd(&s_before[4u * q + i], bef[i]);
-            }
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += blockDim.x) s_mask[e] = 0ull;
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS / 2u; e += blockDim.x) s_all[e] = s_bef[e] = 0u;
+    __syncthreads();
+    if (tid < n_pairs) {                                /* at most 64 tokens of 16 choices: one a thread */
+        atomicOr(&s_mask[id], 1ull << (tid / a.k));
     }
+    if (tid < slices * chunks)
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (all[i]) atomicAdd(&s_all[8u * c + i], all[i]);
+            if (bef[i]) atomicAdd(&s_bef[8u * c + i], bef[i]);
+        }
+    __syncthreads();
+    /* expert 4q + r of the words: word 2q + (r & 1), half r >> 1 */
+    auto half = [](const uint32_t *w, uint32_t e) { return (w[2u * (e / 4u) + (e & 1u)] >> (8u * (e & 2u))) & 0xFFFFu; };
+    for (uint32_t e = tid; e < E; e += blockDim.x) s_total[e] = half(s_all, e);
     __syncthreads();
     if (wave == 0u) sel_scan(s_total, s_base, E, lane);
     __syncthreads();
@@ -290,11 +333,11 @@ __global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
         }
         if (tid == 0u) a.offsets[E] = a.n_tok * a.k;
     }
-    for (uint32_t i = tid; i < here * a.k; i += blockDim.x) {
-        const uint32_t tt = i / a.k, e = s_id[i];
-        const uint32_t pos = s_base[e] + s_before[e] + (uint32_t)__popcll(s_mask[e] & ((1ull << tt) - 1ull));
+    if (tid < n_pairs) {
+        const uint32_t tt = tid / a.k;
+        const uint32_t pos = s_base[id] + half(s_bef, id) + (uint32_t)__popcll(s_mask[id] & ((1ull << tt) - 1ull));
         a.perm[pos] = t0 + tt;
-        a.slot_pos[(size_t)t0 * a.k + i] = pos;
+        a.slot_pos[(size_t)t0 * a.k + tid] = pos;
     }
 }
 
@@ -306,7 +349,7 @@ static uint32_t sel_tok_per_wg(size_t n_tok)
     return n_tok <= 16u * 256u ? 16u : n_tok <= 32u * 256u ? 32u : SEL_TOKENS;
 }
 
-static uint32_t sel_hist_stride(size_t n_expert) { return ((uint32_t)n_expert + 3u) & ~3u; }
+static uint32_t sel_hist_stride(size_t n_expert) { return ((uint32_t)n_expert + 15u) & ~15u; }
 
 static int sel_check(const OxhMoeRouter *r, size_t n_tok, const char *who)
 {
