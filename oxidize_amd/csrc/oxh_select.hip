@@ -21,7 +21,14 @@
 #define SEL_TOKENS 64u              /* a workgroup's tokens, at most: bits of a mask */
 #define SEL_WAVES 16u
 
+/* 1 / 13! .. 1 / 0!, an argument of the kernel so that they are scalar operands, not registers that every wave fills one by one */
+#define EXP_TERMS 14
+struct ExpSeries {
+    double c[EXP_TERMS];
+};
+
 struct SelectArgs {
+    ExpSeries exp;
     const void *logits;
     size_t stride;
     const float *bias;
@@ -33,12 +40,32 @@ struct SelectArgs {
     float scale;
 };
 
-/* The order of 64-bit keys as the order of integers; 0 is left for experts that cannot be chosen, 1 for masked ones
- * (the least key there is, -inf, maps to more). */
+/* The order of 64-bit keys as the order of integers. */
 __device__ __forceinline__ uint64_t sortable(double key)
 {
     const uint64_t b = (uint64_t)__double_as_longlong(key);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
+}
+
+/* An expert's key for the choice: the 43 leading bits of its key's mantissa, then the expert's number turned round, so that of equal
+ * keys the lowest expert has the largest and no two are equal.  Masked experts come after all others, 0 cannot be chosen. */
+__device__ __forceinline__ uint64_t expert_key(double key, bool live, uint32_t e)
+{
+    return (live ? sortable(key) & ~511ull : 512ull) | (511u - e);
+}
+
+/* e^x for x <= 709: x = k ln 2 + r, the series of e^r to its thirteenth power (|r| <= 0.347: what is left out is 4e-18 of it).  Half of
+ * the instructions of the library's, which also looks after what cannot come here. */
+__device__ __forceinline__ double exp64(double x, const ExpSeries &s)
+{
+    x = fmax(x, -750.0);
+    const double k = rint(x * 1.4426950408889634074);
+    double r = __builtin_fma(-k, 0x1.62e42fee00000p-1, x);          /* ln 2 in two parts, the first of 32 bits: k times it is exact */
+    r = __builtin_fma(-k, 0x1.a39ef35793c76p-33, r);
+    double e = s.c[0];
+#pragma unroll
+    for (int i = 1; i < EXP_TERMS; i++) e = __builtin_fma(e, r, s.c[i]);
+    return __builtin_ldexp(e, (int)k);
 }
 
 /* v's neighbour in a step of a reduction over 16 lanes (lane ^ 1, lane ^ 2, mirrored in 8, mirrored in 16): no trip through LDS */
@@ -79,8 +106,8 @@ __device__ __forceinline__ uint32_t wave_max32(uint32_t v)
                max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
-/* The lanes that hold the largest 64-bit key: by its upper half, and by the lower one only where that does not tell. */
-__device__ __forceinline__ unsigned long long wave_argmax64(uint64_t key)
+/* The lane that holds the largest of different 64-bit keys: by its upper half, and by the lower one only where that does not tell. */
+__device__ __forceinline__ int wave_argmax64(uint64_t key)
 {
     const uint32_t hi = (uint32_t)(key >> 32), top = wave_max32(hi);
     unsigned long long who = __ballot(hi == top);
@@ -88,7 +115,7 @@ __device__ __forceinline__ unsigned long long wave_argmax64(uint64_t key)
         const uint32_t lo = hi == top ? (uint32_t)key : 0u, low = wave_max32(lo);
         who = __ballot(hi == top && lo == low);
     }
-    return who;
+    return __builtin_ctzll(who);
 }
 
 /* what a wave's lanes wrote to LDS before, its other lanes read after */
@@ -135,6 +162,7 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
 {
     __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
     __shared__ double s_key[SEL_WAVES][NPL * 64];
+    __shared__ double s_score[SEL_WAVES][NPL * 64];
     __shared__ uint16_t s_id[SEL_TOKENS * OXH_SELECT_MAX_TOPK];
     __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6;
@@ -143,108 +171,113 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
     __syncthreads();
     for (uint32_t tt = wave; tt < here; tt += SEL_WAVES) {
         const size_t row = (size_t)(t0 + tt) * a.stride;
-        double p[NPL];
+        const double ninf = -__builtin_inf();
+        const bool softmax = a.score == OXH_SCORE_SOFTMAX;
         uint64_t key[NPL];
-        float x[NPL], top = -__builtin_inff();
+        float x[NPL], bias[NPL], top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < NPL; i++) x[i] = sel_load<T>(a.logits, row + min(lane + 64u * i, E - 1u));
+#pragma unroll
+        for (int i = 0; i < NPL; i++) bias[i] = a.bias ? a.bias[min(lane + 64u * i, E - 1u)] : 0.0f;
 #pragma unroll
         for (int i = 0; i < NPL; i++) {
-            const uint32_t e = lane + 64u * i;
-            float v = e < E ? sel_load<T>(a.logits, row + e) : -__builtin_inff();
-            v = v != v ? -__builtin_inff() : fminf(v, 3.402823466e38f);
-            x[i] = v;
-            top = fmaxf(top, v);
+            /* a NaN is masked as -inf is */
+            x[i] = lane + 64u * i < E && x[i] == x[i] ? fminf(x[i], 3.402823466e38f) : -__builtin_inff();
+            top = fmaxf(top, x[i]);
+            s_score[wave][lane + 64u * i] = (double)x[i];
         }
-        top = wave_max(top);
-        if (a.score == OXH_SCORE_SOFTMAX) {
-            double z = 0.0;
-#pragma unroll
-            for (int i = 0; i < NPL; i++) {
-                p[i] = x[i] > -__builtin_inff() ? exp((double)x[i] - (double)top) : 0.0;
-                z += p[i];
-            }
+        /* A lane's experts one after the other, in a loop that stays a loop: a wave comes here once, and what it does not have to
+         * fetch of the program it does not wait for.  e^(x - top), or 1 / (1 + e^-x) with the sum within range (below e^-708 it is 0) */
+        top = softmax ? wave_max(top) : 0.0f;
+        double z = 0.0;
+#pragma unroll 1
+        for (uint32_t e = lane; e < NPL * 64u; e += 64u) {
+            const double v = s_score[wave][e];
+            const double d = exp64(softmax ? v - (double)top : fmin(-v, 708.0), a.exp);
+            double r = __builtin_amdgcn_rcp(1.0 + d);
+            r = __builtin_fma(__builtin_fma(-(1.0 + d), r, 1.0), r, r);
+            r = __builtin_fma(__builtin_fma(-(1.0 + d), r, 1.0), r, r);
+            r = softmax ? d : r;
+            r = v < (softmax ? -3.5e38 : -708.0) ? 0.0 : r;
+            z += r;
+            s_score[wave][e] = r;
+        }
+        double factor = 1.0;
+        if (softmax) {
             z = wave_sum64(z);
-            const double inv = z > 0.0 ? 1.0 / z : 0.0;
-#pragma unroll
-            for (int i = 0; i < NPL; i++) p[i] *= inv;
-        } else {
-#pragma unroll
-            for (int i = 0; i < NPL; i++) p[i] = 1.0 / (1.0 + exp(-(double)x[i]));
+            factor = z > 0.0 ? 1.0 / z : 0.0;
         }
 #pragma unroll
         for (int i = 0; i < NPL; i++) {
             const uint32_t e = lane + 64u * i;
-            double kv = p[i];
-            if (a.bias && e < E) kv += (double)a.bias[e];
-            const bool live = x[i] > -__builtin_inff() && kv > -__builtin_inf();      /* a NaN is not */
-            key[i] = e >= E ? 0ull : live ? sortable(kv) : 1ull;
-            if (!live) p[i] = 0.0;
-            if (a.n_group > 1u) s_key[wave][e] = live ? kv : -__builtin_inf();
+            const double p = s_score[wave][e] * factor, kv = p + (double)bias[i];
+            const bool live = x[i] > -__builtin_inff() && kv > ninf;        /* a NaN is not */
+            key[i] = e < E ? expert_key(kv, live, e) : 0ull;
+            s_score[wave][e] = live ? p : 0.0;
+            if (a.n_group > 1u) s_key[wave][e] = live ? kv : ninf;
         }
+        sel_wave_sync();
         if (a.n_group > 1u) {
-            sel_wave_sync();
             /* `share` neighbouring lanes look through a group, every one at each share-th of its keys, and put their best two
              * together */
             const uint32_t size = E / a.n_group, share = 1u << (31u - (uint32_t)__builtin_clz(64u / a.n_group));
             const uint32_t mine = lane / share, from = lane % share;
-            double b1 = -__builtin_inf(), b2 = -__builtin_inf();
+            double b1 = ninf, b2 = ninf;
             if (mine < a.n_group)
-#pragma unroll 4
+#pragma unroll 2
                 for (uint32_t j = from; j < size; j += share) {
                     const double v = s_key[wave][mine * size + j];
                     b2 = fmax(b2, fmin(b1, v));
                     b1 = fmax(b1, v);
                 }
+#pragma unroll 1
             for (uint32_t d = 1; d < share; d <<= 1) {
                 const double o1 = __shfl_xor(b1, (int)d), o2 = __shfl_xor(b2, (int)d);
                 b2 = fmax(fmin(b1, o1), fmax(b2, o2));
                 b1 = fmax(b1, o1);
             }
-            /* group g's at lane g */
-            b1 = __shfl(b1, (int)min(lane * share, 63u));
-            b2 = __shfl(b2, (int)min(lane * share, 63u));
-            const uint64_t rank = sortable(a.group_best == 2u && b2 > -__builtin_inf() ? b1 + b2 : b1);
+            /* a masked expert does not count */
+            const uint64_t rank = sortable(a.group_best == 2u && b2 > ninf ? b1 + b2 : b1);
             uint32_t before = 0;
+#pragma unroll 1
             for (uint32_t g = 0; g < a.n_group; g++) {
-                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, (int)g);
-                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(rank >> 32), (int)g);
+                const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)rank, (int)(g * share));
+                const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(rank >> 32), (int)(g * share));
                 const uint64_t other = ((uint64_t)hi << 32) | lo;
-                before += other > rank || (other == rank && g < lane) ? 1u : 0u;
+                before += other > rank || (other == rank && g < mine) ? 1u : 0u;
             }
-            const unsigned long long kept = __ballot(lane < a.n_group && before < a.top_group);
+            /* bit g * share: whether group g is kept */
+            const unsigned long long kept = __ballot(mine < a.n_group && before < a.top_group);
 #pragma unroll
             for (int i = 0; i < NPL; i++) {
                 const uint32_t e = lane + 64u * i;
-                if (e < E && !((kept >> (e / size)) & 1ull)) key[i] = 0ull;
+                if (e < E && !((kept >> (e / size * share)) & 1ull)) key[i] = 0ull;
             }
-            sel_wave_sync();
         }
-        double my_p = 0.0;
+        /* a lane's keys in descending order, of which only the first one is looked at */
+#pragma unroll
+        for (int n = NPL - 1; n > 0; n--)
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const bool swap = key[i + 1] > key[i];
+                const uint64_t high = swap ? key[i + 1] : key[i], low = swap ? key[i] : key[i + 1];
+                key[i] = high;
+                key[i + 1] = low;
+            }
         uint32_t my_id = 0;
+#pragma unroll 1
         for (uint32_t j = 0; j < a.k; j++) {
-            uint64_t best = key[0];
-            uint32_t at = lane;
-            double bp = p[0];
+            const int owner = wave_argmax64(key[0]);
+            const uint32_t id = 511u - ((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key[0], owner) & 511u);
+            my_id = lane == j ? id : my_id;
+            if ((int)lane == owner) {
 #pragma unroll
-            for (int i = 1; i < NPL; i++)
-                if (key[i] > best) {
-                    best = key[i];
-                    at = lane + 64u * i;
-                    bp = p[i];
-                }
-            const unsigned long long who = wave_argmax64(best);
-            uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)at, __builtin_ctzll(who));
-            /* equal keys: the lowest expert, which is the first lane's unless a lane holds several */
-            if (NPL > 1 && (who & (who - 1ull))) id = ~wave_max32((who >> lane) & 1ull ? ~at : 0u);
-            const double chosen = lane_double(bp, (int)(id & 63u));
-            if (lane == j) {
-                my_id = id;
-                my_p = chosen;
+                for (int i = 0; i + 1 < NPL; i++) key[i] = key[i + 1];
+                key[NPL - 1] = 0ull;
             }
-#pragma unroll
-            for (int i = 0; i < NPL; i++)
-                if (id == lane + 64u * i) key[i] = 0ull;
         }
-        const double sum = wave_sum64(my_p);                    /* lanes from k on hold 0 */
+        const double my_p = lane < a.k ? s_score[wave][my_id] : 0.0;
+        const double sum = wave_sum64(my_p);
         double w = my_p;
         if (a.renorm) w = sum > 0.0 ? my_p / sum : 0.0;
         if (lane < a.k) {
@@ -254,6 +287,7 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
             s_id[tt * a.k + lane] = (uint16_t)my_id;
             atomicOr(&s_mask[my_id], 1ull << tt);
         }
+        sel_wave_sync();
     }
     __syncthreads();
     if (a.hist) {
@@ -278,10 +312,12 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
     }
 }
 
+#define PLACE_THREADS 1024u
+
 /* The positions of the pairs of many workgroups' tokens: the counts of all workgroups give the experts' runs, those of
  * the workgroups before this one where its own pairs start in them.  Sixteen counts to a load, rows dealt to the threads;
  * they are added up two to a word (an expert has at most one pair of a token, 65535 in all). */
-__global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
+__global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
 {
     __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
     __shared__ uint32_t s_all[OXH_SELECT_MAX_EXPERTS / 2u], s_bef[OXH_SELECT_MAX_EXPERTS / 2u];
@@ -289,9 +325,11 @@ __global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_expert;
     const uint32_t t0 = blockIdx.x * a.tok_per_wg, here = min(a.tok_per_wg, a.n_tok - t0);
     /* the loads first: this workgroup's choices, the first rows of counts */
-    const uint32_t chunks = a.hist_stride / 16u, slices = blockDim.x / chunks, c = tid % chunks, first = tid / chunks;
-    const uint32_t n_pairs = here * a.k;
-    const uint32_t id = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid, n_pairs - 1u)];
+    const uint32_t chunks = a.hist_stride / 16u, slices = PLACE_THREADS / chunks, c = tid % chunks, first = tid / chunks;
+    const uint32_t n_pairs = here * a.k;                /* at most 64 tokens of 16 choices: four a thread */
+    uint32_t id[4];
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++) id[i] = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid + PLACE_THREADS * i, n_pairs - 1u)];
     uint32_t all[8] = { 0u }, bef[8] = { 0u };         /* experts 4i, 4i + 2 and 4i + 1, 4i + 3 of the chunk */
     if (tid < slices * chunks)
 #pragma unroll 4
@@ -307,12 +345,12 @@ __global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
                 bef[2 * i + 1] += odd & on;
             }
         }
-    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += blockDim.x) s_mask[e] = 0ull;
-    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS / 2u; e += blockDim.x) s_all[e] = s_bef[e] = 0u;
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += PLACE_THREADS) s_mask[e] = 0ull;
+    for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS / 2u; e += PLACE_THREADS) s_all[e] = s_bef[e] = 0u;
     __syncthreads();
-    if (tid < n_pairs) {                                /* at most 64 tokens of 16 choices: one a thread */
-        atomicOr(&s_mask[id], 1ull << (tid / a.k));
-    }
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++)
+        if (tid + PLACE_THREADS * i < n_pairs) atomicOr(&s_mask[id[i]], 1ull << ((tid + PLACE_THREADS * i) / a.k));
     if (tid < slices * chunks)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -322,22 +360,24 @@ __global__ __launch_bounds__(1024) void k_moe_place(const SelectArgs a)
     __syncthreads();
     /* expert 4q + r of the words: word 2q + (r & 1), half r >> 1 */
     auto half = [](const uint32_t *w, uint32_t e) { return (w[2u * (e / 4u) + (e & 1u)] >> (8u * (e & 2u))) & 0xFFFFu; };
-    for (uint32_t e = tid; e < E; e += blockDim.x) s_total[e] = half(s_all, e);
+    for (uint32_t e = tid; e < E; e += PLACE_THREADS) s_total[e] = half(s_all, e);
     __syncthreads();
     if (wave == 0u) sel_scan(s_total, s_base, E, lane);
     __syncthreads();
     if (blockIdx.x == 0u) {
-        for (uint32_t e = tid; e < E; e += blockDim.x) {
+        for (uint32_t e = tid; e < E; e += PLACE_THREADS) {
             a.counts[e] = s_total[e];
             a.offsets[e] = s_base[e];
         }
         if (tid == 0u) a.offsets[E] = a.n_tok * a.k;
     }
-    if (tid < n_pairs) {
-        const uint32_t tt = tid / a.k;
-        const uint32_t pos = s_base[id] + half(s_bef, id) + (uint32_t)__popcll(s_mask[id] & ((1ull << tt) - 1ull));
+#pragma unroll
+    for (uint32_t i = 0; i < 4u; i++) {
+        const uint32_t pair = tid + PLACE_THREADS * i, tt = pair / a.k;
+        if (pair >= n_pairs) break;
+        const uint32_t pos = s_base[id[i]] + half(s_bef, id[i]) + (uint32_t)__popcll(s_mask[id[i]] & ((1ull << tt) - 1ull));
         a.perm[pos] = t0 + tt;
-        a.slot_pos[(size_t)t0 * a.k + tid] = pos;
+        a.slot_pos[(size_t)t0 * a.k + pair] = pos;
     }
 }
 
@@ -421,6 +461,11 @@ extern "C" int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const
         return oxh_internal_errorf(OXH_ERR_ARG, "invalid argument: %s: workspace must be 16-byte aligned", who);
     if (oxh_internal_device() < 0 && (rc = oxh_init(0))) return rc;
     SelectArgs a = {};
+    double term = 1.0;                              /* n!, exact */
+    for (int n = 0; n < EXP_TERMS; n++) {
+        a.exp.c[EXP_TERMS - 1 - n] = 1.0 / term;
+        term *= n + 1;
+    }
     a.logits = d_logits;
     a.stride = logits_stride;
     a.bias = r->d_bias;
@@ -449,7 +494,7 @@ extern "C" int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const
     else sel_launch<__bf16>(a, wgs, st);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && need) {
-        hipLaunchKernelGGL(k_moe_place, dim3(wgs), dim3(1024), 0, st, a);
+        hipLaunchKernelGGL(k_moe_place, dim3(wgs), dim3(PLACE_THREADS), 0, st, a);
         e = hipGetLastError();
     }
     if (e != hipSuccess) return oxh_internal_errorf(OXH_ERR_HIP, "HIP error in %s: %s", who, hipGetErrorString(e));
