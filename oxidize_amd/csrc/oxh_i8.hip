@@ -325,17 +325,27 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles_tail(const I8Prod
     }
 }
 
-/* The sums of a product whose columns were shared out: integers, the same in any order.  Four rows to a thread. */
+/* The sums of a product whose columns were shared out: integers, the same in any order.  Four rows to a thread, four parts under
+ * way at a time (one after the other, 333 x 4096 in five parts took 9 us). */
 __global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
 {
     const uint32_t r = (blockIdx.x * 256u + threadIdx.x) * 4u, t = blockIdx.y;
     if (r >= (uint32_t)p.w.rows) return;
-    v4i sums = { 0, 0, 0, 0 };
-    for (uint32_t s = 0; s < p.splits; s++)
-        sums += *reinterpret_cast<const v4i *>(p.parts + ((size_t)s * p.n_vec + t) * p.rows_pad + r);
+    const size_t part = (size_t)p.n_vec * p.rows_pad;
+    const int *from = p.parts + (size_t)t * p.rows_pad + r;
     float sw[4], b[4];
     i8_row_factors(p, r, sw, b);
-    i8_results(p, r, t, sums, sw, b, p.q_scale[t]);
+    const float st = p.q_scale[t];
+    v4i sums = { 0, 0, 0, 0 };
+    for (uint32_t s0 = 0; s0 < p.splits; s0 += 4u) {
+        v4i v[4];
+#pragma unroll
+        for (uint32_t s = 0; s < 4u; s++) v[s] = *reinterpret_cast<const v4i *>(from + part * min(s0 + s, p.splits - 1u));
+#pragma unroll
+        for (uint32_t s = 0; s < 4u; s++)
+            if (s0 + s < p.splits) sums += v[s];
+    }
+    i8_results(p, r, t, sums, sw, b, st);
 }
 
 /* ─── few tokens ──────────────────────────────────────────────────────── */
@@ -456,6 +466,87 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_few(const I8Produc
     if (ST > 2) factors();
     __syncthreads();
     if (wave < teams && g < groups && r < rows && r16 < p.n_vec) i8_results(p, r, r16, few_join(turns, wave * team, team), sw, b, st);
+}
+
+/* 17 to 64 tokens, TF fragments of sixteen: the same, but a stage's tokens come as the weights do, eight rows of 128 bytes an
+ * instruction, and are turned the same way, the next stage's requested as soon as these are in LDS. */
+template <int ST, int TF>
+__global__ __launch_bounds__(1024) void k_i8_few_wide(const I8Product p, uint32_t team, uint32_t groups)
+{
+    constexpr uint32_t TURN = TF > 2 ? TF * 1024u : 2048u;
+    __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_WAVES * TURN];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    const uint32_t rows = (uint32_t)p.w.rows, cols = (uint32_t)p.w.cols, teams = FEW_WAVES / team, r16 = lane & 15u, kq = lane >> 4;
+    const uint32_t r0 = 16u * min(blockIdx.x * teams + wave / team, groups - 1u);
+    const uint32_t stages = (cols + 127u) / 128u, last_piece = (cols - 1u) / 16u;
+    uint32_t first, mine;
+    few_part(stages, wave % team, team, first, mine);
+    uint8_t *const turn = turns + TURN * wave;
+    const int8_t *wrow[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; h++) wrow[h] = p.w.d_w + (size_t)min(r0 + 8u * h + (lane >> 3), rows - 1u) * p.w.stride;
+    v4i w[ST][2], q[TF][2];
+    few_weights<ST>(w, wrow, first, stages, last_piece);
+    auto tokens = [&](uint32_t i) {
+        const uint32_t at = 16u * min(8u * min(first + i, stages - 1u) + (lane & 7u), last_piece);
+#pragma unroll
+        for (uint32_t j = 0; j < TF; j++)
+#pragma unroll
+            for (uint32_t h = 0; h < 2u; h++)
+                q[j][h] = *reinterpret_cast<const v4i *>(p.q + (size_t)min(16u * j + 8u * h + (lane >> 3), p.n_vec - 1u) * p.q_stride + at);
+    };
+    tokens(0u);
+    const uint32_t swz = (r16 >> 1) & 7u, wr = 128u * (lane >> 3) + 16u * ((lane & 7u) ^ ((lane >> 4) & 7u));
+    const uint32_t rd[2] = { 128u * r16 + 16u * (kq ^ swz), 128u * r16 + 16u * ((4u + kq) ^ swz) };
+    auto turned = [&](const v4i (&from)[2], v4i (&to)[2]) {
+        *reinterpret_cast<v4i *>(turn + wr) = from[0];
+        *reinterpret_cast<v4i *>(turn + 1024u + (wr ^ 64u)) = from[1];
+        i8_wave_sync();
+        to[0] = *reinterpret_cast<const v4i *>(turn + rd[0]);
+        to[1] = *reinterpret_cast<const v4i *>(turn + rd[1]);
+        i8_wave_sync();
+    };
+    v4i acc[TF];
+#pragma unroll
+    for (uint32_t j = 0; j < TF; j++) acc[j] = v4i{ 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t i = 0; i < ST; i++) {
+        if (i < mine) {
+            if (128u * (first + i + 1u) > cols) {           /* the weights' columns behind the last one count as 0 */
+#pragma unroll
+                for (uint32_t d = 0; d < 4u; d++) {
+                    const uint32_t at = 128u * (first + i) + 16u * (lane & 7u) + 4u * d, left = cols > at ? cols - at : 0u;
+                    const int mask = left < 4u ? (int)((1u << (8u * left)) - 1u) : -1;
+                    w[i][0][d] &= mask;
+                    w[i][1][d] &= mask;
+                }
+            }
+            v4i a[2], b[TF][2];
+            turned(w[i], a);
+#pragma unroll
+            for (uint32_t j = 0; j < TF; j++) turned(q[j], b[j]);
+            if (i + 1u < ST) tokens(i + 1u);
+#pragma unroll
+            for (uint32_t j = 0; j < TF; j++) {
+                acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[0], b[j][0], acc[j], 0, 0, 0);
+                acc[j] = __builtin_amdgcn_mfma_i32_16x16x64_i8(a[1], b[j][1], acc[j], 0, 0, 0);
+            }
+        }
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < TF; j++) *reinterpret_cast<v4i *>(turn + 1024u * j + 16u * lane) = acc[j];
+    __syncthreads();
+    /* a wave joins a fragment of a team's, or several */
+    for (uint32_t x = wave; x < teams * TF; x += FEW_WAVES) {
+        const uint32_t mate = x / TF, j = x % TF, g = blockIdx.x * teams + mate, r = 16u * g + 4u * kq, t = 16u * j + r16;
+        if (g >= groups || r >= rows || t >= p.n_vec) continue;
+        float sw[4], b[4];
+        i8_row_factors(p, r, sw, b);
+        const float st = p.q_scale[t];
+        v4i sums = { 0, 0, 0, 0 };
+        for (uint32_t k = 0; k < team; k++) sums += *reinterpret_cast<const v4i *>(turns + TURN * (mate * team + k) + 1024u * j + 16u * lane);
+        i8_results(p, r, t, sums, sw, b, st);
+    }
 }
 
 /* Float tokens, which every workgroup quantises for itself (k_i8_quantize's codes): their values are requested before the weights
@@ -996,14 +1087,19 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
 
 /* The kernels for few tokens: how many waves share a group of 16 rows (0: they do not take the product).  Four stages a wave
  * leave room for two workgroups on a CU (151936 x 896 under one token: 27 us, 33 with eight); where the groups are few, all
- * of a CU's sixteen waves are wanted. */
+ * of a CU's sixteen waves are wanted.  More than sixteen tokens only where that is one workgroup per CU and four stages a wave: the
+ * tiles reach such a matrix late (4096 x 4096 under 17 to 64 tokens: 6.2 to 8.3 us, the tiles 9.3 to 10.8; 500 x 3001: 5 to 6.2 and
+ * 7.7 to 8.1), but tokens read once per group of rows cost more than they do in tiles (14336 x 4096: 15.7 to 21.7 us, the
+ * tiles 13.8 to 17.4). */
+#define FEW_WIDE_TOKENS 64u
 #define FEW_MAX_STAGES 8u
 static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
 {
     const size_t groups = (rows + 15u) / 16u, stages = (cols + 127u) / 128u;
-    if (n > FEW_TOKENS || stages > FEW_MAX_STAGES * FEW_WAVES) return 0;
+    if (n > FEW_WIDE_TOKENS || stages > FEW_MAX_STAGES * FEW_WAVES) return 0;
     uint32_t team = 1;
     while (team < FEW_WAVES && (stages > 4u * team || groups * team < cus * FEW_WAVES)) team *= 2u;
+    if (n > FEW_TOKENS && (stages > 4u * team || groups * team > cus * FEW_WAVES)) return 0;
     return team;
 }
 
@@ -1019,10 +1115,20 @@ static FewGrid few_grid(size_t rows, size_t cols, uint32_t team)
     return g;
 }
 
+template <int TF> static void few_wide_launch(const I8Product &p, uint32_t team, const FewGrid &g, hipStream_t st)
+{
+    const dim3 grid(g.wgs), block(64u * FEW_WAVES);
+    if (g.stages <= 2u) hipLaunchKernelGGL((k_i8_few_wide<2, TF>), grid, block, 0, st, p, team, g.groups);
+    else hipLaunchKernelGGL((k_i8_few_wide<4, TF>), grid, block, 0, st, p, team, g.groups);
+}
+
 static void few_launch(const I8Product &p, uint32_t team, hipStream_t st)
 {
     const FewGrid g = few_grid(p.w.rows, p.w.cols, team);
     const dim3 grid(g.wgs), block(64u * FEW_WAVES);
+    if (p.n_vec > 48u) return few_wide_launch<4>(p, team, g, st);
+    if (p.n_vec > 32u) return few_wide_launch<3>(p, team, g, st);
+    if (p.n_vec > 16u) return few_wide_launch<2>(p, team, g, st);
     if (g.stages <= 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
     else if (g.stages <= 4u) hipLaunchKernelGGL(k_i8_few<4>, grid, block, 0, st, p, team, g.groups);
     else hipLaunchKernelGGL(k_i8_few<8>, grid, block, 0, st, p, team, g.groups);
@@ -1110,7 +1216,7 @@ static bool linear_fused(size_t rows, size_t cols, size_t n)
 {
     const size_t per = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;      /* waves a token, as in the kernel */
     const uint32_t team = few_team(rows, cols, n, i8_cus());
-    return team && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= i8_cus();
+    return team && n <= FEW_TOKENS && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= i8_cus();
 }
 
 /* the workspace otherwise: codes and scales of the tokens, the partial sums of the product */
