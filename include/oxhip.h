@@ -593,7 +593,7 @@ typedef struct OxhRouting {
     float    *d_weights;
     uint32_t *d_counts, *d_offsets, *d_perm, *d_slot_pos;
 } OxhRouting;
-/* Bytes of workspace a call takes (0 up to 64 tokens). */
+/* Bytes of workspace a call takes (0 up to 64 tokens; never less for more). */
 int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes);
 /* d_logits: n_tok rows of n_expert values of `logits_type` (OXH_F32, OXH_F16,
  * OXH_BF16), logits_stride elements apart.  d_workspace: 16-byte aligned,
@@ -642,7 +642,7 @@ int oxh_i8_quantize(uint32_t x_type, const void *d_x, size_t x_stride, size_t n_
  * aligned to its elements.  Few results over long rows are shared out over
  * the columns when there is a workspace (oxh_i8_matmul_workspace bytes,
  * 16-byte aligned, overwritten; with less, or NULL, the call does without,
- * and with the same results). */
+ * and with the same results).  d_out may overlap no input, here and below. */
 size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec);
 int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
                   const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,
@@ -651,7 +651,8 @@ int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, cons
  * codes and scales; the results are those of the two calls): one launch for a
  * few tokens, so that a decode step needs no quantiser of its own.  The
  * workspace is not optional here: oxh_i8_linear_workspace bytes, 16-byte
- * aligned, overwritten (0 where the call needs none). */
+ * aligned, overwritten (0 where the call needs none); that of a larger n_vec
+ * serves a smaller one too. */
 size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec);
 int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
                   const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,

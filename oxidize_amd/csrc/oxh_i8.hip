@@ -680,7 +680,7 @@ k_i8_experts_begin(const T *__restrict__ x, size_t x_stride, uint32_t cols, int8
             t.first = s_first[lo] + tok * (i - s_tile[lo]);
             t.n = min(tok, s_first[lo + 1u] - t.first);
             t.base = s_tile[lo];
-            t.count = s_tile[lo + 1u] - t.base;
+            t.count = min(s_tile[lo + 1u], n_tiles) - t.base;       /* offsets out of order can ask for more tiles than any routing has */
         }
         tiles[i] = t;
     }
@@ -913,6 +913,11 @@ static int launched(const char *who)
 /* a tile's rows lie within 32 bits of its first one */
 #define I8_MAX_STRIDE ((size_t)1 << 23)
 
+/* results of a product: 2^37 are 2^30 threads in tiles of 256 x 256, and do not fit this memory in f32 */
+#define I8_MAX_RESULTS ((size_t)1 << 37)
+/* pairs times the longer side of an expert: tiles of 128 x 64 below 2^32 threads, and 128 GiB of h or y */
+#define I8_MAX_PAIR_VALUES ((size_t)1 << 35)
+
 static int check_rows(const char *who, const char *name, const void *d, size_t stride, size_t cols)
 {
     if (!d) return I8_ARG("%s: NULL pointer (%s)", who, name);
@@ -1030,12 +1035,19 @@ static double stage_us(int tile, size_t c, bool full)
     }
 }
 
+static size_t tile_count(int tile, size_t rows, size_t n)
+{
+    static const size_t tile_rows[I8_TILES] = { 256, 128, 128, 64 }, tile_tok[I8_TILES] = { 256, 256, 128, 64 };
+    return ((rows + tile_rows[tile] - 1) / tile_rows[tile]) * ((n + tile_tok[tile] - 1) / tile_tok[tile]);
+}
+#define I8_MAX_TILES ((size_t)1 << 23)      /* of 512 threads: a grid of 2^32 */
+
 /* What a product takes: rounds of what the CUs hold at a time, the last one with as many tiles to a CU as are left; results
  * at 5 TB/s; partial sums written and read at 4 TB/s and a second launch. */
 static double product_us(int tile, uint32_t splits, size_t rows, size_t stages, size_t n, size_t cus)
 {
-    static const size_t tile_rows[I8_TILES] = { 256, 128, 128, 64 }, tile_tok[I8_TILES] = { 256, 256, 128, 64 }, held[I8_TILES] = { 1, 1, 2, 4 };
-    const size_t tiles = ((rows + tile_rows[tile] - 1) / tile_rows[tile]) * ((n + tile_tok[tile] - 1) / tile_tok[tile]) * splits;
+    static const size_t held[I8_TILES] = { 1, 1, 2, 4 };
+    const size_t tiles = tile_count(tile, rows, n) * splits;
     const size_t k = (stages + splits - 1) / splits, rounds = tiles / (cus * held[tile]), rest = tiles - rounds * cus * held[tile];
     double us = 3.0 + (double)rounds * ((double)k * stage_us(tile, held[tile], true) + 1.5);
     if (rest) {
@@ -1056,6 +1068,7 @@ static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes, size_t 
         const size_t need = parts_bytes(rows, n, splits);
         if (splits > 1 && (need > ws_bytes || need > I8_MAX_PARTS_BYTES || n > 65535u)) break;
         for (int tile = 0; tile < I8_TILES; tile++) {
+            if (tile > I8_LARGE && tile_count(tile, rows, n) * splits >= I8_MAX_TILES) continue;
             const double us = product_us(tile, splits, rows, stages, n, cus);
             if (us < least) {
                 least = us;
@@ -1203,6 +1216,7 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
         return rc;
     if (!d_q_scale) return I8_ARG("%s: NULL pointer (d_q_scale)", who);
     if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
+    if (n_vec * w->rows > I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, I8_MAX_RESULTS);
     if (d_workspace && workspace_bytes && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
     if ((rc = ready())) return rc;
     return matmul_launch(w, d_q, q_stride, d_q_scale, n_vec, d_bias, out_type, d_out, out_stride, d_workspace,
@@ -1242,6 +1256,15 @@ extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
     return linear_parts(w->rows, w->cols, n_vec).total;
 }
 
+/* codes and scales have to fit; partial sums are used where they do, so a buffer for more tokens serves fewer as well */
+static int check_linear_workspace(const char *who, const OxhI8Matrix *w, size_t n_vec, const void *d_workspace, size_t bytes)
+{
+    const LinearParts l = linear_parts(w->rows, w->cols, n_vec);
+    if (l.total && (!d_workspace || bytes < l.parts)) return I8_ARG("%s: workspace too small (see oxh_i8_linear_workspace)", who);
+    if (l.total && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
+    return OXH_OK;
+}
+
 extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
                              const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
                              size_t workspace_bytes, void *stream)
@@ -1254,10 +1277,11 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
         (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)))
         return rc;
     if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
+    if (n_vec * w->rows > I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, I8_MAX_RESULTS);
+    if ((rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
+        (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)))    /* once more: the way depends on the device */
+        return rc;
     const LinearParts l = linear_parts(w->rows, w->cols, n_vec);
-    if (l.total && (!d_workspace || workspace_bytes < l.total)) return I8_ARG("%s: workspace too small (see oxh_i8_linear_workspace)", who);
-    if (l.total && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
-    if ((rc = ready())) return rc;
     hipStream_t st = stream_of(stream);
     if (l.total == 0) {
         I8Product p = { *w, nullptr, 0, nullptr, d_bias, d_out, out_stride, nullptr, (uint32_t)n_vec, 1u, 0u, 0u, 0u, 0u, out_type };
@@ -1270,8 +1294,8 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
     int8_t *q = (int8_t *)d_workspace;
     float *scale = (float *)((uint8_t *)d_workspace + l.scale);
     if ((rc = quantize_launch(x_type, d_x, x_stride, n_vec, w->cols, nullptr, q, l.q_stride, scale, st, who))) return rc;
-    return matmul_launch(w, q, l.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, (uint8_t *)d_workspace + l.parts, l.parts_bytes,
-                         st, who);
+    return matmul_launch(w, q, l.q_stride, scale, n_vec, d_bias, out_type, d_out, out_stride, (uint8_t *)d_workspace + l.parts,
+                         workspace_bytes - l.parts, st, who);
 }
 
 /* ─── experts ─────────────────────────────────────────────────────────── */
@@ -1310,12 +1334,14 @@ static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Part
     p->qh_stride = up64(m->ffn);
     p->h_stride = up64(m->ffn);
     p->y_stride = up64(m->hidden);
+    if (pairs * (m->hidden > m->ffn ? m->hidden : m->ffn) > I8_MAX_PAIR_VALUES)
+        return I8_ARG("%s: n_tok * top_k * max(hidden, ffn) is more than %zu", who, I8_MAX_PAIR_VALUES);
     if (n_tok * p->q_stride > 0xFFFFFFFFull) return I8_ARG("%s: the tokens' codes exceed 4 GiB", who);
     p->tok = experts_tok(pairs, m->n_expert);
     p->n_tiles = (uint32_t)experts_tiles(pairs, m->n_expert, p->tok);
     size_t at = 0;
 #define OXH_PART(FIELD, BYTES) p->FIELD = at; at = up256(at + (BYTES))
-    OXH_PART(tiles, p->n_tiles * sizeof(I8ExpertTile));
+    OXH_PART(tiles, experts_tiles(pairs, m->n_expert, FEW_TOKENS) * sizeof(I8ExpertTile));   /* more tokens never need less */
     OXH_PART(q, n_tok * p->q_stride);
     OXH_PART(q_scale, n_tok * 4u);
     OXH_PART(h, pairs * p->h_stride * 4u);

@@ -386,7 +386,7 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
 static uint32_t sel_tok_per_wg(size_t n_tok)
 {
     if (n_tok <= SEL_TOKENS) return SEL_TOKENS;
-    return n_tok <= 16u * 256u ? 16u : n_tok <= 32u * 256u ? 32u : SEL_TOKENS;
+    return n_tok <= 4096u ? 16u : n_tok <= 8192u ? 32u : SEL_TOKENS;
 }
 
 static uint32_t sel_hist_stride(size_t n_expert) { return ((uint32_t)n_expert + 15u) & ~15u; }
@@ -420,7 +420,9 @@ static int sel_check(const OxhMoeRouter *r, size_t n_tok, const char *who)
 static size_t sel_workspace(const OxhMoeRouter *r, size_t n_tok)
 {
     const uint32_t per = sel_tok_per_wg(n_tok);
-    return n_tok <= SEL_TOKENS ? 0 : (n_tok + per - 1u) / per * sel_hist_stride(r->n_expert);
+    const size_t wgs = (n_tok + per - 1u) / per;
+    /* where a workgroup takes more tokens there are fewer of them: never less than for fewer tokens */
+    return n_tok <= SEL_TOKENS ? 0 : (n_tok > 4096u && wgs < 256u ? 256u : wgs) * sel_hist_stride(r->n_expert);
 }
 
 extern "C" int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes)

@@ -228,6 +228,83 @@ def test_from_packed(oxh):
     assert np.array_equal(keep[1].download(np.float32, rows), s)
 
 
+WIDE = [(17, 1, 1), (18, 500, 3001), (32, 4096, 4096), (33, 1000, 900), (40, 17, 8192), (47, 16, 16), (48, 2048, 2049), (49, 64, 130),
+        (63, 4095, 4090), (64, 300, 8100), (64, 4097, 128)]
+
+
+@pytest.mark.parametrize("n,rows,cols", WIDE)
+@pytest.mark.parametrize("kind", [F32, BF16], ids=["f32", "bf16"])
+def test_matmul_of_17_to_64_tokens_on_small_matrices(oxh, kind, n, rows, cols):
+    c = Case(n, rows, cols, n + rows, up_to_16(cols) + 16 * (n % 3), up_to_16(cols) + 16 * (n % 2), bias=n % 2 == 0, kind=kind)
+    assert same_bits(c.matmul(rows + n % 4), c.want())
+    x = floats(n, cols, kind, 12)
+    assert same_bits(linear(c, x, kind), c.want(*ref.quantize(ref.decode(x, kind))))
+
+
+@pytest.mark.parametrize("n,rows,cols", [(4400, 4400, 144), (4099, 4500, 130), (8193, 257, 64)])
+def test_matmul_of_more_than_a_round_of_large_tiles(oxh, n, rows, cols):
+    c = Case(n, rows, cols, 3, bias=True, kind=BF16)
+    assert same_bits(c.matmul(), c.want())
+
+
+def test_a_workspace_for_more_tokens_serves_fewer(oxh):
+    big = Case(700, 600, 5000, 1)
+    need = big.m.linear_workspace(700)
+    buf = mv.DeviceBuffer(need)
+    for n in (1, 17, 64, 65, 130, 333, 699):
+        c = Case(n, 600, 5000, 1)
+        x = floats(n, 5000, F32, n)
+        d_x = mv.DeviceBuffer.from_host(x)
+        for size in (need, (5000 + 63) // 64 * 64 * n + (4 * n + 15) // 16 * 16):      # the least: codes and scales
+            got = c.out(lambda d, s: c.m.linear(F32, d_x.ptr, 5000, n, F32, d, s, None, buf.ptr, size))
+            assert same_bits(got, c.want(*ref.quantize(x)))
+
+
+# ─── offsets that pass 32 bits ──────────────────────────────────────────
+
+
+def filled(oxh, size, byte):
+    d = mv.DeviceBuffer(size)
+    _lib.check(oxh.oxh_memset(d.ptr, byte, size, None))
+    return d
+
+
+@pytest.mark.parametrize("n", [3, 40, 150])
+def test_a_matrix_of_more_than_4_gib(oxh, n):
+    rows, cols, stride, last = 1100000, 70, 4096, 130
+    w = filled(oxh, rows * stride, 1)
+    tail, q = codes(last, cols, 5), codes(n, cols, 6)
+    w.upload(ref.padded(tail, stride, 3), (rows - last) * stride)
+    ws, qs = np.full(rows, 0.5, np.float32), np.arange(1, n + 1, dtype=np.float32)
+    d_ws, d_q, d_qs = (mv.DeviceBuffer.from_host(a) for a in (ws, ref.padded(q, 80, 9), qs))
+    out = mv.DeviceBuffer(2 * n * rows)
+    m = int8.Matrix(w.ptr, d_ws.ptr, rows, cols, stride)
+    m.matmul(d_q.ptr, 80, d_qs.ptr, n, F16, out.ptr, rows)
+    mv.sync()
+    for t in (0, n - 1):
+        got = out.download(np.uint16, rows, 2 * t * rows)
+        whole = np.concatenate([np.ones((1, cols), np.int8), tail])
+        want = ref.encode(ref.product(q[t:t + 1], qs[t:t + 1], whole, ws[:last + 1]), F16).view(np.uint16)[0]
+        assert (got[:rows - last] == want[0]).all() and np.array_equal(got[rows - last:], want[1:])
+
+
+def test_tokens_and_results_of_more_than_4_gib(oxh):
+    n, rows, cols, x_stride, out_stride, last = 300000, 20, 33, 4096, 4000, 300
+    d_x, out = filled(oxh, 4 * n * x_stride, 0x3F), filled(oxh, 4 * n * out_stride, 0x5A)
+    c = Case(n, rows, cols, 8)
+    x = floats(last, cols, F32, 9)
+    d_x.upload(ref.padded(x, x_stride, 7), 4 * (n - last) * x_stride)
+    buf = mv.DeviceBuffer(c.m.linear_workspace(n))
+    c.m.linear(F32, d_x.ptr, x_stride, n, F32, out.ptr, out_stride, None, buf.ptr, c.m.linear_workspace(n))
+    mv.sync()
+    first = np.full((1, cols), np.frombuffer(b"\x3f" * 4, np.float32)[0])
+    want = c.want(*ref.quantize(np.concatenate([first, x])))
+    got = out.download(np.float32, last * out_stride, 4 * (n - last) * out_stride).reshape(last, out_stride)
+    assert same_bits(got[:, :rows], want[1:]) and (got[:, rows:].view(np.uint32) == 0x5A5A5A5A).all()
+    got = out.download(np.float32, 1000 * out_stride).reshape(1000, out_stride)
+    assert same_bits(got[:, :rows], np.repeat(want[:1], 1000, axis=0)) and (got[:, rows:].view(np.uint32) == 0x5A5A5A5A).all()
+
+
 # ─── experts ────────────────────────────────────────────────────────────
 
 
@@ -326,6 +403,47 @@ def test_the_layer_takes_the_routing_of_moe_route_too(oxh):
     got = lay.run(x, F32, mv.make_routing(*[b.ptr for b in d]), F32)
     ids, w = d[0].download(np.int32, n * k).reshape(n, k), d[1].download(np.float32, n * k).reshape(n, k)
     lay.check(got, x, F32, ids, w, F32)
+
+
+@pytest.mark.parametrize("n", [3, 60, 300])
+def test_a_routing_that_is_none_stays_in_bounds(oxh, n):
+    """Offsets that fall, positions behind the last pair: clamped; the layer's next call is not touched by it."""
+    e, k = 8, 2
+    lay = Layer(e, k, 64, 48, n)
+    x, (ids, w) = floats(n, 64, F32, 3), choices(np.random.default_rng(n), n, e, k)
+    routing, keep = lay.route(ids, w)
+    good = [b.download(np.uint32, b.nbytes // 4) for b in keep]
+    for offsets in ([0, n * k] * 4 + [0], [0xFFFFFFFF] * 9, [0, 0, 0xFFFFFFFF, 1, n * k, 0, n * k, 2, n * k], [n * k] * 9):
+        keep[3].upload(np.array(offsets, np.uint32))
+        keep[4].upload(np.random.default_rng(1).integers(0, 2 ** 32, size=n * k).astype(np.uint32))
+        keep[5].upload(np.random.default_rng(2).integers(0, 2 ** 32, size=n * k).astype(np.uint32))
+        lay.run(x, F32, routing, F32)
+    for b, a in zip(keep, good):
+        b.upload(a)
+    lay.check(lay.run(x, F32, routing, F32), x, F32, ids, w, F32)
+
+
+@pytest.mark.parametrize("n", [2, 50, 200])
+def test_expert_stacks_of_more_than_4_gib(oxh, n):
+    """All tokens go to the last expert of 512; a layer of that expert alone has to give the same bits."""
+    e, hidden, ffn, stride = 512, 64, 2100, 4112
+    one = Layer(1, 1, hidden, ffn, n)
+    stacks = []
+    for name, rows in (("gate", ffn), ("up", ffn), ("down", hidden)):
+        wide = stride if name != "down" else 2112 + 65536 * 2
+        d = filled(oxh, e * rows * wide, 0)
+        d.upload(ref.padded(one.host[name][0][0], wide), (e - 1) * rows * wide)
+        s = mv.DeviceBuffer.from_host(np.concatenate([np.zeros((e - 1) * rows, np.float32), one.host[name][1][0]]))
+        stacks += [d, s]
+    all_ = Layer.__new__(Layer)
+    all_.e, all_.k, all_.hidden, all_.ffn = e, 1, hidden, ffn
+    all_.layer = int8.MoeLayer(*[b.ptr for b in stacks], e, 1, hidden, ffn, stride, 2112 + 65536 * 2, n)
+    x = floats(n, hidden, F32, 3)
+    got = []
+    for lay in (one, all_):
+        routing, keep = lay.route(np.full((n, 1), lay.e - 1), np.full((n, 1), 0.75))
+        got.append(lay.run(x, F32, routing, F32))
+    assert np.array_equal(got[0], got[1]) and np.abs(got[0]).max() > 0
 
 
 # ─── as they are used together ──────────────────────────────────────────

@@ -147,6 +147,30 @@ def test_expert_layers_refused():
         assert call(Layer(), routing=mv.make_routing(*[0 if j == i else A for j in range(6)])) == _lib.ERR_ARG
 
 
+def test_more_results_than_any_memory_holds_are_refused():
+    big = int8.Matrix(A, A, 1 << 21, 64, 64)
+    refused(big.matmul, A, 64, A, (1 << 16) + 1, int8.F32, A, 1 << 21)
+    refused(big.linear, int8.F32, A, 64, (1 << 16) + 1, int8.F32, A, 1 << 21, d_ws=A, ws_bytes=1 << 40)
+    need, wide = ctypes.c_size_t(), Layer(n_expert=64, top_k=16, ffn=131071, down_stride=131072)
+    assert _lib.lib().oxh_moe_i8_workspace_bytes(ctypes.byref(wide.desc), 16384, ctypes.byref(need)) == _lib.OK
+    assert _lib.lib().oxh_moe_i8_workspace_bytes(ctypes.byref(wide.desc), 16385, ctypes.byref(need)) == _lib.ERR_ARG
+
+
+def test_workspaces_for_more_tokens_serve_fewer():
+    for rows, cols in ((8, 100), (4096, 14336), (600, 5000), (128, 131071), (5000, 64)):
+        m = int8.Matrix(A, A, rows, cols, (cols + 15) // 16 * 16)
+        least = [n * ((cols + 63) // 64 * 64) + (4 * n + 15) // 16 * 16 for n in range(1, 700)]
+        assert all(m.linear_workspace(n) >= least[n - 1] for n in range(17, 700))
+    need, last = ctypes.c_size_t(), 0
+    for n in range(1, 3000):
+        layer = Layer(n_expert=512, top_k=8, hidden=64, ffn=32)
+        assert _lib.lib().oxh_moe_i8_workspace_bytes(ctypes.byref(layer.desc), n, ctypes.byref(need)) == _lib.OK
+        assert need.value >= last
+        last = need.value
+    sizes = [mv.MoeRouter(384, 8).workspace_bytes(n) for n in range(1, 20000)]
+    assert all(a <= b for a, b in zip(sizes, sizes[1:]))
+
+
 def test_a_valid_call_without_a_device_says_so():
     import torch
     if torch.cuda.is_available():
