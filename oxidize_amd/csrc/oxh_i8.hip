@@ -1002,6 +1002,7 @@ static int check_matrix(const char *who, const OxhI8Matrix *w)
 
 typedef I8Geom<8, 4, 2, 4, 5> I8Large;        /* 256 x 256, a workgroup per CU */
 typedef I8Geom<4, 4, 2, 4, 5> I8Half;         /* 128 x 256, one */
+typedef I8Geom<4, 3, 2, 4, 5> I8Wide;         /* 128 x 192, one */
 typedef I8Geom<2, 4, 4, 2, 5> I8Mid;          /* 128 x 128, two */
 typedef I8Geom<2, 2, 2, 2, 5> I8Small;        /* 64 x 64, four */
 
@@ -1012,7 +1013,7 @@ typedef I8Geom<2, 2, 2, 2, 5> I8Small64;    /* 64 rows x 64, 32 pairs */
 typedef I8Geom<2, 1, 2, 2, 5> I8Small32;
 
 /* How a product runs: on which tile, its columns in how many parts. */
-enum { I8_LARGE = 0, I8_HALF, I8_MID, I8_SMALL, I8_TILES };
+enum { I8_LARGE = 0, I8_HALF, I8_WIDE, I8_MID, I8_SMALL, I8_TILES };
 struct I8Way {
     int tile;
     uint32_t splits;
@@ -1021,41 +1022,45 @@ struct I8Way {
 static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return splits > 1 ? (size_t)splits * n * ((rows + 3u) & ~(size_t)3u) * 4u : 0; }
 #define I8_MAX_PARTS_BYTES ((size_t)64 << 20)
 
-/* Microseconds that a stage of 128 columns takes a CU that works on `c` tiles at a time: 1.3 (large; 1.5 round after round), 0.88 (0.95), 0.48 / 0.8
- * and 0.36 / 0.4 / 0.55 / 0.75, from launches that give every CU exactly that many (for instance 512 x 4096 x 4096 in small
- * tiles, two to a CU, 32 stages: 18.5 us, of which 3 are launch and first loads and 1.7 the results). */
-static double stage_us(int tile, size_t c, bool full)
-{
-    static const double mid[3] = { 0, 0.48, 0.8 }, small[5] = { 0, 0.36, 0.40, 0.55, 0.75 };
-    switch (tile) {
-    case I8_LARGE: return full ? 1.5 : 1.3;
-    case I8_HALF:  return full ? 0.95 : 0.88;
-    case I8_MID:   return mid[c];
-    default:       return small[c];
-    }
-}
+/* The tiles: how many a CU holds at a time, and the microseconds that a stage of 128 columns takes a CU that works on so many of them, in a
+ * launch that is done at once and round after round.  These, and the other times of product_us(), are fitted to 1600 launches
+ * (256 to 151936 rows, 896 to 16000 columns, 65 to 4096 tokens, every tile, 1 to 8 parts): the way they choose takes 1.3 % more than the best of
+ * its launches on the average, 16 % at the worst (6000 x 16000 under 512 tokens, 82 us against 73).  128 x 192 is there for token counts
+ * that leave tiles of 128 and 256 half empty (4096 x 14336 under 333: 36.9 us in three parts, 39.2 the best without it;
+ * 160: 24.2 and 25.5). */
+struct I8Pace {
+    uint32_t rows, tok, held;
+    double alone[4], rounds;
+};
+static const I8Pace i8_pace[I8_TILES] = {
+    { 256, 256, 1, { 1.14 }, 1.30 },
+    { 128, 256, 1, { 0.79 }, 0.79 },
+    { 128, 192, 1, { 0.60 }, 0.74 },
+    { 128, 128, 2, { 0.56, 0.82 }, 0.85 },
+    { 64, 64, 4, { 0.33, 0.37, 0.52, 0.76 }, 0.58 },
+};
 
-static size_t tile_count(int tile, size_t rows, size_t n)
+static size_t tile_count(const I8Pace &t, size_t rows, size_t n)
 {
-    static const size_t tile_rows[I8_TILES] = { 256, 128, 128, 64 }, tile_tok[I8_TILES] = { 256, 256, 128, 64 };
-    return ((rows + tile_rows[tile] - 1) / tile_rows[tile]) * ((n + tile_tok[tile] - 1) / tile_tok[tile]);
+    return ((rows + t.rows - 1) / t.rows) * ((n + t.tok - 1) / t.tok);
 }
 #define I8_MAX_TILES ((size_t)1 << 23)      /* of 512 threads: a grid of 2^32 */
 
 /* What a product takes: rounds of what the CUs hold at a time, the last one with as many tiles to a CU as are left; results
- * at 5 TB/s; partial sums written and read at 4 TB/s and a second launch. */
+ * and partial sums, written and read, and the second launch that those take. */
 static double product_us(int tile, uint32_t splits, size_t rows, size_t stages, size_t n, size_t cus)
 {
-    static const size_t held[I8_TILES] = { 1, 1, 2, 4 };
-    const size_t tiles = tile_count(tile, rows, n) * splits;
-    const size_t k = (stages + splits - 1) / splits, rounds = tiles / (cus * held[tile]), rest = tiles - rounds * cus * held[tile];
-    double us = 3.0 + (double)rounds * ((double)k * stage_us(tile, held[tile], true) + 1.5);
+    const I8Pace &t = i8_pace[tile];
+    const size_t tiles = tile_count(t, rows, n) * splits;
+    const size_t k = (stages + splits - 1) / splits, rounds = tiles / (cus * t.held), rest = tiles - rounds * cus * t.held;
+    double us = 1.8 + (double)rounds * ((double)k * t.rounds + 0.66);
     if (rest) {
         const bool halves = tile == I8_LARGE && splits == 1 && rest <= cus / 2;
-        us += (double)k * stage_us(halves ? I8_HALF : tile, (rest + cus - 1) / cus, rounds != 0) + 1.5;
+        const I8Pace &last = halves ? i8_pace[I8_HALF] : t;
+        us += (double)k * (rounds && t.held == 1 ? last.rounds : last.alone[(rest + cus - 1) / cus - 1]) + 0.66;
     }
-    us += (double)n * (double)rows * 4.0 / 5e6;
-    if (splits > 1) us += 2.5 + (double)splits * (double)n * (double)rows * 8.0 / 4e6;
+    us += (double)n * (double)rows * 4.0 / 2.8e6;
+    if (splits > 1) us += 3.9 + (double)splits * (double)n * (double)rows * 8.0 / 4.7e6;
     return us;
 }
 
@@ -1068,7 +1073,7 @@ static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes, size_t 
         const size_t need = parts_bytes(rows, n, splits);
         if (splits > 1 && (need > ws_bytes || need > I8_MAX_PARTS_BYTES || n > 65535u)) break;
         for (int tile = 0; tile < I8_TILES; tile++) {
-            if (tile > I8_LARGE && tile_count(tile, rows, n) * splits >= I8_MAX_TILES) continue;
+            if (tile > I8_LARGE && tile_count(i8_pace[tile], rows, n) * splits >= I8_MAX_TILES) continue;
             const double us = product_us(tile, splits, rows, stages, n, cus);
             if (us < least) {
                 least = us;
@@ -1173,6 +1178,7 @@ static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride,
     if (way.splits > 1) p.parts = (int *)ws;
     if (way.tile == I8_LARGE) tiles_launch<I8Large>(p, st);
     else if (way.tile == I8_HALF) tiles_launch<I8Half>(p, st);
+    else if (way.tile == I8_WIDE) tiles_launch<I8Wide>(p, st);
     else if (way.tile == I8_MID) tiles_launch<I8Mid>(p, st);
     else tiles_launch<I8Small>(p, st);
     if (way.splits > 1) hipLaunchKernelGGL(k_i8_join, dim3((p.rows_pad / 4u + 255u) / 256u, p.n_vec), dim3(256), 0, st, p);
@@ -1190,6 +1196,7 @@ extern "C" int oxh_internal_i8_init(void)
     if ((e = whole_lds(k_i8_tiles<I8Large>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles_tail<I8Large, I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_tiles<I8Wide>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, true>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, false>)) != hipSuccess) return (int)e;
