@@ -666,7 +666,9 @@ int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t
  * [e*ffn, (e+1)*ffn), of down at rows [e*hidden, (e+1)*hidden)), a scale per
  * row.  n_expert <= 512, top_k <= 16, n_tok <= 65535.  The routing must be one
  * of n_tok tokens over n_expert experts with top_k choices; entries out of
- * range are clamped, never followed.  A fixed sequence of launches, capturable.
+ * range are clamped, never followed.  d_counts is not read; d_ids is, by a way
+ * for few pairs with the same results (NULL: not taken).  Launches that the
+ * sizes alone decide, capturable.
  * No output may overlap an input. */
 typedef struct OxhMoeI8 {
     const int8_t *d_w_gate, *d_w_up, *d_w_down;

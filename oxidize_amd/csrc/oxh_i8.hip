@@ -91,11 +91,19 @@ __device__ __forceinline__ uint32_t i8_top8(const float (&v)[8])
     return top;
 }
 
+/* the largest of sixteen neighbouring lanes' values, and of the wave's; every lane receives it, all lanes take part */
+__device__ __forceinline__ uint32_t row_top(uint32_t top)
+{
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0xB1, 0xF, 0xF, false));       /* lane ^ 1 */
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x4E, 0xF, 0xF, false));       /* lane ^ 2 */
+    top = max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x141, 0xF, 0xF, false));      /* mirrored in 8 */
+    return max(top, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)top, 0x140, 0xF, 0xF, false));     /* mirrored in 16 */
+}
 __device__ __forceinline__ uint32_t wave_top(uint32_t top)
 {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) top = max(top, (uint32_t)__shfl_xor((int)top, d));
-    return top;
+    const int row = (int)row_top(top);
+    return max(max((uint32_t)__builtin_amdgcn_readlane(row, 0), (uint32_t)__builtin_amdgcn_readlane(row, 16)),
+               max((uint32_t)__builtin_amdgcn_readlane(row, 32), (uint32_t)__builtin_amdgcn_readlane(row, 48)));
 }
 
 /* scale and 1 / scale of a row whose largest magnitude has the bits `top` (those of an infinity or a NaN are the
@@ -435,7 +443,15 @@ __device__ __forceinline__ void few_part(uint32_t stages, uint32_t part, uint32_
 __device__ __forceinline__ v4i few_join(const uint8_t *turns, uint32_t wave, uint32_t count)
 {
     v4i sums = { 0, 0, 0, 0 };
-    for (uint32_t k = 0; k < count; k++) sums += *reinterpret_cast<const v4i *>(turns + 2048u * (wave + k) + 16u * (threadIdx.x & 63u));
+    for (uint32_t k = 0; k < count; k += 4u) {                      /* four reads under way at a time */
+        v4i v[4];
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            v[i] = *reinterpret_cast<const v4i *>(turns + 2048u * (wave + min(k + i, count - 1u)) + 16u * (threadIdx.x & 63u));
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            if (k + i < count) sums += v[i];
+    }
     return sums;
 }
 
@@ -554,6 +570,33 @@ __global__ __launch_bounds__(1024) void k_i8_few_wide(const I8Product p, uint32_
 #define FEW_HELD 4u                                    /* times eight values of a token that a lane holds */
 #define FEW_HEAD_BYTES (FEW_TURN_BYTES + 128u)         /* and the scales, a maximum per wave */
 
+/* Codes of a row that `per` neighbouring waves hold, wave - w0 the first of them, this one from value 8 * (64 * w0 + lane) on, 512 * per apart;
+ * piece after piece n pieces apart, up to `end` codes.  Returns the scale; `store`: whether there is a row. */
+template <uint32_t HELD>
+__device__ __forceinline__ float few_codes(const float (&v)[HELD][8], uint32_t per, uint32_t w0, uint32_t wave, uint32_t *s_top, bool store,
+                                           uint8_t *codes, uint32_t n, uint32_t end)
+{
+    const uint32_t lane = threadIdx.x & 63u;
+    uint32_t top = 0;
+#pragma unroll
+    for (uint32_t i = 0; i < HELD; i++) top = max(top, i8_top8(v[i]));
+    top = wave_top(top);
+    if (lane == 0u) s_top[wave] = top;
+    __syncthreads();
+    top = row_top((lane & 15u) < per ? s_top[min(wave - w0 + (lane & 15u), FEW_WAVES - 1u)] : top);
+    float inv;
+    const float s = i8_scale(top, inv);
+    if (store) {
+#pragma unroll
+        for (uint32_t i = 0; i < HELD; i++) {
+            const uint32_t c = 8u * (64u * w0 + lane) + 512u * per * i;
+            if (c < end)
+                *reinterpret_cast<uint2 *>(codes + 16u * n * (c / 16u) + (c & 8u)) = inv != 0.0f ? i8_codes8(v[i], s, inv) : make_uint2(0u, 0u);
+        }
+    }
+    return s;
+}
+
 template <typename XT, int ST>
 __global__ __launch_bounds__(1024) void
 k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uint32_t team, uint32_t groups)
@@ -586,24 +629,8 @@ k_i8_few_float(const I8Product p, const XT *__restrict__ x, size_t x_stride, uin
     v4i w[ST][2];
     few_weights<ST>(w, wrow, first, stages, (cols - 1u) / 16u);
 
-    uint32_t top = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < FEW_HELD; i++) top = max(top, i8_top8(v[i]));
-    top = wave_top(top);
-    if (lane == 0u) s_top[wave] = top;
-    __syncthreads();
-    for (uint32_t k = 0; k < per; k++) top = max(top, s_top[wave - w0 + k]);
-    float inv;
-    const float s = i8_scale(top, inv);
-    if (t < n) {
-        if (w0 == 0u && lane == 0u) s_scale[t] = s;
-#pragma unroll
-        for (uint32_t i = 0; i < FEW_HELD; i++) {
-            const uint32_t c = c0 + step * i;
-            if (c < 16u * pieces)
-                *reinterpret_cast<uint2 *>(codes + 16u * ((c / 16u) * n + t) + (c & 8u)) = inv != 0.0f ? i8_codes8(v[i], s, inv) : make_uint2(0u, 0u);
-        }
-    }
+    const float s = few_codes(v, per, w0, wave, s_top, t < n, codes + 16u * t, n, 16u * pieces);
+    if (t < n && w0 == 0u && lane == 0u) s_scale[t] = s;
     __syncthreads();
 
     const uint8_t *mine_codes = codes + 16u * (kq * n + min(r16, n - 1u));
@@ -858,6 +885,114 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const 
         const v4i a = few_join(turns, wave * team, parts);
         const Run<float, 4> v = i8_pair_values<UP>(a, UP ? few_join(turns, wave * team + parts, parts) : a, s0, s1, st);
         i8_store4(p.out + (size_t)(t.first + r16) * p.out_stride + r, v.v, p.rows - r);
+    }
+}
+
+/* ─── the experts of a few tokens, pair by pair ───────────────────────── */
+
+/* A decode step has a handful of pairs, hardly two of one expert, and what it takes is launches: here there are two.  Nothing is sorted or
+ * tabled; a pair's expert is read from its id, and each launch quantises what it multiplies by itself, as k_i8_few_float does.  The sums are
+ * integers and the float steps those of the other kernels: the same results, bit by bit. */
+struct I8Pairs {
+    I8Experts e;
+    const int32_t *ids;
+    const float *weights;
+    uint32_t k, n_expert;
+};
+__device__ __forceinline__ uint32_t i8_pair_expert(const I8Pairs &p, uint32_t pair) { return min((uint32_t)p.ids[pair], p.n_expert - 1u); }
+
+/* h of pair blockIdx.y: `team` waves to a group of 16 rows, half of them gate, half up (k_i8_experts_few) */
+template <typename XT, int ST>
+__global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void
+k_i8_pair_up(const I8Pairs p, const XT *__restrict__ x, size_t x_stride, uint32_t team, uint32_t groups)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t few_shared[];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    uint32_t *const s_top = reinterpret_cast<uint32_t *>(few_shared + FEW_TURN_BYTES + 64u);
+    uint8_t *const codes = few_shared + FEW_HEAD_BYTES, *const turn = few_shared + 2048u * wave;
+    const uint32_t rows = p.e.rows, cols = p.e.cols, stages = (cols + 127u) / 128u, kq = lane >> 4;
+    const uint32_t teams = FEW_WAVES / team, parts = team / 2u, which = wave % team / parts;
+    float v[1][8];                                  /* 8192 columns a workgroup, as many as eight waves take of an expert's rows */
+    i8_values8<XT, false>(x + (size_t)(blockIdx.y / p.k) * x_stride, nullptr, 8u * (64u * wave + lane), cols, v[0]);
+    const I8ExpertTile t = { i8_pair_expert(p, blockIdx.y), blockIdx.y, 1u, 0u, 0u, 0u, { 0u, 0u } };
+    const uint32_t r0 = 16u * min(blockIdx.x * teams + wave / team, groups - 1u);
+    uint32_t first, mine;
+    few_part(stages, wave % parts, parts, first, mine);
+    const int8_t *wrow[2];
+#pragma unroll
+    for (uint32_t h = 0; h < 2u; h++)
+        wrow[h] = p.e.w[which] + ((size_t)t.expert * rows + min(r0 + 8u * h + (lane >> 3), rows - 1u)) * p.e.stride;
+    v4i w[ST][2];
+    few_weights<ST>(w, wrow, first, stages, (cols - 1u) / 16u);
+    const uint32_t g = blockIdx.x * teams + wave, r = 16u * g + 4u * kq;
+    float s0[4], s1[4];
+    if (ST <= 2) i8_pair_scales<true>(p.e, t, min(r, rows - 1u), s0, s1);
+    const float st = few_codes(v, FEW_WAVES, wave, wave, s_top, true, codes, 1u, 128u * stages);
+    __syncthreads();
+    v4i acc = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t i = 0; i < ST; i++)
+        if (i < mine)
+            few_stage(acc, w[i], turn, [&](uint32_t h) { return *reinterpret_cast<const v4i *>(codes + 16u * (8u * (first + i) + 4u * h + kq)); });
+    *reinterpret_cast<v4i *>(turn + 16u * lane) = acc;
+    if (ST > 2) i8_pair_scales<true>(p.e, t, min(r, rows - 1u), s0, s1);
+    __syncthreads();
+    if (wave < teams && g < groups && r < rows && (lane & 15u) == 0u) {
+        const Run<float, 4> hv = i8_pair_values<true>(few_join(few_shared, wave * team, parts), few_join(few_shared, wave * team + parts, parts), s0, s1, st);
+        i8_store4(p.e.out + (size_t)blockIdx.y * p.e.out_stride + r, hv.v, rows - r);
+    }
+}
+
+/* Results of token blockIdx.y, 16 rows of them: `per` waves to each of its pairs. */
+#define FEW_PAIRS_BYTES (FEW_HEAD_BYTES + 64u * OXH_SELECT_MAX_TOPK)       /* and a term per pair and row */
+template <typename T, int ST, int HELD>
+__global__ __launch_bounds__(1024, ST * HELD <= 4 ? 8 : 4) void
+k_i8_pair_down(const I8Pairs p, const float *__restrict__ h, size_t h_stride, T *__restrict__ out, size_t out_stride, uint32_t per)
+{
+    extern __shared__ __attribute__((aligned(16))) uint8_t few_shared[];
+    const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
+    float *const s_scale = reinterpret_cast<float *>(few_shared + FEW_TURN_BYTES), *const s_term = reinterpret_cast<float *>(few_shared + FEW_HEAD_BYTES);
+    uint32_t *const s_top = reinterpret_cast<uint32_t *>(few_shared + FEW_TURN_BYTES + 64u);
+    const uint32_t rows = p.e.rows, cols = p.e.cols, stages = (cols + 127u) / 128u, kq = lane >> 4, r0 = 16u * blockIdx.x;
+    const uint32_t j = min(wave / per, p.k - 1u), w0 = wave % per, pair = blockIdx.y * p.k + j;
+    const bool live = wave < per * p.k;
+    uint8_t *const codes = few_shared + FEW_PAIRS_BYTES + 128u * stages * j, *const turn = few_shared + 2048u * wave;
+    float v[HELD][8];
+#pragma unroll
+    for (uint32_t i = 0; i < HELD; i++)
+        i8_values8<float, false>(h + (size_t)pair * h_stride, nullptr, 8u * (64u * w0 + lane) + 512u * per * i, cols, v[i]);
+    uint32_t first, mine;
+    few_part(stages, w0, per, first, mine);
+    const int8_t *wrow[2];
+    const size_t row0 = (size_t)i8_pair_expert(p, pair) * rows;
+#pragma unroll
+    for (uint32_t i = 0; i < 2u; i++) wrow[i] = p.e.w[0] + (row0 + min(r0 + 8u * i + (lane >> 3), rows - 1u)) * p.e.stride;
+    v4i w[ST][2];
+    few_weights<ST>(w, wrow, first, stages, (cols - 1u) / 16u);
+    /* a thread per pair and row for the terms */
+    const uint32_t tj = min(threadIdx.x / 16u, p.k - 1u), tr = threadIdx.x % 16u, t_pair = blockIdx.y * p.k + tj;
+    const float sw = p.e.s[0][(size_t)i8_pair_expert(p, t_pair) * rows + min(r0 + tr, rows - 1u)], weight = p.weights[t_pair];
+    const float st = few_codes(v, per, w0, wave, s_top, live, codes, 1u, 128u * stages);
+    if (live && w0 == 0u && lane == 0u) s_scale[j] = st;
+    __syncthreads();
+    v4i acc = { 0, 0, 0, 0 };
+#pragma unroll
+    for (uint32_t i = 0; i < ST; i++)
+        if (i < mine)
+            few_stage(acc, w[i], turn, [&](uint32_t q) { return *reinterpret_cast<const v4i *>(codes + 16u * (8u * (first + i) + 4u * q + kq)); });
+    if ((lane & 15u) == 0u) *reinterpret_cast<v4i *>(turn + 16u * kq) = acc;
+    __syncthreads();
+    if (threadIdx.x < 16u * p.k) {
+        int sum = 0;
+#pragma unroll 4
+        for (uint32_t i = 0; i < per; i++) sum += *reinterpret_cast<const int *>(few_shared + 2048u * (tj * per + i) + 4u * tr);
+        s_term[threadIdx.x] = weight * ((float)sum * s_scale[tj] * sw);
+    }
+    __syncthreads();
+    if (threadIdx.x < 16u && r0 + threadIdx.x < rows) {
+        float total = 0.0f;
+        for (uint32_t i = 0; i < p.k; i++) total += s_term[16u * i + threadIdx.x];
+        out[blockIdx.y * out_stride + r0 + threadIdx.x] = from_f32<T>(total);
     }
 }
 
@@ -1380,6 +1515,50 @@ template <bool UP> static void experts_few_launch(I8Experts &e, hipStream_t st)
     else hipLaunchKernelGGL((k_i8_experts_few<8, UP>), grid, block, 0, st, e, team, groups);
 }
 
+/* Whether a layer goes pair by pair, in two launches instead of five.  It saves 5 to 7 us and pays in two ways: every workgroup quantises again,
+ * which shows once the weights take longer than that (7168 x 2048, 8 pairs of 44 MB: 82.2 us, 81.9 sorted; 128 experts of 2048 x 768, 8 pairs
+ * of 4.7 MB: 15.6 and 21.0, 32 of them: 31.0 and 38.7; 64 of 2048 x 1408, 18 of 8.7 MB: 41.8 and 40.7); and pairs of one expert read its weights
+ * each for itself (8 experts of 1024 x 2048, 32 pairs: 28.7 and 23.2).  A wave's columns of an expert's rows are loaded at once, and the
+ * codes have to fit. */
+#define PAIRS_MAX_BYTES ((size_t)160 << 20)
+struct PairsPlan {
+    uint32_t team, per;             /* waves to 16 rows of h; to a pair of the results */
+    size_t up_lds, down_lds;
+    bool taken;
+};
+static PairsPlan pairs_plan(const OxhMoeI8 *m, size_t n_tok)
+{
+    PairsPlan l = { 2u, FEW_WAVES / (uint32_t)m->top_k, 0, 0, false };
+    const size_t up_stages = (m->hidden + 127u) / 128u, down_stages = (m->ffn + 127u) / 128u, groups = (m->ffn + 15u) / 16u, pairs = n_tok * m->top_k;
+    while (l.team < FEW_WAVES && (up_stages * 2u > 4u * l.team || groups * pairs * l.team < i8_cus() * FEW_WAVES)) l.team *= 2u;
+    l.up_lds = FEW_HEAD_BYTES + 128u * up_stages;
+    l.down_lds = FEW_PAIRS_BYTES + 128u * down_stages * m->top_k;
+    l.taken = pairs <= 2u * m->n_expert && pairs * 3u * m->hidden * m->ffn <= PAIRS_MAX_BYTES && pairs <= 65535u &&
+              up_stages <= FEW_MAX_STAGES * FEW_WAVES / 2u && down_stages <= FEW_MAX_STAGES * l.per && m->ffn <= 512u * l.per * FEW_HELD &&
+              l.up_lds <= 65536u && l.down_lds <= 65536u;
+    return l;
+}
+
+template <typename T> static void pair_up_launch(const I8Pairs &p, const PairsPlan &l, uint32_t pairs, const void *x, size_t x_stride, hipStream_t st)
+{
+    const uint32_t groups = (p.e.rows + 15u) / 16u, teams = FEW_WAVES / l.team, stages = ((p.e.cols + 127u) / 128u + l.team / 2u - 1u) / (l.team / 2u);
+    const dim3 grid((groups + teams - 1u) / teams, pairs), block(64u * FEW_WAVES);
+    if (stages <= 2u) hipLaunchKernelGGL((k_i8_pair_up<T, 2>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
+    else if (stages <= 4u) hipLaunchKernelGGL((k_i8_pair_up<T, 4>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
+    else hipLaunchKernelGGL((k_i8_pair_up<T, 8>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
+}
+
+template <typename T> static void pair_down_launch(const I8Pairs &p, const PairsPlan &l, uint32_t n_tok, const float *h, size_t h_stride, void *out, size_t out_stride, hipStream_t st)
+{
+    const uint32_t stages = ((p.e.cols + 127u) / 128u + l.per - 1u) / l.per;
+    const dim3 grid((p.e.rows + 15u) / 16u, n_tok), block(64u * FEW_WAVES);
+#define OXH_DOWN(ST, HELD) hipLaunchKernelGGL((k_i8_pair_down<T, ST, HELD>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per)
+    if (stages <= 4u && p.e.cols <= 512u * l.per) OXH_DOWN(4, 1);
+    else if (stages <= 4u) OXH_DOWN(4, 4);
+    else OXH_DOWN(8, 4);
+#undef OXH_DOWN
+}
+
 template <bool UP> static void experts_run(I8Experts &e, uint32_t tok, hipStream_t st)
 {
     const uint32_t stages = (e.cols + 127u) / 128u;
@@ -1436,6 +1615,21 @@ extern "C" int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint
     int8_t *q = (int8_t *)(ws + p.q), *qh = (int8_t *)(ws + p.qh);
     float *q_scale = (float *)(ws + p.q_scale), *qh_scale = (float *)(ws + p.qh_scale), *h = (float *)(ws + p.h), *y = (float *)(ws + p.y);
     const size_t pairs = n_tok * m->top_k;
+    const PairsPlan few = pairs_plan(m, n_tok);
+    if (few.taken && routing->d_ids) {
+        I8Pairs a = { { { m->d_w_gate, m->d_w_up }, { m->d_s_gate, m->d_s_up }, m->gate_up_stride, nullptr, 0, nullptr, nullptr, nullptr, h, p.h_stride,
+                        (uint32_t)m->ffn, (uint32_t)m->hidden, (uint32_t)n_tok, 0u, 0u }, routing->d_ids, routing->d_weights, (uint32_t)m->top_k, (uint32_t)m->n_expert };
+        if (x_type == OXH_F32) pair_up_launch<float>(a, few, (uint32_t)pairs, d_x, x_stride, st);
+        else if (x_type == OXH_F16) pair_up_launch<_Float16>(a, few, (uint32_t)pairs, d_x, x_stride, st);
+        else pair_up_launch<__bf16>(a, few, (uint32_t)pairs, d_x, x_stride, st);
+        if ((rc = launched(who))) return rc;
+        a.e = { { m->d_w_down, m->d_w_down }, { m->d_s_down, m->d_s_down }, m->down_stride, nullptr, 0, nullptr, nullptr, nullptr, nullptr, 0,
+                (uint32_t)m->hidden, (uint32_t)m->ffn, (uint32_t)n_tok, 0u, 0u };
+        if (out_type == OXH_F32) pair_down_launch<float>(a, few, (uint32_t)n_tok, h, p.h_stride, d_out, out_stride, st);
+        else if (out_type == OXH_F16) pair_down_launch<_Float16>(a, few, (uint32_t)n_tok, h, p.h_stride, d_out, out_stride, st);
+        else pair_down_launch<__bf16>(a, few, (uint32_t)n_tok, h, p.h_stride, d_out, out_stride, st);
+        return launched(who);
+    }
     I8ExpertTile *tiles = (I8ExpertTile *)(ws + p.tiles);
     if (x_type == OXH_F32) experts_begin<float>(d_x, x_stride, n_tok, m->hidden, q, p.q_stride, q_scale, routing->d_offsets, m->n_expert, pairs, p.tok, tiles, p.n_tiles, st);
     else if (x_type == OXH_F16) experts_begin<_Float16>(d_x, x_stride, n_tok, m->hidden, q, p.q_stride, q_scale, routing->d_offsets, m->n_expert, pairs, p.tok, tiles, p.n_tiles, st);

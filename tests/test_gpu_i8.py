@@ -370,6 +370,36 @@ def test_expert_layer(oxh, n, e, k, hidden, ffn, kind, out_kind):
     lay.check(got, x, kind, ids, w, out_kind)
 
 
+@pytest.mark.parametrize("n,e,k,hidden,ffn", [(1, 8, 2, 64, 96), (3, 32, 5, 200, 1000), (1, 16, 16, 130, 77), (2, 12, 1, 2048, 8000), (5, 64, 8, 2048, 768),
+                                              (1, 4, 3, 8190, 2500), (4, 40, 6, 1111, 1408), (1, 1, 1, 1, 1), (16, 8, 1, 48, 4100)])
+@pytest.mark.parametrize("kind,out_kind", [(F32, F32), (BF16, BF16), (F16, F16)], ids=["f32", "bf16", "f16"])
+def test_few_pairs_give_the_same_bits_both_ways(oxh, n, e, k, hidden, ffn, kind, out_kind):
+    """With the choices' ids the layer may go pair by pair, without them it goes by the sorted pairs."""
+    lay = Layer(e, k, hidden, ffn, n, pad=16 * (n % 2))
+    ids, w = choices(np.random.default_rng(n + k), n, e, k)
+    x = floats(n, hidden, kind, 6)
+    routing, keep = lay.route(ids, w)
+    got = lay.run(x, kind, routing, out_kind, hidden + n % 3, hidden + n % 2)
+    sorted_ = mv.make_routing(0, *[b.ptr for b in keep[1:]])
+    assert np.array_equal(got, lay.run(x, kind, sorted_, out_kind))
+    lay.check(got, x, kind, ids, w, out_kind)
+
+
+def test_few_pairs_with_spoiled_tokens_and_ids_out_of_range(oxh):
+    n, e, k = 4, 16, 2
+    lay = Layer(e, k, 100, 70, n)
+    x = floats(n, 100, F32, 1)
+    x[1, 3], x[2] = np.nan, 0.0
+    ids, w = choices(np.random.default_rng(2), n, e, k)
+    w[3] = 0.0
+    routing, keep = lay.route(ids, w)
+    got = lay.run(x, F32, routing, F32)
+    assert np.isnan(got[1]).all() and not got[2].any() and not got[3].any()
+    lay.check(got[[0, 2, 3]], x[[0, 2, 3]], F32, ids[[0, 2, 3]], w[[0, 2, 3]], F32)
+    keep[0].upload(np.array([-1, 16, 2 ** 31 - 1, -2 ** 31, 5, 999, 0, 15], np.int32))
+    lay.run(x, F32, routing, F32)
+
+
 @pytest.mark.parametrize("n", [40, 200])
 def test_expert_layer_with_uneven_loads(oxh, n):
     """Most tokens on the first expert, several without any; and all of them on one."""
