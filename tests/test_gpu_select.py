@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 import i8_ref as ref
+from oxidize_amd import _lib
 from oxidize_amd import matvec as mv
 
 pytestmark = pytest.mark.gpu
@@ -45,7 +46,7 @@ def check(got, logits, k, score, n_group=1, top_group=1, group_best=1, bias=None
 @pytest.mark.parametrize("n,e,k,groups,top,best", [
     (1, 1, 1, 1, 1, 1), (1, 8, 2, 1, 1, 1), (16, 8, 8, 1, 1, 1), (63, 60, 4, 4, 2, 2), (64, 64, 6, 8, 3, 1), (65, 64, 6, 8, 3, 2),
     (100, 65, 5, 5, 1, 1), (129, 128, 16, 1, 1, 1), (500, 160, 6, 8, 3, 1), (1000, 256, 8, 8, 4, 2), (4096, 16, 2, 1, 1, 1),
-    (4097, 32, 4, 4, 2, 2), (8200, 12, 3, 3, 2, 2), (300, 512, 16, 64, 2, 2), (77, 511, 7, 7, 3, 2), (17000, 4, 1, 1, 1, 1)])
+    (4097, 32, 4, 4, 2, 2), (1024, 48, 5, 3, 2, 2), (1025, 48, 5, 1, 1, 1), (2049, 300, 12, 4, 3, 2), (65535, 24, 2, 1, 1, 1), (8200, 12, 3, 3, 2, 2), (300, 512, 16, 64, 2, 2), (77, 511, 7, 7, 3, 2), (17000, 4, 1, 1, 1, 1)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])
 def test_select(oxh, n, e, k, groups, top, best, score):
     rng = np.random.default_rng(n + e)
@@ -118,3 +119,19 @@ def test_calls_may_follow_each_other_over_one_workspace(oxh):
     for n in (5000, 200, 30, 900):
         x = rng.normal(size=(n, 64)).astype(np.float32)
         check(select(x, ref.F32, 4, score="softmax"), x, 4, "softmax")
+
+
+def test_logits_of_more_than_4_gib(oxh):
+    n, e, k, stride, last = 65535, 40, 3, 20000, 50
+    d_l = mv.DeviceBuffer(4 * n * stride)
+    _lib.check(oxh.oxh_memset(d_l.ptr, 0, 4 * n * stride, None))
+    x = np.random.default_rng(3).normal(size=(last, e)).astype(np.float32)
+    d_l.upload(ref.padded(x, stride, 9), 4 * (n - last) * stride)
+    r = mv.MoeRouter(e, k)
+    sizes = dict(ids=n * k, weights=n * k, counts=e, offsets=e + 1, perm=n * k, slot_pos=n * k)
+    d = {name: mv.DeviceBuffer(4 * size) for name, size in sizes.items()}
+    ws = mv.DeviceBuffer(r.workspace_bytes(n))
+    r.select(ref.F32, d_l.ptr, stride, n, mv.make_routing(*[b.ptr for b in d.values()]), ws.ptr, ws.nbytes)
+    mv.sync()
+    got = {name: d[name].download(np.float32 if name == "weights" else np.int32, size) for name, size in sizes.items()}
+    check(got, np.concatenate([np.zeros((n - last, e), np.float32), x]), k, "softmax")
