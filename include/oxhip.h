@@ -593,7 +593,7 @@ typedef struct OxhRouting {
     float    *d_weights;
     uint32_t *d_counts, *d_offsets, *d_perm, *d_slot_pos;
 } OxhRouting;
-/* Bytes of workspace a call takes (0 up to 64 tokens; never less for more). */
+/* Bytes of workspace a call takes (0 up to 16 tokens; never less for more). */
 int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes);
 /* d_logits: n_tok rows of n_expert values of `logits_type` (OXH_F32, OXH_F16,
  * OXH_BF16), logits_stride elements apart.  d_workspace: 16-byte aligned,

@@ -7,7 +7,7 @@
  *
  * Sorting needs no sort: a workgroup takes at most 64 tokens, and a token chooses an expert at most once, so the
  * tokens of an expert are a 64-bit mask in LDS; its count is the mask's population and a pair's rank the population
- * below its token.  Up to 64 tokens one workgroup does all of it in one launch.  Above, every workgroup leaves its
+ * below its token.  For a few tokens one workgroup does all of it in one launch.  Above, every workgroup leaves its
  * counts (a byte each) and a second launch adds up those of the workgroups before it. */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
@@ -383,11 +383,14 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
 
 /* ─── host side ───────────────────────────────────────────────────────── */
 
-/* A workgroup's tokens: one wave to a SIMD while there are CUs left (256 experts, 65 tokens: 10.3 us in workgroups of four, 13.5 of
+/* One workgroup and one launch for as many tokens as it has waves; few experts take less of a wave's time (256 experts, 16 tokens: 10.5 us,
+ * in two launches 10.3; 64 tokens: 29.3 and 10.6; 64 experts, 24 tokens: 6.3 and 8.0). */
+static bool sel_single(const OxhMoeRouter *r, size_t n_tok) { return n_tok <= (r->n_expert <= 64u ? 2u : 1u) * SEL_WAVES; }
+
+/* A workgroup's tokens otherwise: one wave to a SIMD while there are CUs left (256 experts, 65 tokens: 10.3 us in workgroups of four, 13.5 of
  * sixteen), then more, for the second launch looks through the counts of all workgroups: no more than 256 of them up to 8192 tokens. */
 static uint32_t sel_tok_per_wg(size_t n_tok)
 {
-    if (n_tok <= SEL_TOKENS) return SEL_TOKENS;
     if (n_tok <= 1024u) return 4u;
     if (n_tok <= 2048u) return 8u;
     return n_tok <= 4096u ? 16u : n_tok <= 8192u ? 32u : SEL_TOKENS;
@@ -426,7 +429,7 @@ static size_t sel_workspace(const OxhMoeRouter *r, size_t n_tok)
     const uint32_t per = sel_tok_per_wg(n_tok);
     const size_t wgs = (n_tok + per - 1u) / per;
     /* where a workgroup takes more tokens there are fewer of them: never less than for fewer tokens */
-    return n_tok <= SEL_TOKENS ? 0 : (n_tok > 1024u && wgs < 256u ? 256u : wgs) * sel_hist_stride(r->n_expert);
+    return sel_single(r, n_tok) ? 0 : (n_tok > 1024u && wgs < 256u ? 256u : wgs) * sel_hist_stride(r->n_expert);
 }
 
 extern "C" int oxh_moe_select_workspace(const OxhMoeRouter *r, size_t n_tok, size_t *bytes)
@@ -483,7 +486,7 @@ extern "C" int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const
     a.slot_pos = out->d_slot_pos;
     a.hist = need ? (uint8_t *)d_workspace : nullptr;
     a.n_tok = (uint32_t)n_tok;
-    a.tok_per_wg = sel_tok_per_wg(n_tok);
+    a.tok_per_wg = need ? sel_tok_per_wg(n_tok) : SEL_TOKENS;
     a.n_expert = (uint32_t)r->n_expert;
     a.k = (uint32_t)r->top_k;
     a.n_group = r->n_group > 1 ? (uint32_t)r->n_group : 1u;

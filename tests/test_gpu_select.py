@@ -44,7 +44,7 @@ def check(got, logits, k, score, n_group=1, top_group=1, group_best=1, bias=None
 
 
 @pytest.mark.parametrize("n,e,k,groups,top,best", [
-    (1, 1, 1, 1, 1, 1), (1, 8, 2, 1, 1, 1), (16, 8, 8, 1, 1, 1), (63, 60, 4, 4, 2, 2), (64, 64, 6, 8, 3, 1), (65, 64, 6, 8, 3, 2),
+    (1, 1, 1, 1, 1, 1), (1, 8, 2, 1, 1, 1), (16, 8, 8, 1, 1, 1), (16, 300, 9, 1, 1, 1), (17, 300, 9, 6, 4, 2), (32, 64, 5, 1, 1, 1), (33, 64, 5, 2, 1, 1), (63, 60, 4, 4, 2, 2), (64, 64, 6, 8, 3, 1), (65, 64, 6, 8, 3, 2),
     (100, 65, 5, 5, 1, 1), (129, 128, 16, 1, 1, 1), (500, 160, 6, 8, 3, 1), (1000, 256, 8, 8, 4, 2), (4096, 16, 2, 1, 1, 1),
     (4097, 32, 4, 4, 2, 2), (1024, 48, 5, 3, 2, 2), (1025, 48, 5, 1, 1, 1), (2049, 300, 12, 4, 3, 2), (65535, 24, 2, 1, 1, 1), (8200, 12, 3, 3, 2, 2), (300, 512, 16, 64, 2, 2), (77, 511, 7, 7, 3, 2), (17000, 4, 1, 1, 1, 1)])
 @pytest.mark.parametrize("score", ["softmax", "sigmoid"])

@@ -97,7 +97,7 @@ def test_routers_refused(change):
 
 def test_select_refuses():
     r, rt = mv.MoeRouter(**ROUTER), mv.make_routing(A, A, A, A, A, A)
-    assert r.workspace_bytes(64) == 0
+    assert r.workspace_bytes(16) == 0
     need = r.workspace_bytes(1000)
     assert 0 < need <= 1000 * 64
     refused(r.workspace_bytes, 65536)
