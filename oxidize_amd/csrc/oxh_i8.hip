@@ -1139,7 +1139,10 @@ typedef I8Geom<8, 4, 2, 4, 5> I8Large;        /* 256 x 256, a workgroup per CU *
 typedef I8Geom<4, 4, 2, 4, 5> I8Half;         /* 128 x 256, one */
 typedef I8Geom<4, 3, 2, 4, 5> I8Wide;         /* 128 x 192, one */
 typedef I8Geom<2, 4, 4, 2, 5> I8Mid;          /* 128 x 128, two */
-typedef I8Geom<2, 2, 2, 2, 5> I8Small;        /* 64 x 64, four */
+/* 64 x 64, two, with a ring of nine: where there is hardly a tile per CU, loads have to be under way for four stages (4096 x 4096 under 96
+ * to 256 tokens: 10.1 to 11.4 us, with five blocks and four tiles to a CU 12.7 to 16.5) */
+typedef I8Geom<2, 2, 2, 2, 9> I8Small;
+typedef I8Geom<2, 2, 2, 2, 5> I8Many;         /* 64 x 64, four: many tiles of few columns (151936 x 896 under 64 tokens: 42.8 us, 45.5 in I8Small) */
 
 typedef I8Geom<2, 4, 4, 2, 5> I8Mid128;     /* 128 rows x 128, 64, 32 pairs */
 typedef I8Geom<2, 2, 4, 2, 5> I8Mid64;
@@ -1148,7 +1151,7 @@ typedef I8Geom<2, 2, 2, 2, 5> I8Small64;    /* 64 rows x 64, 32 pairs */
 typedef I8Geom<2, 1, 2, 2, 5> I8Small32;
 
 /* How a product runs: on which tile, its columns in how many parts. */
-enum { I8_LARGE = 0, I8_HALF, I8_WIDE, I8_MID, I8_SMALL, I8_TILES };
+enum { I8_LARGE = 0, I8_HALF, I8_WIDE, I8_MID, I8_SMALL, I8_MANY, I8_TILES };
 struct I8Way {
     int tile;
     uint32_t splits;
@@ -1158,21 +1161,21 @@ static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return split
 #define I8_MAX_PARTS_BYTES ((size_t)64 << 20)
 
 /* The tiles: how many a CU holds at a time, and the microseconds that a stage of 128 columns takes a CU that works on so many of them, in a
- * launch that is done at once and round after round.  These, and the other times of product_us(), are fitted to 1600 launches
- * (256 to 151936 rows, 896 to 16000 columns, 65 to 4096 tokens, every tile, 1 to 8 parts): the way they choose takes 1.3 % more than the best of
- * its launches on the average, 16 % at the worst (6000 x 16000 under 512 tokens, 82 us against 73).  128 x 192 is there for token counts
- * that leave tiles of 128 and 256 half empty (4096 x 14336 under 333: 36.9 us in three parts, 39.2 the best without it;
- * 160: 24.2 and 25.5). */
+ * launch that is done at once and round after round.  These, and the other times of product_us(), are fitted to 5000 launches
+ * (256 to 151936 rows, 512 to 16000 columns, 17 to 4096 tokens, every tile, 1 to 8 parts): the way they choose takes 0.9 % more than the best of
+ * its launches on the average, 14 % at the worst (6416 x 512 under 1400 tokens, 20.2 us against 17.7).  128 x 192 is there for token counts
+ * that leave tiles of 128 and 256 half empty (4096 x 14336 under 333: 36.9 us in three parts, 39.2 the best without it). */
 struct I8Pace {
     uint32_t rows, tok, held;
     double alone[4], rounds;
 };
 static const I8Pace i8_pace[I8_TILES] = {
-    { 256, 256, 1, { 1.14 }, 1.30 },
-    { 128, 256, 1, { 0.79 }, 0.79 },
-    { 128, 192, 1, { 0.60 }, 0.74 },
-    { 128, 128, 2, { 0.56, 0.82 }, 0.85 },
-    { 64, 64, 4, { 0.33, 0.37, 0.52, 0.76 }, 0.58 },
+    { 256, 256, 1, { 1.28 }, 1.41 },
+    { 128, 256, 1, { 0.89 }, 0.72 },
+    { 128, 192, 1, { 0.74 }, 0.71 },
+    { 128, 128, 2, { 0.55, 0.94 }, 0.86 },
+    { 64, 64, 2, { 0.20, 0.39 }, 0.46 },
+    { 64, 64, 4, { 0.27, 0.46, 0.55, 0.92 }, 0.90 },
 };
 
 static size_t tile_count(const I8Pace &t, size_t rows, size_t n)
@@ -1181,21 +1184,23 @@ static size_t tile_count(const I8Pace &t, size_t rows, size_t n)
 }
 #define I8_MAX_TILES ((size_t)1 << 23)      /* of 512 threads: a grid of 2^32 */
 
-/* What a product takes: rounds of what the CUs hold at a time, the last one with as many tiles to a CU as are left; results
- * and partial sums, written and read, and the second launch that those take. */
+/* What a product takes: rounds of what the CUs hold at a time, the last one with as many tiles to a CU as are left, and a tile's results, which
+ * take a CU's time where no other tile is multiplied meanwhile; results and partial sums in memory, and the second launch that
+ * those take. */
 static double product_us(int tile, uint32_t splits, size_t rows, size_t stages, size_t n, size_t cus)
 {
     const I8Pace &t = i8_pace[tile];
     const size_t tiles = tile_count(t, rows, n) * splits;
     const size_t k = (stages + splits - 1) / splits, rounds = tiles / (cus * t.held), rest = tiles - rounds * cus * t.held;
-    double us = 1.8 + (double)rounds * ((double)k * t.rounds + 0.66);
+    const double end = 0.61 + (t.held == 1 ? 1.2 * t.rows * t.tok / 65536.0 : 0.0);
+    double us = 3.0 + (double)rounds * ((double)k * t.rounds + end);
     if (rest) {
         const bool halves = tile == I8_LARGE && splits == 1 && rest <= cus / 2;
         const I8Pace &last = halves ? i8_pace[I8_HALF] : t;
-        us += (double)k * (rounds && t.held == 1 ? last.rounds : last.alone[(rest + cus - 1) / cus - 1]) + 0.66;
+        us += (double)k * (rounds && t.held == 1 ? last.rounds : last.alone[(rest + cus - 1) / cus - 1]) + end;
     }
-    us += (double)n * (double)rows * 4.0 / 2.8e6;
-    if (splits > 1) us += 3.9 + (double)splits * (double)n * (double)rows * 8.0 / 4.7e6;
+    us += (double)n * (double)rows * 4.0 / 3.1e6;
+    if (splits > 1) us += 3.6 + (double)splits * (double)n * (double)rows * 8.0 / 5.2e6;
     return us;
 }
 
@@ -1315,7 +1320,8 @@ static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride,
     else if (way.tile == I8_HALF) tiles_launch<I8Half>(p, st);
     else if (way.tile == I8_WIDE) tiles_launch<I8Wide>(p, st);
     else if (way.tile == I8_MID) tiles_launch<I8Mid>(p, st);
-    else tiles_launch<I8Small>(p, st);
+    else if (way.tile == I8_SMALL) tiles_launch<I8Small>(p, st);
+    else tiles_launch<I8Many>(p, st);
     if (way.splits > 1) hipLaunchKernelGGL(k_i8_join, dim3((p.rows_pad / 4u + 255u) / 256u, p.n_vec), dim3(256), 0, st, p);
     return launched(who);
 }
@@ -1333,6 +1339,7 @@ extern "C" int oxh_internal_i8_init(void)
     if ((e = whole_lds(k_i8_tiles<I8Half>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Wide>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_tiles<I8Mid>)) != hipSuccess) return (int)e;
+    if ((e = whole_lds(k_i8_tiles<I8Small>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, true>)) != hipSuccess) return (int)e;
     if ((e = whole_lds(k_i8_experts<I8Mid128, I8Mid64, I8Mid32, false>)) != hipSuccess) return (int)e;
     return (int)hipSuccess;

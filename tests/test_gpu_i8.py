@@ -242,7 +242,8 @@ def test_matmul_of_17_to_64_tokens_on_small_matrices(oxh, kind, n, rows, cols):
 
 
 @pytest.mark.parametrize("n,rows,cols", [(4400, 4400, 144), (4099, 4500, 130), (8193, 257, 64), (191, 4090, 14300),
-                                         (333, 28600, 700), (1000, 4090, 1100), (1400, 3000, 1100), (450, 4096, 14300)])
+                                         (333, 28600, 700), (1000, 4090, 1100), (1400, 3000, 1100), (450, 4096, 14300),
+                                         (4400, 5001, 1100), (40, 70000, 200), (33, 15000, 900)])
 def test_matmul_in_every_tile(oxh, n, rows, cols):
     c = Case(n, rows, cols, 3, bias=True, kind=BF16)
     assert same_bits(c.matmul(), c.want())
