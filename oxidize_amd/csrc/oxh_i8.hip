@@ -1449,11 +1449,13 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
 
 /* ─── experts ─────────────────────────────────────────────────────────── */
 
-/* Pairs of a table entry: by how many an expert gets on average. */
+/* Pairs of a table entry: by how many an expert gets on average (6: 64 experts of 2048 x 1408 take 120 us in tiles of 64, 127 in the few
+ * tokens' way; 9: 122 and 137; 4: 118 and 121, and 8 of 4096 x 14336 277 and 269.  62: 128 of 2048 x 768 take 190 us in tiles of 128, 202 of 64; 25:
+ * 16 of 568 x 6448 take 86 and 75). */
 static uint32_t experts_tok(size_t pairs, size_t n_expert)
 {
     const size_t avg = pairs / n_expert;
-    return avg <= 10 ? FEW_TOKENS : avg <= 44 ? 64u : 128u;
+    return avg <= 4 ? FEW_TOKENS : avg <= 44 ? 64u : 128u;
 }
 
 /* The most tiles any routing can need: an expert's runs make at most one tile that is not full. */
