@@ -1243,22 +1243,25 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
     hipLaunchKernelGGL(k_i8_tiles<G>, dim3(tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
 }
 
-/* The kernels for few tokens: how many waves share a group of 16 rows (0: they do not take the product).  Four stages a wave
- * leave room for two workgroups on a CU (151936 x 896 under one token: 27 us, 33 with eight); where the groups are few, all
- * of a CU's sixteen waves are wanted.  More than sixteen tokens only where that is one workgroup per CU and four stages a wave: the
- * tiles reach such a matrix late (4096 x 4096 under 17 to 64 tokens: 6.2 to 8.3 us, the tiles 9.3 to 10.8; 500 x 3001: 5 to 6.2 and
- * 7.7 to 8.1), but tokens read once per group of rows cost more than they do in tiles (14336 x 4096: 15.7 to 21.7 us, the
- * tiles 13.8 to 17.4). */
+/* The kernels for few tokens: how many waves share a group of 16 rows (0: they do not take the product); four stages a wave leave room for two
+ * workgroups on a CU, and where the groups are few, all of a CU's sixteen waves are wanted.  They reach a matrix sooner than the
+ * tiles, which need the first two stages of a tile before they multiply, but tokens read once per group of rows cost more than they
+ * do in tiles.  So they take, with the tiles' time behind theirs:
+ *  - what is a workgroup per CU and four stages a wave, up to 64 tokens (4096 x 4096 under 1 to 16: 5.7 to 6.4 us, 8.1 to 8.9;
+ *    under 17 to 64: 6.2 to 8.3, 9.1 to 10; 500 x 3001: 5.0 to 6.2, 8.2);
+ *  - what is a workgroup per CU, up to four (1404 x 13515 under one: 7.8, 9.3; under eight: 9.9, 9.6);
+ *  - many rounds of workgroups under one or two (151936 x 896: 27.1 and 27.9, 30.5 and 29.5; but 6000 x 16000, a round and a half:
+ *    21.0, 19.8). */
 #define FEW_WIDE_TOKENS 64u
 #define FEW_MAX_STAGES 8u
 static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
 {
     const size_t groups = (rows + 15u) / 16u, stages = (cols + 127u) / 128u;
-    if (n > FEW_WIDE_TOKENS || stages > FEW_MAX_STAGES * FEW_WAVES) return 0;
     uint32_t team = 1;
     while (team < FEW_WAVES && (stages > 4u * team || groups * team < cus * FEW_WAVES)) team *= 2u;
-    if (n > FEW_TOKENS && (stages > 4u * team || groups * team > cus * FEW_WAVES)) return 0;
-    return team;
+    if (stages > FEW_MAX_STAGES * team) return 0;
+    const size_t most = groups * team >= 3u * cus * FEW_WAVES ? 2u : groups * team > cus * FEW_WAVES ? 0u : stages > 4u * team ? 4u : FEW_WIDE_TOKENS;
+    return n <= most ? team : 0u;
 }
 
 struct FewGrid {
