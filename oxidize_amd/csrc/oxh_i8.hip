@@ -486,9 +486,10 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_few(const I8Produc
 
 /* 17 to 64 tokens, TF fragments of sixteen: the same, but a stage's tokens come as the weights do, eight rows of 128 bytes an
  * instruction, and are turned the same way, the next stage's requested as soon as these are in LDS. */
-template <int ST, int TF>
+template <int TF>
 __global__ __launch_bounds__(1024) void k_i8_few_wide(const I8Product p, uint32_t team, uint32_t groups)
 {
+    constexpr uint32_t ST = 2;                      /* few_team() gives these tokens no more */
     constexpr uint32_t TURN = TF > 2 ? TF * 1024u : 2048u;
     __shared__ __attribute__((aligned(16))) uint8_t turns[FEW_WAVES * TURN];
     const uint32_t lane = threadIdx.x & 63u, wave = (uint32_t)__builtin_amdgcn_readfirstlane((int)(threadIdx.x >> 6));
@@ -1243,24 +1244,35 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
     hipLaunchKernelGGL(k_i8_tiles<G>, dim3(tiles * p.splits), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
 }
 
-/* The kernels for few tokens: how many waves share a group of 16 rows (0: they do not take the product); four stages a wave leave room for two
- * workgroups on a CU, and where the groups are few, all of a CU's sixteen waves are wanted.  They reach a matrix sooner than the
- * tiles, which need the first two stages of a tile before they multiply, but tokens read once per group of rows cost more than they
- * do in tiles.  So they take, with the tiles' time behind theirs:
- *  - what is a workgroup per CU and four stages a wave, up to 64 tokens (4096 x 4096 under 1 to 16: 5.7 to 6.4 us, 8.1 to 8.9;
- *    under 17 to 64: 6.2 to 8.3, 9.1 to 10; 500 x 3001: 5.0 to 6.2, 8.2);
- *  - what is a workgroup per CU, up to four (1404 x 13515 under one: 7.8, 9.3; under eight: 9.9, 9.6);
- *  - many rounds of workgroups under one or two (151936 x 896: 27.1 and 27.9, 30.5 and 29.5; but 6000 x 16000, a round and a half:
- *    21.0, 19.8). */
+/* The kernels for few tokens: how many waves share a group of 16 rows (0: they cannot take the product).  Four stages a wave leave room
+ * for two workgroups on a CU, and where the groups are few, all of a CU's sixteen waves are wanted. */
 #define FEW_WIDE_TOKENS 64u
 #define FEW_MAX_STAGES 8u
-static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
+static uint32_t few_waves(size_t rows, size_t cols, size_t cus)
 {
     const size_t groups = (rows + 15u) / 16u, stages = (cols + 127u) / 128u;
     uint32_t team = 1;
     while (team < FEW_WAVES && (stages > 4u * team || groups * team < cus * FEW_WAVES)) team *= 2u;
-    if (stages > FEW_MAX_STAGES * team) return 0;
-    const size_t most = groups * team >= 3u * cus * FEW_WAVES ? 2u : groups * team > cus * FEW_WAVES ? 0u : stages > 4u * team ? 4u : FEW_WIDE_TOKENS;
+    return stages > FEW_MAX_STAGES * team ? 0u : team;
+}
+
+/* Whether they should.  They reach a matrix sooner than the tiles, which need the first two stages of a tile before they multiply, but
+ * tokens read once per group of rows cost more than they do in tiles.  So they take, with matrices that come from memory and the
+ * tiles' time behind theirs:
+ *  - what is a workgroup per CU and two stages a wave, up to 64 tokens (4096 x 4096 under one: 6.7 us, 8.2; sixteen: 7.4, 9.0; 64:
+ *    9.3, 12.8; 500 x 3001 under sixteen: 5.5, 7.6);
+ *  - up to eight of what is a workgroup per CU and four stages (2048 x 7000: 8.1, 8.5; sixteen: 9.4, 8.6), or more on most of the
+ *    CUs (4096 x 14336: 15.0, 15.2; but 571 x 11128 under one: 9.3, 8.0);
+ *  - up to eight of what is more, if it is one and a half and a wave has two stages (14336 x 4096: 14.6, 15.5; 151936 x 896 under one:
+ *    27.3, 29.7; but 6000 x 16000 under one: 23.2, 22.8; 14631 x 629: 6.4, 5.4). */
+static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
+{
+    const size_t groups = (rows + 15u) / 16u, stages = (cols + 127u) / 128u, all = cus * FEW_WAVES;
+    const uint32_t team = few_waves(rows, cols, cus);
+    size_t most = 0;
+    if (groups * team > all) most = 2u * groups * team >= 3u * all && stages >= 2u * team ? 8u : 0u;
+    else if (stages <= 2u * team) most = FEW_WIDE_TOKENS;
+    else if (stages <= 4u * team || 4u * groups * team >= 3u * all) most = 8u;
     return n <= most ? team : 0u;
 }
 
@@ -1276,21 +1288,14 @@ static FewGrid few_grid(size_t rows, size_t cols, uint32_t team)
     return g;
 }
 
-template <int TF> static void few_wide_launch(const I8Product &p, uint32_t team, const FewGrid &g, hipStream_t st)
-{
-    const dim3 grid(g.wgs), block(64u * FEW_WAVES);
-    if (g.stages <= 2u) hipLaunchKernelGGL((k_i8_few_wide<2, TF>), grid, block, 0, st, p, team, g.groups);
-    else hipLaunchKernelGGL((k_i8_few_wide<4, TF>), grid, block, 0, st, p, team, g.groups);
-}
-
 static void few_launch(const I8Product &p, uint32_t team, hipStream_t st)
 {
     const FewGrid g = few_grid(p.w.rows, p.w.cols, team);
     const dim3 grid(g.wgs), block(64u * FEW_WAVES);
-    if (p.n_vec > 48u) return few_wide_launch<4>(p, team, g, st);
-    if (p.n_vec > 32u) return few_wide_launch<3>(p, team, g, st);
-    if (p.n_vec > 16u) return few_wide_launch<2>(p, team, g, st);
-    if (g.stages <= 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
+    if (p.n_vec > 48u) hipLaunchKernelGGL(k_i8_few_wide<4>, grid, block, 0, st, p, team, g.groups);
+    else if (p.n_vec > 32u) hipLaunchKernelGGL(k_i8_few_wide<3>, grid, block, 0, st, p, team, g.groups);
+    else if (p.n_vec > 16u) hipLaunchKernelGGL(k_i8_few_wide<2>, grid, block, 0, st, p, team, g.groups);
+    else if (g.stages <= 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
     else if (g.stages <= 4u) hipLaunchKernelGGL(k_i8_few<4>, grid, block, 0, st, p, team, g.groups);
     else hipLaunchKernelGGL(k_i8_few<8>, grid, block, 0, st, p, team, g.groups);
 }
@@ -1381,7 +1386,7 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
 static bool linear_fused(size_t rows, size_t cols, size_t n)
 {
     const size_t per = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;      /* waves a token, as in the kernel */
-    const uint32_t team = few_team(rows, cols, n, i8_cus());
+    const uint32_t team = few_waves(rows, cols, i8_cus());
     return team && n <= FEW_TOKENS && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= i8_cus();
 }
 
@@ -1437,7 +1442,7 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
     hipStream_t st = stream_of(stream);
     if (l.total == 0) {
         I8Product p = { *w, nullptr, 0, nullptr, d_bias, d_out, out_stride, nullptr, (uint32_t)n_vec, 1u, 0u, 0u, 0u, 0u, out_type };
-        const uint32_t team = few_team(w->rows, w->cols, n_vec, i8_cus());
+        const uint32_t team = few_waves(w->rows, w->cols, i8_cus());
         if (x_type == OXH_F32) few_float_launch(p, (const float *)d_x, x_stride, team, st);
         else if (x_type == OXH_F16) few_float_launch(p, (const _Float16 *)d_x, x_stride, team, st);
         else few_float_launch(p, (const __bf16 *)d_x, x_stride, team, st);
