@@ -119,7 +119,8 @@ __device__ __forceinline__ float i8_scale(uint32_t top, float &inv)
 }
 
 /* A row by a workgroup, eight values to a thread and step: once for the largest magnitude, once for the codes.  The first
- * HELD steps' values stay in registers; what is longer is read (and, GLU, computed) a second time. */
+ * HELD steps' values stay in registers; what is longer is read (and, GLU, computed) a second time.  Bound by memory: 4096 x 14336 bf16
+ * in 35 us, 5.1 TB/s read and written; one row of 4096 in 2.3 us, a trip to memory and two barriers. */
 template <typename T, bool GLU, int THREADS, int HELD>
 __device__ __forceinline__ void i8_quantize_row(const T *__restrict__ xr, const T *__restrict__ ur, uint32_t cols, int8_t *__restrict__ qr,
                                                 float *__restrict__ scale)
@@ -334,7 +335,7 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_tiles_tail(const I8Prod
 }
 
 /* The sums of a product whose columns were shared out: integers, the same in any order.  Four rows to a thread, four parts under
- * way at a time (one after the other, 333 x 4096 in five parts took 9 us). */
+ * way at a time (333 x 4096 in five parts: 9 us one after the other, 7.7 like this). */
 __global__ __launch_bounds__(256) void k_i8_join(const I8Product p)
 {
     const uint32_t r = (blockIdx.x * 256u + threadIdx.x) * 4u, t = blockIdx.y;
@@ -840,7 +841,9 @@ template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(c
         p.out + (size_t)t.first * p.out_stride + r0, p.out_stride, p.rows - r0, t.n);
 }
 
-/* G: as many pairs as a table entry can have; H, Q: fewer, for the last ones of an expert's. */
+/* G: as many pairs as a table entry can have; H, Q: fewer, for the last ones of an expert's.  2000 tokens, 8 of 128 experts of 2048 x 768:
+ * gate and up in 113 us (403 MB of weights, which take 65 alone, and 100 Gop, which take 42, with the empty places of the tiles 54), down in 83 (201 MB, and 131 of
+ * results). */
 template <typename G, typename H, typename Q, bool UP>
 __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts p)
 {
@@ -856,7 +859,8 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts
     else i8_experts_tile<G, UP>(p, t, row_tile);
 }
 
-/* Up to sixteen pairs of an expert, as k_i8_few: `team` waves share a group of 16 rows; UP: half of them take gate, half up. */
+/* Up to sixteen pairs of an expert, as k_i8_few: `team` waves share a group of 16 rows; UP: half of them take gate, half up.  Bound by
+ * memory: 8 experts of 4096 x 14336, 16 tokens of two: gate and up in 158 us, 5.9 TB/s, down in 97, 4.8 TB/s. */
 template <int ST, bool UP>
 __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const I8Experts p, uint32_t team, uint32_t groups)
 {
@@ -893,7 +897,8 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const 
 
 /* A decode step has a handful of pairs, hardly two of one expert, and what it takes is launches: here there are two.  Nothing is sorted or
  * tabled; a pair's expert is read from its id, and each launch quantises what it multiplies by itself, as k_i8_few_float does.  The sums are
- * integers and the float steps those of the other kernels: the same results, bit by bit. */
+ * integers and the float steps those of the other kernels: the same results, bit by bit.  One token, 8 experts of 2048 x 768: 8.8 and
+ * 6.0 us for 25 and 13 MB, a chain of id, weights and tokens, quantisation and joins behind the memory's 4.1 and 2. */
 struct I8Pairs {
     I8Experts e;
     const int32_t *ids;
@@ -997,7 +1002,8 @@ k_i8_pair_down(const I8Pairs p, const float *__restrict__ h, size_t h_stride, T 
     }
 }
 
-/* out[t] = sum over t's pairs, in their order, of weight * y.  Four columns to a thread, eight of the token's pairs under way at a time. */
+/* out[t] = sum over t's pairs, in their order, of weight * y.  Four columns to a thread, eight of the token's pairs under way at a
+ * time.  Bound by memory: 2000 tokens, 8 x 2048 each, in 21 us, 6.6 TB/s. */
 template <typename T>
 __global__ __launch_bounds__(256) void
 k_i8_combine(const float *__restrict__ y, size_t y_stride, const float *__restrict__ weights, const uint32_t *__restrict__ slot_pos,
