@@ -1239,11 +1239,11 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
     p.row_tiles = (uint32_t)((p.w.rows + G::ROWS - 1u) / G::ROWS);
     p.tok_tiles = (p.n_vec + G::TOK - 1u) / G::TOK;
     const uint32_t tiles = p.row_tiles * p.tok_tiles;
-    if constexpr (G::ROWS == I8Large::ROWS) {
+    if constexpr (G::ROWS == I8Large::ROWS && G::TOK == I8Large::TOK) {
         const uint32_t cus = (uint32_t)i8_cus(), rest = tiles % cus;
         if (p.splits == 1u && rest && rest <= cus / 2u) {
             p.whole = tiles - rest;
-            hipLaunchKernelGGL((k_i8_tiles_tail<I8Large, I8Half>), dim3(p.whole + 2u * rest), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
+            hipLaunchKernelGGL((k_i8_tiles_tail<G, I8Half>), dim3(p.whole + 2u * rest), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
             return;
         }
     }
