@@ -559,7 +559,8 @@ int oxh_moe_route(const float *d_logits, size_t n_tok, size_t n_expert, size_t t
  *           (group_best 1 or 2), and only the experts of the top_group best
  *           groups can be chosen.  n_group <= 1: all experts
  *   choice  the top_k largest keys, largest first; equal keys, and equal
- *           groups, go to the lower index
+ *           groups, go to the lower index.  Keys are held in 64 bits and
+ *           compared by the 43 leading bits of their mantissa
  *   weight  score, divided by the sum of the chosen scores when `renorm`,
  *           times `scale`; rounded once, to f32
  * An expert whose logit is -inf or NaN, or whose key is NaN or -inf, is
@@ -660,7 +661,8 @@ int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t
 /* A mixture-of-experts feed-forward over int8 stacks under a given routing
  * (oxh_moe_select's, or oxh_moe_route's):
  *   x of every token to codes; per expert and only for its own pairs gate and
- *   up, h = silu(gate) * up in f32, h to codes, down in f32;
+ *   up, h = silu(gate) * up in f32 (the hardware's exponential and
+ *   reciprocal, a unit in the last place each), h to codes, down in f32;
  *   out[t] = sum over t's pairs j, in their order, of weight[t][j] * down.
  * Matrices are stacked expert-major as in OxhMoe (expert e of gate / up at rows
  * [e*ffn, (e+1)*ffn), of down at rows [e*hidden, (e+1)*hidden)), a scale per

@@ -951,8 +951,8 @@ k_i8_pair_up(const I8Pairs p, const XT *__restrict__ x, size_t x_stride, uint32_
 
 /* Results of token blockIdx.y, 16 rows of them: `per` waves to each of its pairs. */
 #define FEW_PAIRS_BYTES (FEW_HEAD_BYTES + 64u * OXH_SELECT_MAX_TOPK)       /* and a term per pair and row */
-template <typename T, int ST, int HELD>
-__global__ __launch_bounds__(1024, ST * HELD <= 4 ? 8 : 4) void
+template <typename T, int ST>
+__global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void
 k_i8_pair_down(const I8Pairs p, const float *__restrict__ h, size_t h_stride, T *__restrict__ out, size_t out_stride, uint32_t per)
 {
     extern __shared__ __attribute__((aligned(16))) uint8_t few_shared[];
@@ -962,6 +962,7 @@ k_i8_pair_down(const I8Pairs p, const float *__restrict__ h, size_t h_stride, T 
     const uint32_t rows = p.e.rows, cols = p.e.cols, stages = (cols + 127u) / 128u, kq = lane >> 4, r0 = 16u * blockIdx.x;
     const uint32_t j = min(wave / per, p.k - 1u), w0 = wave % per, pair = blockIdx.y * p.k + j;
     const bool live = wave < per * p.k;
+    constexpr int HELD = ST <= 4 ? 1 : 2;           /* 512 columns a wave */
     uint8_t *const codes = few_shared + FEW_PAIRS_BYTES + 128u * stages * j, *const turn = few_shared + 2048u * wave;
     float v[HELD][8];
 #pragma unroll
@@ -1557,8 +1558,7 @@ static PairsPlan pairs_plan(const OxhMoeI8 *m, size_t n_tok)
     l.up_lds = FEW_HEAD_BYTES + 128u * up_stages;
     l.down_lds = FEW_PAIRS_BYTES + 128u * down_stages * m->top_k;
     l.taken = pairs <= 2u * m->n_expert && pairs * 3u * m->hidden * m->ffn <= PAIRS_MAX_BYTES && pairs <= 65535u &&
-              up_stages <= FEW_MAX_STAGES * FEW_WAVES / 2u && down_stages <= FEW_MAX_STAGES * l.per && m->ffn <= 512u * l.per * FEW_HELD &&
-              l.up_lds <= 65536u && l.down_lds <= 65536u;
+              up_stages <= FEW_MAX_STAGES * FEW_WAVES / 2u && down_stages <= FEW_MAX_STAGES * l.per && l.up_lds <= 65536u && l.down_lds <= 65536u;
     return l;
 }
 
@@ -1575,11 +1575,8 @@ template <typename T> static void pair_down_launch(const I8Pairs &p, const Pairs
 {
     const uint32_t stages = ((p.e.cols + 127u) / 128u + l.per - 1u) / l.per;
     const dim3 grid((p.e.rows + 15u) / 16u, n_tok), block(64u * FEW_WAVES);
-#define OXH_DOWN(ST, HELD) hipLaunchKernelGGL((k_i8_pair_down<T, ST, HELD>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per)
-    if (stages <= 4u && p.e.cols <= 512u * l.per) OXH_DOWN(4, 1);
-    else if (stages <= 4u) OXH_DOWN(4, 4);
-    else OXH_DOWN(8, 4);
-#undef OXH_DOWN
+    if (stages <= 4u) hipLaunchKernelGGL((k_i8_pair_down<T, 4>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per);
+    else hipLaunchKernelGGL((k_i8_pair_down<T, 8>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per);
 }
 
 template <bool UP> static void experts_run(I8Experts &e, uint32_t tok, hipStream_t st)
