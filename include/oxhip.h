@@ -609,10 +609,10 @@ int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const void *d_lo
  * calls: oxh_get_rows expands rows to f32, oxh_i8_quantize writes codes and
  * scales.  No counterpart in the reference.
  * Row r of such a matrix: `cols` codes at d + r * stride; d 16-byte aligned,
- * stride a multiple of 16, at least cols and at most 2^23.  The
- * bytes between cols and the next multiple of 16 are read and not used.  Any
- * cols from 1 to OXH_I8_MAX_COLS (the int32 sums of codes -128..127 cannot
- * overflow); more is OXH_ERR_TOO_WIDE. */
+ * stride a multiple of 16, at least cols and at most 2^23 (fastest: a multiple
+ * of 128 that is none of 4096).  The bytes between cols and the next multiple
+ * of 16 are read and not used.  Any cols from 1 to OXH_I8_MAX_COLS (the int32
+ * sums of codes -128..127 cannot overflow); more is OXH_ERR_TOO_WIDE. */
 #define OXH_I8_MAX_COLS 131071u
 /* element types of the float side (not GGUF type ids) */
 #define OXH_F32  0u

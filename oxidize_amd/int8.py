@@ -16,8 +16,10 @@ MAX_COLS = 131071
 
 
 def stride_of(cols):
-    """The row stride in bytes that rows of `cols` codes are best kept at."""
-    return (cols + 63) // 64 * 64
+    """The row stride in bytes that rows of `cols` codes are best kept at: whole lines of memory, and not a multiple of 4096, which sends
+    the same columns of all rows to the same channels (28672 x 4096 under 16 tokens: 24.1 us at 4224 bytes, 26.4 at 4096)."""
+    stride = (cols + 127) // 128 * 128
+    return stride + 128 if stride % 4096 == 0 else stride
 
 
 def quantize(x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, d_up=None, stream=None):
