@@ -52,7 +52,8 @@ def same_scale(a, b):
 @KINDS
 @pytest.mark.parametrize("n,cols,stride", [(1, 1, 1), (3, 2, 7), (2, 15, 15), (5, 16, 17), (4, 17, 32), (9, 255, 255), (1, 4096, 4096),
                                            (300, 100, 103), (2, 8191, 8200), (3, 14336, 14336), (2, 16384, 16384), (2, 16385, 16390),
-                                           (2, 40001, 40001), (1, 131071, 131071), (2000, 64, 64), (70, 1024, 1025), (513, 2050, 2050)])
+                                           (2, 40001, 40001), (1, 131071, 131071), (2000, 64, 64), (70, 1024, 1025), (513, 2050, 2050), (1100, 2049, 2051),
+                                           (1024, 8192, 8192)])
 def test_quantize(oxh, kind, n, cols, stride):
     x = floats(n, cols, kind, n * 31 + cols)
     q, s = run_quantize(x, kind, stride)
@@ -95,7 +96,7 @@ def test_quantize_rows_without_codes(oxh, kind):
 
 
 @KINDS
-@pytest.mark.parametrize("n,cols,stride", [(1, 1, 1), (3, 100, 101), (40, 4096, 4096), (2, 20000, 20000)])
+@pytest.mark.parametrize("n,cols,stride", [(1, 1, 1), (3, 100, 101), (40, 4096, 4096), (2, 20000, 20000), (1030, 2500, 2501)])
 def test_quantize_swiglu(oxh, kind, n, cols, stride):
     """v = silu(x) * up in f32 is within 12 * 2^-24 of itself (an exponential of two units in the last place whose argument is
     exact, a sum, a quotient, a product), so the scale within 13 and a code within half of one and 127 * 25 * 2^-24 of v / scale."""
