@@ -1600,7 +1600,8 @@ static void experts_begin(const void *x, size_t x_stride, size_t n_tok, size_t c
 #define OXH_BEGIN(THREADS, HELD)                                                                                                 \
     hipLaunchKernelGGL((k_i8_experts_begin<T, THREADS, HELD>), grid, dim3(THREADS), 0, st, (const T *)x, x_stride, (uint32_t)cols, q, \
                        q_stride, scale, offsets, (uint32_t)n_expert, (uint32_t)pairs, tok, tiles, n_tiles)
-    if (cols <= 2048u) OXH_BEGIN(256, 1);
+    if (cols <= 2048u) OXH_BEGIN(256, 1);           /* as quantize_launch(); the table wants 256 threads */
+    else if (cols <= 8192u && n_tok >= 1024u) OXH_BEGIN(256, 4);
     else OXH_BEGIN(1024, 2);
 #undef OXH_BEGIN
 }

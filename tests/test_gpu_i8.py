@@ -360,7 +360,7 @@ def choices(rng, n, e, k, skew=False):
 
 @pytest.mark.parametrize("n,e,k,hidden,ffn", [(1, 1, 1, 1, 1), (1, 8, 2, 64, 96), (2, 4, 3, 33, 50), (16, 8, 2, 256, 512), (7, 128, 8, 128, 48),
                                               (100, 3, 2, 200, 130), (300, 16, 4, 128, 160), (65, 512, 16, 96, 32), (64, 2, 1, 1000, 520),
-                                              (150, 5, 5, 300, 257), (1, 300, 16, 2048, 768), (3, 2, 2, 4096, 64), (2, 8, 2, 64, 5000)])
+                                              (150, 5, 5, 300, 257), (1, 300, 16, 2048, 768), (3, 2, 2, 4096, 64), (2, 8, 2, 64, 5000), (1030, 4, 1, 2100, 40)])
 @pytest.mark.parametrize("kind,out_kind", [(F32, F32), (BF16, BF16), (F16, F32)], ids=["f32", "bf16", "f16-f32"])
 def test_expert_layer(oxh, n, e, k, hidden, ffn, kind, out_kind):
     rng = np.random.default_rng(n + e + hidden)
