@@ -28,10 +28,11 @@ def quantize(x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, d_up=No
 
 
 class Matrix:
-    """An int8 matrix resident on the device, a scale per row; the memory is the caller's."""
+    """An int8 matrix resident on the device, a scale per row; the memory is the caller's.  `stride`: bytes from row to row (cols: rows
+    next to each other; :func:`stride_of` is fastest)."""
 
     def __init__(self, d_w, d_scale, rows, cols, stride=None):
-        self.desc = _lib.OxhI8Matrix(d_w, stride or stride_of(cols), d_scale, rows, cols)
+        self.desc = _lib.OxhI8Matrix(d_w, stride or cols, d_scale, rows, cols)
         self._ref = ctypes.byref(self.desc)
 
     def matmul_workspace(self, n_vec):
@@ -67,12 +68,12 @@ def from_packed(qtype, d_w, rows, cols, stream=None):
 
 class MoeLayer:
     """A mixture-of-experts feed-forward over int8 stacks under a given routing; owns its workspace, sized for
-    `max_tok` tokens."""
+    `max_tok` tokens.  Strides as :class:`Matrix`'s."""
 
     def __init__(self, d_w_gate, d_s_gate, d_w_up, d_s_up, d_w_down, d_s_down, n_expert, top_k, hidden, ffn, gate_up_stride=None,
                  down_stride=None, max_tok=16):
-        self.desc = _lib.OxhMoeI8(d_w_gate, d_w_up, d_w_down, d_s_gate, d_s_up, d_s_down, gate_up_stride or stride_of(hidden),
-                                  down_stride or stride_of(ffn), n_expert, top_k, hidden, ffn)
+        self.desc = _lib.OxhMoeI8(d_w_gate, d_w_up, d_w_down, d_s_gate, d_s_up, d_s_down, gate_up_stride or hidden,
+                                  down_stride or ffn, n_expert, top_k, hidden, ffn)
         self.hidden, self.max_tok = hidden, max_tok
         need = ctypes.c_size_t()
         check(lib().oxh_moe_i8_workspace_bytes(ctypes.byref(self.desc), max_tok, ctypes.byref(need)))

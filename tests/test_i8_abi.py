@@ -201,3 +201,9 @@ def test_oracle_selects_by_hand_worked_cases():
     assert ids[0].tolist() == [2, 0, 1] and w[0].tolist() == [1, 0, 0]
     ids, w = ref.select(np.full((1, 4), -np.inf), 2, "softmax")
     assert ids[0].tolist() == [0, 1] and w[0].tolist() == [0, 0]
+
+
+def test_strides_that_are_not_given_are_those_of_rows_next_to_each_other():
+    assert int8.Matrix(A, A, 8, 4096).desc.stride == 4096
+    refused(int8.Matrix(A, A, 8, 100).linear, int8.F32, A, 100, 1, int8.F32, A, 8)       # 100 is no multiple of 16
+    assert [int8.stride_of(c) for c in (1, 128, 129, 4000, 4096, 8190)] == [128, 128, 256, 4224, 4224, 8320]
