@@ -37,7 +37,7 @@ struct SelectArgs {
     float *weights;
     uint32_t *counts, *offsets, *perm, *slot_pos;
     uint8_t *hist;                  /* [workgroup][hist_stride] counts; NULL for a launch of one workgroup */
-    uint32_t n_tok, tok_per_wg, n_expert, k, n_group, top_group, group_best, score, renorm, hist_stride;
+    uint32_t n_tok, tok_per_wg, rows, rows_per_wg, n_expert, k, n_group, top_group, group_best, score, renorm, hist_stride;
     float scale;
 };
 
@@ -319,7 +319,9 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
 
 /* The positions of the pairs of many workgroups' tokens: the counts of all workgroups give the experts' runs, those of
  * the workgroups before this one where its own pairs start in them.  Sixteen counts to a load, rows dealt to the threads;
- * they are added up two to a word (an expert has at most one pair of a token, 65535 in all). */
+ * they are added up two to a word (an expert has at most one pair of a token, 65535 in all).  Up to 256 rows of counts have a workgroup
+ * each; more are taken several by one, for each looks through all of them (65535 tokens over 128 experts, both launches: 71 us, 87.9 with a
+ * workgroup to each of 1024 rows). */
 __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
 {
     __shared__ unsigned long long s_mask[OXH_SELECT_MAX_EXPERTS];
@@ -328,34 +330,49 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
     __shared__ uint32_t s_all[PLACE_COPIES][PLACE_WORDS + 8u], s_bef[PLACE_COPIES][PLACE_WORDS + 8u];
     __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_expert;
-    const uint32_t t0 = blockIdx.x * a.tok_per_wg, here = min(a.tok_per_wg, a.n_tok - t0);
-    /* the loads first: this workgroup's choices, the first rows of counts */
-    const uint32_t chunks = a.hist_stride / 16u, slices = PLACE_THREADS / chunks, c = tid % chunks, first = tid / chunks;
-    const uint32_t n_pairs = here * a.k;                /* at most 64 tokens of 16 choices: four a thread */
+    const uint32_t row0 = blockIdx.x * a.rows_per_wg, rows = min(a.rows_per_wg, a.rows - row0);
     uint32_t id[4];
+    /* a row's choices: at most 64 tokens of 16, four a thread */
+    auto choices = [&](uint32_t row) {
+        const uint32_t t0 = row * a.tok_per_wg, n_pairs = min(a.tok_per_wg, a.n_tok - t0) * a.k;
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; i++) id[i] = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid + PLACE_THREADS * i, n_pairs - 1u)];
+        for (uint32_t i = 0; i < 4u; i++) id[i] = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid + PLACE_THREADS * i, n_pairs - 1u)];
+    };
+    auto marks = [&](uint32_t n_pairs) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4u; i++)
+            if (tid + PLACE_THREADS * i < n_pairs) atomicOr(&s_mask[id[i]], 1ull << ((tid + PLACE_THREADS * i) / a.k));
+    };
+    /* the loads first: this workgroup's first choices, the first rows of counts */
+    choices(row0);
+    const uint32_t chunks = a.hist_stride / 16u, slices = PLACE_THREADS / chunks, c = tid % chunks, first = tid / chunks;
     uint32_t all[8] = { 0u }, bef[8] = { 0u };         /* experts 4i, 4i + 2 and 4i + 1, 4i + 3 of the chunk */
-    if (tid < slices * chunks)
-#pragma unroll 4
-        for (uint32_t b = first; b < gridDim.x; b += slices) {
-            const u32x4 v = *reinterpret_cast<const u32x4 *>(a.hist + (size_t)b * a.hist_stride + 16u * c);
-            const uint32_t on = b < blockIdx.x ? 0xFFFFFFFFu : 0u;
+    auto counts = [&](uint32_t b) { return *reinterpret_cast<const u32x4 *>(a.hist + (size_t)min(b, a.rows - 1u) * a.hist_stride + 16u * c); };
+    auto add = [&](const u32x4 &v, uint32_t b) {
+        const uint32_t there = b < a.rows ? 0x00FF00FFu : 0u, before = b < row0 ? 0x00FF00FFu : 0u;
 #pragma unroll
-            for (int i = 0; i < 4; i++) {
-                const uint32_t even = v[i] & 0x00FF00FFu, odd = (v[i] >> 8) & 0x00FF00FFu;
-                all[2 * i] += even;
-                all[2 * i + 1] += odd;
-                bef[2 * i] += even & on;
-                bef[2 * i + 1] += odd & on;
-            }
+        for (int i = 0; i < 4; i++) {
+            all[2 * i] += v[i] & there;
+            all[2 * i + 1] += (v[i] >> 8) & there;
+            bef[2 * i] += v[i] & before;
+            bef[2 * i + 1] += (v[i] >> 8) & before;
         }
+    };
+    if (tid < slices * chunks) {
+        if (a.rows <= slices) add(counts(first), first);
+        else
+            for (uint32_t b = first; b < a.rows; b += 4u * slices) {       /* four loads under way at a time */
+                u32x4 v[4];
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) v[j] = counts(b + j * slices);
+#pragma unroll
+                for (uint32_t j = 0; j < 4u; j++) add(v[j], b + j * slices);
+            }
+    }
     for (uint32_t e = tid; e < OXH_SELECT_MAX_EXPERTS; e += PLACE_THREADS) s_mask[e] = 0ull;
     for (uint32_t i = tid; i < PLACE_COPIES * (PLACE_WORDS + 8u); i += PLACE_THREADS) s_all[0][i] = s_bef[0][i] = 0u;
     __syncthreads();
-#pragma unroll
-    for (uint32_t i = 0; i < 4u; i++)
-        if (tid + PLACE_THREADS * i < n_pairs) atomicOr(&s_mask[id[i]], 1ull << ((tid + PLACE_THREADS * i) / a.k));
+    marks(min(a.tok_per_wg, a.n_tok - row0 * a.tok_per_wg) * a.k);
     if (tid < slices * chunks)
 #pragma unroll
         for (int i = 0; i < 8; i++) {
@@ -384,13 +401,27 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
         }
         if (tid == 0u) a.offsets[E] = a.n_tok * a.k;
     }
+    for (uint32_t row = row0; row < row0 + rows; row++) {
+        const uint32_t t0 = row * a.tok_per_wg, n_pairs = min(a.tok_per_wg, a.n_tok - t0) * a.k;
+        if (row > row0) {                               /* the row before is done: its pairs lie before this one's */
+            choices(row);
+            __syncthreads();
+            for (uint32_t e = tid; e < E; e += PLACE_THREADS) {
+                s_base[e] += (uint32_t)__popcll(s_mask[e]);
+                s_mask[e] = 0ull;
+            }
+            __syncthreads();
+            marks(n_pairs);
+            __syncthreads();
+        }
 #pragma unroll
-    for (uint32_t i = 0; i < 4u; i++) {
-        const uint32_t pair = tid + PLACE_THREADS * i, tt = pair / a.k;
-        if (pair >= n_pairs) break;
-        const uint32_t pos = s_base[id[i]] + half(s_bef[0], id[i]) + (uint32_t)__popcll(s_mask[id[i]] & ((1ull << tt) - 1ull));
-        a.perm[pos] = t0 + tt;
-        a.slot_pos[(size_t)t0 * a.k + pair] = pos;
+        for (uint32_t i = 0; i < 4u; i++) {
+            const uint32_t pair = tid + PLACE_THREADS * i, tt = pair / a.k;
+            if (pair >= n_pairs) break;
+            const uint32_t pos = s_base[id[i]] + half(s_bef[0], id[i]) + (uint32_t)__popcll(s_mask[id[i]] & ((1ull << tt) - 1ull));
+            a.perm[pos] = t0 + tt;
+            a.slot_pos[(size_t)t0 * a.k + pair] = pos;
+        }
     }
 }
 
@@ -510,13 +541,15 @@ extern "C" int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const
     a.hist_stride = sel_hist_stride(r->n_expert);
     a.scale = r->scale;
     const uint32_t wgs = (a.n_tok + a.tok_per_wg - 1u) / a.tok_per_wg;
+    a.rows = wgs;
+    a.rows_per_wg = (wgs + 255u) / 256u;
     hipStream_t st = (hipStream_t)(stream ? stream : oxh_internal_stream());
     if (logits_type == OXH_F32) sel_launch<float>(a, wgs, st);
     else if (logits_type == OXH_F16) sel_launch<_Float16>(a, wgs, st);
     else sel_launch<__bf16>(a, wgs, st);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && need) {
-        hipLaunchKernelGGL(k_moe_place, dim3(wgs), dim3(PLACE_THREADS), 0, st, a);
+        hipLaunchKernelGGL(k_moe_place, dim3((wgs + a.rows_per_wg - 1u) / a.rows_per_wg), dim3(PLACE_THREADS), 0, st, a);
         e = hipGetLastError();
     }
     if (e != hipSuccess) return oxh_internal_errorf(OXH_ERR_HIP, "HIP error in %s: %s", who, hipGetErrorString(e));
