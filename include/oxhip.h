@@ -661,8 +661,8 @@ int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t
 /* A mixture-of-experts feed-forward over int8 stacks under a given routing
  * (oxh_moe_select's, or oxh_moe_route's):
  *   x of every token to codes; per expert and only for its own pairs gate and
- *   up, h = silu(gate) * up in f32 (the hardware's exponential and
- *   reciprocal, a unit in the last place each), h to codes, down in f32;
+ *   up, h = silu(gate) * up in f32, h to codes (oxh_i8_quantize's of gate and
+ *   up as they lie in f32), down in f32;
  *   out[t] = sum over t's pairs j, in their order, of weight[t][j] * down.
  * Matrices are stacked expert-major as in OxhMoe (expert e of gate / up at rows
  * [e*ffn, (e+1)*ffn), of down at rows [e*hidden, (e+1)*hidden)), a scale per

@@ -479,6 +479,53 @@ def test_expert_stacks_of_more_than_4_gib(oxh, n):
     assert np.array_equal(got[0], got[1]) and np.abs(got[0]).max() > 0
 
 
+@pytest.mark.parametrize("e,by_ids", [(1, False), (10, False), (100, False), (150, True)], ids=["tiles-128", "tiles-64", "few", "pairs"])
+def test_silu_keeps_its_bits_far_from_zero(oxh, e, by_ids):
+    """One column of h: its code is 127 or -127 and its scale |h| / 127, so that the output is h itself but for three roundings, and
+    h = silu(g) * g for a g that the host knows to the bit.  Units of 2^-24: an exponential of two units in the last place 4, a sum, a quotient and a
+    product 3, the scale 1, its way back 1, none of them growing with g."""
+    n = 300
+    x = np.linspace(-87, 88, n).astype(np.float32)[np.random.default_rng(1).permutation(n)][:, None]
+    ones = mv.DeviceBuffer.from_host(np.full((e, 16), 1, np.int8))
+    unit = mv.DeviceBuffer.from_host(np.ones(e, np.float32))
+    lay = Layer.__new__(Layer)
+    lay.e, lay.k, lay.hidden, lay.ffn = e, 1, 1, 1
+    lay.layer = int8.MoeLayer(*[b.ptr for b in (ones, unit) * 3], e, 1, 1, 1, 16, 16, n)
+    routing, keep = lay.route(np.arange(n)[:, None] % e, np.ones((n, 1)))
+    got = lay.run(x, F32, routing if by_ids else mv.make_routing(0, *[b.ptr for b in keep[1:]]), F32)[:, 0]
+    q, s = ref.quantize(x)
+    g = (q[:, 0].astype(np.float32) * s).astype(np.float64)
+    want = ref.silu(g) * g
+    assert (np.abs(got - want) / np.abs(want)).max() <= 9.001 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("n,by_ids", [(2, True), (4, False), (44, False), (4000, False)], ids=["pairs", "few", "tiles-64", "tiles-128"])
+def test_codes_of_h_are_the_quantisers(oxh, n, by_ids):
+    """Down is the identity and one expert has all weight, so the output is code times scale: those of the quantiser and the products, called one
+    after the other."""
+    hidden = ffn = 512
+    lay = Layer(1, 1, hidden, ffn, n)
+    eye, unit = mv.DeviceBuffer.from_host(np.eye(ffn, dtype=np.int8)), mv.DeviceBuffer.from_host(np.ones(ffn, np.float32))
+    d_gate, d_up = lay.keep[:2], lay.keep[2:4]
+    d_gate[1].upload(lay.host["gate"][1][0] * np.float32(2))             # |g| up to about 10
+    lay.layer = int8.MoeLayer(*[b.ptr for b in (*d_gate, *d_up, eye, unit)], 1, 1, hidden, ffn, hidden, ffn, n)
+    routing, keep = lay.route(np.zeros((n, 1), np.int64), np.ones((n, 1)))
+    x = floats(n, hidden, F32, 12)
+    got = lay.run(x, F32, routing if by_ids else mv.make_routing(0, *[b.ptr for b in keep[1:]]), F32)
+    d_x, glu = mv.DeviceBuffer.from_host(x), [mv.DeviceBuffer(4 * n * ffn) for _ in range(2)]
+    for (w, s), out in zip((d_gate, d_up), glu):
+        m = int8.Matrix(w.ptr, s.ptr, ffn, hidden)
+        need = m.linear_workspace(n)
+        ws = mv.DeviceBuffer(max(16, need))
+        m.linear(F32, d_x.ptr, hidden, n, F32, out.ptr, ffn, None, ws.ptr, need)
+        mv.sync()
+    d_q, d_s = mv.DeviceBuffer(n * ffn), mv.DeviceBuffer(4 * n)
+    int8.quantize(F32, glu[0].ptr, ffn, n, ffn, d_q.ptr, ffn, d_s.ptr, glu[1].ptr)
+    mv.sync()
+    q, s = d_q.download(np.int8, n * ffn).reshape(n, ffn), d_s.download(np.float32, n)
+    assert np.array_equal(got.astype(np.float32), q.astype(np.float32) * s[:, None])
+
+
 # ─── as they are used together ──────────────────────────────────────────
 
 
