@@ -559,8 +559,7 @@ int oxh_moe_route(const float *d_logits, size_t n_tok, size_t n_expert, size_t t
  *           (group_best 1 or 2), and only the experts of the top_group best
  *           groups can be chosen.  n_group <= 1: all experts
  *   choice  the top_k largest keys, largest first; equal keys, and equal
- *           groups, go to the lower index.  Keys are held in 64 bits and
- *           compared by the 43 leading bits of their mantissa
+ *           groups, go to the lower index.  Keys are 64-bit floats
  *   weight  score, divided by the sum of the chosen scores when `renorm`,
  *           times `scale`; rounded once, to f32
  * An expert whose logit is -inf or NaN, or whose key is NaN or -inf, is

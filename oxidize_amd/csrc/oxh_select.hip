@@ -41,19 +41,14 @@ struct SelectArgs {
     float scale;
 };
 
-/* The order of 64-bit keys as the order of integers. */
+/* The order of 64-bit keys as the order of integers; the least key there is, -inf, maps to more than the two below. */
 __device__ __forceinline__ uint64_t sortable(double key)
 {
     const uint64_t b = (uint64_t)__double_as_longlong(key);
     return b >> 63 ? ~b : b | 0x8000000000000000ull;
 }
-
-/* An expert's key for the choice: the 43 leading bits of its key's mantissa, then the expert's number turned round, so that of equal
- * keys the lowest expert has the largest and no two are equal.  Masked experts come after all others, 0 cannot be chosen. */
-__device__ __forceinline__ uint64_t expert_key(double key, bool live, uint32_t e)
-{
-    return (live ? sortable(key) & ~511ull : 512ull) | (511u - e);
-}
+#define KEY_MASKED 1ull             /* chosen after all others */
+#define KEY_NONE 0ull               /* never chosen */
 
 /* e^x for x <= 709: x = k ln 2 + r, the series of e^r to its thirteenth power (|r| <= 0.347: what is left out is 4e-18 of it).  Half of
  * the instructions of the library's, which also looks after what cannot come here. */
@@ -107,14 +102,17 @@ __device__ __forceinline__ uint32_t wave_max32(uint32_t v)
                max((uint32_t)__builtin_amdgcn_readlane((int)v, 32), (uint32_t)__builtin_amdgcn_readlane((int)v, 48)));
 }
 
-/* The lane that holds the largest of different 64-bit keys: by its upper half, and by the lower one only where that does not tell. */
-__device__ __forceinline__ int wave_argmax64(uint64_t key)
+/* The lane that holds the largest 64-bit key: by its upper half, by the lower one only where that does not tell, and of equal keys the one
+ * of the lowest expert, `at` (expert e is lane e % 64's). */
+__device__ __forceinline__ int wave_argmax64(uint64_t key, uint32_t at)
 {
     const uint32_t hi = (uint32_t)(key >> 32), top = wave_max32(hi);
     unsigned long long who = __ballot(hi == top);
     if (who & (who - 1ull)) {
         const uint32_t lo = hi == top ? (uint32_t)key : 0u, low = wave_max32(lo);
-        who = __ballot(hi == top && lo == low);
+        const bool equal = hi == top && lo == low;
+        who = __ballot(equal);
+        if (who & (who - 1ull)) return (int)(~wave_max32(equal ? ~at : 0u) & 63u);
     }
     return __builtin_ctzll(who);
 }
@@ -175,6 +173,7 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
         const double ninf = -__builtin_inf();
         const bool softmax = a.score == OXH_SCORE_SOFTMAX;
         uint64_t key[NPL];
+        uint32_t at[NPL];
         float x[NPL], bias[NPL], top = -__builtin_inff();
 #pragma unroll
         for (int i = 0; i < NPL; i++) x[i] = sel_load<T>(a.logits, row + min(lane + 64u * i, E - 1u));
@@ -213,7 +212,8 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
             const uint32_t e = lane + 64u * i;
             const double p = s_score[wave][e] * factor, kv = p + (double)bias[i];
             const bool live = x[i] > -__builtin_inff() && kv > ninf;        /* a NaN is not */
-            key[i] = e < E ? expert_key(kv, live, e) : 0ull;
+            key[i] = e < E ? live ? sortable(kv) : KEY_MASKED : KEY_NONE;
+            at[i] = e;
             s_score[wave][e] = live ? p : 0.0;
             if (a.n_group > 1u) s_key[wave][e] = live ? kv : ninf;
         }
@@ -252,29 +252,35 @@ __global__ __launch_bounds__(1024) void k_moe_select(const SelectArgs a)
 #pragma unroll
             for (int i = 0; i < NPL; i++) {
                 const uint32_t e = lane + 64u * i;
-                if (e < E && !((kept >> (e / size * share)) & 1ull)) key[i] = 0ull;
+                if (e < E && !((kept >> (e / size * share)) & 1ull)) key[i] = KEY_NONE;
             }
         }
-        /* a lane's keys in descending order, of which only the first one is looked at */
+        /* a lane's keys in descending order, equal ones in the experts', of which only the first one is looked at */
 #pragma unroll
         for (int n = NPL - 1; n > 0; n--)
 #pragma unroll
             for (int i = 0; i < n; i++) {
                 const bool swap = key[i + 1] > key[i];
                 const uint64_t high = swap ? key[i + 1] : key[i], low = swap ? key[i] : key[i + 1];
+                const uint32_t first = swap ? at[i + 1] : at[i], second = swap ? at[i] : at[i + 1];
                 key[i] = high;
                 key[i + 1] = low;
+                at[i] = first;
+                at[i + 1] = second;
             }
         uint32_t my_id = 0;
 #pragma unroll 1
         for (uint32_t j = 0; j < a.k; j++) {
-            const int owner = wave_argmax64(key[0]);
-            const uint32_t id = 511u - ((uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)key[0], owner) & 511u);
+            const int owner = wave_argmax64(key[0], at[0]);
+            const uint32_t id = (uint32_t)__builtin_amdgcn_readlane((int)at[0], owner);
             my_id = lane == j ? id : my_id;
             if ((int)lane == owner) {
 #pragma unroll
-                for (int i = 0; i + 1 < NPL; i++) key[i] = key[i + 1];
-                key[NPL - 1] = 0ull;
+                for (int i = 0; i + 1 < NPL; i++) {
+                    key[i] = key[i + 1];
+                    at[i] = at[i + 1];
+                }
+                key[NPL - 1] = KEY_NONE;
             }
         }
         const double my_p = lane < a.k ? s_score[wave][my_id] : 0.0;

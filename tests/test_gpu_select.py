@@ -135,3 +135,22 @@ def test_logits_of_more_than_4_gib(oxh):
     mv.sync()
     got = {name: d[name].download(np.float32 if name == "weights" else np.int32, size) for name, size in sizes.items()}
     check(got, np.concatenate([np.zeros((n - last, e), np.float32), x]), k, "softmax")
+
+
+@pytest.mark.parametrize("e", [64, 130, 500])
+def test_keys_that_differ_in_their_last_bits(oxh, e):
+    """Sigmoids between 1 - 2^-43 and 1, and scores of 0.5 with biases down to the last bit of the sum, 2^-53: largest first,
+    wherever the experts lie among the lanes; equal ones by their number."""
+    rng = np.random.default_rng(e)
+    x = np.zeros((40, e), np.float32)
+    far = np.linspace(29.8, 35.8, 16).astype(np.float32)              # neighbours 4e-14 to 1e-16 apart
+    for t in range(40):
+        x[t, rng.choice(e, size=16, replace=False)] = far
+    got = select(x, ref.F32, 12, score="sigmoid", renorm=False)
+    check(got, x, 12, "sigmoid", renorm=False)
+    assert np.array_equal(np.take_along_axis(x, got["ids"].reshape(40, 12), 1), np.tile(far[:3:-1], (40, 1)))
+    bias, at = np.zeros(e, np.float32), rng.choice(e, size=8, replace=False)
+    bias[at] = np.arange(1, 9) * 2.0 ** -53
+    got = select(np.zeros((40, e), np.float32), ref.F32, 10, bias=bias, score="sigmoid")
+    zeros = np.setdiff1d(np.arange(e), at)[:2]
+    assert got["ids"].reshape(40, 10).tolist() == [at[::-1].tolist() + zeros.tolist()] * 40
