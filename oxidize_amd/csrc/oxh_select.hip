@@ -337,17 +337,15 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
     __shared__ uint32_t s_total[OXH_SELECT_MAX_EXPERTS], s_base[OXH_SELECT_MAX_EXPERTS];
     const uint32_t tid = threadIdx.x, lane = tid & 63u, wave = tid >> 6, E = a.n_expert;
     const uint32_t row0 = blockIdx.x * a.rows_per_wg, rows = min(a.rows_per_wg, a.rows - row0);
-    uint32_t id[4];
-    /* a row's choices: at most 64 tokens of 16, four a thread */
+    static_assert(SEL_TOKENS * OXH_SELECT_MAX_TOPK <= PLACE_THREADS, "a row's choices are one a thread at most");
+    uint32_t id;
+    const uint32_t tt = tid / a.k;                      /* the row's token whose choice this thread has */
     auto choices = [&](uint32_t row) {
         const uint32_t t0 = row * a.tok_per_wg, n_pairs = min(a.tok_per_wg, a.n_tok - t0) * a.k;
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) id[i] = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid + PLACE_THREADS * i, n_pairs - 1u)];
+        id = (uint32_t)a.ids[(size_t)t0 * a.k + min(tid, n_pairs - 1u)];
     };
     auto marks = [&](uint32_t n_pairs) {
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; i++)
-            if (tid + PLACE_THREADS * i < n_pairs) atomicOr(&s_mask[id[i]], 1ull << ((tid + PLACE_THREADS * i) / a.k));
+        if (tid < n_pairs) atomicOr(&s_mask[id], 1ull << tt);
     };
     /* the loads first: this workgroup's first choices, the first rows of counts */
     choices(row0);
@@ -420,13 +418,10 @@ __global__ __launch_bounds__(PLACE_THREADS) void k_moe_place(const SelectArgs a)
             marks(n_pairs);
             __syncthreads();
         }
-#pragma unroll
-        for (uint32_t i = 0; i < 4u; i++) {
-            const uint32_t pair = tid + PLACE_THREADS * i, tt = pair / a.k;
-            if (pair >= n_pairs) break;
-            const uint32_t pos = s_base[id[i]] + half(s_bef[0], id[i]) + (uint32_t)__popcll(s_mask[id[i]] & ((1ull << tt) - 1ull));
+        if (tid < n_pairs) {
+            const uint32_t pos = s_base[id] + half(s_bef[0], id) + (uint32_t)__popcll(s_mask[id] & ((1ull << tt) - 1ull));
             a.perm[pos] = t0 + tt;
-            a.slot_pos[(size_t)t0 * a.k + pair] = pos;
+            a.slot_pos[(size_t)t0 * a.k + tid] = pos;
         }
     }
 }

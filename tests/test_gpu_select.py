@@ -154,3 +154,9 @@ def test_keys_that_differ_in_their_last_bits(oxh, e):
     got = select(np.zeros((40, e), np.float32), ref.F32, 10, bias=bias, score="sigmoid")
     zeros = np.setdiff1d(np.arange(e), at)[:2]
     assert got["ids"].reshape(40, 10).tolist() == [at[::-1].tolist() + zeros.tolist()] * 40
+
+
+def test_rows_of_counts_with_a_choice_for_every_thread(oxh):
+    """64 tokens of 16 choices to a workgroup, the last one with a single token; ids that cover a row's 1024 threads."""
+    x = np.random.default_rng(6).normal(size=(8193 + 64, 20)).astype(np.float32)
+    check(select(x, ref.F32, 16, score="sigmoid"), x, 16, "sigmoid")
