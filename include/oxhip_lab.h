@@ -98,6 +98,22 @@ typedef struct OxhLab {
      * Else: 0, or 1 + the operation that has to be complete, and the first
      * five of the rest. */
     int (*plan_draft)(const OxhPlanOp *ops, size_t n_ops, uint32_t n_cu, uint64_t *out);
+    /* Which kernel an int8 product of these sizes runs on, on a device of n_cu
+     * compute units and with ws_bytes of workspace for partial sums: what the
+     * launch itself asks, as host arithmetic.  floats: oxh_i8_linear, else
+     * oxh_i8_matmul.  out[0]: 0 tiles, 1 the kernel of up to 16 tokens, 2 that
+     * of 17 to 64, 3 the one that quantises up to 16 itself.  Tiles: which
+     * (256 x 256, 128 x 256, 128 x 192, 128 x 128, 64 x 64 with a ring of nine
+     * blocks, 64 x 64 with one of five), parts of the columns, tiles of the
+     * last round that are done in halves.  Else: waves that share 16 rows, the
+     * stages of 128 columns that a wave's registers hold, tokens in sixteens
+     * (kernel 3: tokens). */
+    int (*i8_kernel)(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int floats, uint32_t out[4]);
+    /* The same for oxh_moe_ffn_i8, with or without d_ids: whether it goes pair
+     * by pair (1); else the pairs a tile may have (16, 64 or 128); and for gate
+     * and up, then for down, the stages that a wave of the few pairs' kernels
+     * holds, or 0 for tiles. */
+    int (*moe_i8_kernels)(const OxhMoeI8 *m, size_t n_tok, int ids, size_t n_cu, uint32_t out[4]);
 } OxhLab;
 
 const OxhLab *oxh_lab(void);

@@ -81,7 +81,9 @@ class OxhLab(ctypes.Structure):
                 ("experts_batch", ctypes.CFUNCTYPE(I, U32, Z, Z, Z, Z, Z, Z, Z)),
                 ("plan_by_value", ctypes.CFUNCTYPE(I, V)),
                 ("mmq32_fetched", ctypes.CFUNCTYPE(ctypes.c_uint64, U32, U32, U32, U32, U32)),
-                ("plan_draft", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhPlanOp), Z, U32, ctypes.POINTER(ctypes.c_uint64)))]
+                ("plan_draft", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhPlanOp), Z, U32, ctypes.POINTER(ctypes.c_uint64))),
+                ("i8_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, I, ctypes.POINTER(U32 * 4))),
+                ("moe_i8_kernels", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhMoeI8), Z, I, Z, ctypes.POINTER(U32 * 4)))]
 
 
 # name -> (restype, argtypes); every symbol include/oxhip.h and include/oxhip_lab.h declare

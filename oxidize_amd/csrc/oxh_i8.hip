@@ -1231,8 +1231,21 @@ static I8Way i8_way(size_t rows, size_t cols, size_t n, size_t ws_bytes, size_t 
     return best;
 }
 
+/* The kernel of a product over quantised tokens: `tile` in `splits` parts, or with `team` the few tokens'. */
+struct I8Choice {
+    uint32_t team;
+    I8Way way;
+};
+
 /* compute units; a count to plan a workspace with when there is no device yet */
 static size_t i8_cus(void) { return oxh_internal_n_cu() > 0 ? (size_t)oxh_internal_n_cu() : 256u; }
+
+/* the large tiles whose last round is done in half tiles: places behind the whole ones, or 0 */
+static uint32_t i8_tail(uint32_t tiles, uint32_t splits, size_t cus)
+{
+    const uint32_t rest = tiles % (uint32_t)cus;
+    return splits == 1u && rest <= cus / 2u ? rest : 0u;
+}
 
 template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
 {
@@ -1240,8 +1253,8 @@ template <typename G> static void tiles_launch(I8Product &p, hipStream_t st)
     p.tok_tiles = (p.n_vec + G::TOK - 1u) / G::TOK;
     const uint32_t tiles = p.row_tiles * p.tok_tiles;
     if constexpr (G::ROWS == I8Large::ROWS && G::TOK == I8Large::TOK) {
-        const uint32_t cus = (uint32_t)i8_cus(), rest = tiles % cus;
-        if (p.splits == 1u && rest && rest <= cus / 2u) {
+        const uint32_t rest = i8_tail(tiles, p.splits, i8_cus());
+        if (rest) {
             p.whole = tiles - rest;
             hipLaunchKernelGGL((k_i8_tiles_tail<G, I8Half>), dim3(p.whole + 2u * rest), dim3(G::WAVES * 64u), G::LDS_BYTES, st, p);
             return;
@@ -1282,15 +1295,18 @@ static uint32_t few_team(size_t rows, size_t cols, size_t n, size_t cus)
     return n <= most ? team : 0u;
 }
 
+/* the kernels' instance for waves of up to so many stages */
+static uint32_t few_held(uint32_t stages) { return stages <= 2u ? 2u : stages <= 4u ? 4u : FEW_MAX_STAGES; }
+
 struct FewGrid {
-    uint32_t groups, wgs, stages;   /* stages of a wave, at most */
+    uint32_t groups, wgs, held;     /* held: few_held() of a wave's stages */
 };
 static FewGrid few_grid(size_t rows, size_t cols, uint32_t team)
 {
     FewGrid g;
     g.groups = (uint32_t)((rows + 15u) / 16u);
     g.wgs = (g.groups + FEW_WAVES / team - 1u) / (FEW_WAVES / team);
-    g.stages = ((uint32_t)((cols + 127u) / 128u) + team - 1u) / team;
+    g.held = few_held(((uint32_t)((cols + 127u) / 128u) + team - 1u) / team);
     return g;
 }
 
@@ -1301,8 +1317,8 @@ static void few_launch(const I8Product &p, uint32_t team, hipStream_t st)
     if (p.n_vec > 48u) hipLaunchKernelGGL(k_i8_few_wide<4>, grid, block, 0, st, p, team, g.groups);
     else if (p.n_vec > 32u) hipLaunchKernelGGL(k_i8_few_wide<3>, grid, block, 0, st, p, team, g.groups);
     else if (p.n_vec > 16u) hipLaunchKernelGGL(k_i8_few_wide<2>, grid, block, 0, st, p, team, g.groups);
-    else if (g.stages <= 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
-    else if (g.stages <= 4u) hipLaunchKernelGGL(k_i8_few<4>, grid, block, 0, st, p, team, g.groups);
+    else if (g.held == 2u) hipLaunchKernelGGL(k_i8_few<2>, grid, block, 0, st, p, team, g.groups);
+    else if (g.held == 4u) hipLaunchKernelGGL(k_i8_few<4>, grid, block, 0, st, p, team, g.groups);
     else hipLaunchKernelGGL(k_i8_few<8>, grid, block, 0, st, p, team, g.groups);
 }
 
@@ -1312,9 +1328,16 @@ template <typename XT> static void few_float_launch(const I8Product &p, const XT
     const FewGrid g = few_grid(p.w.rows, p.w.cols, team);
     const dim3 grid(g.wgs), block(64u * FEW_WAVES);
     const size_t lds = few_float_lds(p.w.cols, p.n_vec);
-    if (g.stages <= 2u) hipLaunchKernelGGL((k_i8_few_float<XT, 2>), grid, block, lds, st, p, x, x_stride, team, g.groups);
-    else if (g.stages <= 4u) hipLaunchKernelGGL((k_i8_few_float<XT, 4>), grid, block, lds, st, p, x, x_stride, team, g.groups);
+    if (g.held == 2u) hipLaunchKernelGGL((k_i8_few_float<XT, 2>), grid, block, lds, st, p, x, x_stride, team, g.groups);
+    else if (g.held == 4u) hipLaunchKernelGGL((k_i8_few_float<XT, 4>), grid, block, lds, st, p, x, x_stride, team, g.groups);
     else hipLaunchKernelGGL((k_i8_few_float<XT, 8>), grid, block, lds, st, p, x, x_stride, team, g.groups);
+}
+
+static I8Choice i8_choice(size_t rows, size_t cols, size_t n, size_t ws_bytes, size_t cus)
+{
+    I8Choice c = { few_team(rows, cols, n, cus), { 0, 1u } };
+    if (!c.team) c.way = i8_way(rows, cols, n, ws_bytes, cus);
+    return c;
 }
 
 static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, const float *bias,
@@ -1322,12 +1345,12 @@ static int matmul_launch(const OxhI8Matrix *w, const int8_t *q, size_t q_stride,
 {
     I8Product p = { *w, q, q_stride, q_scale, bias, out, out_stride, nullptr, (uint32_t)n, 1u, 0u, 0u, 0u,
                     (uint32_t)((w->rows + 3u) & ~(size_t)3u), out_type };
-    const uint32_t team = few_team(w->rows, w->cols, n, i8_cus());
-    if (team) {
-        few_launch(p, team, st);
+    const I8Choice choice = i8_choice(w->rows, w->cols, n, ws_bytes, i8_cus());
+    if (choice.team) {
+        few_launch(p, choice.team, st);
         return launched(who);
     }
-    const I8Way way = i8_way(w->rows, w->cols, n, ws_bytes, i8_cus());
+    const I8Way way = choice.way;
     p.splits = way.splits;
     if (way.splits > 1) p.parts = (int *)ws;
     if (way.tile == I8_LARGE) tiles_launch<I8Large>(p, st);
@@ -1389,11 +1412,11 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
 /* Whether a product quantises its tokens in the launch itself: every workgroup does it again, so for few values (a second
  * launch costs about 3 us, the values of one token of 4096 about 1) and while there is no more than a workgroup per CU
  * (14336 x 4096 under one token, 448 workgroups: 16.5 us fused, 15.2 in two). */
-static bool linear_fused(size_t rows, size_t cols, size_t n)
+static bool linear_fused(size_t rows, size_t cols, size_t n, size_t cus)
 {
     const size_t per = n == 1 ? 16 : n == 2 ? 8 : n <= 4 ? 4 : n <= 8 ? 2 : 1;      /* waves a token, as in the kernel */
-    const uint32_t team = few_waves(rows, cols, i8_cus());
-    return team && n <= FEW_TOKENS && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= i8_cus();
+    const uint32_t team = few_waves(rows, cols, cus);
+    return team && n <= FEW_TOKENS && n * cols <= 16384u && cols <= 512u * per * FEW_HELD && few_grid(rows, cols, team).wgs <= cus;
 }
 
 /* the workspace otherwise: codes and scales of the tokens, the partial sums of the product */
@@ -1408,7 +1431,7 @@ static LinearParts linear_parts(size_t rows, size_t cols, size_t n)
     p.scale = p.q_stride * n;
     p.parts = p.scale + up16(4u * n);
     p.parts_bytes = few_team(rows, cols, n, i8_cus()) ? 0 : parts_bytes(rows, n, i8_way(rows, cols, n, SIZE_MAX, i8_cus()).splits);
-    p.total = linear_fused(rows, cols, n) ? 0 : p.parts + p.parts_bytes;
+    p.total = linear_fused(rows, cols, n, i8_cus()) ? 0 : p.parts + p.parts_bytes;
     return p;
 }
 
@@ -1525,17 +1548,27 @@ template <typename G, typename H, typename Q, bool UP> static void experts_launc
     hipLaunchKernelGGL((k_i8_experts<G, H, Q, UP>), dim3(e.row_tiles * e.n_tiles), dim3(G::WAVES * 64u), G::LDS_BYTES, st, e);
 }
 
-/* the experts' kernel for few pairs: waves to a group of rows, as few_team() */
-template <bool UP> static void experts_few_launch(I8Experts &e, hipStream_t st)
+/* How a product of the experts runs under a table whose entries have up to `tok` pairs: on the kernel for few pairs, `team` waves to a group of
+ * rows as few_team(), half of them gate where it is up's, or (held 0) on tiles. */
+struct ExpertsWay {
+    uint32_t team, held;
+};
+static ExpertsWay experts_way(bool up, size_t rows, size_t cols, uint32_t tok, size_t n_tiles, size_t cus)
 {
-    const uint32_t groups = (e.rows + 15u) / 16u, stages = (e.cols + 127u) / 128u, cus = (uint32_t)i8_cus();
-    uint32_t team = UP ? 2u : 1u;
-    while (team < FEW_WAVES && (stages * (UP ? 2u : 1u) > 4u * team || (size_t)groups * e.n_tiles * team < cus * FEW_WAVES)) team *= 2u;
-    const uint32_t teams = FEW_WAVES / team, parts = UP ? team / 2u : team, mine = (stages + parts - 1u) / parts;
+    const uint32_t groups = (uint32_t)((rows + 15u) / 16u), stages = (uint32_t)((cols + 127u) / 128u), halves = up ? 2u : 1u;
+    if (tok != FEW_TOKENS || stages > FEW_MAX_STAGES * FEW_WAVES / halves) return { 0u, 0u };
+    uint32_t team = halves;
+    while (team < FEW_WAVES && (stages * halves > 4u * team || (size_t)groups * n_tiles * team < cus * FEW_WAVES)) team *= 2u;
+    const uint32_t parts = team / halves;
+    return { team, few_held((stages + parts - 1u) / parts) };
+}
+template <bool UP> static void experts_few_launch(I8Experts &e, ExpertsWay way, hipStream_t st)
+{
+    const uint32_t groups = (e.rows + 15u) / 16u, teams = FEW_WAVES / way.team;
     const dim3 grid((groups + teams - 1u) / teams, e.n_tiles), block(64u * FEW_WAVES);
-    if (mine <= 2u) hipLaunchKernelGGL((k_i8_experts_few<2, UP>), grid, block, 0, st, e, team, groups);
-    else if (mine <= 4u) hipLaunchKernelGGL((k_i8_experts_few<4, UP>), grid, block, 0, st, e, team, groups);
-    else hipLaunchKernelGGL((k_i8_experts_few<8, UP>), grid, block, 0, st, e, team, groups);
+    if (way.held == 2u) hipLaunchKernelGGL((k_i8_experts_few<2, UP>), grid, block, 0, st, e, way.team, groups);
+    else if (way.held == 4u) hipLaunchKernelGGL((k_i8_experts_few<4, UP>), grid, block, 0, st, e, way.team, groups);
+    else hipLaunchKernelGGL((k_i8_experts_few<8, UP>), grid, block, 0, st, e, way.team, groups);
 }
 
 /* Whether a layer goes pair by pair, in two launches instead of five.  It saves 5 to 7 us and pays in two ways: every workgroup quantises again,
@@ -1546,14 +1579,17 @@ template <bool UP> static void experts_few_launch(I8Experts &e, hipStream_t st)
 #define PAIRS_MAX_BYTES ((size_t)160 << 20)
 struct PairsPlan {
     uint32_t team, per;             /* waves to 16 rows of h; to a pair of the results */
+    uint32_t up_held, down_held;    /* the kernels' instances; down has no <2> */
     size_t up_lds, down_lds;
     bool taken;
 };
-static PairsPlan pairs_plan(const OxhMoeI8 *m, size_t n_tok)
+static PairsPlan pairs_plan(const OxhMoeI8 *m, size_t n_tok, size_t cus)
 {
-    PairsPlan l = { 2u, FEW_WAVES / (uint32_t)m->top_k, 0, 0, false };
+    PairsPlan l = { 2u, FEW_WAVES / (uint32_t)m->top_k, 0, 0, 0, 0, false };
     const size_t up_stages = (m->hidden + 127u) / 128u, down_stages = (m->ffn + 127u) / 128u, groups = (m->ffn + 15u) / 16u, pairs = n_tok * m->top_k;
-    while (l.team < FEW_WAVES && (up_stages * 2u > 4u * l.team || groups * pairs * l.team < i8_cus() * FEW_WAVES)) l.team *= 2u;
+    while (l.team < FEW_WAVES && (up_stages * 2u > 4u * l.team || groups * pairs * l.team < cus * FEW_WAVES)) l.team *= 2u;
+    l.up_held = few_held(((uint32_t)up_stages + l.team / 2u - 1u) / (l.team / 2u));
+    l.down_held = ((uint32_t)down_stages + l.per - 1u) / l.per <= 4u ? 4u : FEW_MAX_STAGES;
     l.up_lds = FEW_HEAD_BYTES + 128u * up_stages;
     l.down_lds = FEW_PAIRS_BYTES + 128u * down_stages * m->top_k;
     l.taken = pairs <= 2u * m->n_expert && pairs * 3u * m->hidden * m->ffn <= PAIRS_MAX_BYTES && pairs <= 65535u &&
@@ -1563,25 +1599,24 @@ static PairsPlan pairs_plan(const OxhMoeI8 *m, size_t n_tok)
 
 template <typename T> static void pair_up_launch(const I8Pairs &p, const PairsPlan &l, uint32_t pairs, const void *x, size_t x_stride, hipStream_t st)
 {
-    const uint32_t groups = (p.e.rows + 15u) / 16u, teams = FEW_WAVES / l.team, stages = ((p.e.cols + 127u) / 128u + l.team / 2u - 1u) / (l.team / 2u);
+    const uint32_t groups = (p.e.rows + 15u) / 16u, teams = FEW_WAVES / l.team;
     const dim3 grid((groups + teams - 1u) / teams, pairs), block(64u * FEW_WAVES);
-    if (stages <= 2u) hipLaunchKernelGGL((k_i8_pair_up<T, 2>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
-    else if (stages <= 4u) hipLaunchKernelGGL((k_i8_pair_up<T, 4>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
+    if (l.up_held == 2u) hipLaunchKernelGGL((k_i8_pair_up<T, 2>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
+    else if (l.up_held == 4u) hipLaunchKernelGGL((k_i8_pair_up<T, 4>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
     else hipLaunchKernelGGL((k_i8_pair_up<T, 8>), grid, block, l.up_lds, st, p, (const T *)x, x_stride, l.team, groups);
 }
 
 template <typename T> static void pair_down_launch(const I8Pairs &p, const PairsPlan &l, uint32_t n_tok, const float *h, size_t h_stride, void *out, size_t out_stride, hipStream_t st)
 {
-    const uint32_t stages = ((p.e.cols + 127u) / 128u + l.per - 1u) / l.per;
     const dim3 grid((p.e.rows + 15u) / 16u, n_tok), block(64u * FEW_WAVES);
-    if (stages <= 4u) hipLaunchKernelGGL((k_i8_pair_down<T, 4>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per);
+    if (l.down_held == 4u) hipLaunchKernelGGL((k_i8_pair_down<T, 4>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per);
     else hipLaunchKernelGGL((k_i8_pair_down<T, 8>), grid, block, l.down_lds, st, p, h, h_stride, (T *)out, out_stride, l.per);
 }
 
 template <bool UP> static void experts_run(I8Experts &e, uint32_t tok, hipStream_t st)
 {
-    const uint32_t stages = (e.cols + 127u) / 128u;
-    if (tok == FEW_TOKENS && stages <= FEW_MAX_STAGES * FEW_WAVES / (UP ? 2u : 1u)) experts_few_launch<UP>(e, st);
+    const ExpertsWay way = experts_way(UP, e.rows, e.cols, tok, e.n_tiles, i8_cus());
+    if (way.held) experts_few_launch<UP>(e, way, st);
     else if (tok <= 64u) experts_launch<I8Small64, I8Small32, I8Small32, UP>(e, st);
     else experts_launch<I8Mid128, I8Mid64, I8Mid32, UP>(e, st);
 }
@@ -1635,7 +1670,7 @@ extern "C" int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint
     int8_t *q = (int8_t *)(ws + p.q), *qh = (int8_t *)(ws + p.qh);
     float *q_scale = (float *)(ws + p.q_scale), *qh_scale = (float *)(ws + p.qh_scale), *h = (float *)(ws + p.h), *y = (float *)(ws + p.y);
     const size_t pairs = n_tok * m->top_k;
-    const PairsPlan few = pairs_plan(m, n_tok);
+    const PairsPlan few = pairs_plan(m, n_tok, i8_cus());
     if (few.taken && routing->d_ids) {
         I8Pairs a = { { { m->d_w_gate, m->d_w_up }, { m->d_s_gate, m->d_s_up }, m->gate_up_stride, nullptr, 0, nullptr, nullptr, nullptr, h, p.h_stride,
                         (uint32_t)m->ffn, (uint32_t)m->hidden, (uint32_t)n_tok, 0u, 0u }, routing->d_ids, routing->d_weights, (uint32_t)m->top_k, (uint32_t)m->n_expert };
@@ -1673,4 +1708,49 @@ extern "C" int oxh_moe_ffn_i8(const OxhMoeI8 *m, const OxhRouting *routing, uint
     else OXH_COMBINE(__bf16);
 #undef OXH_COMBINE
     return launched(who);
+}
+
+/* ─── which kernels run, for tests ────────────────────────────────────── */
+
+extern "C" int oxh_debug_i8_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int floats, uint32_t out[4])
+{
+    static const char who[] = "oxh_debug_i8_kernel";
+    if (!out || !rows || !n_vec || !n_cu) return I8_ARG("%s: NULL or empty", who);
+    const int rc = check_cols(who, cols);
+    if (rc) return rc;
+    if (floats && linear_fused(rows, cols, n_vec, n_cu)) {
+        out[0] = 3u;
+        out[1] = few_waves(rows, cols, n_cu);
+        out[2] = few_grid(rows, cols, out[1]).held;
+        out[3] = (uint32_t)n_vec;
+        return OXH_OK;
+    }
+    const I8Choice c = i8_choice(rows, cols, n_vec, ws_bytes, n_cu);
+    if (c.team) {
+        out[0] = n_vec > FEW_TOKENS ? 2u : 1u;
+        out[1] = c.team;
+        out[2] = few_grid(rows, cols, c.team).held;
+        out[3] = (uint32_t)((n_vec + 15u) / 16u);
+        return OXH_OK;
+    }
+    out[0] = 0u;
+    out[1] = (uint32_t)c.way.tile;
+    out[2] = c.way.splits;
+    out[3] = c.way.tile == I8_LARGE ? i8_tail((uint32_t)tile_count(i8_pace[I8_LARGE], rows, n_vec), c.way.splits, n_cu) : 0u;
+    return OXH_OK;
+}
+
+extern "C" int oxh_debug_moe_i8_kernels(const OxhMoeI8 *m, size_t n_tok, int ids, size_t n_cu, uint32_t out[4])
+{
+    static const char who[] = "oxh_debug_moe_i8_kernels";
+    MoeI8Parts p;
+    if (!out || !n_cu) return I8_ARG("%s: NULL or empty", who);
+    const int rc = moe_parts(who, m, n_tok, &p);
+    if (rc) return rc;
+    const PairsPlan few = pairs_plan(m, n_tok, n_cu);
+    out[0] = few.taken && ids;
+    out[1] = out[0] ? 1u : p.tok;
+    out[2] = out[0] ? few.up_held : experts_way(true, m->ffn, m->hidden, p.tok, p.n_tiles, n_cu).held;
+    out[3] = out[0] ? few.down_held : experts_way(false, m->hidden, m->ffn, p.tok, p.n_tiles, n_cu).held;
+    return OXH_OK;
 }

@@ -108,6 +108,9 @@ int oxh_debug_mmq_kernel(uint32_t qtype, size_t rows, size_t cols, size_t n_vec,
 int oxh_debug_experts_batch(uint32_t qtype, size_t n_mat, size_t n_expert, size_t rows, size_t cols, size_t top_k, size_t n_tok,
                             size_t n_cu);
 int oxh_debug_experts_tile(uint32_t qtype, size_t n_mat, size_t n_expert, size_t rows, size_t pairs, size_t n_cu, uint32_t tile[2]);
+int oxh_debug_i8_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int floats, uint32_t out[4]);
+struct OxhMoeI8;
+int oxh_debug_moe_i8_kernels(const struct OxhMoeI8 *m, size_t n_tok, int ids, size_t n_cu, uint32_t out[4]);
 uint64_t oxh_debug_mmq32_fetched(uint32_t block_bytes, uint32_t blocks, uint32_t row, uint32_t blk, uint32_t step);
 int oxh_debug_subblock_sums(uint32_t qtype, const void *d_w, size_t rows, size_t cols, const void *d_act,
                             int32_t *d_sums, void *stream);

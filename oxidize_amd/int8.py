@@ -27,6 +27,25 @@ def quantize(x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, d_up=No
     check(lib().oxh_i8_quantize(x_type, d_x, x_stride, n_vec, cols, d_up, d_q, q_stride, d_scale, stream))
 
 
+TILE_256x256, TILE_128x256, TILE_128x192, TILE_128x128, TILE_64x64_RING, TILE_64x64 = range(6)
+TILES, FEW, FEW_WIDE, FEW_FLOAT = range(4)
+
+
+def kernel(rows, cols, n_vec, floats=False, ws_bytes=1 << 40, n_cu=256):
+    """Which kernel a product of these sizes runs on: (TILES, tile, parts, half tiles), or one of FEW.. with (waves to 16 rows, stages
+    a wave holds, tokens in sixteens); host arithmetic (include/oxhip_lab.h)."""
+    out = (ctypes.c_uint32 * 4)()
+    check(_lib.lab().i8_kernel(rows, cols, n_vec, n_cu, ws_bytes, int(floats), ctypes.byref(out)))
+    return tuple(out)
+
+
+def moe_kernels(desc, n_tok, ids=True, n_cu=256):
+    """(pair by pair?, pairs of a tile, stages gate and up hold or 0 for tiles, stages down holds) of a layer's launch."""
+    out = (ctypes.c_uint32 * 4)()
+    check(_lib.lab().moe_i8_kernels(ctypes.byref(desc), n_tok, int(ids), n_cu, ctypes.byref(out)))
+    return tuple(out)
+
+
 class Matrix:
     """An int8 matrix resident on the device, a scale per row; the memory is the caller's.  `stride`: bytes from row to row (cols: rows
     next to each other; :func:`stride_of` is fastest)."""

@@ -7,6 +7,7 @@ import numpy as np
 import pytest
 
 import i8_ref as ref
+import i8_shapes as shapes
 from oxidize_amd import _lib, int8
 from oxidize_amd import matvec as mv
 
@@ -207,3 +208,47 @@ def test_strides_that_are_not_given_are_those_of_rows_next_to_each_other():
     assert int8.Matrix(A, A, 8, 4096).desc.stride == 4096
     refused(int8.Matrix(A, A, 8, 100).linear, int8.F32, A, 100, 1, int8.F32, A, 8)       # 100 is no multiple of 16
     assert [int8.stride_of(c) for c in (1, 128, 129, 4000, 4096, 8190)] == [128, 128, 256, 4224, 4224, 8320]
+
+
+# ─── which kernels run ──────────────────────────────────────────────────
+
+
+def matmul_key(n, rows, cols, ws_bytes=1 << 40):
+    kernel, a, b, c = int8.kernel(rows, cols, n, ws_bytes=ws_bytes)
+    return (kernel, a, b > 1, c > 0) if kernel == int8.TILES else (kernel, b, c)
+
+
+def test_listed_sizes_run_on_the_kernels_they_are_listed_for():
+    for key, sizes in shapes.MATMUL.items():
+        for n, rows, cols in sizes:
+            assert matmul_key(n, rows, cols) == key, (n, rows, cols)
+            need = int8.Matrix(A, A, rows, cols, (cols + 15) // 16 * 16).matmul_workspace(n)
+            assert (need > 0) == (key[0] == int8.TILES and key[2])
+            assert matmul_key(n, rows, cols, need) == key
+    for held, sizes in shapes.LINEAR.items():
+        for n, rows, cols in sizes:
+            kernel, _, got, tokens = int8.kernel(rows, cols, n, floats=True)
+            assert (kernel, got, tokens) == (int8.FEW_FLOAT, held, n), (n, rows, cols)
+    for key, sizes in shapes.EXPERTS.items():
+        for n, e, k, hidden, ffn in sizes:
+            assert int8.moe_kernels(Layer(n_expert=e, top_k=k, hidden=hidden, ffn=ffn).desc, n, key[0]) == key, (n, e, k, hidden, ffn)
+
+
+def test_no_size_runs_on_a_kernel_that_has_none_listed():
+    """Sizes of all lengths: whatever kernel they run on is among the listed ones."""
+    rng = np.random.default_rng(1)
+    up, down = ({(key[0], key[1], key[i]) for key in shapes.EXPERTS} for i in (2, 3))
+
+    def length(lo, hi):
+        return int(round(np.exp(rng.uniform(np.log(lo), np.log(hi)))))
+
+    for _ in range(20000):
+        n, rows, cols = length(1, 5000), length(1, 160000), length(1, int8.MAX_COLS)
+        assert matmul_key(n, rows, cols, rng.choice([0, 1 << 40])) in shapes.MATMUL, (n, rows, cols)
+        kernel, _, held, _ = int8.kernel(rows, cols, n, floats=True)
+        assert kernel != int8.FEW_FLOAT or held in shapes.LINEAR, (n, rows, cols)
+        e = length(1, 512)
+        k, n = int(rng.integers(1, min(16, e) + 1)), length(1, 3000)
+        layer, ids = Layer(n_expert=e, top_k=k, hidden=length(1, 20000), ffn=length(1, 40000)), int(rng.integers(0, 2))
+        pairs, tok, up_held, down_held = int8.moe_kernels(layer.desc, n, ids)
+        assert (pairs, tok, up_held) in up and (pairs, tok, down_held) in down, (n, e, k, layer.desc.hidden, layer.desc.ffn)
