@@ -551,7 +551,8 @@ int oxh_moe_route(const float *d_logits, size_t n_tok, size_t n_expert, size_t t
 
 /* Routers of models with many experts, beside oxh_moe_route (which keeps the
  * reference's softmax and its order among equal probabilities).  Per token:
- *   score   softmax over the experts, or a sigmoid of each logit, in 64 bits
+ *   score   softmax over the experts, or a sigmoid of each logit (0 below
+ *           -708), in 64 bits
  *   key     score + d_bias[e] (d_bias NULL: the score).  The bias keeps the
  *           experts' loads even: it takes part in the choice, not in the weight
  *   groups  n_group > 1: the experts are n_group runs of n_expert / n_group;
@@ -611,8 +612,12 @@ int oxh_moe_select(const OxhMoeRouter *r, uint32_t logits_type, const void *d_lo
  * stride a multiple of 16, at least cols and at most 2^23 (fastest: a multiple
  * of 128 that is none of 4096).  The bytes between cols and the next multiple
  * of 16 are read and not used.  Any cols from 1 to OXH_I8_MAX_COLS (the int32
- * sums of codes -128..127 cannot overflow); more is OXH_ERR_TOO_WIDE. */
+ * sums of codes -128..127 cannot overflow); more is OXH_ERR_TOO_WIDE.  At most
+ * OXH_I8_MAX_ROWS rows, of a matrix or of tokens, and OXH_I8_MAX_RESULTS
+ * results a call; more is OXH_ERR_ARG, and the workspace functions say 0. */
 #define OXH_I8_MAX_COLS 131071u
+#define OXH_I8_MAX_ROWS ((size_t)1 << 21)
+#define OXH_I8_MAX_RESULTS ((size_t)1 << 37)
 /* element types of the float side (not GGUF type ids) */
 #define OXH_F32  0u
 #define OXH_F16  1u
@@ -637,7 +642,7 @@ typedef struct OxhI8Matrix {
 int oxh_i8_quantize(uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, size_t cols,
                     const void *d_up, int8_t *d_q, size_t q_stride, float *d_scale, void *stream);
 /* out[t * out_stride + r] = (sum_k q[t][k] * w[r][k]) * q_scale[t] * w_scale[r]
- * + bias[r], for t < n_vec (any count) in out_type; the sum is an exact
+ * + bias[r], for t < n_vec in out_type; the sum is an exact
  * integer, the rest f32, rounded once.  d_bias NULL or `rows` floats.  d_out
  * aligned to its elements.  Few results over long rows are shared out over
  * the columns when there is a workspace (oxh_i8_matmul_workspace bytes,
@@ -665,12 +670,15 @@ int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t
  *   out[t] = sum over t's pairs j, in their order, of weight[t][j] * down.
  * Matrices are stacked expert-major as in OxhMoe (expert e of gate / up at rows
  * [e*ffn, (e+1)*ffn), of down at rows [e*hidden, (e+1)*hidden)), a scale per
- * row.  n_expert <= 512, top_k <= 16, n_tok <= 65535.  The routing must be one
+ * row.  n_expert <= 512, top_k <= 16, n_tok 1..65535, and of what lies in the
+ * workspace n_tok * top_k * max(hidden, ffn) <= OXH_MOE_I8_MAX_VALUES and
+ * n_tok times hidden, rounded up to 64, < 2^32.  The routing must be one
  * of n_tok tokens over n_expert experts with top_k choices; entries out of
  * range are clamped, never followed.  d_counts is not read; d_ids is, by a way
  * for few pairs with the same results (NULL: not taken).  Launches that the
  * sizes alone decide, capturable.
  * No output may overlap an input. */
+#define OXH_MOE_I8_MAX_VALUES ((size_t)1 << 35)
 typedef struct OxhMoeI8 {
     const int8_t *d_w_gate, *d_w_up, *d_w_down;
     const float  *d_s_gate, *d_s_up, *d_s_down;

@@ -1045,16 +1045,11 @@ static int launched(const char *who)
     return e == hipSuccess ? OXH_OK : oxh_internal_errorf(OXH_ERR_HIP, "HIP error in %s: %s", who, hipGetErrorString(e));
 }
 
-/* rows or tokens: a workgroup of 1024 threads each is a grid of 2^31 threads */
-#define I8_MAX_ROWS ((size_t)1 << 21)
+/* OXH_I8_MAX_ROWS: a workgroup of 1024 threads each is a grid of 2^31 threads.  OXH_I8_MAX_RESULTS: 2^30 threads in tiles of 256 x 256, and
+ * they do not fit this memory in f32.  OXH_MOE_I8_MAX_VALUES: tiles of 128 x 64 below 2^32 threads, and 128 GiB of h or y. */
 
 /* a tile's rows lie within 32 bits of its first one */
 #define I8_MAX_STRIDE ((size_t)1 << 23)
-
-/* results of a product: 2^37 are 2^30 threads in tiles of 256 x 256, and do not fit this memory in f32 */
-#define I8_MAX_RESULTS ((size_t)1 << 37)
-/* pairs times the longer side of an expert: tiles of 128 x 64 below 2^32 threads, and 128 GiB of h or y */
-#define I8_MAX_PAIR_VALUES ((size_t)1 << 35)
 
 static int check_rows(const char *who, const char *name, const void *d, size_t stride, size_t cols)
 {
@@ -1127,7 +1122,7 @@ extern "C" int oxh_i8_quantize(uint32_t x_type, const void *d_x, size_t x_stride
         return rc;
     if (d_up && (rc = check_floats(who, "d_up", x_type, d_up, x_stride, cols))) return rc;
     if (!d_scale) return I8_ARG("%s: NULL pointer (d_scale)", who);
-    if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows per call", who, I8_MAX_ROWS);
+    if (n_vec > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows per call", who, OXH_I8_MAX_ROWS);
     if ((rc = ready())) return rc;
     return quantize_launch(x_type, d_x, x_stride, n_vec, cols, d_up, d_q, q_stride, d_scale, stream_of(stream), who);
 }
@@ -1138,7 +1133,7 @@ static int check_matrix(const char *who, const OxhI8Matrix *w)
     if (!w) return I8_ARG("%s: NULL matrix", who);
     if ((rc = check_cols(who, w->cols)) || (rc = check_rows(who, "the matrix", w->d_w, w->stride, w->cols))) return rc;
     if (!w->d_scale) return I8_ARG("%s: NULL pointer (the matrix's scales)", who);
-    if (w->rows > I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows", who, I8_MAX_ROWS);
+    if (w->rows > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows", who, OXH_I8_MAX_ROWS);
     return OXH_OK;
 }
 
@@ -1384,7 +1379,7 @@ extern "C" int oxh_internal_i8_init(void)
 
 extern "C" size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > I8_MAX_ROWS || n_vec > I8_MAX_ROWS)
+    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
         return 0;
     if (few_team(w->rows, w->cols, n_vec, i8_cus())) return 0;
     return parts_bytes(w->rows, n_vec, i8_way(w->rows, w->cols, n_vec, SIZE_MAX, i8_cus()).splits);
@@ -1401,8 +1396,8 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
     if ((rc = check_rows(who, "d_q", d_q, q_stride, w->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)))
         return rc;
     if (!d_q_scale) return I8_ARG("%s: NULL pointer (d_q_scale)", who);
-    if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
-    if (n_vec * w->rows > I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, I8_MAX_RESULTS);
+    if (n_vec > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, OXH_I8_MAX_ROWS);
+    if (n_vec * w->rows > OXH_I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, OXH_I8_MAX_RESULTS);
     if (d_workspace && workspace_bytes && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
     if ((rc = ready())) return rc;
     return matmul_launch(w, d_q, q_stride, d_q_scale, n_vec, d_bias, out_type, d_out, out_stride, d_workspace,
@@ -1437,7 +1432,7 @@ static LinearParts linear_parts(size_t rows, size_t cols, size_t n)
 
 extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > I8_MAX_ROWS || n_vec > I8_MAX_ROWS)
+    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
         return 0;
     return linear_parts(w->rows, w->cols, n_vec).total;
 }
@@ -1462,8 +1457,8 @@ extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *
     if ((rc = check_floats(who, "d_x", x_type, d_x, x_stride, w->cols)) ||
         (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)))
         return rc;
-    if (n_vec > I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, I8_MAX_ROWS);
-    if (n_vec * w->rows > I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, I8_MAX_RESULTS);
+    if (n_vec > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, OXH_I8_MAX_ROWS);
+    if (n_vec * w->rows > OXH_I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, OXH_I8_MAX_RESULTS);
     if ((rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
         (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)))    /* once more: the way depends on the device */
         return rc;
@@ -1522,8 +1517,8 @@ static int moe_parts(const char *who, const OxhMoeI8 *m, size_t n_tok, MoeI8Part
     p->qh_stride = up64(m->ffn);
     p->h_stride = up64(m->ffn);
     p->y_stride = up64(m->hidden);
-    if (pairs * (m->hidden > m->ffn ? m->hidden : m->ffn) > I8_MAX_PAIR_VALUES)
-        return I8_ARG("%s: n_tok * top_k * max(hidden, ffn) is more than %zu", who, I8_MAX_PAIR_VALUES);
+    if (pairs * (m->hidden > m->ffn ? m->hidden : m->ffn) > OXH_MOE_I8_MAX_VALUES)
+        return I8_ARG("%s: n_tok * top_k * max(hidden, ffn) is more than %zu", who, OXH_MOE_I8_MAX_VALUES);
     if (n_tok * p->q_stride > 0xFFFFFFFFull) return I8_ARG("%s: the tokens' codes exceed 4 GiB", who);
     p->tok = experts_tok(pairs, m->n_expert);
     p->n_tiles = (uint32_t)experts_tiles(pairs, m->n_expert, p->tok);

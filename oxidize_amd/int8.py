@@ -12,7 +12,7 @@ from . import matvec as mv
 from ._lib import check, lib
 
 F32, F16, BF16 = 0, 1, 2
-MAX_COLS = 131071
+MAX_COLS, MAX_ROWS, MAX_RESULTS, MOE_MAX_VALUES = 131071, 1 << 21, 1 << 37, 1 << 35
 
 
 def stride_of(cols):

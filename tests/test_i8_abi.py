@@ -252,3 +252,52 @@ def test_no_size_runs_on_a_kernel_that_has_none_listed():
         layer, ids = Layer(n_expert=e, top_k=k, hidden=length(1, 20000), ffn=length(1, 40000)), int(rng.integers(0, 2))
         pairs, tok, up_held, down_held = int8.moe_kernels(layer.desc, n, ids)
         assert (pairs, tok, up_held) in up and (pairs, tok, down_held) in down, (n, e, k, layer.desc.hidden, layer.desc.ffn)
+
+
+# ─── limits ─────────────────────────────────────────────────────────────
+
+
+def test_the_limits_are_the_headers(tmp_path):
+    names = {"OXH_I8_MAX_COLS": int8.MAX_COLS, "OXH_I8_MAX_ROWS": int8.MAX_ROWS, "OXH_I8_MAX_RESULTS": int8.MAX_RESULTS,
+             "OXH_MOE_I8_MAX_VALUES": int8.MOE_MAX_VALUES}
+    src, exe = tmp_path / "limits.c", tmp_path / "limits"
+    src.write_text('#include <stdio.h>\n#include "oxhip.h"\nint main(void) {' +
+                   "".join('printf("%s %%zu\\n", (size_t)%s);' % (n, n) for n in names) + "return 0; }")
+    subprocess.run(["gcc", "-std=c11", "-I", os.path.join(ROOT, "include"), "-o", str(exe), str(src)], check=True)
+    out = subprocess.run([str(exe)], check=True, capture_output=True, text=True).stdout
+    assert {a: int(b) for a, b in (line.split() for line in out.splitlines())} == names
+
+
+def test_what_lies_next_to_a_limit():
+    """The largest sizes are planned for and one more is refused."""
+    most, need = int8.MAX_ROWS, ctypes.c_size_t()
+    refused(int8.quantize, **{**QUANT, "n_vec": most + 1})
+    m = int8.Matrix(**MAT)
+    refused(m.matmul, **{**MUL, "n_vec": most + 1})
+    assert m.linear_workspace(most) >= most * 128 and m.linear_workspace(most + 1) == 0 and m.matmul_workspace(most + 1) == 0
+    high = dict(MAT, rows=most + 1)
+    refused(int8.Matrix(**high).matmul, **{**MUL, "out_stride": most + 1})
+    assert int8.Matrix(**dict(MAT, rows=most)).linear_workspace(100) > 0 and int8.Matrix(**high).linear_workspace(100) == 0
+    large = int8.Matrix(**dict(MAT, rows=most))                        # 2^21 rows: 2^16 tokens have 2^37 results
+    refused(large.matmul, **{**MUL, "n_vec": (1 << 16) + 1, "out_stride": most})
+    wide = 1 << 23
+    refused(int8.quantize, **{**QUANT, "q_stride": wide + 16})
+    refused(int8.Matrix(**dict(MAT, stride=wide + 16)).matmul, **MUL)
+
+    def layer(n, **sizes):
+        return _lib.lib().oxh_moe_i8_workspace_bytes(ctypes.byref(Layer(**sizes).desc), n, ctypes.byref(need))
+
+    assert layer(65535, hidden=65536, top_k=1) == _lib.OK and need.value > 65535 * 65536
+    assert layer(65535, hidden=65537, top_k=1) == _lib.ERR_ARG         # 65600 bytes of codes a token: more than 4 GiB
+    assert layer(1 << 14, n_expert=64, top_k=16, ffn=131071) == _lib.OK
+    assert layer((1 << 14) + 1, n_expert=64, top_k=16, ffn=131071) == _lib.ERR_ARG
+
+
+def test_the_largest_sizes_pass_the_checks():
+    import torch
+    if torch.cuda.is_available():
+        pytest.skip("there is a device")                               # the addresses are not real
+    most = int8.MAX_ROWS
+    refused(int8.quantize, **{**QUANT, "n_vec": most, "q_stride": 1 << 23}, status=_lib.ERR_NO_DEVICE)
+    refused(int8.Matrix(**dict(MAT, rows=most, stride=1 << 23)).matmul, **{**MUL, "n_vec": 1 << 16, "out_stride": most},
+            status=_lib.ERR_NO_DEVICE)
