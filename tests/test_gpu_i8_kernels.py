@@ -94,3 +94,24 @@ def test_select(oxh, kind, e, n):
     logits = ref.encode(np.random.default_rng(e).normal(size=(n, e)).astype(np.float32), kind)
     got = sel.select(logits, kind, 7, e + 3, score="sigmoid", n_group=2, top_group=1, group_best=2)
     sel.check(got, ref.decode(logits, kind), 7, "sigmoid", 2, 1, 2)
+
+
+def test_calls_of_one_stream_share_a_workspace(oxh):
+    """An expert layer under several token counts, pair by pair, by few pairs and by tiles, and products of one matrix, each in one workspace that
+    holds the call before: outputs of their own, one wait at the end."""
+    lay, rng = base.Layer(20, 2, 200, 300, 700), np.random.default_rng(2)
+    m = base.Case(700, 600, 5000, 1)
+    need = m.m.linear_workspace(700)
+    ws, calls = mv.DeviceBuffer.from_host(np.full(need, 0xFF, np.uint8)), []
+    for n in (700, 3, 40, 400, 1, 200, 60):
+        ids, w = base.choices(rng, n, 20, 2)
+        x, y = base.floats(n, 200, F32, n), base.floats(n, 5000, F32, n)
+        calls.append((n, x, ids, w, *lay.route(ids, w), mv.DeviceBuffer.from_host(x), mv.DeviceBuffer(4 * n * 200), y,
+                      mv.DeviceBuffer.from_host(y), mv.DeviceBuffer(4 * n * 600)))
+    for n, x, ids, w, routing, keep, d_x, d_o, y, d_y, d_p in calls:
+        lay.layer.forward(routing, F32, d_x.ptr, n, F32, d_o.ptr)
+        m.m.linear(F32, d_y.ptr, 5000, n, F32, d_p.ptr, 600, None, ws.ptr, need)
+    mv.sync()
+    for n, x, ids, w, routing, keep, d_x, d_o, y, d_y, d_p in calls:
+        lay.check(d_o.download(np.float32, n * 200).reshape(n, 200).astype(np.float64), x, F32, ids, w, F32)
+        assert base.same_bits(d_p.download(np.float32, n * 600).reshape(n, 600), ref.product(*ref.quantize(y), m.w, m.ws))

@@ -160,3 +160,22 @@ def test_rows_of_counts_with_a_choice_for_every_thread(oxh):
     """64 tokens of 16 choices to a workgroup, the last one with a single token; ids that cover a row's 1024 threads."""
     x = np.random.default_rng(6).normal(size=(8193 + 64, 20)).astype(np.float32)
     check(select(x, ref.F32, 16, score="sigmoid"), x, 16, "sigmoid")
+
+
+def test_calls_of_one_stream_share_a_workspace(oxh):
+    """Large and small calls over several expert counts, one after the other on one stream into ONE workspace, which holds other counts before
+    each; outputs of their own, one wait at the end."""
+    rng = np.random.default_rng(4)
+    calls, need = [], 0
+    for n, e, k in ((5000, 64, 4), (200, 64, 4), (30, 300, 5), (900, 20, 3), (5000, 500, 8), (17, 64, 4), (2100, 33, 16), (70, 512, 2)):
+        x, r = rng.normal(size=(n, e)).astype(np.float32), mv.MoeRouter(e, k, "sigmoid")
+        sizes = dict(ids=n * k, weights=n * k, counts=e, offsets=e + 1, perm=n * k, slot_pos=n * k)
+        calls.append((x, k, r, mv.DeviceBuffer.from_host(x), {name: mv.DeviceBuffer(4 * size) for name, size in sizes.items()}, sizes))
+        need = max(need, r.workspace_bytes(n))
+    ws = mv.DeviceBuffer.from_host(np.full(need, 0xFF, np.uint8))
+    for x, k, r, d_x, d, sizes in calls:
+        r.select(ref.F32, d_x.ptr, x.shape[1], x.shape[0], mv.make_routing(*[b.ptr for b in d.values()]), ws.ptr, need)
+    mv.sync()
+    for x, k, r, d_x, d, sizes in calls:
+        got = {name: d[name].download(np.float32 if name == "weights" else np.int32, size) for name, size in sizes.items()}
+        check(got, x, k, "sigmoid")
