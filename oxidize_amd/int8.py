@@ -72,7 +72,10 @@ class Matrix:
 
 
 def from_packed(qtype, d_w, rows, cols, stream=None):
-    """A packed matrix (any type oxh_get_rows expands) as int8 rows: (Matrix, [the buffers it lives in])."""
+    """A packed matrix (any type oxh_get_rows expands) as int8 rows: (Matrix, [the buffers it lives in]).
+
+    What one scale a row costs beside the packed format's own: a weight moves by at most half a code, its row's largest magnitude / 254.
+    That is 1.3 % of the weights' rms for random Q4_K, Q5_K and Q6_K rows of 4096 columns, 1.1 % for Q8_0."""
     stride, step = stride_of(cols), max(1, min(65535, rows, (256 << 20) // (4 * cols)))
     pad = (cols + 3) // 4 * 4
     codes, scale = mv.DeviceBuffer(rows * stride), mv.DeviceBuffer(4 * rows)

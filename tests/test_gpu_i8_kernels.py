@@ -7,7 +7,7 @@ import i8_ref as ref
 import i8_shapes as shapes
 import test_gpu_i8 as base
 import test_gpu_select as sel
-from oxidize_amd import int8
+from oxidize_amd import int8, synth
 from oxidize_amd import matvec as mv
 
 pytestmark = pytest.mark.gpu
@@ -115,3 +115,36 @@ def test_calls_of_one_stream_share_a_workspace(oxh):
     for n, x, ids, w, routing, keep, d_x, d_o, y, d_y, d_p in calls:
         lay.check(d_o.download(np.float32, n * 200).reshape(n, 200).astype(np.float64), x, F32, ids, w, F32)
         assert base.same_bits(d_p.download(np.float32, n * 600).reshape(n, 600), ref.product(*ref.quantize(y), m.w, m.ws))
+
+
+def test_from_packed_in_several_blocks_of_rows(oxh):
+    """More rows than one expansion takes (65535), the last block a short one."""
+    rows, cols = 65535 + 700, 256
+    w = synth.weights(13, rows, cols, seed=3, stream=1)
+    d_w, d_ids = mv.DeviceBuffer.from_host(w), mv.DeviceBuffer.from_host(np.arange(rows, dtype=np.uint32))
+    m, keep = int8.from_packed(13, d_w.ptr, rows, cols)
+    q = keep[0].download(np.int8, rows * m.desc.stride).reshape(rows, -1)[:, :cols]
+    s = keep[1].download(np.float32, rows)
+    d_f = mv.DeviceBuffer(4 * 1000 * cols)
+    for r in (0, 65000, rows - 1000):
+        mv.get_rows(13, d_w.ptr, rows, cols, d_ids.ptr + 4 * r, 1000, d_f.ptr, cols)
+        mv.sync()
+        want_q, want_s = ref.quantize(d_f.download(np.float32, 1000 * cols).reshape(1000, cols))
+        n = min(1000, rows - r)
+        assert np.array_equal(q[r:r + n], want_q[:n]) and np.array_equal(s[r:r + n], want_s[:n])
+
+
+@pytest.mark.parametrize("qtype", [13, 15, 16, 7], ids=["q4_k", "q5_k", "q6_k", "q8_0"])
+def test_what_one_scale_a_row_costs(oxh, qtype):
+    """A weight moves by at most half a code, the row's largest magnitude / 254 (and its f32 roundings)."""
+    rows, cols = 64, 4096
+    w = synth.weights(qtype, rows, cols, seed=5, stream=1)
+    d_w, d_ids = mv.DeviceBuffer.from_host(w), mv.DeviceBuffer.from_host(np.arange(rows, dtype=np.uint32))
+    d_f = mv.DeviceBuffer(4 * rows * cols)
+    mv.get_rows(qtype, d_w.ptr, rows, cols, d_ids.ptr, rows, d_f.ptr, cols)
+    m, keep = int8.from_packed(qtype, d_w.ptr, rows, cols)
+    f = d_f.download(np.float32, rows * cols).reshape(rows, cols).astype(np.float64)
+    q, s = keep[0].download(np.int8, rows * m.desc.stride).reshape(rows, -1)[:, :cols], keep[1].download(np.float32, rows)
+    off = np.abs(q * s[:, None].astype(np.float64) - f)
+    assert np.all(off <= np.abs(f).max(axis=1, keepdims=True) / 254 * (1 + 256 * 2.0 ** -24))
+    print("relative to the rows' rms: %.4f" % np.sqrt((off ** 2).mean() / (f ** 2).mean()))
