@@ -120,7 +120,7 @@ __device__ __forceinline__ float i8_scale(uint32_t top, float &inv)
 
 /* A row by a workgroup, eight values to a thread and step: once for the largest magnitude, once for the codes.  The first
  * HELD steps' values stay in registers; what is longer is read (and, GLU, computed) a second time.  Bound by memory: 4096 x 14336 bf16
- * in 35 us, 5.1 TB/s read and written; one row of 4096 in 2.3 us, a trip to memory and two barriers. */
+ * in 35 us, 5.1 TB/s read and written, of silu(x) * up in 66, 4.5 TB/s; one row of 4096 in 2.2 us, a trip to memory and two barriers. */
 template <typename T, bool GLU, int THREADS, int HELD>
 __device__ __forceinline__ void i8_quantize_row(const T *__restrict__ xr, const T *__restrict__ ur, uint32_t cols, int8_t *__restrict__ qr,
                                                 float *__restrict__ scale)
@@ -220,7 +220,7 @@ __device__ __forceinline__ uint32_t i8_place(uint32_t b, uint32_t n)
 
 /* The tile at place i: an order that goes through the token tiles with up to eight row tiles at each, so that what an XCD's
  * 32 CUs read at a time is 8 + 4 operand tiles through its L2, where one row tile under 32 token tiles is 33 (8192 x
- * 8192 x 8192: 473 us, 435 in this order). */
+ * 8192 x 8192: 473 us, 435 in this order; 406 with what i8_tile has learnt since, 2700 TOPS). */
 __device__ __forceinline__ void i8_tile_at(uint32_t i, uint32_t row_tiles, uint32_t tok_tiles, uint32_t &row, uint32_t &tok)
 {
     const uint32_t group = i / (8u * tok_tiles), in = i - group * 8u * tok_tiles, high = min(8u, row_tiles - 8u * group);
@@ -837,7 +837,7 @@ template <typename G, bool UP> __device__ __forceinline__ void i8_experts_tile(c
 }
 
 /* G: as many pairs as a table entry can have; H, Q: fewer, for the last ones of an expert's.  2000 tokens, 8 of 128 experts of 2048 x 768:
- * gate and up in 113 us (403 MB of weights, which take 65 alone, and 100 Gop, which take 42, with the empty places of the tiles 54), down in 83 (201 MB, and 131 of
+ * gate and up in 113 us (403 MB of weights, which take 65 alone, and 100 Gop, which take 37, with the empty places of the tiles 47), down in 79 (201 MB, and 131 of
  * results). */
 template <typename G, typename H, typename Q, bool UP>
 __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts p)
@@ -855,7 +855,7 @@ __global__ __launch_bounds__(G::WAVES * 64, 2) void k_i8_experts(const I8Experts
 }
 
 /* Up to sixteen pairs of an expert, as k_i8_few: `team` waves share a group of 16 rows; UP: half of them take gate, half up.  Bound by
- * memory: 8 experts of 4096 x 14336, 16 tokens of two: gate and up in 158 us, 5.9 TB/s, down in 97, 4.8 TB/s. */
+ * memory: 8 experts of 4096 x 14336, 16 tokens of two: gate and up in 155 us, 6.1 TB/s, down in 98, 4.8 TB/s. */
 template <int ST, bool UP>
 __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const I8Experts p, uint32_t team, uint32_t groups)
 {
@@ -892,8 +892,8 @@ __global__ __launch_bounds__(1024, ST <= 4 ? 8 : 4) void k_i8_experts_few(const 
 
 /* A decode step has a handful of pairs, hardly two of one expert, and what it takes is launches: here there are two.  Nothing is sorted or
  * tabled; a pair's expert is read from its id, and each launch quantises what it multiplies by itself, as k_i8_few_float does.  The sums are
- * integers and the float steps those of the other kernels: the same results, bit by bit.  One token, 8 experts of 2048 x 768: 8.8 and
- * 6.0 us for 25 and 13 MB, a chain of id, weights and tokens, quantisation and joins behind the memory's 4.1 and 2. */
+ * integers and the float steps those of the other kernels: the same results, bit by bit.  One token, 8 experts of 2048 x 768: 9.4 and
+ * 6.5 us for 25 and 13 MB, a chain of id, weights and tokens, quantisation and joins behind the memory's 4.1 and 2. */
 struct I8Pairs {
     I8Experts e;
     const int32_t *ids;
@@ -999,7 +999,7 @@ k_i8_pair_down(const I8Pairs p, const float *__restrict__ h, size_t h_stride, T 
 }
 
 /* out[t] = sum over t's pairs, in their order, of weight * y.  Four columns to a thread, eight of the token's pairs under way at a
- * time.  Bound by memory: 2000 tokens, 8 x 2048 each, in 21 us, 6.6 TB/s. */
+ * time.  Bound by memory: 2000 tokens, 8 x 2048 each, in 21.6 us, 6.4 TB/s. */
 template <typename T>
 __global__ __launch_bounds__(256) void
 k_i8_combine(const float *__restrict__ y, size_t y_stride, const float *__restrict__ weights, const uint32_t *__restrict__ slot_pos,
@@ -1164,9 +1164,13 @@ static size_t parts_bytes(size_t rows, size_t n, uint32_t splits) { return split
 
 /* The tiles: how many a CU holds at a time, and the microseconds that a stage of 128 columns takes a CU that works on so many of them, in a
  * launch that is done at once and round after round.  These, and the other times of product_us(), are fitted to 5000 launches
- * (256 to 151936 rows, 512 to 16000 columns, 17 to 4096 tokens, every tile, 1 to 8 parts): the way they choose takes 0.9 % more than the best of
- * its launches on the average, 14 % at the worst (6416 x 512 under 1400 tokens, 20.2 us against 17.7).  128 x 192 is there for token counts
- * that leave tiles of 128 and 256 half empty (4096 x 14336 under 333: 36.9 us in three parts, 39.2 the best without it). */
+ * (256 to 151936 rows, 512 to 16000 columns, 17 to 4096 tokens, every tile, 1 to 8 parts) over three to six matrices in turn, which the
+ * last cache holds wholly or in part: the way they choose takes 0.9 % more than the best of its launches on the average, 14 % at the worst
+ * (6416 x 512 under 1400 tokens, 20.2 us against 17.7).  They serve matrices that come from memory as well, though a launch of 65 to 500 tokens takes up to
+ * half as long again: over 800 MB of matrices in turn 0.8 % and 15 % (76 sizes, 2048 x 2048 to 28672 x 4096 and 6000 x 16000, 17 to 2048 tokens;
+ * 6000 x 16000 under 333, 67.2 us against 58.4), over three of the same 0.9 % and 17 %; where they choose nine to twelve parts
+ * (60 sizes, 64 to 9000 rows) 0.6 % and 5 %, over three 2.2 % and 15 %.  128 x 192 is there for token counts that leave tiles of 128 and 256 half empty (4096 x 14336 under
+ * 333: 34.8 us in four parts, 37.0 the best without it; from memory 38.8 and 41.5). */
 struct I8Pace {
     uint32_t rows, tok, held;
     double alone[4], rounds;

@@ -8,7 +8,7 @@
  * Sorting needs no sort: a workgroup takes at most 64 tokens, and a token chooses an expert at most once, so the
  * tokens of an expert are a 64-bit mask in LDS; its count is the mask's population and a pair's rank the population
  * below its token.  Bound by the instructions of 64-bit exponentials and of the rounds of the choice (about 5000 cycles a token, four
- * waves to a SIMD): 4096 tokens, 8 of 256 sigmoids in groups, in 11 us and the positions in 6.  For a few tokens one workgroup does all of it in one launch.  Above, every workgroup leaves its
+ * waves to a SIMD): 4096 tokens, 8 of 256 sigmoids in groups, in 12 us and the positions in 5.5.  For a few tokens one workgroup does all of it in one launch.  Above, every workgroup leaves its
  * counts (a byte each) and a second launch adds up those of the workgroups before it. */
 #include <hip/hip_runtime.h>
 #include <stdint.h>
