@@ -90,7 +90,7 @@ def from_packed(qtype, d_w, rows, cols, stream=None):
 
 class MoeLayer:
     """A mixture-of-experts feed-forward over int8 stacks under a given routing; owns its workspace, sized for
-    `max_tok` tokens.  Strides as :class:`Matrix`'s."""
+    `max_tok` tokens: calls that overlap in time need a layer each.  Strides as :class:`Matrix`'s."""
 
     def __init__(self, d_w_gate, d_s_gate, d_w_up, d_s_up, d_w_down, d_s_down, n_expert, top_k, hidden, ffn, gate_up_stride=None,
                  down_stride=None, max_tok=16):
