@@ -662,6 +662,84 @@ size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec);
 int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
                   const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,
                   void *d_workspace, size_t workspace_bytes, void *stream);
+/* What stands around those products in a layer.  Results are the same bits for
+ * any number of rows, order of rows and workspace.
+ *
+ * The norm that makes a product's tokens, oxh_i8_quantize behind it:
+ *   s = x + add in f32,  r = 1 / sqrt(mean of s^2 + eps) in 64 bits,
+ *   y = s * r * weight in 64 bits, rounded once to f32,
+ *   code and scale of y as oxh_i8_quantize's.
+ * d_add, d_sum, d_y and d_weight may be NULL: no addition, s and y not kept,
+ * a weight of 1.  s and y are rounded to the type of x, in which add comes too;
+ * strides are in elements and at least cols.  eps >= 0.  d_sum and d_y may each
+ * be d_x or d_add, at that one's stride: the residual stream is brought up to
+ * date in place.  Nothing else may overlap.  A row that holds an infinity or
+ * a NaN, or zeros alone with eps 0, gets scale NaN and codes 0. */
+typedef struct OxhI8Norm {
+    const float *d_weight;            /* NULL or cols values                             */
+    float        eps;
+    const void  *d_add;
+    size_t       add_stride;
+    void        *d_sum;
+    size_t       sum_stride;
+    void        *d_y;
+    size_t       y_stride;
+} OxhI8Norm;
+int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, size_t cols,
+                   int8_t *d_q, size_t q_stride, float *d_scale, void *stream);
+/* oxh_i8_matmul and oxh_i8_linear with an epilogue:
+ *   out = act(sum * q_scale * w_scale + bias) + residual
+ * in f32, rounded once to out_type.  The residual is n_vec rows of out_type,
+ * residual_stride elements apart, and may be d_out itself, at out_stride.
+ * Workspaces are those of the products without one.  e NULL: none.  act(v):
+ *   RELU       max(v, 0)               SILU  v / (1 + exp(-v))
+ *   GELU       v * (1 + erf(v / sqrt(2))) / 2
+ *   GELU_TANH  v * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) / 2
+ * of a NaN NaN; of -inf 0 (RELU) or NaN. */
+#define OXH_ACT_NONE      0u
+#define OXH_ACT_RELU      1u
+#define OXH_ACT_SILU      2u
+#define OXH_ACT_GELU      3u
+#define OXH_ACT_GELU_TANH 4u
+typedef struct OxhI8Epilogue {
+    const float *d_bias;              /* NULL or rows values                             */
+    uint32_t     act;                 /* OXH_ACT_*                                       */
+    const void  *d_residual;          /* NULL: none                                      */
+    size_t       residual_stride;
+} OxhI8Epilogue;
+int oxh_i8_matmul_ex(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
+                     const OxhI8Epilogue *e, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
+                     size_t workspace_bytes, void *stream);
+int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,
+                     const OxhI8Epilogue *e, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
+                     size_t workspace_bytes, void *stream);
+/* Both first projections of a gated feed-forward in one launch:
+ *   out[t][r] = act(g) * u,  g = sum(q[t], gate[r]) * q_scale[t] * s_gate[r]
+ *   + b_gate[r],  u likewise, in f32, rounded once to out_type.
+ * Sizes, strides and workspace (oxh_i8_gated_workspace bytes, or less, or none)
+ * as oxh_i8_matmul's. */
+typedef struct OxhI8Gated {
+    const int8_t *d_w_gate, *d_w_up;  /* rows x cols each                                */
+    size_t        stride;             /* bytes from row to row, of both                  */
+    const float  *d_s_gate, *d_s_up;  /* rows values                                     */
+    const float  *d_b_gate, *d_b_up;  /* NULL or rows values                             */
+    size_t        rows, cols;
+    uint32_t      act;                /* OXH_ACT_*                                       */
+} OxhI8Gated;
+size_t oxh_i8_gated_workspace(const OxhI8Gated *g, size_t n_vec);
+int oxh_i8_gated(const OxhI8Gated *g, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
+                 uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream);
+/* The gated feed-forward block: oxh_i8_gated into f32 rows, then
+ * oxh_i8_linear_ex of those over `down` (down->cols = g->rows), with its bias
+ * and the layer's residual in e; the results are those of the two calls.  Tokens
+ * come as codes: oxh_i8_rmsnorm's, or oxh_i8_quantize's.  d_workspace:
+ * oxh_i8_ffn_workspace() of device memory, 256-byte aligned, overwritten by every
+ * call: calls that overlap in time need one each.  That of more tokens serves
+ * fewer. */
+size_t oxh_i8_ffn_workspace(const OxhI8Gated *g, const OxhI8Matrix *down, size_t n_vec);
+int oxh_i8_ffn(const OxhI8Gated *g, const OxhI8Matrix *down, const int8_t *d_q, size_t q_stride, const float *d_q_scale,
+               size_t n_vec, const OxhI8Epilogue *e, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
+               size_t workspace_bytes, void *stream);
 /* A mixture-of-experts feed-forward over int8 stacks under a given routing
  * (oxh_moe_select's, or oxh_moe_route's):
  *   x of every token to codes; per expert and only for its own pairs gate and

@@ -51,6 +51,20 @@ class OxhI8Matrix(ctypes.Structure):
     _fields_ = [("d_w", V), ("stride", Z), ("d_scale", V), ("rows", Z), ("cols", Z)]
 
 
+class OxhI8Norm(ctypes.Structure):
+    _fields_ = [("d_weight", V), ("eps", ctypes.c_float), ("d_add", V), ("add_stride", Z), ("d_sum", V), ("sum_stride", Z),
+                ("d_y", V), ("y_stride", Z)]
+
+
+class OxhI8Epilogue(ctypes.Structure):
+    _fields_ = [("d_bias", V), ("act", U32), ("d_residual", V), ("residual_stride", Z)]
+
+
+class OxhI8Gated(ctypes.Structure):
+    _fields_ = [("d_w_gate", V), ("d_w_up", V), ("stride", Z), ("d_s_gate", V), ("d_s_up", V), ("d_b_gate", V), ("d_b_up", V),
+                ("rows", Z), ("cols", Z), ("act", U32)]
+
+
 class OxhMoeI8(ctypes.Structure):
     _fields_ = [("d_w_gate", V), ("d_w_up", V), ("d_w_down", V), ("d_s_gate", V), ("d_s_up", V), ("d_s_down", V),
                 ("gate_up_stride", Z), ("down_stride", Z), ("n_expert", Z), ("top_k", Z), ("hidden", Z), ("ffn", Z)]
@@ -83,7 +97,8 @@ class OxhLab(ctypes.Structure):
                 ("mmq32_fetched", ctypes.CFUNCTYPE(ctypes.c_uint64, U32, U32, U32, U32, U32)),
                 ("plan_draft", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhPlanOp), Z, U32, ctypes.POINTER(ctypes.c_uint64))),
                 ("i8_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, I, ctypes.POINTER(U32 * 4))),
-                ("moe_i8_kernels", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhMoeI8), Z, I, Z, ctypes.POINTER(U32 * 4)))]
+                ("moe_i8_kernels", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhMoeI8), Z, I, Z, ctypes.POINTER(U32 * 4))),
+                ("i8_gated_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, ctypes.POINTER(U32 * 4)))]
 
 
 # name -> (restype, argtypes); every symbol include/oxhip.h and include/oxhip_lab.h declare
@@ -133,6 +148,14 @@ SIGNATURES = {
     "oxh_i8_matmul": (I, [ctypes.POINTER(OxhI8Matrix), V, Z, V, Z, V, U32, V, Z, V, Z, V]),
     "oxh_i8_linear_workspace": (Z, [ctypes.POINTER(OxhI8Matrix), Z]),
     "oxh_i8_linear": (I, [ctypes.POINTER(OxhI8Matrix), U32, V, Z, Z, V, U32, V, Z, V, Z, V]),
+    "oxh_i8_rmsnorm": (I, [ctypes.POINTER(OxhI8Norm), U32, V, Z, Z, Z, V, Z, V, V]),
+    "oxh_i8_matmul_ex": (I, [ctypes.POINTER(OxhI8Matrix), V, Z, V, Z, ctypes.POINTER(OxhI8Epilogue), U32, V, Z, V, Z, V]),
+    "oxh_i8_linear_ex": (I, [ctypes.POINTER(OxhI8Matrix), U32, V, Z, Z, ctypes.POINTER(OxhI8Epilogue), U32, V, Z, V, Z, V]),
+    "oxh_i8_gated_workspace": (Z, [ctypes.POINTER(OxhI8Gated), Z]),
+    "oxh_i8_gated": (I, [ctypes.POINTER(OxhI8Gated), V, Z, V, Z, U32, V, Z, V, Z, V]),
+    "oxh_i8_ffn_workspace": (Z, [ctypes.POINTER(OxhI8Gated), ctypes.POINTER(OxhI8Matrix), Z]),
+    "oxh_i8_ffn": (I, [ctypes.POINTER(OxhI8Gated), ctypes.POINTER(OxhI8Matrix), V, Z, V, Z, ctypes.POINTER(OxhI8Epilogue), U32, V, Z, V,
+                       Z, V]),
     "oxh_moe_i8_workspace_bytes": (I, [ctypes.POINTER(OxhMoeI8), Z, ctypes.POINTER(Z)]),
     "oxh_moe_ffn_i8": (I, [ctypes.POINTER(OxhMoeI8), ctypes.POINTER(OxhRouting), U32, V, Z, Z, U32, V, Z, V, Z, V]),
     "oxh_malloc": (I, [ctypes.POINTER(V), Z]),

@@ -1,0 +1,485 @@
+/* oxh_i8_layer.hip — what stands around the int8 products of a layer: the norm that makes their tokens, products with bias,
+ * activation and residual, the gated product and the feed-forward block (oxh_i8_rmsnorm, oxh_i8_matmul_ex, oxh_i8_linear_ex,
+ * oxh_i8_gated, oxh_i8_ffn). */
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "oxhip.h"
+#include "oxh_internal.h"
+#include "oxh_device.inc"
+#include "i8_tiles.inc"
+#include "i8_products.inc"
+#include "i8_host.inc"
+
+/* ─── norm ────────────────────────────────────────────────────────────── */
+
+struct I8Norm {
+    const void *x, *add;
+    void *sum, *y;
+    size_t x_stride, add_stride, sum_stride, y_stride;
+    const float *weight;
+    int8_t *q;
+    size_t q_stride;
+    float *scale;
+    double eps;
+    uint32_t cols;
+};
+
+/* Values c .. c + 7 of a row, those behind the last one `other`. */
+template <typename T> __device__ __forceinline__ void norm_load8(const T *from, uint32_t c, uint32_t cols, float other, float (&v)[8])
+{
+    if (c + 8u <= cols) {
+        const Run<T, 8> r = *reinterpret_cast<const Run<T, 8> *>(from + c);
+#pragma unroll
+        for (int i = 0; i < 8; i++) v[i] = to_f32(r.v[i]);
+    } else
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++) v[i] = c + i < cols ? to_f32(from[c + i]) : other;
+}
+
+template <typename T> __device__ __forceinline__ void norm_store8(T *to, uint32_t c, uint32_t cols, const float (&v)[8])
+{
+    if (c + 8u <= cols) {
+        Run<T, 8> r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r.v[i] = from_f32<T>(v[i]);
+        *reinterpret_cast<Run<T, 8> *>(to + c) = r;
+    } else
+#pragma unroll
+        for (uint32_t i = 0; i < 8u; i++)
+            if (c + i < cols) to[c + i] = from_f32<T>(v[i]);
+}
+
+/* A row by a workgroup, eight values to a thread and step: s = x + add in 32 bits, the sum of its squares (each exact) and the norm in 64, so that
+ * y, rounded once, does not depend on how a row is dealt to threads, and neither do its codes.  The first HELD steps' values stay in registers; what is longer is
+ * read three times.  sum and y are written by the thread that has read those places, behind the last read: they may be x or
+ * add. */
+template <typename T, int THREADS, int HELD>
+__global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
+{
+    constexpr uint32_t STEP = 8u * THREADS;
+    __shared__ double s_sum[THREADS / 64];
+    __shared__ uint32_t s_top[THREADS / 64];
+    const size_t row = blockIdx.x;
+    const T *x = (const T *)p.x + row * p.x_stride, *add = p.add ? (const T *)p.add + row * p.add_stride : nullptr;
+    const uint32_t cols = p.cols, c0 = 8u * threadIdx.x, wave = threadIdx.x >> 6;
+    auto load = [&](uint32_t c, float (&v)[8]) {
+        norm_load8(x, c, cols, 0.0f, v);
+        if (add) {
+            float a[8];
+            norm_load8(add, c, cols, 0.0f, a);
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] += a[i];
+        }
+    };
+    double squares = 0.0;
+    auto square = [&](const float (&v)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) squares = __builtin_fma((double)v[i], (double)v[i], squares);
+    };
+    float s[HELD][8], w[HELD][8];
+#pragma unroll
+    for (int i = 0; i < HELD; i++) load(c0 + STEP * i, s[i]);
+#pragma unroll
+    for (int i = 0; i < HELD; i++) square(s[i]);
+    for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
+        float v[8];
+        load(c, v);
+        square(v);
+    }
+#pragma unroll
+    for (uint32_t d = 32u; d; d >>= 1) squares += __shfl_xor(squares, (int)d);
+    if (THREADS > 64) {
+        if ((threadIdx.x & 63u) == 0u) s_sum[wave] = squares;
+        __syncthreads();
+        squares = 0.0;
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) squares += s_sum[i];
+    }
+    const double r = 1.0 / sqrt(squares / (double)cols + p.eps);
+    auto weights = [&](uint32_t c, float (&v)[8]) {
+        if (p.weight) norm_load8(p.weight, c, cols, 0.0f, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 1.0f;
+    };
+    auto normed = [&](const float (&v)[8], const float (&g)[8], float (&y)[8]) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) y[i] = (float)((double)v[i] * r * (double)g[i]);
+    };
+    uint32_t top = 0;               /* what stands for places behind the last column is 0 or, where r is no number, as little one as the row itself */
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        float y[8];
+        weights(c0 + STEP * i, w[i]);
+        normed(s[i], w[i], y);
+        top = max(top, i8_top8(y));
+    }
+    for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
+        float v[8], g[8], y[8];
+        load(c, v);
+        weights(c, g);
+        normed(v, g, y);
+        top = max(top, i8_top8(y));
+    }
+    top = wave_top(top);
+    if (THREADS > 64) {
+        if ((threadIdx.x & 63u) == 0u) s_top[wave] = top;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < THREADS / 64; i++) top = max(top, s_top[i]);
+    }
+    float inv;
+    const float scale = i8_scale(top, inv);
+    if (threadIdx.x == 0u) p.scale[row] = scale;
+    const uint32_t end = (cols + 15u) & ~15u;
+    auto store = [&](uint32_t c, const float (&v)[8], const float (&g)[8]) {
+        if (c >= end) return;
+        float y[8];
+        normed(v, g, y);
+        *reinterpret_cast<uint2 *>(p.q + row * p.q_stride + c) = inv != 0.0f ? i8_codes8(y, scale, inv) : make_uint2(0u, 0u);
+        if (p.sum) norm_store8((T *)p.sum + row * p.sum_stride, c, cols, v);
+        if (p.y) norm_store8((T *)p.y + row * p.y_stride, c, cols, y);
+    };
+#pragma unroll
+    for (int i = 0; i < HELD; i++) store(c0 + STEP * i, s[i], w[i]);
+    for (uint32_t c = c0 + STEP * HELD; c < end; c += STEP) {
+        float v[8], g[8];
+        load(c, v);
+        weights(c, g);
+        store(c, v, g);
+    }
+}
+
+/* ─── products with an epilogue ───────────────────────────────────────── */
+
+/* In 32 bits; a NaN stays one. */
+__device__ __forceinline__ float i8_activate(uint32_t act, float v)
+{
+    if (act == OXH_ACT_RELU) return v < 0.0f ? 0.0f : v;
+    if (act == OXH_ACT_SILU) return silu(v);
+    if (act == OXH_ACT_GELU) return 0.5f * v * erfcf(v * -0.70710678f);
+    if (act == OXH_ACT_GELU_TANH) return v / (1.0f + expf(-1.59576912f * (v + 0.044715f * v * v * v)));     /* (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u)) */
+    return v;
+}
+
+struct I8ProductEx : I8Product {
+    const void *residual;
+    size_t residual_stride;
+    uint32_t act;
+};
+
+template <typename T> __device__ __forceinline__ void add_residual4(const T *from, uint32_t left, float (&v)[4])
+{
+    if (left >= 4u) {
+        const Run<T, 4> r = *reinterpret_cast<const Run<T, 4> *>(from);
+#pragma unroll
+        for (int i = 0; i < 4; i++) v[i] += to_f32(r.v[i]);
+    } else
+#pragma unroll
+        for (uint32_t i = 0; i < 3u; i++)
+            if (i < left) v[i] += to_f32(from[i]);
+}
+
+__device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[1], const I8RowFactors (&f)[1], float st)
+{
+    float v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        v[k] = (float)sums[0][k] * st * f[0].s[k];
+        if (p.bias) v[k] += f[0].b[k];
+        v[k] = i8_activate(p.act, v[k]);
+    }
+    if (p.residual) {
+        const size_t at = (size_t)t * p.residual_stride + r;
+        const uint32_t left = (uint32_t)p.w.rows - r;
+        if (p.out_type == OXH_F32) add_residual4((const float *)p.residual + at, left, v);
+        else if (p.out_type == OXH_F16) add_residual4((const _Float16 *)p.residual + at, left, v);
+        else add_residual4((const __bf16 *)p.residual + at, left, v);
+    }
+    i8_put(p, r, t, v);
+}
+
+/* ─── gated products ──────────────────────────────────────────────────── */
+
+/* w and bias are the gate's */
+struct I8GatedProduct : I8Product {
+    static constexpr uint32_t MATRICES = 2;
+    const int8_t *up;
+    const float *up_scale, *up_bias;
+    uint32_t act;
+};
+
+__device__ __forceinline__ const int8_t *i8_codes_of(const I8GatedProduct &p, uint32_t m) { return m ? p.up : p.w.d_w; }
+
+__device__ __forceinline__ void i8_row_factors(const I8GatedProduct &p, uint32_t r, I8RowFactors (&f)[2])
+{
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        const uint32_t rk = min(r + k, (uint32_t)p.w.rows - 1u);
+        f[0].s[k] = p.w.d_scale[rk];
+        f[1].s[k] = p.up_scale[rk];
+        f[0].b[k] = p.bias ? p.bias[rk] : 0.0f;
+        f[1].b[k] = p.up_bias ? p.up_bias[rk] : 0.0f;
+    }
+}
+
+__device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, uint32_t t, const v4i (&sums)[2], const I8RowFactors (&f)[2], float st)
+{
+    float v[4];
+#pragma unroll
+    for (uint32_t k = 0; k < 4u; k++) {
+        float g = (float)sums[0][k] * st * f[0].s[k], u = (float)sums[1][k] * st * f[1].s[k];
+        if (p.bias) g += f[0].b[k];
+        if (p.up_bias) u += f[1].b[k];
+        v[k] = i8_activate(p.act, g) * u;
+    }
+    i8_put(p, r, t, v);
+}
+
+/* ─── host side ───────────────────────────────────────────────────────── */
+
+static int check_again(const char *who, const char *name, const void *d, uint32_t type, size_t stride, size_t cols)
+{
+    return d ? check_floats(who, name, type, d, stride, cols) : OXH_OK;
+}
+
+extern "C" int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, size_t cols, int8_t *d_q,
+                              size_t q_stride, float *d_scale, void *stream)
+{
+    static const char who[] = "oxh_i8_rmsnorm";
+    int rc;
+    if (!norm) return I8_ARG("%s: NULL norm", who);
+    if (!(norm->eps >= 0.0f)) return I8_ARG("%s: eps must be >= 0", who);
+    if (n_vec == 0) return OXH_OK;
+    if ((rc = check_cols(who, cols)) || (rc = check_floats(who, "d_x", x_type, d_x, x_stride, cols)) ||
+        (rc = check_rows(who, "d_q", d_q, q_stride, cols)) || (rc = check_again(who, "d_add", norm->d_add, x_type, norm->add_stride, cols)) ||
+        (rc = check_again(who, "d_sum", norm->d_sum, x_type, norm->sum_stride, cols)) ||
+        (rc = check_again(who, "d_y", norm->d_y, x_type, norm->y_stride, cols)) ||
+        (rc = check_again(who, "d_weight", norm->d_weight, OXH_F32, cols, cols)))
+        return rc;
+    if (!d_scale) return I8_ARG("%s: NULL pointer (d_scale)", who);
+    if (norm->d_sum && norm->d_sum == norm->d_y) return I8_ARG("%s: d_sum and d_y are the same memory", who);
+    const void *const outs[2] = { norm->d_sum, norm->d_y }, *const ins[2] = { d_x, norm->d_add };
+    const size_t out_strides[2] = { norm->sum_stride, norm->y_stride }, in_strides[2] = { x_stride, norm->add_stride };
+    for (int o = 0; o < 2; o++)
+        for (int i = 0; i < 2; i++)
+            if (outs[o] && outs[o] == ins[i] && out_strides[o] != in_strides[i])
+                return I8_ARG("%s: an output in place of an input must have its stride", who);
+    if (n_vec > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows per call", who, OXH_I8_MAX_ROWS);
+    if ((rc = ready())) return rc;
+    const I8Norm p = { d_x, norm->d_add, norm->d_sum, norm->d_y, x_stride, norm->add_stride, norm->sum_stride, norm->y_stride, norm->d_weight,
+                       d_q, q_stride, d_scale, (double)norm->eps, (uint32_t)cols };
+    const dim3 grid((uint32_t)n_vec);
+    const hipStream_t st = stream_of(stream);
+#define OXH_NORM_K(T, THREADS, HELD) hipLaunchKernelGGL((k_i8_rmsnorm<T, THREADS, HELD>), grid, dim3(THREADS), 0, st, p)
+#define OXH_NORM(T)                                                                                                              \
+    do {                                                                                                                         \
+        if (cols <= 512u) OXH_NORM_K(T, 64, 1);                                                                                  \
+        else if (cols <= 2048u) OXH_NORM_K(T, 256, 1);                                                                           \
+        else OXH_NORM_K(T, 1024, 2);                                                                                             \
+    } while (0)
+    if (x_type == OXH_F32) OXH_NORM(float);
+    else if (x_type == OXH_F16) OXH_NORM(_Float16);
+    else OXH_NORM(__bf16);
+#undef OXH_NORM
+#undef OXH_NORM_K
+    return launched(who);
+}
+
+static int check_activation(const char *who, uint32_t act)
+{
+    return act <= OXH_ACT_GELU_TANH ? OXH_OK : I8_ARG("%s: the activation is not an OXH_ACT_", who);
+}
+
+static int check_epilogue(const char *who, const OxhI8Epilogue *e, uint32_t out_type, const void *d_out, size_t out_stride, size_t rows)
+{
+    int rc;
+    if (!e) return OXH_OK;
+    if ((rc = check_activation(who, e->act)) || (rc = check_again(who, "d_bias", e->d_bias, OXH_F32, rows, rows)) ||
+        (rc = check_again(who, "d_residual", e->d_residual, out_type, e->residual_stride, rows)))
+        return rc;
+    if (e->d_residual && e->d_residual == d_out && e->residual_stride != out_stride)
+        return I8_ARG("%s: results in place of the residual must have its stride", who);
+    return OXH_OK;
+}
+
+static I8ProductEx product_ex(const I8Product &p, const OxhI8Epilogue *e)
+{
+    I8ProductEx x = { p, nullptr, 0, OXH_ACT_NONE };
+    if (e) {
+        x.bias = e->d_bias;
+        x.residual = e->d_residual;
+        x.residual_stride = e->residual_stride;
+        x.act = e->act;
+    }
+    return x;
+}
+
+/* sizes that every product here has to keep to */
+static int check_sizes(const char *who, size_t n_vec, size_t rows)
+{
+    if (n_vec > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu tokens per call", who, OXH_I8_MAX_ROWS);
+    if (n_vec * rows > OXH_I8_MAX_RESULTS) return I8_ARG("%s: at most %zu results per call", who, OXH_I8_MAX_RESULTS);
+    return OXH_OK;
+}
+
+static int check_tokens(const char *who, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t cols)
+{
+    const int rc = check_rows(who, "d_q", d_q, q_stride, cols);
+    if (rc) return rc;
+    return d_q_scale ? OXH_OK : I8_ARG("%s: NULL pointer (d_q_scale)", who);
+}
+
+static int check_optional_workspace(const char *who, const void *d_workspace, size_t bytes)
+{
+    if (d_workspace && bytes && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
+    return OXH_OK;
+}
+
+extern "C" int oxh_i8_matmul_ex(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
+                                const OxhI8Epilogue *e, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace,
+                                size_t workspace_bytes, void *stream)
+{
+    static const char who[] = "oxh_i8_matmul_ex";
+    int rc;
+    if ((rc = check_matrix(who, w))) return rc;
+    if (n_vec == 0 || w->rows == 0) return OXH_OK;
+    if ((rc = check_tokens(who, d_q, q_stride, d_q_scale, w->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)) ||
+        (rc = check_epilogue(who, e, out_type, d_out, out_stride, w->rows)) || (rc = check_sizes(who, n_vec, w->rows)) ||
+        (rc = check_optional_workspace(who, d_workspace, workspace_bytes)) || (rc = ready()))
+        return rc;
+    I8ProductEx p = product_ex(i8_product(w, d_q, q_stride, d_q_scale, n_vec, nullptr, out_type, d_out, out_stride), e);
+    return product_launch(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus()), d_workspace, stream_of(stream), who);
+}
+
+extern "C" int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, const OxhI8Epilogue *e,
+                                uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream)
+{
+    static const char who[] = "oxh_i8_linear_ex";
+    int rc;
+    if ((rc = check_matrix(who, w))) return rc;
+    if (n_vec == 0 || w->rows == 0) return OXH_OK;
+    if ((rc = check_floats(who, "d_x", x_type, d_x, x_stride, w->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)) ||
+        (rc = check_epilogue(who, e, out_type, d_out, out_stride, w->rows)) || (rc = check_sizes(who, n_vec, w->rows)) ||
+        (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
+        (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)))    /* once more: the way depends on the device */
+        return rc;
+    I8ProductEx p = product_ex(i8_product(w, nullptr, 0, nullptr, n_vec, nullptr, out_type, d_out, out_stride), e);
+    return linear_launch(p, x_type, d_x, x_stride, d_workspace, workspace_bytes, stream_of(stream), who);
+}
+
+static OxhI8Matrix gate_of(const OxhI8Gated *g) { return { g->d_w_gate, g->stride, g->d_s_gate, g->rows, g->cols }; }
+
+static int check_gated(const char *who, const OxhI8Gated *g)
+{
+    int rc;
+    if (!g) return I8_ARG("%s: NULL matrices", who);
+    if ((rc = check_cols(who, g->cols)) || (rc = check_rows(who, "d_w_gate", g->d_w_gate, g->stride, g->cols)) ||
+        (rc = check_rows(who, "d_w_up", g->d_w_up, g->stride, g->cols)))
+        return rc;
+    if (!g->d_s_gate || !g->d_s_up) return I8_ARG("%s: NULL pointer (the matrices' scales)", who);
+    if ((rc = check_again(who, "d_b_gate", g->d_b_gate, OXH_F32, g->rows, g->rows)) ||
+        (rc = check_again(who, "d_b_up", g->d_b_up, OXH_F32, g->rows, g->rows)))
+        return rc;
+    if (g->rows > OXH_I8_MAX_ROWS) return I8_ARG("%s: at most %zu rows", who, OXH_I8_MAX_ROWS);
+    return check_activation(who, g->act);
+}
+
+static int gated_launch(const OxhI8Gated *g, const int8_t *q, size_t q_stride, const float *q_scale, size_t n, uint32_t out_type, void *out,
+                        size_t out_stride, void *ws, size_t ws_bytes, hipStream_t st, const char *who)
+{
+    const OxhI8Matrix gate = gate_of(g);
+    I8GatedProduct p = { i8_product(&gate, q, q_stride, q_scale, n, g->d_b_gate, out_type, out, out_stride), g->d_w_up, g->d_s_up, g->d_b_up, g->act };
+    return product_launch(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), 2u), ws, st, who);
+}
+
+static bool workable(size_t rows, size_t cols, size_t n)
+{
+    return n != 0 && rows != 0 && cols != 0 && cols <= OXH_I8_MAX_COLS && rows <= OXH_I8_MAX_ROWS && n <= OXH_I8_MAX_ROWS;
+}
+
+static size_t gated_parts(size_t rows, size_t cols, size_t n)
+{
+    const I8Choice c = i8_choice(rows, cols, n, SIZE_MAX, i8_cus(), 2u);
+    return c.team ? 0 : parts_bytes(i8_rows_in_all(rows, 2u), n, c.way.splits);
+}
+
+extern "C" size_t oxh_i8_gated_workspace(const OxhI8Gated *g, size_t n_vec)
+{
+    return g && workable(g->rows, g->cols, n_vec) ? gated_parts(g->rows, g->cols, n_vec) : 0;
+}
+
+extern "C" int oxh_i8_gated(const OxhI8Gated *g, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec, uint32_t out_type,
+                            void *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes, void *stream)
+{
+    static const char who[] = "oxh_i8_gated";
+    int rc;
+    if ((rc = check_gated(who, g))) return rc;
+    if (n_vec == 0 || g->rows == 0) return OXH_OK;
+    if ((rc = check_tokens(who, d_q, q_stride, d_q_scale, g->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, g->rows)) ||
+        (rc = check_sizes(who, n_vec, g->rows)) || (rc = check_optional_workspace(who, d_workspace, workspace_bytes)) || (rc = ready()))
+        return rc;
+    return gated_launch(g, d_q, q_stride, d_q_scale, n_vec, out_type, d_out, out_stride, d_workspace, d_workspace ? workspace_bytes : 0,
+                        stream_of(stream), who);
+}
+
+/* The block's workspace: h in f32, rows of up64(ffn); behind it the gated product's partial sums, and when those are done the codes
+ * and sums of the down projection. */
+static size_t ffn_h_bytes(size_t ffn, size_t n) { return up256(n * up64(ffn) * 4u); }
+
+extern "C" size_t oxh_i8_ffn_workspace(const OxhI8Gated *g, const OxhI8Matrix *down, size_t n_vec)
+{
+    if (!g || !down || !workable(g->rows, g->cols, n_vec) || !workable(down->rows, down->cols, n_vec)) return 0;
+    const size_t first = gated_parts(g->rows, g->cols, n_vec), second = linear_parts(down->rows, down->cols, n_vec).total;
+    return ffn_h_bytes(g->rows, n_vec) + (first > second ? first : second);
+}
+
+/* h and the codes have to fit, partial sums are used where they do */
+static int check_ffn_workspace(const char *who, const OxhI8Gated *g, const OxhI8Matrix *down, size_t n_vec, const void *d_workspace, size_t bytes)
+{
+    const LinearParts l = linear_parts(down->rows, down->cols, n_vec);
+    if (!d_workspace || bytes < ffn_h_bytes(g->rows, n_vec) + (l.total ? l.parts : 0)) return I8_ARG("%s: workspace too small (see oxh_i8_ffn_workspace)", who);
+    if ((uintptr_t)d_workspace & 255u) return I8_ARG("%s: workspace must be 256-byte aligned", who);
+    return OXH_OK;
+}
+
+extern "C" int oxh_i8_ffn(const OxhI8Gated *g, const OxhI8Matrix *down, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
+                          const OxhI8Epilogue *e, uint32_t out_type, void *d_out, size_t out_stride, void *d_workspace, size_t workspace_bytes,
+                          void *stream)
+{
+    static const char who[] = "oxh_i8_ffn";
+    int rc;
+    if ((rc = check_gated(who, g)) || (rc = check_matrix(who, down))) return rc;
+    if (g->rows == 0 || down->cols != g->rows) return I8_ARG("%s: the down matrix must have as many columns as the gate has rows", who);
+    if (n_vec == 0 || down->rows == 0) return OXH_OK;
+    if ((rc = check_tokens(who, d_q, q_stride, d_q_scale, g->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, down->rows)) ||
+        (rc = check_epilogue(who, e, out_type, d_out, out_stride, down->rows)) || (rc = check_sizes(who, n_vec, g->rows)) ||
+        (rc = check_sizes(who, n_vec, down->rows)) || (rc = check_ffn_workspace(who, g, down, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
+        (rc = check_ffn_workspace(who, g, down, n_vec, d_workspace, workspace_bytes)))
+        return rc;
+    const hipStream_t st = stream_of(stream);
+    const size_t h_bytes = ffn_h_bytes(g->rows, n_vec), h_stride = up64(g->rows);
+    uint8_t *rest = (uint8_t *)d_workspace + h_bytes;
+    if ((rc = gated_launch(g, d_q, q_stride, d_q_scale, n_vec, OXH_F32, d_workspace, h_stride, rest, workspace_bytes - h_bytes, st, who))) return rc;
+    I8ProductEx p = product_ex(i8_product(down, nullptr, 0, nullptr, n_vec, nullptr, out_type, d_out, out_stride), e);
+    return linear_launch(p, OXH_F32, d_workspace, h_stride, rest, workspace_bytes - h_bytes, st, who);
+}
+
+extern "C" int oxh_internal_i8_layer_init(void)
+{
+    const hipError_t e = product_init<I8ProductEx>();
+    return (int)(e == hipSuccess ? product_init<I8GatedProduct>() : e);
+}
+
+/* ─── which kernels run, for tests ────────────────────────────────────── */
+
+extern "C" int oxh_debug_i8_gated_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, uint32_t out[4])
+{
+    static const char who[] = "oxh_debug_i8_gated_kernel";
+    if (!out || !rows || !n_vec || !n_cu) return I8_ARG("%s: NULL or empty", who);
+    const int rc = check_cols(who, cols);
+    if (rc) return rc;
+    i8_describe(i8_choice(rows, cols, n_vec, ws_bytes, n_cu, 2u), rows, cols, n_vec, n_cu, 2u, out);
+    return OXH_OK;
+}

@@ -79,8 +79,12 @@ int oxh_internal_experts_batch_takes(int fmt, size_t n_mat, size_t n_expert, siz
 int oxh_internal_experts_batch(int fmt, int tile_major, const void *const *d_w, float *const *d_out, size_t n_mat,
                                size_t n_expert, size_t rows, size_t blocks, const void *d_acts, size_t out_stride,
                                const uint32_t *d_counts, const uint32_t *d_offsets, size_t pairs, size_t max_tokens, void *stream);
-/* Products over int8 rows (oxh_i8.hip); a hipError_t. */
+/* Products over int8 rows (oxh_i8.hip); init returns a hipError_t, the quantiser's launch a status.  Arguments checked by the
+ * caller, whose name `who` is. */
 int oxh_internal_i8_init(void);
+int oxh_internal_i8_layer_init(void);      /* oxh_i8_layer.hip */
+int oxh_internal_i8_quantize(uint32_t type, const void *x, size_t x_stride, size_t n, size_t cols, const void *up, int8_t *q,
+                             size_t q_stride, float *scale, void *stream, const char *who);
 /* Whether the runtime knows all of this memory (page-locked, managed or on the device) and so copies it without a
  * detour through staging of its own. */
 int oxh_internal_runtime_memory(const void *p, size_t bytes);
@@ -109,6 +113,7 @@ int oxh_debug_experts_batch(uint32_t qtype, size_t n_mat, size_t n_expert, size_
                             size_t n_cu);
 int oxh_debug_experts_tile(uint32_t qtype, size_t n_mat, size_t n_expert, size_t rows, size_t pairs, size_t n_cu, uint32_t tile[2]);
 int oxh_debug_i8_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int floats, uint32_t out[4]);
+int oxh_debug_i8_gated_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, uint32_t out[4]);
 struct OxhMoeI8;
 int oxh_debug_moe_i8_kernels(const struct OxhMoeI8 *m, size_t n_tok, int ids, size_t n_cu, uint32_t out[4]);
 uint64_t oxh_debug_mmq32_fetched(uint32_t block_bytes, uint32_t blocks, uint32_t row, uint32_t blk, uint32_t step);

@@ -1,7 +1,8 @@
-"""int8 rows with one scale per row: the quantiser, products and the expert layer (oxh_i8_*, oxh_moe_ffn_i8).
+"""int8 rows with one scale per row: the quantiser and the norm in front of it, products, plain and with an epilogue, the gated
+feed-forward block and the expert layer (oxh_i8_*, oxh_moe_ffn_i8).
 
-Addresses are integers, as everywhere in the device-resident layer; nothing here allocates but :class:`MoeLayer`, which
-owns its workspace, and :func:`from_packed`, which returns what it made.
+Addresses are integers, as everywhere in the device-resident layer; nothing here allocates but :class:`MoeLayer` and
+:class:`FeedForward`, which own their workspaces, and :func:`from_packed`, which returns what it made.
 """
 import ctypes
 
@@ -12,6 +13,7 @@ from . import matvec as mv
 from ._lib import check, lib
 
 F32, F16, BF16 = 0, 1, 2
+NONE, RELU, SILU, GELU, GELU_TANH = range(5)
 MAX_COLS, MAX_ROWS, MAX_RESULTS, MOE_MAX_VALUES = 131071, 1 << 21, 1 << 37, 1 << 35
 
 
@@ -46,6 +48,33 @@ def moe_kernels(desc, n_tok, ids=True, n_cu=256):
     return tuple(out)
 
 
+def gated_kernel(rows, cols, n_vec, ws_bytes=1 << 40, n_cu=256):
+    """:func:`kernel` for :class:`Gated`."""
+    out = (ctypes.c_uint32 * 4)()
+    check(_lib.lab().i8_gated_kernel(rows, cols, n_vec, n_cu, ws_bytes, ctypes.byref(out)))
+    return tuple(out)
+
+
+class Norm:
+    """A root-mean-square norm that leaves its rows as codes and scales; `d_add`: what is added first, `d_sum` and `d_y`: where the sum and
+    the normed floats are kept too, all in the type of x and at strides in elements.  Keeps the addresses it is given."""
+
+    def __init__(self, d_weight, eps, d_add=None, add_stride=0, d_sum=None, sum_stride=0, d_y=None, y_stride=0):
+        self.desc = _lib.OxhI8Norm(d_weight, eps, d_add, add_stride, d_sum, sum_stride, d_y, y_stride)
+        self._ref = ctypes.byref(self.desc)
+
+    def quantize(self, x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, stream=None):
+        check(lib().oxh_i8_rmsnorm(self._ref, x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, stream))
+
+
+class Epilogue:
+    """What a product does with its sums: act(sum * scales + bias) + residual.  Keeps the addresses it is given."""
+
+    def __init__(self, d_bias=None, act=NONE, d_residual=None, residual_stride=0):
+        self.desc = _lib.OxhI8Epilogue(d_bias, act, d_residual, residual_stride)
+        self._ref = ctypes.byref(self.desc)
+
+
 class Matrix:
     """An int8 matrix resident on the device, a scale per row; the memory is the caller's.  `stride`: bytes from row to row (cols: rows
     next to each other; :func:`stride_of` is fastest)."""
@@ -69,6 +98,47 @@ class Matrix:
         """Float tokens against the matrix, quantised on the way."""
         check(lib().oxh_i8_linear(self._ref, x_type, d_x, x_stride, n_vec, d_bias, out_type, d_out, out_stride, d_ws, ws_bytes,
                                   stream))
+
+    def matmul_ex(self, d_q, q_stride, d_q_scale, n_vec, epilogue, out_type, d_out, out_stride, d_ws=None, ws_bytes=0, stream=None):
+        """:meth:`matmul` with an :class:`Epilogue` (None: without); the same workspace."""
+        check(lib().oxh_i8_matmul_ex(self._ref, d_q, q_stride, d_q_scale, n_vec, epilogue._ref if epilogue else None, out_type, d_out,
+                                     out_stride, d_ws, ws_bytes, stream))
+
+    def linear_ex(self, x_type, d_x, x_stride, n_vec, epilogue, out_type, d_out, out_stride, d_ws=None, ws_bytes=0, stream=None):
+        """:meth:`linear` with an :class:`Epilogue` (None: without); the same workspace."""
+        check(lib().oxh_i8_linear_ex(self._ref, x_type, d_x, x_stride, n_vec, epilogue._ref if epilogue else None, out_type, d_out,
+                                     out_stride, d_ws, ws_bytes, stream))
+
+
+class Gated:
+    """The gate and up matrices of a feed-forward, resident on the device: act(gate) * up of quantised tokens in one launch.  Stride as
+    :class:`Matrix`'s, the same for both."""
+
+    def __init__(self, d_w_gate, d_s_gate, d_w_up, d_s_up, rows, cols, stride=None, act=SILU, d_b_gate=None, d_b_up=None):
+        self.desc = _lib.OxhI8Gated(d_w_gate, d_w_up, stride or cols, d_s_gate, d_s_up, d_b_gate, d_b_up, rows, cols, act)
+        self._ref = ctypes.byref(self.desc)
+
+    def workspace(self, n_vec):
+        return int(lib().oxh_i8_gated_workspace(self._ref, n_vec))
+
+    def matmul(self, d_q, q_stride, d_q_scale, n_vec, out_type, d_out, out_stride, d_ws=None, ws_bytes=0, stream=None):
+        check(lib().oxh_i8_gated(self._ref, d_q, q_stride, d_q_scale, n_vec, out_type, d_out, out_stride, d_ws, ws_bytes, stream))
+
+
+class FeedForward:
+    """A gated feed-forward block over quantised tokens (:class:`Gated`, then `down`, a :class:`Matrix`); owns its workspace, sized for
+    `max_tok` tokens: calls that overlap in time need a block each."""
+
+    def __init__(self, gated, down, max_tok=16):
+        self.gated, self.down, self.max_tok = gated, down, max_tok
+        self.workspace = mv.DeviceBuffer(max(256, int(lib().oxh_i8_ffn_workspace(gated._ref, down._ref, max_tok))))
+
+    def forward(self, d_q, q_stride, d_q_scale, n_tok, epilogue, out_type, d_out, out_stride, stream=None):
+        """`epilogue`: the down projection's bias and the residual (None: neither)."""
+        if n_tok > self.max_tok:
+            raise ValueError("n_tok %d beyond the workspace's %d" % (n_tok, self.max_tok))
+        check(lib().oxh_i8_ffn(self.gated._ref, self.down._ref, d_q, q_stride, d_q_scale, n_tok, epilogue._ref if epilogue else None,
+                               out_type, d_out, out_stride, self.workspace.ptr, self.workspace.nbytes, stream))
 
 
 def from_packed(qtype, d_w, rows, cols, stream=None):
