@@ -25,8 +25,8 @@ struct I8Norm {
     uint32_t cols;
 };
 
-/* Values c .. c + 7 of a row, those behind the last one `other`. */
-template <typename T> __device__ __forceinline__ void norm_load8(const T *from, uint32_t c, uint32_t cols, float other, float (&v)[8])
+/* Values c .. c + 7 of a row, those behind the last one 0. */
+template <typename T> __device__ __forceinline__ void norm_load8(const T *from, uint32_t c, uint32_t cols, float (&v)[8])
 {
     if (c + 8u <= cols) {
         const Run<T, 8> r = *reinterpret_cast<const Run<T, 8> *>(from + c);
@@ -34,7 +34,7 @@ template <typename T> __device__ __forceinline__ void norm_load8(const T *from, 
         for (int i = 0; i < 8; i++) v[i] = to_f32(r.v[i]);
     } else
 #pragma unroll
-        for (uint32_t i = 0; i < 8u; i++) v[i] = c + i < cols ? to_f32(from[c + i]) : other;
+        for (uint32_t i = 0; i < 8u; i++) v[i] = c + i < cols ? to_f32(from[c + i]) : 0.0f;
 }
 
 template <typename T> __device__ __forceinline__ void norm_store8(T *to, uint32_t c, uint32_t cols, const float (&v)[8])
@@ -50,10 +50,27 @@ template <typename T> __device__ __forceinline__ void norm_store8(T *to, uint32_
             if (c + i < cols) to[c + i] = from_f32<T>(v[i]);
 }
 
+/* the sum over the wave's lanes, in every lane, by exchanges within rows of sixteen and four scalar reads */
+__device__ __forceinline__ double wave_sum(double v)
+{
+    auto with = [&](auto exchange) {
+        const uint2 bits = __builtin_bit_cast(uint2, v);
+        v += __builtin_bit_cast(double, make_uint2((uint32_t)exchange((int)bits.x), (uint32_t)exchange((int)bits.y)));
+    };
+    with([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0xB1, 0xF, 0xF, false); });       /* lane ^ 1 */
+    with([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x4E, 0xF, 0xF, false); });       /* lane ^ 2 */
+    with([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x141, 0xF, 0xF, false); });      /* mirrored in 8 */
+    with([](int x) { return __builtin_amdgcn_update_dpp(0, x, 0x140, 0xF, 0xF, false); });      /* mirrored in 16 */
+    auto row = [&](int lane) {
+        const uint2 bits = __builtin_bit_cast(uint2, v);
+        return __builtin_bit_cast(double, make_uint2((uint32_t)__builtin_amdgcn_readlane((int)bits.x, lane), (uint32_t)__builtin_amdgcn_readlane((int)bits.y, lane)));
+    };
+    return (row(0) + row(16)) + (row(32) + row(48));
+}
+
 /* A row by a workgroup, eight values to a thread and step: s = x + add in 32 bits, the sum of its squares (each exact) and the norm in 64, so that
  * y, rounded once, does not depend on how a row is dealt to threads, and neither do its codes.  The first HELD steps' values stay in registers; what is longer is
- * read three times.  sum and y are written by the thread that has read those places, behind the last read: they may be x or
- * add. */
+ * read three times.  sum and y go only to places that the same thread has read for the last time: they may be x or add. */
 template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
 {
@@ -63,11 +80,17 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
     const size_t row = blockIdx.x;
     const T *x = (const T *)p.x + row * p.x_stride, *add = p.add ? (const T *)p.add + row * p.add_stride : nullptr;
     const uint32_t cols = p.cols, c0 = 8u * threadIdx.x, wave = threadIdx.x >> 6;
+    auto weights = [&](uint32_t c, float (&v)[8]) {
+        if (p.weight) norm_load8(p.weight, c, cols, v);
+        else
+#pragma unroll
+            for (int i = 0; i < 8; i++) v[i] = 1.0f;
+    };
     auto load = [&](uint32_t c, float (&v)[8]) {
-        norm_load8(x, c, cols, 0.0f, v);
+        norm_load8(x, c, cols, v);
         if (add) {
             float a[8];
-            norm_load8(add, c, cols, 0.0f, a);
+            norm_load8(add, c, cols, a);
 #pragma unroll
             for (int i = 0; i < 8; i++) v[i] += a[i];
         }
@@ -81,14 +104,18 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
 #pragma unroll
     for (int i = 0; i < HELD; i++) load(c0 + STEP * i, s[i]);
 #pragma unroll
-    for (int i = 0; i < HELD; i++) square(s[i]);
+    for (int i = 0; i < HELD; i++) weights(c0 + STEP * i, w[i]);
+#pragma unroll
+    for (int i = 0; i < HELD; i++) {
+        square(s[i]);
+        if (p.sum) norm_store8((T *)p.sum + row * p.sum_stride, c0 + STEP * i, cols, s[i]);
+    }
     for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
         float v[8];
         load(c, v);
         square(v);
     }
-#pragma unroll
-    for (uint32_t d = 32u; d; d >>= 1) squares += __shfl_xor(squares, (int)d);
+    squares = wave_sum(squares);
     if (THREADS > 64) {
         if ((threadIdx.x & 63u) == 0u) s_sum[wave] = squares;
         __syncthreads();
@@ -97,30 +124,23 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
         for (int i = 0; i < THREADS / 64; i++) squares += s_sum[i];
     }
     const double r = 1.0 / sqrt(squares / (double)cols + p.eps);
-    auto weights = [&](uint32_t c, float (&v)[8]) {
-        if (p.weight) norm_load8(p.weight, c, cols, 0.0f, v);
-        else
+    /* what stands for places behind the last column is 0 or, where r is no number, as little one as the row itself */
+    auto normed = [&](float (&v)[8], const float (&g)[8]) {
 #pragma unroll
-            for (int i = 0; i < 8; i++) v[i] = 1.0f;
+        for (int i = 0; i < 8; i++) v[i] = (float)((double)v[i] * r * (double)g[i]);
     };
-    auto normed = [&](const float (&v)[8], const float (&g)[8], float (&y)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; i++) y[i] = (float)((double)v[i] * r * (double)g[i]);
-    };
-    uint32_t top = 0;               /* what stands for places behind the last column is 0 or, where r is no number, as little one as the row itself */
+    uint32_t top = 0;
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-        float y[8];
-        weights(c0 + STEP * i, w[i]);
-        normed(s[i], w[i], y);
-        top = max(top, i8_top8(y));
+        normed(s[i], w[i]);
+        top = max(top, i8_top8(s[i]));
     }
     for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
-        float v[8], g[8], y[8];
+        float v[8], g[8];
         load(c, v);
         weights(c, g);
-        normed(v, g, y);
-        top = max(top, i8_top8(y));
+        normed(v, g);
+        top = max(top, i8_top8(v));
     }
     top = wave_top(top);
     if (THREADS > 64) {
@@ -133,33 +153,53 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
     const float scale = i8_scale(top, inv);
     if (threadIdx.x == 0u) p.scale[row] = scale;
     const uint32_t end = (cols + 15u) & ~15u;
-    auto store = [&](uint32_t c, const float (&v)[8], const float (&g)[8]) {
+    auto store = [&](uint32_t c, const float (&y)[8]) {
         if (c >= end) return;
-        float y[8];
-        normed(v, g, y);
         *reinterpret_cast<uint2 *>(p.q + row * p.q_stride + c) = inv != 0.0f ? i8_codes8(y, scale, inv) : make_uint2(0u, 0u);
-        if (p.sum) norm_store8((T *)p.sum + row * p.sum_stride, c, cols, v);
         if (p.y) norm_store8((T *)p.y + row * p.y_stride, c, cols, y);
     };
 #pragma unroll
-    for (int i = 0; i < HELD; i++) store(c0 + STEP * i, s[i], w[i]);
+    for (int i = 0; i < HELD; i++) store(c0 + STEP * i, s[i]);
     for (uint32_t c = c0 + STEP * HELD; c < end; c += STEP) {
         float v[8], g[8];
         load(c, v);
         weights(c, g);
-        store(c, v, g);
+        if (p.sum) norm_store8((T *)p.sum + row * p.sum_stride, c, cols, v);
+        normed(v, g);
+        store(c, v);
     }
 }
 
 /* ─── products with an epilogue ───────────────────────────────────────── */
 
-/* In 32 bits; a NaN stays one. */
+/* 1 / (1 + 2^t), by the instructions for both (a unit in the last place each; results below 2^-126 are 0) */
+__device__ __forceinline__ float i8_logistic(float t) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)); }
+
+/* v P(X <= v) of a normal X.  P(X > z) = 2^(-z^2 / (2 ln 2)) R(z) falls as fast as its first factor; R = erfcx(z / sqrt(2)) / 2 has no scale of its own and is a
+ * polynomial of degree 8 in 1 / (1 + 0.3 z) without a constant term, fitted to least relative error over 0 <= z <= 13.5, where the first
+ * factor leaves the f32 numbers: 7.2 * 2^-24 off with its own roundings. */
+__device__ __forceinline__ float i8_gelu(float v)
+{
+    const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, fabsf(v), 1.0f));
+    float r = 0.03593168780207634f;
+    r = __builtin_fmaf(r, t, -0.1582757830619812f);
+    r = __builtin_fmaf(r, t, 0.2082061916589737f);
+    r = __builtin_fmaf(r, t, -0.05539347976446152f);
+    r = __builtin_fmaf(r, t, 0.12946900725364685f);
+    r = __builtin_fmaf(r, t, 0.09963755309581757f);
+    r = __builtin_fmaf(r, t, 0.12079835683107376f);
+    r = __builtin_fmaf(r, t, 0.11962639540433884f);
+    const float above = __builtin_amdgcn_exp2f(v * v * -0.72134752f) * (r * t);
+    return v * (v > 0.0f ? 1.0f - above : above);
+}
+
+/* In 32 bits; a NaN stays one.  SILU's exponent is rounded once: -1 / ln 2 is the sum of two f32 numbers. */
 __device__ __forceinline__ float i8_activate(uint32_t act, float v)
 {
     if (act == OXH_ACT_RELU) return v < 0.0f ? 0.0f : v;
-    if (act == OXH_ACT_SILU) return silu(v);
-    if (act == OXH_ACT_GELU) return 0.5f * v * erfcf(v * -0.70710678f);
-    if (act == OXH_ACT_GELU_TANH) return v / (1.0f + expf(-1.59576912f * (v + 0.044715f * v * v * v)));     /* (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u)) */
+    if (act == OXH_ACT_SILU) return v * i8_logistic(__builtin_fmaf(v, -1.44269502f, v * -1.92596299e-8f));
+    if (act == OXH_ACT_GELU) return i8_gelu(v);
+    if (act == OXH_ACT_GELU_TANH) return v * i8_logistic(v * __builtin_fmaf(v * v, -0.10294324f, -2.30220820f));    /* (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u)) */
     return v;
 }
 
@@ -169,16 +209,14 @@ struct I8ProductEx : I8Product {
     uint32_t act;
 };
 
-template <typename T> __device__ __forceinline__ void add_residual4(const T *from, uint32_t left, float (&v)[4])
+/* four neighbouring values of the residual, as i8_store4 stores them */
+template <typename T> __device__ __forceinline__ v4f residual4(const T *from, uint32_t left)
 {
     if (left >= 4u) {
         const Run<T, 4> r = *reinterpret_cast<const Run<T, 4> *>(from);
-#pragma unroll
-        for (int i = 0; i < 4; i++) v[i] += to_f32(r.v[i]);
-    } else
-#pragma unroll
-        for (uint32_t i = 0; i < 3u; i++)
-            if (i < left) v[i] += to_f32(from[i]);
+        return v4f{ to_f32(r.v[0]), to_f32(r.v[1]), to_f32(r.v[2]), to_f32(r.v[3]) };
+    }
+    return v4f{ to_f32(from[0]), left > 1u ? to_f32(from[1]) : 0.0f, left > 2u ? to_f32(from[2]) : 0.0f, 0.0f };
 }
 
 __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[1], const I8RowFactors (&f)[1], float st)
@@ -193,9 +231,11 @@ __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uin
     if (p.residual) {
         const size_t at = (size_t)t * p.residual_stride + r;
         const uint32_t left = (uint32_t)p.w.rows - r;
-        if (p.out_type == OXH_F32) add_residual4((const float *)p.residual + at, left, v);
-        else if (p.out_type == OXH_F16) add_residual4((const _Float16 *)p.residual + at, left, v);
-        else add_residual4((const __bf16 *)p.residual + at, left, v);
+        const v4f more = p.out_type == OXH_F32   ? residual4((const float *)p.residual + at, left)
+                         : p.out_type == OXH_F16 ? residual4((const _Float16 *)p.residual + at, left)
+                                                 : residual4((const __bf16 *)p.residual + at, left);
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) v[k] += more[k];
     }
     i8_put(p, r, t, v);
 }
@@ -276,7 +316,10 @@ extern "C" int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void
 #define OXH_NORM(T)                                                                                                              \
     do {                                                                                                                         \
         if (cols <= 512u) OXH_NORM_K(T, 64, 1);                                                                                  \
+        else if (cols <= 1024u) OXH_NORM_K(T, 128, 1);                                                                           \
         else if (cols <= 2048u) OXH_NORM_K(T, 256, 1);                                                                           \
+        else if (cols <= 4096u) OXH_NORM_K(T, 512, 1);                                                                           \
+        else if (cols <= 8192u) OXH_NORM_K(T, 512, 2);                                                                           \
         else OXH_NORM_K(T, 1024, 2);                                                                                             \
     } while (0)
     if (x_type == OXH_F32) OXH_NORM(float);

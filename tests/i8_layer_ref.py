@@ -7,7 +7,7 @@ import numpy as np
 import i8_ref as ref
 
 HALF = 2.0 ** -24
-LOST = 2.61e-37             # what an activation may lose next to the smallest numbers (activation())
+LOST = 1.03e-36             # what an activation may lose next to the smallest numbers (activation())
 NONE, RELU, SILU, GELU, GELU_TANH = range(5)
 ACTS = {"none": NONE, "relu": RELU, "silu": SILU, "gelu": GELU, "gelu_tanh": GELU_TANH}
 _erfc = np.vectorize(math.erfc, otypes=[np.float64])
@@ -33,9 +33,8 @@ def activation(act, v):
     -v / sqrt(2) with two roundings (a constant, a product), which move erfc by at most (2 z^2 + 2) times theirs, z^2 = v^2 / 2; an exponential of z^2 (three
     roundings of z^2 as an argument), and 32 for erfc's own: 40 + 4 v^2.
 
-    LOST: v / (1 + exp(-v)) is 0 where exp(-v) passes the largest f32, below 2^128: from v = -128 ln 2 = -88.7229 on, where |v| e^v, which falls from there, is
-    88.7229 * 2^-128 = 2.607e-37 at most.  GELU_TANH is lost from 2u = -88.7229, v = -10.1, on: less.  GELU's erfc leaves the
-    normal numbers below 2^-126: |v| / 2 of it, at v = -13, 8e-38."""
+    LOST: an exponential, its reciprocal and erfc count as 0 below 2^-126.  SILU: from v = -126 ln 2 = -87.34 on, where |v| e^v, which falls
+    from there, is 87.34 * 2^-126 = 1.027e-36 at most.  GELU_TANH: from 2u = -87.34, v = -10, on: less.  GELU: |v| of it, at v = -13, 1.6e-37."""
     with np.errstate(all="ignore"):
         x = v.astype(np.float64)
         if act == RELU:
