@@ -194,16 +194,62 @@ __device__ __forceinline__ float i8_gelu(float v)
 }
 
 /* In 32 bits; a NaN stays one.  SILU's exponent is rounded once: -1 / ln 2 is the sum of two f32 numbers. */
-__device__ __forceinline__ float i8_activate(uint32_t act, float v)
+template <uint32_t ACT> __device__ __forceinline__ float i8_activate(float v)
 {
-    if (act == OXH_ACT_RELU) return v < 0.0f ? 0.0f : v;
-    if (act == OXH_ACT_SILU) return v * i8_logistic(__builtin_fmaf(v, -1.44269502f, v * -1.92596299e-8f));
-    if (act == OXH_ACT_GELU) return i8_gelu(v);
-    if (act == OXH_ACT_GELU_TANH) return v * i8_logistic(v * __builtin_fmaf(v * v, -0.10294324f, -2.30220820f));    /* (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u)) */
-    return v;
+    if (ACT == OXH_ACT_RELU) return v < 0.0f ? 0.0f : v;
+    if (ACT == OXH_ACT_SILU) return v * i8_logistic(__builtin_fmaf(v, -1.44269502f, v * -1.92596299e-8f));
+    if (ACT == OXH_ACT_GELU) return i8_gelu(v);
+    return v * i8_logistic(v * __builtin_fmaf(v * v, -0.10294324f, -2.30220820f));      /* (1 + tanh(u)) / 2 = 1 / (1 + exp(-2u)) */
+}
+
+/* Of many values at a time: what an activation waits for, an exponential and a reciprocal, is under way for all of them, where a branch on its kind for each
+ * value would end every one's chain first (4096 tokens over 14336 x 4096, bias and GELU: BEFORE us; like this AFTER). */
+template <uint32_t N> __device__ __forceinline__ void i8_activate_all(uint32_t act, float (&v)[N][4])
+{
+    auto all = [&](auto kind) {
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) v[i][k] = i8_activate<kind.value>(v[i][k]);
+    };
+    if (act == OXH_ACT_RELU) all(I8Num<OXH_ACT_RELU>{});
+    else if (act == OXH_ACT_SILU) all(I8Num<OXH_ACT_SILU>{});
+    else if (act == OXH_ACT_GELU) all(I8Num<OXH_ACT_GELU>{});
+    else if (act == OXH_ACT_GELU_TANH) all(I8Num<OXH_ACT_GELU_TANH>{});
+}
+
+/* sum * q_scale * w_scale + bias */
+template <uint32_t N, uint32_t M> __device__ __forceinline__ void i8_scaled(const v4i (&sums)[N][M], const I8RowFactors (&f)[N][M], uint32_t m, float st, bool bias, float (&v)[N][4])
+{
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) v[i][k] = (float)sums[i][m][k] * st * f[i][m].s[k];
+    if (bias)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) v[i][k] += f[i][m].b[k];
+}
+
+template <typename T, uint32_t N> __device__ __forceinline__ void i8_put_all(T *out, uint32_t left, const float (&v)[N][4])
+{
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++)
+        if (16u * i < left) i8_store4(out + 16u * i, v[i], left - 16u * i);
+}
+template <uint32_t N> __device__ __forceinline__ void i8_put_all(const I8Product &p, uint32_t r, uint32_t t, const float (&v)[N][4])
+{
+    if (r >= (uint32_t)p.w.rows) return;
+    const size_t at = (size_t)t * p.out_stride + r;
+    const uint32_t left = (uint32_t)p.w.rows - r;
+    if (p.out_type == OXH_F32) i8_put_all((float *)p.out + at, left, v);
+    else if (p.out_type == OXH_F16) i8_put_all((_Float16 *)p.out + at, left, v);
+    else i8_put_all((__bf16 *)p.out + at, left, v);
 }
 
 struct I8ProductEx : I8Product {
+    static constexpr bool TOGETHER = true;
     const void *residual;
     size_t residual_stride;
     uint32_t act;
@@ -218,26 +264,31 @@ template <typename T> __device__ __forceinline__ v4f residual4(const T *from, ui
     }
     return v4f{ to_f32(from[0]), left > 1u ? to_f32(from[1]) : 0.0f, left > 2u ? to_f32(from[2]) : 0.0f, 0.0f };
 }
-
-__device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[1], const I8RowFactors (&f)[1], float st)
+template <typename T, uint32_t N> __device__ __forceinline__ void residual_all(const T *from, uint32_t left, float (&v)[N][4])
 {
-    float v[4];
+    v4f more[N];
 #pragma unroll
-    for (uint32_t k = 0; k < 4u; k++) {
-        v[k] = (float)sums[0][k] * st * f[0].s[k];
-        if (p.bias) v[k] += f[0].b[k];
-        v[k] = i8_activate(p.act, v[k]);
-    }
-    if (p.residual) {
+    for (uint32_t i = 0; i < N; i++) more[i] = 16u * i < left ? residual4(from + 16u * i, left - 16u * i) : v4f{ 0.0f, 0.0f, 0.0f, 0.0f };
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) v[i][k] += more[i][k];
+}
+
+template <uint32_t N>
+__device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[N][1], const I8RowFactors (&f)[N][1], float st)
+{
+    float v[N][4];
+    i8_scaled(sums, f, 0u, st, p.bias != nullptr, v);
+    i8_activate_all(p.act, v);
+    if (p.residual && r < (uint32_t)p.w.rows) {
         const size_t at = (size_t)t * p.residual_stride + r;
         const uint32_t left = (uint32_t)p.w.rows - r;
-        const v4f more = p.out_type == OXH_F32   ? residual4((const float *)p.residual + at, left)
-                         : p.out_type == OXH_F16 ? residual4((const _Float16 *)p.residual + at, left)
-                                                 : residual4((const __bf16 *)p.residual + at, left);
-#pragma unroll
-        for (uint32_t k = 0; k < 4u; k++) v[k] += more[k];
+        if (p.out_type == OXH_F32) residual_all((const float *)p.residual + at, left, v);
+        else if (p.out_type == OXH_F16) residual_all((const _Float16 *)p.residual + at, left, v);
+        else residual_all((const __bf16 *)p.residual + at, left, v);
     }
-    i8_put(p, r, t, v);
+    i8_put_all(p, r, t, v);
 }
 
 /* ─── gated products ──────────────────────────────────────────────────── */
@@ -245,6 +296,7 @@ __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uin
 /* w and bias are the gate's */
 struct I8GatedProduct : I8Product {
     static constexpr uint32_t MATRICES = 2;
+    static constexpr bool TOGETHER = true;
     const int8_t *up;
     const float *up_scale, *up_bias;
     uint32_t act;
@@ -264,17 +316,25 @@ __device__ __forceinline__ void i8_row_factors(const I8GatedProduct &p, uint32_t
     }
 }
 
-__device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, uint32_t t, const v4i (&sums)[2], const I8RowFactors (&f)[2], float st)
+template <uint32_t N>
+__device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, uint32_t t, const v4i (&sums)[N][2], const I8RowFactors (&f)[N][2], float st)
 {
-    float v[4];
+    float v[N][4], up[N][4];
+    i8_scaled(sums, f, 0u, st, p.bias != nullptr, v);
+    i8_activate_all(p.act, v);
+    i8_scaled(sums, f, 1u, st, p.up_bias != nullptr, up);
 #pragma unroll
-    for (uint32_t k = 0; k < 4u; k++) {
-        float g = (float)sums[0][k] * st * f[0].s[k], u = (float)sums[1][k] * st * f[1].s[k];
-        if (p.bias) g += f[0].b[k];
-        if (p.up_bias) u += f[1].b[k];
-        v[k] = i8_activate(p.act, g) * u;
-    }
-    i8_put(p, r, t, v);
+    for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) v[i][k] *= up[i][k];
+    i8_put_all(p, r, t, v);
+}
+
+/* the same of one fragment's rows, as the kernels for few tokens and the joined parts have them */
+template <typename P, uint32_t M> __device__ __forceinline__ void i8_results(const P &p, uint32_t r, uint32_t t, const v4i (&sums)[M], const I8RowFactors (&f)[M], float st)
+{
+    const v4i(&one)[1][M] = reinterpret_cast<const v4i(&)[1][M]>(sums);
+    i8_results<1u>(p, r, t, one, reinterpret_cast<const I8RowFactors(&)[1][M]>(f), st);
 }
 
 /* ─── host side ───────────────────────────────────────────────────────── */
