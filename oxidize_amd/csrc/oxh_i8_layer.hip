@@ -232,20 +232,87 @@ template <uint32_t N, uint32_t M> __device__ __forceinline__ void i8_scaled(cons
             for (uint32_t k = 0; k < 4u; k++) v[i][k] += f[i][m].b[k];
 }
 
-template <typename T, uint32_t N> __device__ __forceinline__ void i8_put_all(T *out, uint32_t left, const float (&v)[N][4])
+/* A lane's results, rows r + 16 i .. + 3 of token t, to memory, whole lines at a time.  A wave holds four rows of each of sixteen tokens: a store of those as
+ * they are writes 32 (16-bit results) or 64 neighbouring bytes of a token's row.  So lanes change places first, without LDS: of two fragments of
+ * 16-bit results the lanes of odd rows of sixteen give their share of the first for their neighbours' of the second, and have 16 bytes each of one,
+ * 64 of a token; then of two such the lanes of the upper eight tokens give the first for the lower eight's second, and a store writes 128
+ * bytes of each of eight tokens.  (4096 tokens over 14336 x 4096, bf16: bias and GELU BEFORE us without, BETWEEN with the first change, AFTER with both.)  Every
+ * lane takes part, whether its token is there or not. */
+template <typename T, uint32_t N>
+__device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4])
 {
+    constexpr bool HALF = sizeof(T) == 2;
+    if constexpr (N >= (HALF ? 2u : 1u)) {
+        constexpr uint32_t PIECES = HALF ? N / 2u : N, SPAN = HALF ? 32u : 16u, HAS = 16u / sizeof(T);      /* a lane's pieces of 16 bytes, rows from one to the next, rows of one */
+        uint4 piece[PIECES];
 #pragma unroll
-    for (uint32_t i = 0; i < N; i++)
-        if (16u * i < left) i8_store4(out + 16u * i, v[i], left - 16u * i);
+        for (uint32_t i = 0; i < PIECES; i++) {
+            typedef T T4 __attribute__((ext_vector_type(4)));
+            if constexpr (HALF) {
+                const uint2 a = __builtin_bit_cast(uint2, (T4){ from_f32<T>(v[2u * i][0]), from_f32<T>(v[2u * i][1]), from_f32<T>(v[2u * i][2]), from_f32<T>(v[2u * i][3]) });
+                const uint2 b = __builtin_bit_cast(uint2, (T4){ from_f32<T>(v[2u * i + 1u][0]), from_f32<T>(v[2u * i + 1u][1]), from_f32<T>(v[2u * i + 1u][2]), from_f32<T>(v[2u * i + 1u][3]) });
+                const auto lo = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), hi = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
+                piece[i] = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+            } else piece[i] = __builtin_bit_cast(uint4, (T4){ v[i][0], v[i][1], v[i][2], v[i][3] });
+        }
+        const uint32_t kq = (threadIdx.x >> 4) & 3u;
+        uint32_t row = HALF ? r - 4u * kq + 16u * (kq & 1u) + 8u * (kq >> 1) : r;
+        auto store = [&](uint32_t token, uint32_t at, const uint4 &what) {
+            if (token >= n_vec) return;
+            T *to = out + (size_t)token * stride + at;
+            const Run<T, HAS> all = __builtin_bit_cast(Run<T, HAS>, what);
+            if (at + HAS <= rows) *reinterpret_cast<Run<T, HAS> *>(to) = all;
+            else
+#pragma unroll
+                for (uint32_t k = 0; k < HAS - 1u; k++)
+                    if (at + k < rows) to[k] = all.v[k];
+        };
+        if constexpr (PIECES % 2u == 0u) {
+            const uint32_t upper = (threadIdx.x >> 3) & 1u;
+            row += SPAN * upper;
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; i += 2u) {
+                const uint4 x = piece[i], y = piece[i + 1u];
+                auto low = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xF, 0xC, false); };     /* a, in the upper eight lanes the lower's b */
+                auto high = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xF, 0x3, false); };    /* b, in the lower eight the upper's a */
+                store(t - 8u * upper, row + SPAN * i, make_uint4(low(x.x, y.x), low(x.y, y.y), low(x.z, y.z), low(x.w, y.w)));
+                store(t + 8u - 8u * upper, row + SPAN * i, make_uint4(high(x.x, y.x), high(x.y, y.y), high(x.z, y.z), high(x.w, y.w)));
+            }
+        } else
+#pragma unroll
+            for (uint32_t i = 0; i < PIECES; i++) store(t, row + SPAN * i, piece[i]);
+    } else if (t < n_vec)
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            if (r + 16u * i < rows) i8_store4(out + (size_t)t * stride + r + 16u * i, v[i], rows - r - 16u * i);
 }
 template <uint32_t N> __device__ __forceinline__ void i8_put_all(const I8Product &p, uint32_t r, uint32_t t, const float (&v)[N][4])
 {
-    if (r >= (uint32_t)p.w.rows) return;
-    const size_t at = (size_t)t * p.out_stride + r;
-    const uint32_t left = (uint32_t)p.w.rows - r;
-    if (p.out_type == OXH_F32) i8_put_all((float *)p.out + at, left, v);
-    else if (p.out_type == OXH_F16) i8_put_all((_Float16 *)p.out + at, left, v);
-    else i8_put_all((__bf16 *)p.out + at, left, v);
+    const uint32_t rows = (uint32_t)p.w.rows;
+    if (p.out_type == OXH_F32) i8_put_all((float *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
+    else if (p.out_type == OXH_F16) i8_put_all((_Float16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
+    else i8_put_all((__bf16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
+}
+
+/* Scales (or biases, if there are any) of matrix m's rows r + 16 i .. + 3, 16 bytes a load where all four exist; behind the last row the last
+ * one again. */
+template <uint32_t N, uint32_t M>
+__device__ __forceinline__ void i8_rows4(const float *from, uint32_t r, uint32_t rows, uint32_t m, float (I8RowFactors::*to)[4], I8RowFactors (&f)[N][M])
+{
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) {
+        const uint32_t at = r + 16u * i;
+        if (!from)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) (f[i][m].*to)[k] = 0.0f;
+        else if (at + 4u <= rows) {
+            const Run<float, 4> v = *reinterpret_cast<const Run<float, 4> *>(from + at);
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) (f[i][m].*to)[k] = v.v[k];
+        } else
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) (f[i][m].*to)[k] = from[min(at + k, rows - 1u)];
+    }
 }
 
 struct I8ProductEx : I8Product {
@@ -254,6 +321,12 @@ struct I8ProductEx : I8Product {
     size_t residual_stride;
     uint32_t act;
 };
+
+template <uint32_t N> __device__ __forceinline__ void i8_row_factors(const I8ProductEx &p, uint32_t r, I8RowFactors (&f)[N][1])
+{
+    i8_rows4(p.w.d_scale, r, (uint32_t)p.w.rows, 0u, &I8RowFactors::s, f);
+    i8_rows4(p.bias, r, (uint32_t)p.w.rows, 0u, &I8RowFactors::b, f);
+}
 
 /* four neighbouring values of the residual, as i8_store4 stores them */
 template <typename T> __device__ __forceinline__ v4f residual4(const T *from, uint32_t left)
@@ -282,7 +355,7 @@ __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uin
     i8_scaled(sums, f, 0u, st, p.bias != nullptr, v);
     i8_activate_all(p.act, v);
     if (p.residual && r < (uint32_t)p.w.rows) {
-        const size_t at = (size_t)t * p.residual_stride + r;
+        const size_t at = (size_t)min(t, p.n_vec - 1u) * p.residual_stride + r;
         const uint32_t left = (uint32_t)p.w.rows - r;
         if (p.out_type == OXH_F32) residual_all((const float *)p.residual + at, left, v);
         else if (p.out_type == OXH_F16) residual_all((const _Float16 *)p.residual + at, left, v);
@@ -304,16 +377,13 @@ struct I8GatedProduct : I8Product {
 
 __device__ __forceinline__ const int8_t *i8_codes_of(const I8GatedProduct &p, uint32_t m) { return m ? p.up : p.w.d_w; }
 
-__device__ __forceinline__ void i8_row_factors(const I8GatedProduct &p, uint32_t r, I8RowFactors (&f)[2])
+template <uint32_t N> __device__ __forceinline__ void i8_row_factors(const I8GatedProduct &p, uint32_t r, I8RowFactors (&f)[N][2])
 {
-#pragma unroll
-    for (uint32_t k = 0; k < 4u; k++) {
-        const uint32_t rk = min(r + k, (uint32_t)p.w.rows - 1u);
-        f[0].s[k] = p.w.d_scale[rk];
-        f[1].s[k] = p.up_scale[rk];
-        f[0].b[k] = p.bias ? p.bias[rk] : 0.0f;
-        f[1].b[k] = p.up_bias ? p.up_bias[rk] : 0.0f;
-    }
+    const uint32_t rows = (uint32_t)p.w.rows;
+    i8_rows4(p.w.d_scale, r, rows, 0u, &I8RowFactors::s, f);
+    i8_rows4(p.up_scale, r, rows, 1u, &I8RowFactors::s, f);
+    i8_rows4(p.bias, r, rows, 0u, &I8RowFactors::b, f);
+    i8_rows4(p.up_bias, r, rows, 1u, &I8RowFactors::b, f);
 }
 
 template <uint32_t N>
@@ -331,10 +401,13 @@ __device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, 
 }
 
 /* the same of one fragment's rows, as the kernels for few tokens and the joined parts have them */
+template <typename P, uint32_t M> __device__ __forceinline__ void i8_row_factors(const P &p, uint32_t r, I8RowFactors (&f)[M])
+{
+    i8_row_factors<1u>(p, r, reinterpret_cast<I8RowFactors(&)[1][M]>(f));
+}
 template <typename P, uint32_t M> __device__ __forceinline__ void i8_results(const P &p, uint32_t r, uint32_t t, const v4i (&sums)[M], const I8RowFactors (&f)[M], float st)
 {
-    const v4i(&one)[1][M] = reinterpret_cast<const v4i(&)[1][M]>(sums);
-    i8_results<1u>(p, r, t, one, reinterpret_cast<const I8RowFactors(&)[1][M]>(f), st);
+    i8_results<1u>(p, r, t, reinterpret_cast<const v4i(&)[1][M]>(sums), reinterpret_cast<const I8RowFactors(&)[1][M]>(f), st);
 }
 
 /* ─── host side ───────────────────────────────────────────────────────── */
