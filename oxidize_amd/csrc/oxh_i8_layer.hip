@@ -11,6 +11,18 @@
 #include "i8_products.inc"
 #include "i8_host.inc"
 
+/* Bytes that the L2s are told not to keep: results of a launch, which nobody reads before the next one. */
+typedef uint32_t Stored8 __attribute__((ext_vector_type(2), aligned(2)));
+typedef uint32_t Stored16 __attribute__((ext_vector_type(4), aligned(2)));
+template <typename W, typename V> __device__ __forceinline__ void store_past(void *to, const V &v)
+{
+    static_assert(sizeof(V) % sizeof(W) == 0, "whole stores");
+    struct All { W w[sizeof(V) / sizeof(W)]; };
+    const All all = __builtin_bit_cast(All, v);
+#pragma unroll
+    for (uint32_t i = 0; i < sizeof(V) / sizeof(W); i++) __builtin_nontemporal_store(all.w[i], (W *)to + i);
+}
+
 /* ─── norm ────────────────────────────────────────────────────────────── */
 
 struct I8Norm {
@@ -43,7 +55,7 @@ template <typename T> __device__ __forceinline__ void norm_store8(T *to, uint32_
         Run<T, 8> r;
 #pragma unroll
         for (int i = 0; i < 8; i++) r.v[i] = from_f32<T>(v[i]);
-        *reinterpret_cast<Run<T, 8> *>(to + c) = r;
+        store_past<Stored16>(to + c, r);
     } else
 #pragma unroll
         for (uint32_t i = 0; i < 8u; i++)
@@ -70,7 +82,9 @@ __device__ __forceinline__ double wave_sum(double v)
 
 /* A row by a workgroup, eight values to a thread and step: s = x + add in 32 bits, the sum of its squares (each exact) and the norm in 64, so that
  * y, rounded once, does not depend on how a row is dealt to threads, and neither do its codes.  The first HELD steps' values stay in registers; what is longer is
- * read three times.  sum and y go only to places that the same thread has read for the last time: they may be x or add. */
+ * read three times.  sum and y go only to places that the same thread has read for the last time: they may be x or add.  Bound by memory: 4096 rows
+ * of 4096 bf16 with add and sum in 26 us, 4.5 TB/s read and written (30 with ordinary stores), of 14336 in 92, 4.5 TB/s (114); one row of
+ * 4096 in 3.3, a trip to memory and two barriers. */
 template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
 {
@@ -155,7 +169,7 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
     const uint32_t end = (cols + 15u) & ~15u;
     auto store = [&](uint32_t c, const float (&y)[8]) {
         if (c >= end) return;
-        *reinterpret_cast<uint2 *>(p.q + row * p.q_stride + c) = inv != 0.0f ? i8_codes8(y, scale, inv) : make_uint2(0u, 0u);
+        store_past<Stored8>(p.q + row * p.q_stride + c, inv != 0.0f ? i8_codes8(y, scale, inv) : make_uint2(0u, 0u));
         if (p.y) norm_store8((T *)p.y + row * p.y_stride, c, cols, y);
     };
 #pragma unroll
@@ -203,7 +217,7 @@ template <uint32_t ACT> __device__ __forceinline__ float i8_activate(float v)
 }
 
 /* Of many values at a time: what an activation waits for, an exponential and a reciprocal, is under way for all of them, where a branch on its kind for each
- * value would end every one's chain first (4096 tokens over 14336 x 4096, bias and GELU: BEFORE us; like this AFTER). */
+ * value would end every one's chain first (4096 tokens over 14336 x 4096, bias and GELU: 269 us; like this 262). */
 template <uint32_t N> __device__ __forceinline__ void i8_activate_all(uint32_t act, float (&v)[N][4])
 {
     auto all = [&](auto kind) {
@@ -236,8 +250,9 @@ template <uint32_t N, uint32_t M> __device__ __forceinline__ void i8_scaled(cons
  * they are writes 32 (16-bit results) or 64 neighbouring bytes of a token's row.  So lanes change places first, without LDS: of two fragments of
  * 16-bit results the lanes of odd rows of sixteen give their share of the first for their neighbours' of the second, and have 16 bytes each of one,
  * 64 of a token; then of two such the lanes of the upper eight tokens give the first for the lower eight's second, and a store writes 128
- * bytes of each of eight tokens.  (4096 tokens over 14336 x 4096, bf16: bias and GELU BEFORE us without, BETWEEN with the first change, AFTER with both.)  Every
- * lane takes part, whether its token is there or not. */
+ * bytes of each of eight tokens.  The L2s are told to keep none of it: a launch's results would push the operands of its other tiles out.  (4096 tokens over
+ * 14336 x 4096, bf16, bias and GELU: 259 us without all that, 235 with the first change, 234 with both, 217 with the stores past the L2s; gate and up 413,
+ * 387, 385 and 366.)  Every lane takes part, whether its token is there or not. */
 template <typename T, uint32_t N>
 __device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4])
 {
@@ -260,12 +275,13 @@ __device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, ui
         auto store = [&](uint32_t token, uint32_t at, const uint4 &what) {
             if (token >= n_vec) return;
             T *to = out + (size_t)token * stride + at;
-            const Run<T, HAS> all = __builtin_bit_cast(Run<T, HAS>, what);
-            if (at + HAS <= rows) *reinterpret_cast<Run<T, HAS> *>(to) = all;
-            else
+            if (at + HAS <= rows) store_past<Stored16>(to, what);
+            else {
+                const Run<T, HAS> all = __builtin_bit_cast(Run<T, HAS>, what);
 #pragma unroll
                 for (uint32_t k = 0; k < HAS - 1u; k++)
                     if (at + k < rows) to[k] = all.v[k];
+            }
         };
         if constexpr (PIECES % 2u == 0u) {
             const uint32_t upper = (threadIdx.x >> 3) & 1u;
@@ -446,11 +462,15 @@ extern "C" int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void
     const dim3 grid((uint32_t)n_vec);
     const hipStream_t st = stream_of(stream);
 #define OXH_NORM_K(T, THREADS, HELD) hipLaunchKernelGGL((k_i8_rmsnorm<T, THREADS, HELD>), grid, dim3(THREADS), 0, st, p)
+    /* Threads to a row: as few as hold its values in a step or two, so that they are read once (us of 4096 bf16 rows with 256 threads and two
+     * steps, 512 and one, 512 and two, 1024 and two: of 4096 values 26.0, 28.7, 35.9, 77; one row 3.8, 3.5, 4.5, 5.8; 4096 f32 rows 38.1, 36.4; 2048 bf16 rows of
+     * 8192 with 512 and two, 1024 and one: 27.5, 37.8; 4096 of 14336 with 1024 and two, 512 and two, which reads some twice more: 92, 96). */
 #define OXH_NORM(T)                                                                                                              \
     do {                                                                                                                         \
         if (cols <= 512u) OXH_NORM_K(T, 64, 1);                                                                                  \
         else if (cols <= 1024u) OXH_NORM_K(T, 128, 1);                                                                           \
         else if (cols <= 2048u) OXH_NORM_K(T, 256, 1);                                                                           \
+        else if (cols <= 4096u && sizeof(T) == 2 && n_vec >= 1024u) OXH_NORM_K(T, 256, 2);                                       \
         else if (cols <= 4096u) OXH_NORM_K(T, 512, 1);                                                                           \
         else if (cols <= 8192u) OXH_NORM_K(T, 512, 2);                                                                           \
         else OXH_NORM_K(T, 1024, 2);                                                                                             \
