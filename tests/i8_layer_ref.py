@@ -105,23 +105,20 @@ def ffn(q, qs, gate, up, act, down, residual=None):
 
 # Sizes at which each kernel of the gated product runs on 256 compute units, as in i8_shapes: [(tokens, rows, columns)]
 GATED = {
-    (1, 2, 1): [(1, 1, 1), (16, 200, 2048), (7, 2048, 1000)],
-    (1, 4, 1): [(1, 16, 2103), (8, 40, 4096), (5, 14336, 4096)],
-    (1, 8, 1): [(1, 3415, 4949), (2, 4096, 8192), (8, 3912, 4505)],
-    (2, 2, 2): [(17, 16, 64), (32, 50, 2040)],
-    (2, 2, 3): [(34, 16, 65), (48, 70, 2048)],
-    (2, 2, 4): [(51, 17, 66), (64, 2048, 2000)],
+    (1, 2, 1): [(1, 1, 1), (8, 200, 2048), (7, 2048, 1000)],
+    (1, 4, 1): [(1, 16, 2103), (8, 40, 4096), (5, 4096, 4096)],
+    (1, 8, 1): [(1, 1, 4146), (1, 3415, 4949), (2, 4096, 8192), (4, 3912, 4505)],
     (0, 0, False, False): [(514, 10000, 132)],
     (0, 0, False, True): [(707, 14552, 415)],
     (0, 0, True, False): [(155, 5663, 12638)],
     (0, 1, False, False): [(243, 8805, 1433)],
-    (0, 1, True, False): [(455, 1366, 9055)],
+    (0, 1, True, False): [(204, 2816, 13387)],
     (0, 2, False, False): [(275, 5936, 259)],
-    (0, 2, True, False): [(260, 1891, 6834)],
+    (0, 2, True, False): [(158, 2901, 8183)],
     (0, 3, False, False): [(67, 8328, 65), (333, 4864, 896)],
-    (0, 3, True, False): [(66, 1450, 7728)],
-    (0, 4, False, False): [(67, 16, 64), (70, 150, 1030), (16, 14336, 4096)],
-    (0, 4, True, False): [(9, 16, 4230), (1, 1, 4146), (48, 2048, 8000)],
+    (0, 3, True, False): [(252, 2299, 9671)],
+    (0, 4, False, False): [(67, 16, 64), (70, 150, 1030), (16, 14336, 4096), (5, 14336, 4096), (17, 16, 64), (34, 16, 65), (64, 2048, 2000), (260, 1891, 6834)],
+    (0, 4, True, False): [(9, 16, 8276), (1, 1, 8543), (48, 2048, 8000), (66, 1450, 7728)],
     (0, 5, False, False): [(1, 17582, 64), (33, 20000, 100)],
-    (0, 5, True, False): [(1, 2365, 4614)],
+    (0, 5, True, False): [(1, 4455, 7576)],
 }
