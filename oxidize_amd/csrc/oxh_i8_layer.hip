@@ -364,6 +364,28 @@ template <typename T, uint32_t N> __device__ __forceinline__ void residual_all(c
         for (uint32_t k = 0; k < 4u; k++) v[i][k] += more[i][k];
 }
 
+/* the residual of one fragment's rows; 0 where there is none, or no such row or token */
+__device__ __forceinline__ v4f i8_beside(const I8ProductEx &p, uint32_t r, uint32_t t)
+{
+    const uint32_t rows = (uint32_t)p.w.rows;
+    if (!p.residual || r >= rows || t >= p.n_vec) return v4f{ 0.0f, 0.0f, 0.0f, 0.0f };
+    const size_t at = (size_t)t * p.residual_stride + r;
+    if (p.out_type == OXH_F32) return residual4((const float *)p.residual + at, rows - r);
+    if (p.out_type == OXH_F16) return residual4((const _Float16 *)p.residual + at, rows - r);
+    return residual4((const __bf16 *)p.residual + at, rows - r);
+}
+
+__device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[1], const I8RowFactors (&f)[1], float st, v4f beside)
+{
+    float v[1][4];
+    i8_scaled(reinterpret_cast<const v4i(&)[1][1]>(sums), reinterpret_cast<const I8RowFactors(&)[1][1]>(f), 0u, st, p.bias != nullptr, v);
+    i8_activate_all(p.act, v);
+    if (p.residual)
+#pragma unroll
+        for (uint32_t k = 0; k < 4u; k++) v[0][k] += beside[k];
+    i8_put_all(p, r, t, v);
+}
+
 template <uint32_t N>
 __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uint32_t t, const v4i (&sums)[N][1], const I8RowFactors (&f)[N][1], float st)
 {
@@ -416,14 +438,14 @@ __device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, 
     i8_put_all(p, r, t, v);
 }
 
-/* the same of one fragment's rows, as the kernels for few tokens and the joined parts have them */
+/* of one fragment's rows, as the kernels for few tokens and the joined parts have them */
 template <typename P, uint32_t M> __device__ __forceinline__ void i8_row_factors(const P &p, uint32_t r, I8RowFactors (&f)[M])
 {
     i8_row_factors<1u>(p, r, reinterpret_cast<I8RowFactors(&)[1][M]>(f));
 }
-template <typename P, uint32_t M> __device__ __forceinline__ void i8_results(const P &p, uint32_t r, uint32_t t, const v4i (&sums)[M], const I8RowFactors (&f)[M], float st)
+__device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, uint32_t t, const v4i (&sums)[2], const I8RowFactors (&f)[2], float st, I8Nothing)
 {
-    i8_results<1u>(p, r, t, reinterpret_cast<const v4i(&)[1][M]>(sums), reinterpret_cast<const I8RowFactors(&)[1][M]>(f), st);
+    i8_results<1u>(p, r, t, reinterpret_cast<const v4i(&)[1][2]>(sums), reinterpret_cast<const I8RowFactors(&)[1][2]>(f), st);
 }
 
 /* ─── host side ───────────────────────────────────────────────────────── */
