@@ -80,16 +80,16 @@ __device__ __forceinline__ double wave_sum(double v)
     return (row(0) + row(16)) + (row(32) + row(48));
 }
 
-/* A row by a workgroup, eight values to a thread and step: s = x + add in 32 bits, the sum of its squares (each exact) and the norm in 64, so that
- * y, rounded once, does not depend on how a row is dealt to threads, and neither do its codes.  The first HELD steps' values stay in registers; what is longer is
+/* A row by a workgroup, eight values to a thread and step: s = x + add in 32 bits, the sum of its squares (each exact) and the norm in 64; y is
+ * rounded once.  The first HELD steps' values stay in registers; what is longer is
  * read three times.  sum and y go only to places that the same thread has read for the last time: they may be x or add.  Bound by memory: 4096 rows
  * of 4096 bf16 with add and sum in 26 us, 4.5 TB/s read and written (30 with ordinary stores), of 14336 in 92, 4.5 TB/s (114); one row of
  * 4096 in 3.3, a trip to memory and two barriers. */
 template <typename T, int THREADS, int HELD>
 __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
 {
-    constexpr uint32_t STEP = 8u * THREADS;
-    __shared__ double s_sum[THREADS / 64];
+    constexpr uint32_t STEP = 8u * THREADS, WAVES = THREADS / 64;
+    __shared__ double s_sum[(HELD + 1) * WAVES];
     __shared__ uint32_t s_top[THREADS / 64];
     const size_t row = blockIdx.x;
     const T *x = (const T *)p.x + row * p.x_stride, *add = p.add ? (const T *)p.add + row * p.add_stride : nullptr;
@@ -109,8 +109,7 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
             for (int i = 0; i < 8; i++) v[i] += a[i];
         }
     };
-    double squares = 0.0;
-    auto square = [&](const float (&v)[8]) {
+    auto square = [](const float (&v)[8], double &squares) {
 #pragma unroll
         for (int i = 0; i < 8; i++) squares = __builtin_fma((double)v[i], (double)v[i], squares);
     };
@@ -119,24 +118,38 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
     for (int i = 0; i < HELD; i++) load(c0 + STEP * i, s[i]);
 #pragma unroll
     for (int i = 0; i < HELD; i++) weights(c0 + STEP * i, w[i]);
+    /* 512 neighbouring values' squares by a wave, and those sums in the order of the columns: the same for any THREADS and HELD that hold a row */
+    double sums[HELD + 1];
 #pragma unroll
     for (int i = 0; i < HELD; i++) {
-        square(s[i]);
+        sums[i] = 0.0;
+        square(s[i], sums[i]);
         if (p.sum) norm_store8((T *)p.sum + row * p.sum_stride, c0 + STEP * i, cols, s[i]);
     }
+    const bool longer = cols > STEP * HELD;
+    sums[HELD] = 0.0;
     for (uint32_t c = c0 + STEP * HELD; c < cols; c += STEP) {
         float v[8];
         load(c, v);
-        square(v);
+        square(v, sums[HELD]);
     }
-    squares = wave_sum(squares);
-    if (THREADS > 64) {
-        if ((threadIdx.x & 63u) == 0u) s_sum[wave] = squares;
-        __syncthreads();
-        squares = 0.0;
 #pragma unroll
-        for (int i = 0; i < THREADS / 64; i++) squares += s_sum[i];
-    }
+    for (int i = 0; i < HELD; i++) sums[i] = wave_sum(sums[i]);
+    if (longer) sums[HELD] = wave_sum(sums[HELD]);
+    double squares = 0.0;
+    if (THREADS > 64) {
+        if ((threadIdx.x & 63u) == 0u)
+#pragma unroll
+            for (int i = 0; i <= HELD; i++) s_sum[WAVES * i + wave] = sums[i];
+        __syncthreads();
+#pragma unroll
+        for (uint32_t i = 0; i < HELD * WAVES; i++) squares += s_sum[i];
+        if (longer)
+#pragma unroll
+            for (uint32_t i = HELD * WAVES; i < (HELD + 1) * WAVES; i++) squares += s_sum[i];
+    } else
+#pragma unroll
+        for (int i = 0; i <= HELD; i++) squares += sums[i];
     const double r = 1.0 / sqrt(squares / (double)cols + p.eps);
     /* what stands for places behind the last column is 0 or, where r is no number, as little one as the row itself */
     auto normed = [&](float (&v)[8], const float (&g)[8]) {
