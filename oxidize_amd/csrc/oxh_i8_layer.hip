@@ -323,6 +323,28 @@ template <uint32_t N> __device__ __forceinline__ void i8_put_all(const I8Product
     else i8_put_all((__bf16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
 }
 
+/* Partial sums the same way: rows of rows_pad of a token and matrix, as k_i8_join reads them (333 tokens, 4096 x 14336 in four parts: 39.1 us, 36.8). */
+template <typename P, uint32_t N, uint32_t M> __device__ __forceinline__ void i8_part(const P &p, uint32_t split, uint32_t r, uint32_t t, const v4i (&sums)[N][M])
+{
+#pragma unroll
+    for (uint32_t m = 0; m < M; m++) {
+        float v[N][4];
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+#pragma unroll
+            for (uint32_t k = 0; k < 4u; k++) v[i][k] = __int_as_float(sums[i][m][k]);
+        float *out = (float *)p.parts + ((size_t)split * p.n_vec * M + m) * p.rows_pad;
+        i8_put_all(out, (size_t)M * p.rows_pad, r, p.rows_pad, t, p.n_vec, v);
+    }
+}
+
+/* products whose columns are shared out, without what is made of their sums */
+struct I8Sums : I8Product {
+    static constexpr bool TOGETHER = true, SUMS = true;
+    explicit I8Sums(const I8Product &p) : I8Product(p) {}
+};
+template <uint32_t N> __device__ __forceinline__ void i8_row_factors(const I8Sums &, uint32_t, I8RowFactors (&)[N][1]) {}
+
 /* Scales (or biases, if there are any) of matrix m's rows r + 16 i .. + 3, 16 bytes a load where all four exist; behind the last row the last
  * one again. */
 template <uint32_t N, uint32_t M>
@@ -436,6 +458,11 @@ template <uint32_t N> __device__ __forceinline__ void i8_row_factors(const I8Gat
     i8_rows4(p.bias, r, rows, 0u, &I8RowFactors::b, f);
     i8_rows4(p.up_bias, r, rows, 1u, &I8RowFactors::b, f);
 }
+
+struct I8GatedSums : I8GatedProduct {
+    static constexpr bool SUMS = true;
+    explicit I8GatedSums(const I8GatedProduct &p) : I8GatedProduct(p) {}
+};
 
 template <uint32_t N>
 __device__ __forceinline__ void i8_results(const I8GatedProduct &p, uint32_t r, uint32_t t, const v4i (&sums)[N][2], const I8RowFactors (&f)[N][2], float st)
@@ -581,7 +608,8 @@ extern "C" int oxh_i8_matmul_ex(const OxhI8Matrix *w, const int8_t *d_q, size_t 
         (rc = check_optional_workspace(who, d_workspace, workspace_bytes)) || (rc = ready()))
         return rc;
     I8ProductEx p = product_ex(i8_product(w, d_q, q_stride, d_q_scale, n_vec, nullptr, out_type, d_out, out_stride), e);
-    return product_launch(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus()), d_workspace, stream_of(stream), who);
+    return product_launch<I8ProductEx, I8Sums>(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus()), d_workspace,
+                                               stream_of(stream), who);
 }
 
 extern "C" int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec, const OxhI8Epilogue *e,
@@ -597,7 +625,7 @@ extern "C" int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const voi
         (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)))    /* once more: the way depends on the device */
         return rc;
     I8ProductEx p = product_ex(i8_product(w, nullptr, 0, nullptr, n_vec, nullptr, out_type, d_out, out_stride), e);
-    return linear_launch(p, x_type, d_x, x_stride, d_workspace, workspace_bytes, stream_of(stream), who);
+    return linear_launch<I8ProductEx, I8Sums>(p, x_type, d_x, x_stride, d_workspace, workspace_bytes, stream_of(stream), who);
 }
 
 static OxhI8Matrix gate_of(const OxhI8Gated *g) { return { g->d_w_gate, g->stride, g->d_s_gate, g->rows, g->cols }; }
@@ -622,7 +650,7 @@ static int gated_launch(const OxhI8Gated *g, const int8_t *q, size_t q_stride, c
 {
     const OxhI8Matrix gate = gate_of(g);
     I8GatedProduct p = { i8_product(&gate, q, q_stride, q_scale, n, g->d_b_gate, out_type, out, out_stride), g->d_w_up, g->d_s_up, g->d_b_up, g->act };
-    return product_launch(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), 2u), ws, st, who);
+    return product_launch<I8GatedProduct, I8GatedSums>(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), 2u), ws, st, who);
 }
 
 static bool workable(size_t rows, size_t cols, size_t n)
@@ -694,13 +722,16 @@ extern "C" int oxh_i8_ffn(const OxhI8Gated *g, const OxhI8Matrix *down, const in
     uint8_t *rest = (uint8_t *)d_workspace + h_bytes;
     if ((rc = gated_launch(g, d_q, q_stride, d_q_scale, n_vec, OXH_F32, d_workspace, h_stride, rest, workspace_bytes - h_bytes, st, who))) return rc;
     I8ProductEx p = product_ex(i8_product(down, nullptr, 0, nullptr, n_vec, nullptr, out_type, d_out, out_stride), e);
-    return linear_launch(p, OXH_F32, d_workspace, h_stride, rest, workspace_bytes - h_bytes, st, who);
+    return linear_launch<I8ProductEx, I8Sums>(p, OXH_F32, d_workspace, h_stride, rest, workspace_bytes - h_bytes, st, who);
 }
 
 extern "C" int oxh_internal_i8_layer_init(void)
 {
-    const hipError_t e = product_init<I8ProductEx>();
-    return (int)(e == hipSuccess ? product_init<I8GatedProduct>() : e);
+    hipError_t e;
+    if ((e = product_init<I8ProductEx>()) != hipSuccess) return (int)e;
+    if ((e = product_init<I8Sums>()) != hipSuccess) return (int)e;
+    if ((e = product_init<I8GatedProduct>()) != hipSuccess) return (int)e;
+    return (int)product_init<I8GatedSums>();
 }
 
 /* ─── which kernels run, for tests ────────────────────────────────────── */
