@@ -267,7 +267,8 @@ template <uint32_t N, uint32_t M> __device__ __forceinline__ void i8_scaled(cons
  * 14336 x 4096, bf16, bias and GELU: 259 us without all that, 235 with the first change, 234 with both, 217 with the stores past the L2s; gate and up 413,
  * 387, 385 and 366.)  Every lane takes part, whether its token is there or not. */
 template <typename T, uint32_t N>
-__device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4])
+__device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4],
+                                           bool past = true)
 {
     constexpr bool HALF = sizeof(T) == 2;
     if constexpr (N >= (HALF ? 2u : 1u)) {
@@ -288,8 +289,10 @@ __device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, ui
         auto store = [&](uint32_t token, uint32_t at, const uint4 &what) {
             if (token >= n_vec) return;
             T *to = out + (size_t)token * stride + at;
-            if (at + HAS <= rows) store_past<Stored16>(to, what);
-            else {
+            if (at + HAS <= rows) {
+                if (past) store_past<Stored16>(to, what);
+                else *reinterpret_cast<Run<T, HAS> *>(to) = __builtin_bit_cast(Run<T, HAS>, what);
+            } else {
                 const Run<T, HAS> all = __builtin_bit_cast(Run<T, HAS>, what);
 #pragma unroll
                 for (uint32_t k = 0; k < HAS - 1u; k++)
@@ -323,7 +326,9 @@ template <uint32_t N> __device__ __forceinline__ void i8_put_all(const I8Product
     else i8_put_all((__bf16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
 }
 
-/* Partial sums the same way: rows of rows_pad of a token and matrix, as k_i8_join reads them (333 tokens, 4096 x 14336 in four parts: 39.1 us, 36.8). */
+/* Partial sums the same way: rows of rows_pad of a token and matrix, as k_i8_join reads them.  Up to 8 MB of them stay in the L2s for it (us kept and past
+ * them: 2000 x 9000, gate and up under 60, 3.8 MB: 13.7 and 14.3; 1168 x 14272 under 310, 7.2: 19.8, 20.4; 2000 x 14000 under 260, 10.4: 24.7, 24.2; 4096 x
+ * 14336 under 333, 21.8: 39.4, 36.1, and 39.1 kept in half lines; under 1000, 32.8: 81.8, 78.8). */
 template <typename P, uint32_t N, uint32_t M> __device__ __forceinline__ void i8_part(const P &p, uint32_t split, uint32_t r, uint32_t t, const v4i (&sums)[N][M])
 {
 #pragma unroll
@@ -334,7 +339,7 @@ template <typename P, uint32_t N, uint32_t M> __device__ __forceinline__ void i8
 #pragma unroll
             for (uint32_t k = 0; k < 4u; k++) v[i][k] = __int_as_float(sums[i][m][k]);
         float *out = (float *)p.parts + ((size_t)split * p.n_vec * M + m) * p.rows_pad;
-        i8_put_all(out, (size_t)M * p.rows_pad, r, p.rows_pad, t, p.n_vec, v);
+        i8_put_all(out, (size_t)M * p.rows_pad, r, p.rows_pad, t, p.n_vec, v, (size_t)p.splits * p.n_vec * M * p.rows_pad > ((size_t)2 << 20));
     }
 }
 
