@@ -265,65 +265,89 @@ template <uint32_t N, uint32_t M> __device__ __forceinline__ void i8_scaled(cons
  * 64 of a token; then of two such the lanes of the upper eight tokens give the first for the lower eight's second, and a store writes 128
  * bytes of each of eight tokens.  The L2s are told to keep none of it: a launch's results would push the operands of its other tiles out.  (4096 tokens over
  * 14336 x 4096, bf16, bias and GELU: 259 us without all that, 235 with the first change, 234 with both, 217 with the stores past the L2s; gate and up 413,
- * 387, 385 and 366.)  Every lane takes part, whether its token is there or not. */
-template <typename T, uint32_t N>
-__device__ __forceinline__ void i8_put_all(T *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4],
-                                           bool past = true)
+ * 387, 385 and 366.)  Every lane takes part, whether its token is there or not.
+ *
+ * i8_put_pieces: pieces of 16 bytes that a lane has of its token: `PIECES` of them, SPAN rows apart from `row` on, HAS rows of W's size each. */
+template <typename W, uint32_t PIECES>
+__device__ __forceinline__ void i8_put_pieces(W *out, size_t stride, uint32_t row, uint32_t rows, uint32_t t, uint32_t n_vec, const uint4 (&piece)[PIECES], bool past)
 {
-    constexpr bool HALF = sizeof(T) == 2;
-    if constexpr (N >= (HALF ? 2u : 1u)) {
-        constexpr uint32_t PIECES = HALF ? N / 2u : N, SPAN = HALF ? 32u : 16u, HAS = 16u / sizeof(T);      /* a lane's pieces of 16 bytes, rows from one to the next, rows of one */
-        uint4 piece[PIECES];
-#pragma unroll
-        for (uint32_t i = 0; i < PIECES; i++) {
-            typedef T T4 __attribute__((ext_vector_type(4)));
-            if constexpr (HALF) {
-                const uint2 a = __builtin_bit_cast(uint2, (T4){ from_f32<T>(v[2u * i][0]), from_f32<T>(v[2u * i][1]), from_f32<T>(v[2u * i][2]), from_f32<T>(v[2u * i][3]) });
-                const uint2 b = __builtin_bit_cast(uint2, (T4){ from_f32<T>(v[2u * i + 1u][0]), from_f32<T>(v[2u * i + 1u][1]), from_f32<T>(v[2u * i + 1u][2]), from_f32<T>(v[2u * i + 1u][3]) });
-                const auto lo = __builtin_amdgcn_permlane16_swap(a.x, b.x, false, false), hi = __builtin_amdgcn_permlane16_swap(a.y, b.y, false, false);
-                piece[i] = make_uint4(lo[0], hi[0], lo[1], hi[1]);
-            } else piece[i] = __builtin_bit_cast(uint4, (T4){ v[i][0], v[i][1], v[i][2], v[i][3] });
-        }
-        const uint32_t kq = (threadIdx.x >> 4) & 3u;
-        uint32_t row = HALF ? r - 4u * kq + 16u * (kq & 1u) + 8u * (kq >> 1) : r;
-        auto store = [&](uint32_t token, uint32_t at, const uint4 &what) {
-            if (token >= n_vec) return;
-            T *to = out + (size_t)token * stride + at;
-            if (at + HAS <= rows) {
-                if (past) store_past<Stored16>(to, what);
-                else *reinterpret_cast<Run<T, HAS> *>(to) = __builtin_bit_cast(Run<T, HAS>, what);
-            } else {
-                const Run<T, HAS> all = __builtin_bit_cast(Run<T, HAS>, what);
-#pragma unroll
-                for (uint32_t k = 0; k < HAS - 1u; k++)
-                    if (at + k < rows) to[k] = all.v[k];
-            }
-        };
-        if constexpr (PIECES % 2u == 0u) {
-            const uint32_t upper = (threadIdx.x >> 3) & 1u;
-            row += SPAN * upper;
-#pragma unroll
-            for (uint32_t i = 0; i < PIECES; i += 2u) {
-                const uint4 x = piece[i], y = piece[i + 1u];
-                auto low = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xF, 0xC, false); };     /* a, in the upper eight lanes the lower's b */
-                auto high = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xF, 0x3, false); };    /* b, in the lower eight the upper's a */
-                store(t - 8u * upper, row + SPAN * i, make_uint4(low(x.x, y.x), low(x.y, y.y), low(x.z, y.z), low(x.w, y.w)));
-                store(t + 8u - 8u * upper, row + SPAN * i, make_uint4(high(x.x, y.x), high(x.y, y.y), high(x.z, y.z), high(x.w, y.w)));
-            }
+    constexpr uint32_t HAS = 16u / sizeof(W), SPAN = 4u * HAS;
+    auto store = [&](uint32_t token, uint32_t at, const uint4 &what) {
+        if (token >= n_vec) return;
+        W *to = out + (size_t)token * stride + at;
+        const Run<W, HAS> all = __builtin_bit_cast(Run<W, HAS>, what);
+        if (at + HAS <= rows) {
+            if (past) store_past<Stored16>(to, what);
+            else *reinterpret_cast<Run<W, HAS> *>(to) = all;
         } else
 #pragma unroll
-            for (uint32_t i = 0; i < PIECES; i++) store(t, row + SPAN * i, piece[i]);
-    } else if (t < n_vec)
+            for (uint32_t k = 0; k < HAS - 1u; k++)
+                if (at + k < rows) to[k] = all.v[k];
+    };
+    if constexpr (PIECES % 2u == 0u) {
+        const uint32_t upper = (threadIdx.x >> 3) & 1u;
+        row += SPAN * upper;
 #pragma unroll
-        for (uint32_t i = 0; i < N; i++)
-            if (r + 16u * i < rows) i8_store4(out + (size_t)t * stride + r + 16u * i, v[i], rows - r - 16u * i);
+        for (uint32_t i = 0; i < PIECES; i += 2u) {
+            const uint4 x = piece[i], y = piece[i + 1u];
+            auto low = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)a, (int)b, 0x128, 0xF, 0xC, false); };     /* a, in the upper eight lanes the lower's b */
+            auto high = [](uint32_t a, uint32_t b) { return (uint32_t)__builtin_amdgcn_update_dpp((int)b, (int)a, 0x128, 0xF, 0x3, false); };    /* b, in the lower eight the upper's a */
+            store(t - 8u * upper, row + SPAN * i, make_uint4(low(x.x, y.x), low(x.y, y.y), low(x.z, y.z), low(x.w, y.w)));
+            store(t + 8u - 8u * upper, row + SPAN * i, make_uint4(high(x.x, y.x), high(x.y, y.y), high(x.z, y.z), high(x.w, y.w)));
+        }
+    } else
+#pragma unroll
+        for (uint32_t i = 0; i < PIECES; i++) store(t, row + SPAN * i, piece[i]);
 }
+
+template <uint32_t N>
+__device__ __forceinline__ void i8_put_f32(float *out, size_t stride, uint32_t r, uint32_t rows, uint32_t t, uint32_t n_vec, const float (&v)[N][4], bool past)
+{
+    uint4 piece[N];
+#pragma unroll
+    for (uint32_t i = 0; i < N; i++) piece[i] = __builtin_bit_cast(uint4, (v4f){ v[i][0], v[i][1], v[i][2], v[i][3] });
+    i8_put_pieces((uint32_t *)out, stride, r, rows, t, n_vec, piece, past);
+}
+
 template <uint32_t N> __device__ __forceinline__ void i8_put_all(const I8Product &p, uint32_t r, uint32_t t, const float (&v)[N][4])
 {
     const uint32_t rows = (uint32_t)p.w.rows;
-    if (p.out_type == OXH_F32) i8_put_all((float *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
-    else if (p.out_type == OXH_F16) i8_put_all((_Float16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
-    else i8_put_all((__bf16 *)p.out, p.out_stride, r, rows, t, p.n_vec, v);
+    if (p.out_type == OXH_F32) {
+        i8_put_f32((float *)p.out, p.out_stride, r, rows, t, p.n_vec, v, true);
+        return;
+    }
+    /* the two 16-bit types differ in their rounding only */
+    uint2 four[N];
+    auto round = [&](auto zero) {
+        typedef decltype(zero) T;
+        typedef T T4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+        for (uint32_t i = 0; i < N; i++)
+            four[i] = __builtin_bit_cast(uint2, (T4){ from_f32<T>(v[i][0]), from_f32<T>(v[i][1]), from_f32<T>(v[i][2]), from_f32<T>(v[i][3]) });
+    };
+    if (p.out_type == OXH_F16) round((_Float16)0);
+    else round((__bf16)0.0f);
+    uint16_t *out = (uint16_t *)p.out;
+    if constexpr (N % 2u == 0u) {
+        uint4 piece[N / 2u];
+#pragma unroll
+        for (uint32_t i = 0; i < N; i += 2u) {
+            const auto lo = __builtin_amdgcn_permlane16_swap(four[i].x, four[i + 1u].x, false, false), hi = __builtin_amdgcn_permlane16_swap(four[i].y, four[i + 1u].y, false, false);
+            piece[i / 2u] = make_uint4(lo[0], hi[0], lo[1], hi[1]);
+        }
+        const uint32_t kq = (threadIdx.x >> 4) & 3u;
+        i8_put_pieces(out, p.out_stride, r - 4u * kq + 16u * (kq & 1u) + 8u * (kq >> 1), rows, t, p.n_vec, piece, true);
+    } else {
+        static_assert(N == 1u, "fragments in pairs, or one");
+        if (t >= p.n_vec || r >= rows) return;
+        uint16_t *to = out + (size_t)t * p.out_stride + r;
+        const Run<uint16_t, 4> all = __builtin_bit_cast(Run<uint16_t, 4>, four[0]);
+        if (r + 4u <= rows) *reinterpret_cast<Run<uint16_t, 4> *>(to) = all;
+        else
+#pragma unroll
+            for (uint32_t k = 0; k < 3u; k++)
+                if (r + k < rows) to[k] = all.v[k];
+    }
 }
 
 /* Partial sums the same way: rows of rows_pad of a token and matrix, as k_i8_join reads them.  Up to 8 MB of them stay in the L2s for it (us kept and past
@@ -339,7 +363,7 @@ template <typename P, uint32_t N, uint32_t M> __device__ __forceinline__ void i8
 #pragma unroll
             for (uint32_t k = 0; k < 4u; k++) v[i][k] = __int_as_float(sums[i][m][k]);
         float *out = (float *)p.parts + ((size_t)split * p.n_vec * M + m) * p.rows_pad;
-        i8_put_all(out, (size_t)M * p.rows_pad, r, p.rows_pad, t, p.n_vec, v, (size_t)p.splits * p.n_vec * M * p.rows_pad > ((size_t)2 << 20));
+        i8_put_f32(out, (size_t)M * p.rows_pad, r, p.rows_pad, t, p.n_vec, v, (size_t)p.splits * p.n_vec * M * p.rows_pad > ((size_t)2 << 20));
     }
 }
 
