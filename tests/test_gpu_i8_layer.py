@@ -555,3 +555,122 @@ def test_matrices_of_more_than_4_gib(oxh):
         got = out.download(np.float32, rows, 4 * t * rows)
         assert lref.same_or_near(got[rows - last:], F32, want[t, 1:], far[t, 1:])
         assert (got[:rows - last] == got[0]).all() and lref.same_or_near(got[:1], F32, want[t, :1], far[t, :1])
+
+
+# ─── calls that the documentation allows and the rest does not make ─────
+
+
+@KINDS
+@pytest.mark.parametrize("n,rows,cols", [(1, 100, 600), (7, 97, 333), (40, 131, 500), (130, 259, 700), (16, 130, 9000)])
+def test_pointers_aligned_to_their_elements_only(oxh, kind, n, rows, cols):
+    """Everything but codes lies one element behind a 16-byte border."""
+    e_ = ref.np_type(kind)().itemsize
+    c = Case(n, rows, cols, 3, int8.SILU, kind=kind)
+    want = c.matmul_ex()
+
+    def shifted(a, by):
+        d = mv.DeviceBuffer(a.nbytes + by)
+        d.upload(np.ascontiguousarray(a), by)
+        return d
+
+    ws, bias, qs, res = shifted(c.ws, 4), shifted(c.bias, 4), shifted(c.qs, 4), shifted(ref.padded(c.res, c.res_stride, 1), e_)
+    out = mv.DeviceBuffer(n * (rows + 1) * e_ + e_)
+    m = int8.Matrix(c.d["w"].ptr, ws.ptr + 4, rows, cols, c.m.desc.stride)
+    e = int8.Epilogue(bias.ptr + 4, c.act, res.ptr + e_, c.res_stride)
+    need = m.matmul_workspace(n)
+    buf = mv.DeviceBuffer(max(16, need))
+    m.matmul_ex(c.d["q"].ptr, c.q_stride, qs.ptr + 4, n, e, kind, out.ptr + e_, rows + 1, buf.ptr, need)
+    mv.sync()
+    got = out.download(ref.np_type(kind), n * (rows + 1), e_).reshape(n, rows + 1)[:, :rows]
+    assert same_bits(got, want)
+    x, add = (base.floats(n, cols, kind, i) for i in (1, 2))
+    w = np.random.default_rng(3).normal(1, 0.3, cols).astype(np.float32)
+    d_x, d_a, d_w = shifted(x, e_), shifted(add, e_), shifted(w, 4)
+    total, y = mv.DeviceBuffer(n * cols * e_ + e_), mv.DeviceBuffer(n * cols * e_ + e_)
+    q, s = mv.DeviceBuffer(n * up_to_16(cols)), mv.DeviceBuffer(4 * n + 4)
+    int8.Norm(d_w.ptr + 4, 1e-5, d_a.ptr + e_, cols, total.ptr + e_, cols, y.ptr + e_, cols).quantize(kind, d_x.ptr + e_, cols, n, cols, q.ptr, up_to_16(cols), s.ptr + 4)
+    mv.sync()
+    dt = ref.np_type(kind)
+    check_norm((q.download(np.int8, n * up_to_16(cols)).reshape(n, -1)[:, :cols], s.download(np.float32, n, 4), total.download(dt, n * cols, e_).reshape(n, cols),
+                y.download(dt, n * cols, e_).reshape(n, cols)), x, kind, w, 1e-5, add)
+
+
+@pytest.mark.parametrize("cols", [300, 4096, 20000])
+def test_norm_over_both_inputs_at_once(oxh, cols):
+    n, kind = 5, BF16
+    x, add = (base.floats(n, cols, kind, i) for i in (1, 2))
+    want = run_norm(x, kind, None, 1e-5, add)
+    d_x, d_a, q, s = mv.DeviceBuffer.from_host(x), mv.DeviceBuffer.from_host(add), mv.DeviceBuffer(n * up_to_16(cols)), mv.DeviceBuffer(4 * n)
+    int8.Norm(None, 1e-5, d_a.ptr, cols, d_a.ptr, cols, d_x.ptr, cols).quantize(kind, d_x.ptr, cols, n, cols, q.ptr, up_to_16(cols), s.ptr)
+    mv.sync()
+    assert same_bits(d_a.download(np.uint16, n * cols).reshape(n, cols), want[2]) and same_bits(d_x.download(np.uint16, n * cols).reshape(n, cols), want[3])
+    assert np.array_equal(q.download(np.int8, n * up_to_16(cols)).reshape(n, -1)[:, :cols], want[0])
+
+
+def test_x_added_to_itself(oxh):
+    x = base.floats(3, 700, F32, 4)
+    d, q, s = mv.DeviceBuffer.from_host(x), mv.DeviceBuffer(3 * 704), mv.DeviceBuffer(12)
+    int8.Norm(None, 1e-5, d.ptr, 700, d.ptr, 700).quantize(F32, d.ptr, 700, 3, 700, q.ptr, 704, s.ptr)
+    mv.sync()
+    assert same_bits(d.download(np.float32, 3 * 700).reshape(3, 700), x + x)
+
+
+@pytest.mark.parametrize("rows,cols", [(20, 40), (70, 5000)])
+def test_more_tokens_than_a_grid_has_rows(oxh, rows, cols):
+    """70000 tokens: beyond what the join of parts could take, so the columns stay together."""
+    n = 70000
+    c = Gate(n, rows, cols, 5, kind=BF16)
+    got = c.run()
+    some = np.r_[0:5, 65530:65540, n - 5:n]
+    want, far = lref.gated(c.q[some], c.qs[some], c.mats[0], c.mats[1], c.act)
+    assert lref.same_or_near(got[some], BF16, want, far)
+    e = Case(n, rows, cols, 6, int8.GELU, kind=F16)
+    got = e.matmul_ex()
+    want, far = lref.epilogue(e.q[some], e.qs[some], e.w, e.ws, e.bias, e.act, ref.decode(e.res[some], F16))
+    assert lref.same_or_near(got[some], F16, want, far)
+
+
+def test_two_threads_at_once(oxh):
+    """Calls from two host threads, each on a stream and buffers of its own."""
+    import threading
+    streams = []
+    for _ in range(2):
+        s = ctypes.c_void_p()
+        _lib.check(oxh.oxh_stream_create(ctypes.byref(s)))
+        streams.append(s)
+    steps = [Step(40, 10 * (i + 1), s) for i, s in enumerate(streams)]
+    want = []
+    for st in steps:
+        st.run()
+        want.append(st.results())
+    got, wrong = [None, None], []
+
+    def work(i):
+        try:
+            for _ in range(20):
+                steps[i].run()
+            got[i] = steps[i].results()
+        except Exception as e:                          # shown by the assertion below
+            wrong.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not wrong
+    for g, w in zip(got, want):
+        assert all(np.array_equal(a, b) for a, b in zip(g, w))
+    for s in streams:
+        oxh.oxh_stream_destroy(s)
+
+
+def test_ffn_in_place_at_every_few_tokens(oxh):
+    for n in (1, 2, 5, 17, 33, 65, 200):
+        c = Block(n, 520, 700, n, kind=F16)
+        want = c.run()
+        c.e = int8.Epilogue(c.d["b"].ptr, int8.NONE, c.d["res"].ptr, c.hidden)
+        g = c.gate
+        c.block.forward(g.d["q"].ptr, g.q_stride, g.d["qs"].ptr, n, c.e, F16, c.d["res"].ptr, c.hidden)
+        mv.sync()
+        assert same_bits(c.d["res"].download(np.float16, n * c.hidden).reshape(n, -1), want)
