@@ -114,9 +114,10 @@ typedef struct OxhLab {
      * and up, then for down, the stages that a wave of the few pairs' kernels
      * holds, or 0 for tiles. */
     int (*moe_i8_kernels)(const OxhMoeI8 *m, size_t n_tok, int ids, size_t n_cu, uint32_t out[4]);
-    /* i8_kernel for oxh_i8_gated: kernels 0 to 2; a tile's rows are those of
-     * both matrices, and a team's waves are half the gate's and half up's. */
-    int (*i8_gated_kernel)(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, uint32_t out[4]);
+    /* i8_kernel for oxh_i8_matmul_ex, or (gated) for oxh_i8_gated: kernels 0 to
+     * 2, and two tiles more, 64 x 32 with rings of nine and five.  Gated: a tile's
+     * rows are those of both matrices, a team's waves half the gate's, half up's. */
+    int (*i8_layer_kernel)(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int gated, uint32_t out[4]);
 } OxhLab;
 
 const OxhLab *oxh_lab(void);

@@ -98,7 +98,7 @@ class OxhLab(ctypes.Structure):
                 ("plan_draft", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhPlanOp), Z, U32, ctypes.POINTER(ctypes.c_uint64))),
                 ("i8_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, I, ctypes.POINTER(U32 * 4))),
                 ("moe_i8_kernels", ctypes.CFUNCTYPE(I, ctypes.POINTER(OxhMoeI8), Z, I, Z, ctypes.POINTER(U32 * 4))),
-                ("i8_gated_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, ctypes.POINTER(U32 * 4)))]
+                ("i8_layer_kernel", ctypes.CFUNCTYPE(I, Z, Z, Z, Z, Z, I, ctypes.POINTER(U32 * 4)))]
 
 
 # name -> (restype, argtypes); every symbol include/oxhip.h and include/oxhip_lab.h declare

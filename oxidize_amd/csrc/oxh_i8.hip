@@ -461,8 +461,7 @@ extern "C" size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
     if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
         return 0;
-    if (few_team(w->rows, w->cols, n_vec, i8_cus())) return 0;
-    return parts_bytes(w->rows, n_vec, i8_way(w->rows, w->cols, n_vec, SIZE_MAX, i8_cus()).splits);
+    return product_parts(w->rows, w->cols, n_vec);
 }
 
 extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
@@ -481,7 +480,7 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
     if (d_workspace && workspace_bytes && ((uintptr_t)d_workspace & 15u)) return I8_ARG("%s: workspace must be 16-byte aligned", who);
     if ((rc = ready())) return rc;
     I8Product p = i8_product(w, d_q, q_stride, d_q_scale, n_vec, d_bias, out_type, d_out, out_stride);
-    return product_launch(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus()), d_workspace, stream_of(stream), who);
+    return product_launch(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus(), I8_PLAIN), d_workspace, stream_of(stream), who);
 }
 
 extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
@@ -752,7 +751,7 @@ extern "C" int oxh_debug_i8_kernel(size_t rows, size_t cols, size_t n_vec, size_
         out[3] = (uint32_t)n_vec;
         return OXH_OK;
     }
-    i8_describe(i8_choice(rows, cols, n_vec, ws_bytes, n_cu), rows, cols, n_vec, n_cu, 1u, out);
+    i8_describe(i8_choice(rows, cols, n_vec, ws_bytes, n_cu, I8_PLAIN), rows, cols, n_vec, n_cu, I8_PLAIN, out);
     return OXH_OK;
 }
 

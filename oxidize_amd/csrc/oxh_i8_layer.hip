@@ -396,6 +396,7 @@ __device__ __forceinline__ void i8_rows4(const float *from, uint32_t r, uint32_t
 }
 
 struct I8ProductEx : I8Product {
+    static constexpr uint32_t RULE = I8_EX;
     static constexpr bool TOGETHER = true;
     const void *residual;
     size_t residual_stride;
@@ -470,7 +471,7 @@ __device__ __forceinline__ void i8_results(const I8ProductEx &p, uint32_t r, uin
 
 /* w and bias are the gate's */
 struct I8GatedProduct : I8Product {
-    static constexpr uint32_t MATRICES = 2;
+    static constexpr uint32_t MATRICES = 2, RULE = I8_GATED;
     static constexpr bool TOGETHER = true;
     const int8_t *up;
     const float *up_scale, *up_bias;
@@ -637,7 +638,7 @@ extern "C" int oxh_i8_matmul_ex(const OxhI8Matrix *w, const int8_t *d_q, size_t 
         (rc = check_optional_workspace(who, d_workspace, workspace_bytes)) || (rc = ready()))
         return rc;
     I8ProductEx p = product_ex(i8_product(w, d_q, q_stride, d_q_scale, n_vec, nullptr, out_type, d_out, out_stride), e);
-    return product_launch<I8ProductEx, I8Sums>(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus()), d_workspace,
+    return product_launch<I8ProductEx, I8Sums>(p, i8_choice(w->rows, w->cols, n_vec, d_workspace ? workspace_bytes : 0, i8_cus(), I8_EX), d_workspace,
                                                stream_of(stream), who);
 }
 
@@ -679,7 +680,7 @@ static int gated_launch(const OxhI8Gated *g, const int8_t *q, size_t q_stride, c
 {
     const OxhI8Matrix gate = gate_of(g);
     I8GatedProduct p = { i8_product(&gate, q, q_stride, q_scale, n, g->d_b_gate, out_type, out, out_stride), g->d_w_up, g->d_s_up, g->d_b_up, g->act };
-    return product_launch<I8GatedProduct, I8GatedSums>(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), 2u), ws, st, who);
+    return product_launch<I8GatedProduct, I8GatedSums>(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), I8_GATED), ws, st, who);
 }
 
 static bool workable(size_t rows, size_t cols, size_t n)
@@ -689,7 +690,7 @@ static bool workable(size_t rows, size_t cols, size_t n)
 
 static size_t gated_parts(size_t rows, size_t cols, size_t n)
 {
-    const I8Choice c = i8_choice(rows, cols, n, SIZE_MAX, i8_cus(), 2u);
+    const I8Choice c = i8_choice(rows, cols, n, SIZE_MAX, i8_cus(), I8_GATED);
     return c.team ? 0 : parts_bytes(i8_rows_in_all(rows, 2u), n, c.way.splits);
 }
 
@@ -765,12 +766,13 @@ extern "C" int oxh_internal_i8_layer_init(void)
 
 /* ─── which kernels run, for tests ────────────────────────────────────── */
 
-extern "C" int oxh_debug_i8_gated_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, uint32_t out[4])
+extern "C" int oxh_debug_i8_layer_kernel(size_t rows, size_t cols, size_t n_vec, size_t n_cu, size_t ws_bytes, int gated, uint32_t out[4])
 {
-    static const char who[] = "oxh_debug_i8_gated_kernel";
+    static const char who[] = "oxh_debug_i8_layer_kernel";
     if (!out || !rows || !n_vec || !n_cu) return I8_ARG("%s: NULL or empty", who);
     const int rc = check_cols(who, cols);
     if (rc) return rc;
-    i8_describe(i8_choice(rows, cols, n_vec, ws_bytes, n_cu, 2u), rows, cols, n_vec, n_cu, 2u, out);
+    const uint32_t rule = gated ? I8_GATED : I8_EX;
+    i8_describe(i8_choice(rows, cols, n_vec, ws_bytes, n_cu, rule), rows, cols, n_vec, n_cu, rule, out);
     return OXH_OK;
 }

@@ -3447,7 +3447,7 @@ extern "C" const OxhLab *oxh_lab(void)
                                 oxh_debug_read_probe, oxh_debug_mfma_probe, oxh_debug_subblock_sums,
                                 oxh_debug_mmq_kernel, oxh_debug_experts_tile, oxh_debug_host_ring_chunks, oxh_debug_experts_batch,
                                 oxh_debug_plan_by_value, oxh_debug_mmq32_fetched, oxh_debug_plan_draft, oxh_debug_i8_kernel,
-                                oxh_debug_moe_i8_kernels, oxh_debug_i8_gated_kernel };
+                                oxh_debug_moe_i8_kernels, oxh_debug_i8_layer_kernel };
     return &lab;
 }
 

@@ -29,7 +29,7 @@ def quantize(x_type, d_x, x_stride, n_vec, cols, d_q, q_stride, d_scale, d_up=No
     check(lib().oxh_i8_quantize(x_type, d_x, x_stride, n_vec, cols, d_up, d_q, q_stride, d_scale, stream))
 
 
-TILE_256x256, TILE_128x256, TILE_128x192, TILE_128x128, TILE_64x64_RING, TILE_64x64 = range(6)
+TILE_256x256, TILE_128x256, TILE_128x192, TILE_128x128, TILE_64x64_RING, TILE_64x64, TILE_64x32_RING, TILE_64x32 = range(8)
 TILES, FEW, FEW_WIDE, FEW_FLOAT = range(4)
 
 
@@ -48,10 +48,10 @@ def moe_kernels(desc, n_tok, ids=True, n_cu=256):
     return tuple(out)
 
 
-def gated_kernel(rows, cols, n_vec, ws_bytes=1 << 40, n_cu=256):
-    """:func:`kernel` for :class:`Gated`."""
+def layer_kernel(rows, cols, n_vec, gated, ws_bytes=1 << 40, n_cu=256):
+    """:func:`kernel` for a product with an epilogue, or for :class:`Gated`."""
     out = (ctypes.c_uint32 * 4)()
-    check(_lib.lab().i8_gated_kernel(rows, cols, n_vec, n_cu, ws_bytes, ctypes.byref(out)))
+    check(_lib.lab().i8_layer_kernel(rows, cols, n_vec, n_cu, ws_bytes, int(gated), ctypes.byref(out)))
     return tuple(out)
 
 

@@ -103,7 +103,33 @@ def ffn(q, qs, gate, up, act, down, residual=None):
     return y, off
 
 
-# Sizes at which each kernel of the gated product runs on 256 compute units, as in i8_shapes: [(tokens, rows, columns)]
+# Sizes at which each kernel of a product with an epilogue, and of the gated product, runs on 256 compute units, as in i8_shapes:
+# [(tokens, rows, columns)]
+EX = {
+    (1, 2, 1): [(1, 16, 64), (16, 200, 4096), (7, 4096, 1000), (1, 4107, 3588)],
+    (1, 4, 1): [(1, 16, 4102), (8, 40, 8192), (9, 16, 4230), (16, 2400, 8064), (3, 5888, 6528)],
+    (1, 8, 1): [(1, 3057, 8209), (2, 4096, 14336), (8, 4096, 14336), (8, 3100, 16384)],
+    (2, 2, 2): [(17, 16, 64), (32, 50, 4090)],
+    (2, 2, 3): [(34, 16, 65), (48, 70, 4096)],
+    (2, 2, 4): [(49, 17, 66), (64, 4096, 4000)],
+    (0, 0, False, False): [(514, 19821, 132)],
+    (0, 0, False, True): [(776, 23320, 386)],
+    (0, 0, True, False): [(130, 11042, 8238)],
+    (0, 1, False, False): [(825, 8133, 274)],
+    (0, 1, True, False): [(3990, 130, 12785)],
+    (0, 2, False, False): [(603, 8092, 132)],
+    (0, 2, True, False): [(131, 5498, 5051), (333, 4096, 14336)],
+    (0, 3, False, False): [(66, 16916, 65)],
+    (0, 3, True, False): [(66, 2700, 7728)],
+    (0, 4, False, False): [(67, 16, 64), (70, 300, 1030)],
+    (0, 4, True, False): [(48, 4096, 14336), (37, 65, 4683)],
+    (0, 5, False, False): [(33, 40000, 100)],
+    (0, 5, True, False): [(3777, 1, 4214)],
+    (0, 6, False, False): [(1, 4110, 1), (5, 14336, 4096), (16, 5001, 700), (32, 6000, 900)],
+    (0, 6, True, False): [(1, 1, 8276), (21, 40, 6617), (24, 4096, 14336)],
+    (0, 7, False, False): [(1, 32863, 64), (29, 36260, 70)],
+    (0, 7, True, False): [(4, 6516, 7118), (1, 6648, 4249)],
+}
 GATED = {
     (1, 2, 1): [(1, 1, 1), (8, 200, 2048), (7, 2048, 1000)],
     (1, 4, 1): [(1, 16, 2103), (8, 40, 4096), (5, 4096, 4096)],
@@ -117,8 +143,12 @@ GATED = {
     (0, 2, True, False): [(158, 2901, 8183)],
     (0, 3, False, False): [(67, 8328, 65), (333, 4864, 896)],
     (0, 3, True, False): [(252, 2299, 9671)],
-    (0, 4, False, False): [(67, 16, 64), (70, 150, 1030), (16, 14336, 4096), (5, 14336, 4096), (17, 16, 64), (34, 16, 65), (64, 2048, 2000), (260, 1891, 6834)],
-    (0, 4, True, False): [(9, 16, 8276), (1, 1, 8543), (48, 2048, 8000), (66, 1450, 7728)],
-    (0, 5, False, False): [(1, 17582, 64), (33, 20000, 100)],
-    (0, 5, True, False): [(1, 4455, 7576)],
+    (0, 4, False, False): [(67, 16, 64), (70, 150, 1030), (34, 16, 65), (64, 2048, 2000), (260, 1891, 6834)],
+    (0, 4, True, False): [(48, 2048, 8000), (66, 1450, 7728)],
+    (0, 5, False, False): [(33, 20000, 100)],
+    (0, 5, True, False): [(44, 4218, 15900)],
+    (0, 6, False, False): [(17, 16, 64), (9, 33, 70), (32, 300, 500), (16, 14336, 4096), (5, 14336, 4096)],
+    (0, 6, True, False): [(9, 16, 8276), (1, 1, 8543), (32, 200, 9000)],
+    (0, 7, False, False): [(1, 17582, 64), (8, 24486, 40)],
+    (0, 7, True, False): [(1, 4455, 7576)],
 }

@@ -206,7 +206,7 @@ def listed(table):
     return [pytest.param(*size, id="-".join(str(int(v)) for v in (key if isinstance(key, tuple) else (key,))) + ":" + "x".join(map(str, size))) for key, sizes in table.items() for size in sizes]
 
 
-@pytest.mark.parametrize("n,rows,cols", listed(shapes.MATMUL))
+@pytest.mark.parametrize("n,rows,cols", listed(lref.EX))
 def test_matmul_ex_in_every_kernel(oxh, n, rows, cols):
     kind = (BF16, F32, F16)[(n + rows) % 3]
     c = Case(n, rows, cols, n + cols, list(lref.ACTS.values())[(n + cols) % 5], kind=kind, w_stride=up_to_16(cols) + 16, q_stride=up_to_16(cols) + 32)

@@ -177,23 +177,38 @@ def test_workspaces():
     assert int8.Gated(**{**GATED, "cols": 131072}).workspace(4) == 0
 
 
-def key_of(n, rows, cols):
-    k = int8.gated_kernel(rows, cols, n)
+def key_of(n, rows, cols, gated):
+    k = int8.layer_kernel(rows, cols, n, gated)
     return (k[0], k[1], k[2] > 1, k[3] > 0) if k[0] == int8.TILES else (k[0], k[2], k[3])
 
 
-def test_listed_sizes_run_on_the_kernels_they_are_listed_for():
-    for key, sizes in lref.GATED.items():
+@pytest.mark.parametrize("gated,table", [(False, lref.EX), (True, lref.GATED)], ids=["epilogue", "gated"])
+def test_listed_sizes_run_on_the_kernels_they_are_listed_for(gated, table):
+    for key, sizes in table.items():
         for n, rows, cols in sizes:
-            assert key_of(n, rows, cols) == key, (n, rows, cols)
+            assert key_of(n, rows, cols, gated) == key, (n, rows, cols)
 
 
-def test_no_size_runs_on_a_kernel_that_has_none_listed():
+@pytest.mark.parametrize("gated,table", [(False, lref.EX), (True, lref.GATED)], ids=["epilogue", "gated"])
+def test_no_size_runs_on_a_kernel_that_has_none_listed(gated, table):
     rng = np.random.default_rng(1)
     for _ in range(4000):
         n, rows, cols = (int(np.exp(rng.uniform(np.log(a), np.log(b)))) for a, b in ((1, 5000), (1, 40000), (1, 20000)))
-        assert key_of(n, rows, cols) in lref.GATED, (n, rows, cols)
-    assert set(shapes.MATMUL) >= set(lref.GATED)
+        assert key_of(n, rows, cols, gated) in table, (n, rows, cols)
+    assert {key for key in table if key[:2] not in ((0, int8.TILE_64x32_RING), (0, int8.TILE_64x32))} <= set(shapes.MATMUL)
+
+
+def test_a_product_that_needs_parts_with_an_epilogue_says_so_without():
+    """One workspace serves both: where either goes in parts of its columns there is room for them."""
+    rng = np.random.default_rng(2)
+    for _ in range(2000):
+        n, rows, cols = (int(np.exp(rng.uniform(np.log(a), np.log(b)))) for a, b in ((1, 65), (1, 20000), (1, 20000)))
+        need = int8.Matrix(A, A, rows, cols, int8.stride_of(cols)).matmul_workspace(n)
+        for k in (int8.kernel(rows, cols, n), int8.layer_kernel(rows, cols, n, False)):
+            if k[0] == int8.TILES and k[2] > 1:
+                assert need >= 4 * k[2] * n * rows
+        if need:
+            assert int8.layer_kernel(rows, cols, n, False, need) == int8.layer_kernel(rows, cols, n, False)
 
 
 def test_oracle_activations_at_known_places():
