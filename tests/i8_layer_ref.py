@@ -131,7 +131,7 @@ EX = {
     (0, 7, True, False): [(4, 6516, 7118), (1, 6648, 4249)],
 }
 GATED = {
-    (1, 2, 1): [(1, 1, 1), (8, 200, 2048), (7, 2048, 1000)],
+    (1, 2, 1): [(1, 16, 1300), (8, 200, 2048), (7, 2048, 1700)],
     (1, 4, 1): [(1, 16, 2103), (8, 40, 4096), (5, 4096, 4096)],
     (1, 8, 1): [(1, 1, 4146), (1, 3415, 4949), (2, 4096, 8192), (4, 3912, 4505)],
     (0, 0, False, False): [(514, 10000, 132)],
@@ -147,7 +147,7 @@ GATED = {
     (0, 4, True, False): [(48, 2048, 8000), (66, 1450, 7728)],
     (0, 5, False, False): [(33, 20000, 100)],
     (0, 5, True, False): [(44, 4218, 15900)],
-    (0, 6, False, False): [(17, 16, 64), (9, 33, 70), (32, 300, 500), (16, 14336, 4096), (5, 14336, 4096)],
+    (0, 6, False, False): [(1, 1, 1), (7, 2048, 1000), (17, 16, 64), (9, 33, 70), (32, 300, 500), (16, 14336, 4096), (5, 14336, 4096)],
     (0, 6, True, False): [(9, 16, 8276), (1, 1, 8543), (32, 200, 9000)],
     (0, 7, False, False): [(1, 17582, 64), (8, 24486, 40)],
     (0, 7, True, False): [(1, 4455, 7576)],
