@@ -487,7 +487,7 @@ extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
     if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
         return 0;
-    return linear_parts(w->rows, w->cols, n_vec).total;
+    return linear_bytes(w->rows, w->cols, n_vec);
 }
 
 extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,

@@ -720,7 +720,7 @@ static size_t ffn_h_bytes(size_t ffn, size_t n) { return up256(n * up64(ffn) * 4
 extern "C" size_t oxh_i8_ffn_workspace(const OxhI8Gated *g, const OxhI8Matrix *down, size_t n_vec)
 {
     if (!g || !down || !workable(g->rows, g->cols, n_vec) || !workable(down->rows, down->cols, n_vec)) return 0;
-    const size_t first = gated_parts(g->rows, g->cols, n_vec), second = linear_parts(down->rows, down->cols, n_vec).total;
+    const size_t first = gated_parts(g->rows, g->cols, n_vec), second = linear_bytes(down->rows, down->cols, n_vec);
     return ffn_h_bytes(g->rows, n_vec) + (first > second ? first : second);
 }
 
@@ -728,7 +728,7 @@ extern "C" size_t oxh_i8_ffn_workspace(const OxhI8Gated *g, const OxhI8Matrix *d
 static int check_ffn_workspace(const char *who, const OxhI8Gated *g, const OxhI8Matrix *down, size_t n_vec, const void *d_workspace, size_t bytes)
 {
     const LinearParts l = linear_parts(down->rows, down->cols, n_vec);
-    if (!d_workspace || bytes < ffn_h_bytes(g->rows, n_vec) + (l.total ? l.parts : 0)) return I8_ARG("%s: workspace too small (see oxh_i8_ffn_workspace)", who);
+    if (!d_workspace || bytes < ffn_h_bytes(g->rows, n_vec) + (l.fused ? 0 : l.parts)) return I8_ARG("%s: workspace too small (see oxh_i8_ffn_workspace)", who);
     if ((uintptr_t)d_workspace & 255u) return I8_ARG("%s: workspace must be 256-byte aligned", who);
     return OXH_OK;
 }
