@@ -690,7 +690,8 @@ int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void *d_x, size
 /* oxh_i8_matmul and oxh_i8_linear with an epilogue:
  *   out = act(sum * q_scale * w_scale + bias) + residual
  * in f32, rounded once to out_type.  The residual is n_vec rows of out_type,
- * residual_stride elements apart, and may be d_out itself, at out_stride.
+ * residual_stride elements apart, and may be d_out itself, at out_stride; d_x
+ * may be the residual, but not d_out.
  * Workspaces are those of the products without one.  e NULL: none.  act(v):
  *   RELU       max(v, 0)               SILU  v / (1 + exp(-v))
  *   GELU       v * (1 + erf(v / sqrt(2))) / 2

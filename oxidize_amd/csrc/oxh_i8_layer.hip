@@ -650,8 +650,10 @@ extern "C" int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const voi
     if ((rc = check_matrix(who, w))) return rc;
     if (n_vec == 0 || w->rows == 0) return OXH_OK;
     if ((rc = check_floats(who, "d_x", x_type, d_x, x_stride, w->cols)) || (rc = check_floats(who, "d_out", out_type, d_out, out_stride, w->rows)) ||
-        (rc = check_epilogue(who, e, out_type, d_out, out_stride, w->rows)) || (rc = check_sizes(who, n_vec, w->rows)) ||
-        (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
+        (rc = check_epilogue(who, e, out_type, d_out, out_stride, w->rows)) || (rc = check_sizes(who, n_vec, w->rows)))
+        return rc;
+    if (d_out == d_x) return I8_ARG("%s: results in place of the tokens", who);      /* workgroups that quantise for themselves read all of them */
+    if ((rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)) || (rc = ready()) ||
         (rc = check_linear_workspace(who, w, n_vec, d_workspace, workspace_bytes)))    /* once more: the way depends on the device */
         return rc;
     I8ProductEx p = product_ex(i8_product(w, nullptr, 0, nullptr, n_vec, nullptr, out_type, d_out, out_stride), e);

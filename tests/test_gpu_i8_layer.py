@@ -511,6 +511,33 @@ def test_graphs_on_two_streams_replayed_between_eager_calls(oxh, n):
         oxh.oxh_stream_destroy(s)
 
 
+@pytest.mark.parametrize("n", [1, 24, 130])
+def test_two_graphs_of_one_stream_share_workspaces(oxh, n):
+    stream = ctypes.c_void_p()
+    _lib.check(oxh.oxh_stream_create(ctypes.byref(stream)))
+    steps = [Step(n, seed, stream) for seed in (10, 20)]
+    want = []
+    for st in steps:
+        st.run()
+        want.append(st.results())
+    steps[1].ws, steps[1].b.block.workspace = steps[0].ws, steps[0].b.block.workspace
+    graphs = []
+    for st in steps:
+        with mv.Graph(stream) as g:
+            st.run()
+        graphs.append(g)
+    for _ in range(3):
+        for g in graphs + graphs[::-1]:
+            g.launch()
+        for st, w in zip(steps, want):
+            assert all(np.array_equal(a, b) for a, b in zip(st.results(), w))
+        steps[0].run()                                  # eager work in the same workspaces between the replays
+    for g in graphs:
+        g.destroy()
+    mv.sync(stream)
+    oxh.oxh_stream_destroy(stream)
+
+
 def test_rows_residual_and_results_of_more_than_4_gib(oxh):
     """300000 tokens whose rows lie 16 KB apart: the last ones are far behind 4 GiB in x, add, sum, residual and results."""
     n, cols, stride, last = 300000, 33, 4096, 200

@@ -56,7 +56,7 @@ def test_norm_of_nothing_and_of_too_much():
 
 MAT = dict(d_w=A, d_scale=A, rows=8, cols=100, stride=128)
 MUL = dict(d_q=A, q_stride=128, d_q_scale=A, n_vec=3, epilogue=None, out_type=int8.F32, d_out=A, out_stride=8)
-LIN = dict(x_type=int8.F32, d_x=A, x_stride=100, n_vec=300, epilogue=None, out_type=int8.F32, d_out=A, out_stride=8, d_ws=A)
+LIN = dict(x_type=int8.F32, d_x=2 * A, x_stride=100, n_vec=300, epilogue=None, out_type=int8.F32, d_out=A, out_stride=8, d_ws=A)
 
 
 def epilogues():
@@ -82,7 +82,7 @@ def test_matmul_ex_refuses(mat, mul):
 
 
 @pytest.mark.parametrize("change", [dict(d_x=0), dict(x_stride=99), dict(x_type=9), dict(d_out=0), dict(ws_bytes=-1), dict(d_ws=0),
-                                    dict(d_ws=A + 8), dict(out_stride=7)])
+                                    dict(d_ws=A + 8), dict(out_stride=7), dict(d_x=A)])
 def test_linear_ex_refuses(change):
     m = int8.Matrix(**MAT)
     need = m.linear_workspace(300)
