@@ -10,7 +10,6 @@ Where ``own`` is false ``run`` computes them from elementary torch operations.  
 channel eight times as large; weight codes are round(32 N(0, 1)) within +-127 and their scales 2^-5 / sqrt(cols) on average,
 so that outputs are of unit size; norm weights are N(1, 0.2^2), biases N(0, 0.1^2).
 """
-import functools
 import math
 
 import torch
@@ -172,12 +171,6 @@ def run(s):
 # ─── the framework's calls ──────────────────────────────────────────────
 
 
-@functools.lru_cache(maxsize=None)
-def _program_stream():
-    """A program's stream is one for all of its calls, not made anew for each input."""
-    return torch.cuda.Stream()
-
-
 def _prepare_own(s):
     """The output buffers, workspaces and handles that a program keeps."""
     from oxidize_amd import _lib, int8
@@ -192,7 +185,7 @@ def _prepare_own(s):
     if kind == "norm":
         cols, kept = c["cols"], dict(dtype=TYPES[c["x"]], device="cuda")
         # the codes are turned into the values they stand for by the program's own next operation: a stream that both are put on
-        s["stream"] = _program_stream()
+        s["stream"] = torch.cuda.Stream()
         s["sum"] = torch.empty(n, cols, **kept) if c["add"] else None
         s["y"] = torch.empty(n, cols, **kept) if c["y"] else None
         s["q"], s["scale"], s["values"] = torch.zeros(n, _stride(cols), dtype=torch.int8, device="cuda"), _empty((n, 1), torch.float32), _empty((n, cols), torch.float32)
