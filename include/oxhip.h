@@ -647,7 +647,10 @@ int oxh_i8_quantize(uint32_t x_type, const void *d_x, size_t x_stride, size_t n_
  * aligned to its elements.  Few results over long rows are shared out over
  * the columns when there is a workspace (oxh_i8_matmul_workspace bytes,
  * 16-byte aligned, overwritten; with less, or NULL, the call does without,
- * and with the same results).  d_out may overlap no input, here and below. */
+ * and with the same results).  The function answers for n_vec tokens and for
+ * fewer, with or without an epilogue: never less for more tokens, and a smaller
+ * batch in it goes its fastest way too.  d_out may overlap no input, here and
+ * below. */
 size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec);
 int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
                   const float *d_bias, uint32_t out_type, void *d_out, size_t out_stride,
@@ -717,8 +720,8 @@ int oxh_i8_linear_ex(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, siz
 /* Both first projections of a gated feed-forward in one launch:
  *   out[t][r] = act(g) * u,  g = sum(q[t], gate[r]) * q_scale[t] * s_gate[r]
  *   + b_gate[r],  u likewise, in f32, rounded once to out_type.
- * Sizes, strides and workspace (oxh_i8_gated_workspace bytes, or less, or none)
- * as oxh_i8_matmul's. */
+ * Sizes, strides and workspace (oxh_i8_gated_workspace bytes, for n_vec tokens
+ * and fewer, or less, or none) as oxh_i8_matmul's. */
 typedef struct OxhI8Gated {
     const int8_t *d_w_gate, *d_w_up;  /* rows x cols each                                */
     size_t        stride;             /* bytes from row to row, of both                  */

@@ -690,10 +690,14 @@ static bool workable(size_t rows, size_t cols, size_t n)
     return n != 0 && rows != 0 && cols != 0 && cols <= OXH_I8_MAX_COLS && rows <= OXH_I8_MAX_ROWS && n <= OXH_I8_MAX_ROWS;
 }
 
+/* as product_parts() */
 static size_t gated_parts(size_t rows, size_t cols, size_t n)
 {
-    const I8Choice c = i8_choice(rows, cols, n, SIZE_MAX, i8_cus(), I8_GATED);
-    return c.team ? 0 : parts_bytes(i8_rows_in_all(rows, 2u), n, c.way.splits);
+    const size_t cus = i8_cus(), in_all = i8_rows_in_all(rows, 2u);
+    return most_parts(in_all, cols, n, [&](size_t m) {
+        const I8Choice c = i8_choice(rows, cols, m, SIZE_MAX, cus, I8_GATED);
+        return c.team ? (size_t)0 : parts_bytes(in_all, m, c.way.splits);
+    });
 }
 
 extern "C" size_t oxh_i8_gated_workspace(const OxhI8Gated *g, size_t n_vec)
