@@ -459,9 +459,7 @@ extern "C" int oxh_internal_i8_init(void)
 
 extern "C" size_t oxh_i8_matmul_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
-        return 0;
-    return product_parts(w->rows, w->cols, n_vec);
+    return w && workable(w->rows, w->cols, n_vec) ? product_parts(w->rows, w->cols, n_vec) : 0;
 }
 
 extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_stride, const float *d_q_scale, size_t n_vec,
@@ -485,9 +483,7 @@ extern "C" int oxh_i8_matmul(const OxhI8Matrix *w, const int8_t *d_q, size_t q_s
 
 extern "C" size_t oxh_i8_linear_workspace(const OxhI8Matrix *w, size_t n_vec)
 {
-    if (!w || n_vec == 0 || w->rows == 0 || w->cols == 0 || w->cols > OXH_I8_MAX_COLS || w->rows > OXH_I8_MAX_ROWS || n_vec > OXH_I8_MAX_ROWS)
-        return 0;
-    return linear_bytes(w->rows, w->cols, n_vec);
+    return w && workable(w->rows, w->cols, n_vec) ? linear_bytes(w->rows, w->cols, n_vec) : 0;
 }
 
 extern "C" int oxh_i8_linear(const OxhI8Matrix *w, uint32_t x_type, const void *d_x, size_t x_stride, size_t n_vec,

@@ -685,11 +685,6 @@ static int gated_launch(const OxhI8Gated *g, const int8_t *q, size_t q_stride, c
     return product_launch<I8GatedProduct, I8GatedSums>(p, i8_choice(g->rows, g->cols, n, ws_bytes, i8_cus(), I8_GATED), ws, st, who);
 }
 
-static bool workable(size_t rows, size_t cols, size_t n)
-{
-    return n != 0 && rows != 0 && cols != 0 && cols <= OXH_I8_MAX_COLS && rows <= OXH_I8_MAX_ROWS && n <= OXH_I8_MAX_ROWS;
-}
-
 /* as product_parts() */
 static size_t gated_parts(size_t rows, size_t cols, size_t n)
 {

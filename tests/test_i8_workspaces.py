@@ -93,3 +93,12 @@ def test_calls_accept_the_workspace_of_more_tokens(n, rows, cols):
         refused(m.linear, int8.F32, A, cols, k, int8.F32, A, rows, d_ws=A, ws_bytes=need, status=_lib.ERR_NO_DEVICE)
         b = Block(g, down, int(_lib.lib().oxh_i8_ffn_workspace(g._ref, down._ref, n)))
         refused(b.forward, A, int8.stride_of(cols), A, k, None, int8.F32, A, cols, status=_lib.ERR_NO_DEVICE)
+
+
+def test_sizes_that_are_refused_have_no_workspace():
+    """More than 2^37 results: the calls are refused, and the functions say 0."""
+    rows, n = 1 << 21, 1 << 16
+    assert matrix(rows, 5000).linear_workspace(n) >= codes_bytes(n, 5000) and matrix(rows, 5000).linear_workspace(n + 1) == 0
+    assert matrix(rows, 5000).matmul_workspace(n + 1) == 0 and gated(rows, 5000).workspace(n + 1) == 0
+    refused(matrix(rows, 5000).linear, int8.F32, A, 5000, n + 1, int8.F32, A, rows, d_ws=A, ws_bytes=1 << 40)
+    assert block(100, 100000, 1 << 20) > 0 and block(100, 131071, (1 << 20) + 16) == 0 and block(1 << 17, 100, (1 << 20) + 1) == 0
