@@ -695,11 +695,18 @@ int oxh_i8_rmsnorm(const OxhI8Norm *norm, uint32_t x_type, const void *d_x, size
  * in f32, rounded once to out_type.  The residual is n_vec rows of out_type,
  * residual_stride elements apart, and may be d_out itself, at out_stride; d_x
  * may be the residual, but not d_out.
- * Workspaces are those of the products without one.  e NULL: none.  act(v):
+ * Workspaces are those of the products without one, whose functions answer for
+ * both.  e NULL: none.  act(v):
  *   RELU       max(v, 0)               SILU  v / (1 + exp(-v))
  *   GELU       v * (1 + erf(v / sqrt(2))) / 2
  *   GELU_TANH  v * (1 + tanh(sqrt(2 / pi) * (v + 0.044715 v^3))) / 2
- * of a NaN NaN; of -inf 0 (RELU) or NaN. */
+ * of a NaN NaN; of -inf 0 (RELU) or NaN.  By the instructions for 2^x and 1/x,
+ * within, in units of 2^-24 of the value: SILU 6 + 1.01 |v|, GELU 20 + 1.2 v^2,
+ * GELU_TANH 6 + 3.4 |2 sqrt(2 / pi) (v + 0.044715 v^3)| below 0, and 6, 20 and 6
+ * above; what is less than 1.03e-36 may be lost.  oxh_i8_quantize with d_up and
+ * oxh_moe_ffn_i8 have a SiLU with an exponential and a division, good to 7 units
+ * everywhere: codes made of a gated product's results may differ from theirs in
+ * values next to a half. */
 #define OXH_ACT_NONE      0u
 #define OXH_ACT_RELU      1u
 #define OXH_ACT_SILU      2u

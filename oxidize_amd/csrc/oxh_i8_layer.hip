@@ -203,8 +203,9 @@ __global__ __launch_bounds__(THREADS) void k_i8_rmsnorm(const I8Norm p)
 __device__ __forceinline__ float i8_logistic(float t) { return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(t)); }
 
 /* v P(X <= v) of a normal X.  P(X > z) = 2^(-z^2 / (2 ln 2)) R(z) falls as fast as its first factor; R = erfcx(z / sqrt(2)) / 2 has no scale of its own and is a
- * polynomial of degree 8 in 1 / (1 + 0.3 z) without a constant term, fitted to least relative error over 0 <= z <= 13.5, where the first
- * factor leaves the f32 numbers: 7.2 * 2^-24 off with its own roundings. */
+ * polynomial of degree 8 in 1 / (1 + 0.3 z) without a constant term, fitted to least relative error (2.4 * 2^-24) over 0 <= z <= 13.5, where the first
+ * factor leaves the f32 numbers.  v v times the constant is rounded three times ahead of 2^x, which counts as v^2: in units of 2^-24 the whole is
+ * within 20 + 1.2 v^2 below 0 and within 20 above (2^21 values each: 9.0 off in -1 .. 0, 14 in -4 .. -2, 46 in -8 .. -6, 127 in -13 .. -10; 8.7 above). */
 __device__ __forceinline__ float i8_gelu(float v)
 {
     const float t = __builtin_amdgcn_rcpf(__builtin_fmaf(0.3f, fabsf(v), 1.0f));
@@ -220,7 +221,9 @@ __device__ __forceinline__ float i8_gelu(float v)
     return v * (v > 0.0f ? 1.0f - above : above);
 }
 
-/* In 32 bits; a NaN stays one.  SILU's exponent is rounded once: -1 / ln 2 is the sum of two f32 numbers. */
+/* In 32 bits; a NaN stays one.  SILU's exponent is rounded once: -1 / ln 2 is the sum of two f32 numbers (within 6 + 1.01 |v| units of 2^-24; 8 off in
+ * -8 .. -4, 47 in -80 .. -30).  The tanh form's, -2u / ln 2, is rounded three times and has two rounded constants (6 + 3.4 |2u|; 16 off in -4 .. -2, 155 in -10 ..
+ * -8, where it is below 2^-68). */
 template <uint32_t ACT> __device__ __forceinline__ float i8_activate(float v)
 {
     if (ACT == OXH_ACT_RELU) return v < 0.0f ? 0.0f : v;

@@ -84,6 +84,7 @@ class Matrix:
         self._ref = ctypes.byref(self.desc)
 
     def matmul_workspace(self, n_vec):
+        """What n_vec tokens make use of, or fewer, with or without an epilogue."""
         return int(lib().oxh_i8_matmul_workspace(self._ref, n_vec))
 
     def matmul(self, d_q, q_stride, d_q_scale, n_vec, out_type, d_out, out_stride, d_bias=None, d_ws=None, ws_bytes=0, stream=None):
@@ -119,6 +120,7 @@ class Gated:
         self._ref = ctypes.byref(self.desc)
 
     def workspace(self, n_vec):
+        """What n_vec tokens make use of, or fewer."""
         return int(lib().oxh_i8_gated_workspace(self._ref, n_vec))
 
     def matmul(self, d_q, q_stride, d_q_scale, n_vec, out_type, d_out, out_stride, d_ws=None, ws_bytes=0, stream=None):
